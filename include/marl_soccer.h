@@ -354,6 +354,148 @@ int ms_rollout_record(int64_t n_envs, const float *rew, const uint8_t *term, con
                       const int32_t *score, float *rewards, float *next_done, float *dones_next,
                       int64_t *episodes, int64_t *score_sum, void *stream);
 
+/* ---- sequence memory of a policy: short causal convolution and selective state-space scan ---
+ * (no reference equivalent: the reference's policy sees a stack of 3 frames. marlsoccer.sequence
+ * and marlsoccer.memory wrap these.) Sequences are T steps of R rows of D channels; every
+ * time-dependent array has its own step and row strides (elements, any order) and contiguous
+ * channels. starts (uint8, non-zero = true; NULL: none): starts[t][r] says that row r begins a
+ * new episode at step t, and nothing before t, the given state included, reaches step t or later.
+ * dtype: 0 float32, 1 bfloat16, 2 float16 for the arrays marked [io]; all others are float32.
+ * Asynchronous on `stream`; no atomics, so results repeat bit for bit. Arrays must not overlap
+ * unless stated. T = 0 and R = 0 are allowed (state copied through, gradients zero).
+ *
+ * ms_conv_forward: out[t][r][d] = act(bias[d] + sum_k weight[d][k] x[t - W + 1 + k][r][d]), W = width
+ *   in 2..4, act SiLU or none; steps before 0 come from state (R, W-1, D) [io], oldest first
+ *   (NULL: zeros). new_state (R, W-1, D) [io] (NULL: not written): the W-1 newest inputs, zeros
+ *   for those before the last start. It may be `state` itself when T <= 1 (a step in place).
+ * ms_conv_backward: gradients for dout and dnew_state (NULL: zero) with the same inputs: dx,
+ *   dstate [io], dweight (D, W), dbias (D); NULL gradients are not written (dx is required).
+ *   workspace: ms_conv_workspace() bytes, 16-B aligned.
+ */
+typedef struct ms_conv_io {
+  int32_t dtype, width, silu, pad0;
+  int64_t steps, rows, channels;
+  const void *x;
+  int64_t x_t, x_r;
+  const float *weight, *bias;
+  const void *state;
+  const uint8_t *starts;
+  int64_t starts_t, starts_r;
+  void *out;
+  int64_t out_t, out_r;
+  void *new_state;
+  const void *dout;
+  int64_t dout_t, dout_r;
+  const void *dnew_state;
+  void *dx;
+  int64_t dx_t, dx_r;
+  void *dstate;
+  float *dweight, *dbias;
+  void *workspace;
+  int64_t workspace_bytes;
+} ms_conv_io;
+int ms_conv_forward(const ms_conv_io *io, void *stream);
+int64_t ms_conv_workspace(const ms_conv_io *io);
+int ms_conv_backward(const ms_conv_io *io, void *stream);
+
+/* ms_scan_forward: for every row r, channel d and state n < N (1..64), with the rate
+ *   rate = delta[t][r][d] + delta_bias[d], through softplus when softplus != 0:
+ *     h[n]  = exp(rate A[d][n]) h[n] + rate u[t][r][d] B[t][r][g][n]
+ *     y     = sum_n C[t][r][g][n] h[n] + D[d] u[t][r][d]
+ *     out   = y silu(z[t][r][d])   (y where z is NULL)
+ *   u, delta, z, out (T, R, D) [io]; B, C (T, R, G, N) [io], shared by the D / G channels of group
+ *   g; A (D, N), D (D), delta_bias (D) (the last two may be NULL); state (R, D, N) the states
+ *   before step 0 (NULL: zeros), new_state (R, D, N) after the last (NULL: not written; it may be
+ *   `state` itself). A is meant to be negative (a state that decays). States, sums and rates are
+ *   held in 32 bits; out is rounded once.
+ *   checkpoints: NULL, or ms_scan_checkpoints() bytes that ms_scan_backward reads.
+ *   workspace: ms_scan_workspace(io, 0) bytes (0: may be NULL), 16-B aligned.
+ * ms_scan_step: one step (steps = 1; the t strides are not read) for every row, state renewed in
+ *   place; needs no workspace.
+ * ms_scan_backward: gradients for dout and dnew_state (NULL: zero) with the inputs and checkpoints
+ *   of the forward: du, ddelta, dz [io, the strides given], dB, dC [io, (T, R, G, N) contiguous],
+ *   dA, dD, ddelta_bias, dstate (contiguous). du, ddelta, dB, dC and dA are required, dz with z;
+ *   the others may be NULL. workspace: ms_scan_workspace(io, 1) bytes. */
+typedef struct ms_scan_io {
+  int32_t dtype, softplus, states, groups;
+  int64_t steps, rows, channels;
+  const void *u;
+  int64_t u_t, u_r;
+  const void *delta;
+  int64_t delta_t, delta_r;
+  const void *z;
+  int64_t z_t, z_r;
+  const void *B;
+  int64_t B_t, B_r, B_g;
+  const void *C;
+  int64_t C_t, C_r, C_g;
+  const float *A, *D, *delta_bias;
+  const float *state;
+  const uint8_t *starts;
+  int64_t starts_t, starts_r;
+  void *out;
+  int64_t out_t, out_r;
+  float *new_state;
+  float *checkpoints;
+  const void *dout;
+  int64_t dout_t, dout_r;
+  const float *dnew_state;
+  void *du;
+  int64_t du_t, du_r;
+  void *ddelta;
+  int64_t ddelta_t, ddelta_r;
+  void *dz;
+  int64_t dz_t, dz_r;
+  void *dB, *dC;
+  float *dA, *dD, *ddelta_bias, *dstate;
+  void *workspace;
+  int64_t workspace_bytes;
+} ms_scan_io;
+int ms_scan_forward(const ms_scan_io *io, void *stream);
+int ms_scan_step(const ms_scan_io *io, void *stream);
+int64_t ms_scan_checkpoints(const ms_scan_io *io);
+int64_t ms_scan_workspace(const ms_scan_io *io, int backward);
+int ms_scan_backward(const ms_scan_io *io, void *stream);
+const char *ms_sequence_last_error(void);
+
+/* ---- the optimiser step of a PPO update (the notebook's train cell: Adam and clip_grad_norm_ over
+ * the Agent's parameters; marlsoccer.optim wraps this) -----------------------------------------
+ * ms_adamw_step: for every tensor i < count, with t = ++*step (int64, device), g = grad * clip and
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g g,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps),
+ * computed in float32 and rounded once to p's type. lr_device (float32, device), when non-NULL, is
+ * read in place of lr. clip is the factor that ms_grad_clip left in the workspace when use_clip != 0,
+ * else 1.
+ *   param, grad: dtype 0 float32, 1 bfloat16, 2 float16 (the same for both), numel elements in a row.
+ *   state_bits 32: exp_avg, exp_avg_sq float32. state_bits 8: OCP e4m3 bytes, exp_avg the codes of
+ *   m and exp_avg_sq those of sqrt(v), each with a float32 scale for every MS_ADAMW_BLOCK elements
+ *   (value = code * scale, scale = max|.| / 448) in the *_scale arrays.
+ * ms_grad_clip: factor = min(1, max_norm / (norm + 1e-6)), norm the Euclidean norm of all the
+ *   tensors' gradients (summed in float64, in a fixed order; a non-finite one passes into the
+ *   update, as clip_grad_norm_ has it); also written to *grad_norm (float32, device) when non-NULL.
+ *   Reads param-independent fields only (grad, dtype, numel).
+ * workspace: MS_OPTIM_WORKSPACE floats of device memory, 16-B aligned, zeroed once; one step at a
+ * time may use it. Tensors must not overlap. MS_OPTIM_TENSORS of them go into a launch; a longer
+ * list takes several. Asynchronous on `stream`, nothing read on the host: may be captured. */
+#define MS_OPTIM_WORKSPACE 4096
+#define MS_OPTIM_TENSORS 48
+#define MS_ADAMW_BLOCK 256
+typedef struct ms_optim_tensor {
+  void *param;
+  const void *grad;
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale;
+  int64_t *step;
+  int64_t numel;
+  int32_t dtype, pad0;
+} ms_optim_tensor;
+int ms_grad_clip(const ms_optim_tensor *tensors, int64_t count, double max_norm, float *grad_norm,
+                 float *workspace, void *stream);
+int ms_adamw_step(const ms_optim_tensor *tensors, int64_t count, int state_bits, double lr,
+                  const float *lr_device, double beta1, double beta2, double eps, double weight_decay,
+                  int use_clip, float *workspace, void *stream);
+const char *ms_optim_last_error(void);
+
 /* Synchronises the stream and reads the device counters. */
 int ms_get_stats(ms_env *env, ms_stats *out);
 int ms_reset_stats(ms_env *env);

@@ -18,11 +18,16 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIB_DIR, "libmarlsoccer.so")
-SOURCES = [os.path.join(CSRC, "ms_env.hip"), os.path.join(CSRC, "ms_policy.hip"), os.path.join(CSRC, "ms_kstep.hip")]
+SOURCES = [os.path.join(CSRC, f) for f in ("ms_env.hip", "ms_policy.hip", "ms_kstep.hip", "ms_conv.hip", "ms_scan.hip",
+                                           "ms_optim.hip")]
 # per-source flags: the K-step kernels (ms_kstep.hip) without LLVM's machine loop-invariant code motion,
-# which hoisted per-step values out of their K-step loop and spilled them
-UNIT_FLAGS = {"ms_kstep.hip": ["-mllvm", "-disable-machine-licm"]}
-DEPS = SOURCES + [os.path.join(CSRC, "ms_device.h"), os.path.join(CSRC, "ms_diag.h"), os.path.join(CSRC, "ms_group.inc"), os.path.join(CSRC, "ms_pair.inc"), os.path.join(ROOT, "include", "marl_soccer.h")]
+# which hoisted per-step values out of their K-step loop and spilled them; the sequence and
+# optimiser kernels without packed float32 instructions, some forms of which have given wrong results
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+UNIT_FLAGS = {"ms_kstep.hip": ["-mllvm", "-disable-machine-licm"], "ms_conv.hip": NO_PACKED, "ms_scan.hip": NO_PACKED,
+              "ms_optim.hip": NO_PACKED}
+DEPS = SOURCES + [os.path.join(CSRC, "ms_device.h"), os.path.join(CSRC, "ms_diag.h"), os.path.join(CSRC, "ms_group.inc"), os.path.join(CSRC, "ms_pair.inc"),
+                  os.path.join(CSRC, "ms_sequence.h"), os.path.join(ROOT, "include", "marl_soccer.h")]
 ARCH = os.environ.get("MS_OFFLOAD_ARCH", "gfx950")
 # LLVM's default AMDGPU machine scheduler. The max-ILP strategy (-mllvm
 # -amdgpu-sched-strategy=max-ilp, -2.6 % step time in round 1) produced kernels that fault on the

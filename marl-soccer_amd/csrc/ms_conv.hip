@@ -1,0 +1,366 @@
+// ms_conv.hip — short causal convolution over time, per channel, with its gradients (gfx950).
+//
+//   pre[t] = b + sum_j w[W-1-j] x[t-j],  out = silu(pre) or pre,  j < W <= 4,
+// where x[t-j] counts only if no episode starts in (t-j, t], and steps before 0 are the state's.
+// Backward, with p[t] = dout[t] act'(pre[t]) and the same condition:
+//   dx[t] = sum_j w[W-1-j] p[t+j],  dw[W-1-j] = sum_t p[t] x[t-j],  db = sum_t p[t].
+//
+// Bound by HBM: one read of x and one write of out (backward: x, dout, dx), a few FMAs a value.
+// A thread owns 16 B of neighbouring channels (one 16-B access a step) and walks a span of steps
+// with its window of W - 1 inputs in registers; a span begins by re-reading the W - 1 steps before
+// it, which is what splitting the time axis costs.
+#include "ms_sequence.h"
+
+thread_local char g_sequence_error[256] = "";
+
+extern "C" const char* ms_sequence_last_error(void) { return g_sequence_error; }
+
+namespace conv {
+using namespace seq;
+
+constexpr int THREADS = 256;
+
+struct Shape {  // the launch: a block covers `cols` groups of E channels and `slots` spans at a time
+  int cols_log2;
+  int64_t groups, spans, span, items, blocks_c, blocks_p;
+};
+
+template <typename T, int E, int W>
+__global__ __launch_bounds__(THREADS) void forward(const ms_conv_io io, const Shape sh, bool vec) {
+  const int cols = 1 << sh.cols_log2, slots = THREADS >> sh.cols_log2;
+  const int64_t group = (int64_t)(blockIdx.x % sh.blocks_c) * cols + (threadIdx.x & (cols - 1));
+  const int64_t item = (int64_t)(blockIdx.x / sh.blocks_c) * slots + (threadIdx.x >> sh.cols_log2);
+  if (group >= sh.groups || item >= sh.items) return;
+  const int64_t c = group * E, D = io.channels;
+  const int n = (int)(D - c < E ? D - c : E);
+  const int64_t r = item % io.rows, t0 = item / io.rows * sh.span;
+  const int64_t t1 = t0 + sh.span < io.steps ? t0 + sh.span : io.steps;
+  const T* x = (const T*)io.x + r * io.x_r + c;
+  T* out = (T*)io.out + r * io.out_r + c;
+  const uint8_t* starts = io.starts ? io.starts + r * io.starts_r : nullptr;
+  const T* state = io.state ? (const T*)io.state + r * (W - 1) * D + c : nullptr;
+  float w[W][E], b[E], win[W - 1][E];  // win[k]: the input W - 1 - k steps back
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    b[e] = io.bias && e < n ? io.bias[c + e] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) w[k][e] = e < n ? io.weight[(c + e) * W + k] : 0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k) {
+    const int64_t t = t0 - (W - 1) + k;
+    typename Vec<T, E>::type v;
+    if (t >= 0) {
+      v = load<T, E>(x + t * io.x_t, n, vec);
+      if (starts && starts[t * io.starts_t]) {
+#pragma unroll
+        for (int j = 0; j < k; ++j)
+#pragma unroll
+          for (int e = 0; e < E; ++e) win[j][e] = 0.0f;
+      }
+    } else if (state) {
+      v = load<T, E>(state + (W - 1 + t) * D, n, vec);
+    } else {
+      v = 0;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) win[k][e] = (float)v[e];
+  }
+#pragma unroll 4
+  for (int64_t t = t0; t < t1; ++t) {
+    const typename Vec<T, E>::type v = load<T, E>(x + t * io.x_t, n, vec);
+    if (starts && starts[t * io.starts_t]) {
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+        for (int e = 0; e < E; ++e) win[j][e] = 0.0f;
+    }
+    float y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float a = b[e];
+#pragma unroll
+      for (int k = 0; k < W - 1; ++k) a = __builtin_fmaf(w[k][e], win[k][e], a);
+      a = __builtin_fmaf(w[W - 1][e], (float)v[e], a);
+      y[e] = io.silu ? silu(a) : a;
+#pragma unroll
+      for (int k = 0; k < W - 2; ++k) win[k][e] = win[k + 1][e];
+      win[W - 2][e] = (float)v[e];
+    }
+    store<T, E>(out + t * io.out_t, y, n, vec);
+  }
+  if (io.new_state && t1 == io.steps) {
+    T* ns = (T*)io.new_state + r * (W - 1) * D + c;
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) store<T, E>(ns + k * D, win[k], n, vec);
+  }
+}
+
+// p[t] reaches dx of steps t - W + 1 .. t: pend[j] collects dx[t - j], complete (and stored) when it
+// falls out of the window. reach: how many steps back belong to step t's episode. A span stores the
+// steps of its own and runs W - 1 steps past them, whose p counts for dx but not for dw and db.
+template <typename T, int E, int W>
+__global__ __launch_bounds__(THREADS) void backward(const ms_conv_io io, const Shape sh, bool vec,
+                                                    float* __restrict__ parts) {
+  __shared__ float red[THREADS];
+  const int cols = 1 << sh.cols_log2, slots = THREADS >> sh.cols_log2;
+  const int64_t bc = blockIdx.x % sh.blocks_c, bp = blockIdx.x / sh.blocks_c;
+  const int col = threadIdx.x & (cols - 1), slot = threadIdx.x >> sh.cols_log2;
+  const int64_t group = bc * cols + col, D = io.channels, c = group * E;
+  const int n = group < sh.groups ? (int)(D - c < E ? D - c : E) : 0;
+  float w[W][E], b[E], dw[W][E], db[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    b[e] = io.bias && e < n ? io.bias[c + e] : 0.0f;
+    db[e] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      w[k][e] = e < n ? io.weight[(c + e) * W + k] : 0.0f;
+      dw[k][e] = 0.0f;
+    }
+  }
+  for (int64_t item = bp * slots + slot; n > 0 && item < sh.items; item += sh.blocks_p * slots) {
+    const int64_t r = item % io.rows, t0 = item / io.rows * sh.span;
+    const int64_t t1 = t0 + sh.span < io.steps ? t0 + sh.span : io.steps;
+    const int64_t t2 = t1 + W - 1 < io.steps ? t1 + W - 1 : io.steps;
+    const T* x = (const T*)io.x + r * io.x_r + c;
+    const T* dout = (const T*)io.dout + r * io.dout_r + c;
+    T* dx = (T*)io.dx + r * io.dx_r + c;
+    const uint8_t* starts = io.starts ? io.starts + r * io.starts_r : nullptr;
+    const int64_t row = r * (W - 1) * D + c;
+    float win[W - 1][E], pend[W - 1][E];  // pend[j]: dx of step t - 1 - j as far as it is known
+    int reach = 0;
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) {
+      const int64_t t = t0 - (W - 1) + k;
+      typename Vec<T, E>::type v;
+      v = 0;
+      reach = reach < W - 1 ? reach + 1 : W - 1;
+      if (t >= 0) {
+        v = load<T, E>(x + t * io.x_t, n, vec);
+        if (starts && starts[t * io.starts_t]) {
+          reach = 0;
+#pragma unroll
+          for (int j = 0; j < k; ++j)
+#pragma unroll
+            for (int e = 0; e < E; ++e) win[j][e] = 0.0f;
+        }
+      } else if (io.state) {
+        v = load<T, E>((const T*)io.state + row + (W - 1 + t) * D, n, vec);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        win[k][e] = (float)v[e];
+        pend[k][e] = 0.0f;
+      }
+    }
+    // after the W - 1 steps before t0, reach counts how many of the steps t0 - 1, t0 - 2, ... belong
+    // to step t0 - 1's episode (that step itself not counted)
+    auto flush = [&](int64_t t, const float (&g)[E]) __attribute__((always_inline)) {  // dx[t] is complete
+      if (t >= t0 && t < t1) store<T, E>(dx + t * io.dx_t, g, n, vec);
+      if (t < 0 && t0 == 0 && io.dstate) store<T, E>((T*)io.dstate + row + (W - 1 + t) * D, g, n, vec);
+    };
+#pragma unroll 2
+    for (int64_t t = t0; t < t2; ++t) {
+      const typename Vec<T, E>::type v = load<T, E>(x + t * io.x_t, n, vec);
+      const typename Vec<T, E>::type d = load<T, E>(dout + t * io.dout_t, n, vec);
+      reach = reach < W - 1 ? reach + 1 : W - 1;
+      if (starts && starts[t * io.starts_t]) {
+        reach = 0;
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+          for (int e = 0; e < E; ++e) win[j][e] = 0.0f;
+      }
+      float done[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float a = b[e];
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) a = __builtin_fmaf(w[k][e], win[k][e], a);
+        a = __builtin_fmaf(w[W - 1][e], (float)v[e], a);
+        const float p = io.silu ? (float)d[e] * silu_slope(a) : (float)d[e];
+        if (t < t1) {
+          db[e] += p;
+#pragma unroll
+          for (int k = 0; k < W - 1; ++k) dw[k][e] = __builtin_fmaf(p, win[k][e], dw[k][e]);
+          dw[W - 1][e] = __builtin_fmaf(p, (float)v[e], dw[W - 1][e]);
+        }
+#pragma unroll
+        for (int j = 1; j < W; ++j)
+          if (j <= reach) pend[j - 1][e] = __builtin_fmaf(w[W - 1 - j][e], p, pend[j - 1][e]);
+        done[e] = pend[W - 2][e];
+#pragma unroll
+        for (int j = W - 2; j > 0; --j) pend[j][e] = pend[j - 1][e];
+        pend[0][e] = w[W - 1][e] * p;
+#pragma unroll
+        for (int k = 0; k < W - 2; ++k) win[k][e] = win[k + 1][e];
+        win[W - 2][e] = (float)v[e];
+      }
+      flush(t - (W - 1), done);
+    }
+    if (t2 == io.steps) {  // the last steps, and the gradient of the state handed on
+#pragma unroll
+      for (int j = 0; j < W - 1; ++j) {
+        if (io.dnew_state && j <= reach) {
+          const typename Vec<T, E>::type g = load<T, E>((const T*)io.dnew_state + row + (W - 2 - j) * D, n, vec);
+#pragma unroll
+          for (int e = 0; e < E; ++e) pend[j][e] += (float)g[e];
+        }
+        flush(t2 - 1 - j, pend[j]);
+      }
+    }
+  }
+  // the block's sums: slots of the same channels in turn, in a fixed order
+  float* to = parts + bp * (W + 1) * D;
+#pragma unroll
+  for (int k = 0; k <= W; ++k)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      __syncthreads();
+      red[threadIdx.x] = k < W ? dw[k < W ? k : 0][e] : db[e];
+      __syncthreads();
+      if (slot == 0 && e < n) {
+        float a = 0.0f;
+        for (int s = 0; s < slots; ++s) a += red[s * cols + col];
+        to[(c + e) * (W + 1) + k] = a;
+      }
+    }
+}
+
+// parts (P, D, W + 1) -> dweight (D, W), dbias (D)
+__global__ __launch_bounds__(256) void finish(const float* __restrict__ sums, int64_t D, int W, float* __restrict__ dweight,
+                                              float* __restrict__ dbias) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= D * (W + 1)) return;
+  const int64_t d = i / (W + 1);
+  const int k = (int)(i - d * (W + 1));
+  if (k < W) {
+    if (dweight) dweight[d * W + k] = sums[i];
+  } else if (dbias) {
+    dbias[d] = sums[i];
+  }
+}
+
+// How the work is cut: spans of steps long enough that the W - 1 re-read steps cost little, short
+// enough that there are threads for every SIMD several times over.
+Shape shape(const ms_conv_io& io, bool back) {
+  Shape s = {};
+  const int E = io.dtype == 0 ? 4 : 8;
+  s.groups = (io.channels + E - 1) / E;
+  while ((1 << s.cols_log2) < s.groups && s.cols_log2 < 8) ++s.cols_log2;
+  const int64_t slots = THREADS >> s.cols_log2;
+  s.blocks_c = (s.groups + (1 << s.cols_log2) - 1) >> s.cols_log2;
+  const int64_t want = 262144;  // threads: 256 CUs x 16 waves
+  const int64_t have = s.groups * io.rows;
+  int64_t spans = have > 0 ? (want + have - 1) / have : 1;
+  const int64_t most = (io.steps + 15) / 16;  // 16 steps at least: 3 re-read
+  spans = spans > most ? most : spans;
+  spans = spans < 1 ? 1 : spans;
+  s.span = (io.steps + spans - 1) / spans;
+  s.span = s.span < 1 ? 1 : s.span;
+  s.spans = io.steps > 0 ? (io.steps + s.span - 1) / s.span : 1;
+  s.items = s.spans * io.rows;
+  s.blocks_p = (s.items + slots - 1) / slots;
+  s.blocks_p = s.blocks_p < 1 ? 1 : s.blocks_p;
+  if (back) {  // every block leaves sums to be added: as many as fill the chip
+    const int64_t cap = (1024 + s.blocks_c - 1) / s.blocks_c;
+    if (s.blocks_p > cap) s.blocks_p = cap;
+  }
+  return s;
+}
+
+const char* check(const ms_conv_io* io, bool back) {
+  if (!io) return "no arguments";
+  if (io->dtype < 0 || io->dtype > 2) return "dtype must be 0 (float32), 1 (bfloat16) or 2 (float16)";
+  if (io->width < 2 || io->width > 4) return "width must be 2, 3 or 4";
+  if (io->steps < 0 || io->rows < 0 || io->channels <= 0) return "steps and rows must be >= 0, channels > 0";
+  if (io->rows > 0 && io->steps > (int64_t)1 << 40) return "too many steps";
+  if (!io->weight) return "weight is NULL";
+  const bool some = io->steps > 0 && io->rows > 0;
+  if (some && !io->x) return "x is NULL";
+  if (!back && some && !io->out) return "out is NULL";
+  if (!back && io->new_state && io->new_state == io->state && io->steps > 1)
+    return "new_state may be the state only for one step";
+  if (back && some && (!io->dout || !io->dx)) return "dout or dx is NULL";
+  return nullptr;
+}
+
+template <typename T, int E>
+int run_forward(const ms_conv_io& io, const Shape& s, bool vec, hipStream_t stream) {
+  const int64_t blocks = s.blocks_c * s.blocks_p;
+  if (blocks > 0x7fffffff) return fail(MS_ERR_INVALID_ARGUMENT, "ms_conv_forward", "too large");
+  const dim3 grid((unsigned)blocks), block(THREADS);
+  switch (io.width) {
+    case 2: hipLaunchKernelGGL((forward<T, E, 2>), grid, block, 0, stream, io, s, vec); break;
+    case 3: hipLaunchKernelGGL((forward<T, E, 3>), grid, block, 0, stream, io, s, vec); break;
+    default: hipLaunchKernelGGL((forward<T, E, 4>), grid, block, 0, stream, io, s, vec); break;
+  }
+  return launched("ms_conv_forward");
+}
+template <typename T, int E>
+int run_backward(const ms_conv_io& io, const Shape& s, bool vec, hipStream_t stream) {
+  const dim3 grid((unsigned)(s.blocks_c * s.blocks_p)), block(THREADS);
+  float* parts = (float*)io.workspace;
+  const int64_t columns = io.channels * (io.width + 1);
+  float* sums = parts + s.blocks_p * columns;
+  switch (io.width) {
+    case 2: hipLaunchKernelGGL((backward<T, E, 2>), grid, block, 0, stream, io, s, vec, parts); break;
+    case 3: hipLaunchKernelGGL((backward<T, E, 3>), grid, block, 0, stream, io, s, vec, parts); break;
+    default: hipLaunchKernelGGL((backward<T, E, 4>), grid, block, 0, stream, io, s, vec, parts); break;
+  }
+  if (int rc = launched("ms_conv_backward")) return rc;
+  if (!io.dweight && !io.dbias) return MS_OK;
+  hipLaunchKernelGGL((sum_parts<8>), dim3((unsigned)((columns + 63) / 64)), dim3(512), 0, stream, parts, s.blocks_p,
+                     columns, sums);
+  hipLaunchKernelGGL(finish, dim3((unsigned)((columns + 255) / 256)), dim3(256), 0, stream, sums, io.channels, io.width,
+                     io.dweight, io.dbias);
+  return launched("ms_conv_backward");
+}
+
+bool state_aligned(const ms_conv_io& io, int64_t elem, int64_t E) {
+  return (!io.state || aligned(io.state, io.channels, 0, elem, E)) &&
+         (!io.new_state || aligned(io.new_state, io.channels, 0, elem, E)) &&
+         (!io.dstate || aligned(io.dstate, io.channels, 0, elem, E)) &&
+         (!io.dnew_state || aligned(io.dnew_state, io.channels, 0, elem, E));
+}
+
+}  // namespace conv
+
+extern "C" {
+
+int ms_conv_forward(const ms_conv_io* io, void* stream) {
+  if (const char* why = conv::check(io, false)) return seq::fail(MS_ERR_INVALID_ARGUMENT, "ms_conv_forward", why);
+  if (io->rows == 0 || (io->steps == 0 && !io->new_state)) return MS_OK;
+  const conv::Shape s = conv::shape(*io, false);
+  const int64_t elem = io->dtype == 0 ? 4 : 2, E = 16 / elem;
+  const bool vec = seq::aligned(io->x, io->x_t, io->x_r, elem, E) && seq::aligned(io->out, io->out_t, io->out_r, elem, E) &&
+                   conv::state_aligned(*io, elem, E);
+  const hipStream_t st = (hipStream_t)stream;
+  if (io->dtype == 0) return conv::run_forward<float, 4>(*io, s, vec, st);
+  if (io->dtype == 1) return conv::run_forward<seq::bf16, 8>(*io, s, vec, st);
+  return conv::run_forward<seq::f16, 8>(*io, s, vec, st);
+}
+
+int64_t ms_conv_workspace(const ms_conv_io* io) {
+  if (conv::check(io, true)) return 0;
+  const conv::Shape s = conv::shape(*io, true);
+  return (s.blocks_p + 1) * io->channels * (io->width + 1) * (int64_t)sizeof(float);
+}
+
+int ms_conv_backward(const ms_conv_io* io, void* stream) {
+  if (const char* why = conv::check(io, true)) return seq::fail(MS_ERR_INVALID_ARGUMENT, "ms_conv_backward", why);
+  const conv::Shape s = conv::shape(*io, true);
+  if (!io->workspace || ((uintptr_t)io->workspace & 15u) || io->workspace_bytes < ms_conv_workspace(io))
+    return seq::fail(MS_ERR_INVALID_ARGUMENT, "ms_conv_backward", "the workspace is missing, misaligned or too small");
+  if (s.blocks_c * s.blocks_p > 0x7fffffff) return seq::fail(MS_ERR_INVALID_ARGUMENT, "ms_conv_backward", "too large");
+  const int64_t elem = io->dtype == 0 ? 4 : 2, E = 16 / elem;
+  const bool vec = seq::aligned(io->x, io->x_t, io->x_r, elem, E) && seq::aligned(io->dout, io->dout_t, io->dout_r, elem, E) &&
+                   seq::aligned(io->dx, io->dx_t, io->dx_r, elem, E) && conv::state_aligned(*io, elem, E);
+  const hipStream_t st = (hipStream_t)stream;
+  if (io->dtype == 0) return conv::run_backward<float, 4>(*io, s, vec, st);
+  if (io->dtype == 1) return conv::run_backward<seq::bf16, 8>(*io, s, vec, st);
+  return conv::run_backward<seq::f16, 8>(*io, s, vec, st);
+}
+
+}  // extern "C"

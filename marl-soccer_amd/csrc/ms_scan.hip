@@ -1,0 +1,888 @@
+// ms_scan.hip — selective state-space scan over time, its gradients, and its single step (gfx950).
+//
+// Per row r, channel d, state n:  h[t] = a[t] h[t-1] + rate u B[t],  a = exp(rate A),  rate =
+// softplus(delta + bias);  y = sum_n C h + D u;  out = y silu(z).  starts[t] sets h[t-1] to zero.
+//
+// What bounds it: each (t, r, d) moves 6-8 B in half precision but needs N exponentials (v_exp_f32,
+// a quarter of the rate of an FMA) and 4 N other VALU operations, so at N = 16 the vector units and
+// not HBM set the time. The layout serves them:
+//   * a lane is a channel and holds its states, so nothing is exchanged between lanes in the
+//     recurrence, and B and C, the same for all channels of a row's step, are scalars: they are read
+//     through the constant address space into SGPRs and cost no vector instruction;
+//   * a block is 64 channels of one row; its NW waves share the states (NS each) and add their parts
+//     of y through LDS. u, delta and z are read 16 B a thread, turned into (rate, rate u) once and
+//     laid into LDS as float pairs;
+//   * where rows and channels do not fill the chip, the time axis is split into chunks: one pass
+//     leaves each chunk's end state from zero and its summed rate (the decay over a chunk is
+//     exp(A sum rate)), a small kernel joins the chunks, and the scan proper starts each chunk from
+//     its state. The first pass costs another N exponentials, so chunks are used only then.
+// Backward runs the same tiles from the end: g[t] = C dy + a[t+1] g[t+1]. The states it needs are
+// rebuilt from checkpoints of every KC = 16 steps; dB and dC are sums over channels, folded over the
+// wave's lanes with v_permlane swaps and DPP, and over the channel blocks by a last kernel.
+#include "ms_sequence.h"
+
+namespace scan {
+using namespace seq;
+
+constexpr int KC = 16;     // steps between checkpoints, and a tile of the backward pass
+constexpr float LOG2E = 1.44269504f, LN2 = 0.69314718f;
+
+#define CONSTANT(T) const __attribute__((address_space(4))) T
+
+// How a call is cut. NW waves hold NS states each; `tiles` blocks of 64 channels a group.
+struct Plan {
+  int ns, nw;               // states per wave, waves per block
+  int64_t tiles, blocks_d;  // tiles per group, tiles * groups
+  int64_t chunks, chunk;    // over time; steps per chunk (a multiple of 32)
+  int64_t kc;               // checkpoints
+};
+
+struct Work {  // the workspace, in floats
+  float *bc, *local, *rates, *parts_bc, *parts_a, *parts_d, *sums;
+  int* cut;
+  int64_t floats;
+};
+
+// One launch's view: the caller's arrays and what the kernels share
+struct Args {
+  ms_scan_io io;
+  Plan p;
+  const float *Bf, *Cf;  // float32, padded to ns * nw states
+  int64_t b_t, b_r, b_g, c_t, c_r, c_g;
+  float *local, *rates, *parts_bc, *parts_a, *parts_d;
+  int* cut;
+  int vec;
+};
+
+__device__ __forceinline__ float rate_of(float x, int soft) { return soft ? softplus(x) : x; }
+
+// B and C (T, R, G, N) of any strides and type -> float32 [T][R][G][NP], zeros past N
+template <typename T>
+__global__ __launch_bounds__(256) void widen(const ms_scan_io io, int np, float* __restrict__ to) {
+  const int64_t per = io.steps * io.rows * io.groups * np;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= per) return;
+  const int n = (int)(i % np);
+  int64_t k = i / np;
+  const int64_t g = k % io.groups;
+  k /= io.groups;
+  const int64_t r = k % io.rows, t = k / io.rows;
+  const bool in = n < io.states;
+  to[i] = in ? (float)((const T*)io.B)[t * io.B_t + r * io.B_r + g * io.B_g + n] : 0.0f;
+  to[per + i] = in ? (float)((const T*)io.C)[t * io.C_t + r * io.C_r + g * io.C_g + n] : 0.0f;
+}
+
+// Which steps of a tile begin an episode, as a mask the whole wave shares
+__device__ __forceinline__ uint64_t start_mask(const ms_scan_io& io, int64_t r, int64_t t0, int64_t t1) {
+  if (!io.starts) return 0;
+  const int64_t t = t0 + (threadIdx.x & 63);
+  return __ballot(t < t1 && io.starts[t * io.starts_t + r * io.starts_r] != 0);
+}
+
+struct Place {  // a block's channels
+  int64_t r, chunk, g, c0;  // row, chunk, group, first channel
+  int64_t td;               // tile over all groups
+  int nc;                   // channels of the tile (<= 64)
+};
+__device__ __forceinline__ Place place(const Args& a) {
+  Place p;
+  int64_t b = blockIdx.x;
+  p.td = b % a.p.blocks_d;
+  b /= a.p.blocks_d;
+  p.r = b % a.io.rows;
+  p.chunk = b / a.io.rows;
+  const int64_t per = a.io.channels / a.io.groups;
+  p.g = p.td / a.p.tiles;
+  const int64_t in = (p.td % a.p.tiles) * 64;
+  p.c0 = p.g * per + in;
+  p.nc = (int)(per - in < 64 ? per - in : 64);
+  return p;
+}
+
+// ---------------------------------------------------------------- forward
+// LOCAL: the first pass of a split time axis (states from zero, no outputs).
+template <typename T, int NS, int NW, bool LOCAL>
+__global__ __launch_bounds__(64 * NW) void forward(const Args a) {
+  constexpr int TT = 8 * NW, E = 8;  // a tile: TT steps x 64 channels, 8 channels of one step a thread
+  __shared__ float2 sd[TT][64];
+  __shared__ float sy[LOCAL ? 1 : NW][LOCAL ? 1 : TT][64];
+  const ms_scan_io& io = a.io;
+  const Place at = place(a);
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lt = threadIdx.x >> 3, lc = (threadIdx.x & 7) * 8;  // this thread's step and channels in loads
+  const int n = at.nc - lc < 0 ? 0 : at.nc - lc;
+  const int64_t t_begin = at.chunk * a.p.chunk;
+  const int64_t t_end = t_begin + a.p.chunk < io.steps ? t_begin + a.p.chunk : io.steps;
+  const int64_t cl = at.c0 + lc;
+  const T* u = (const T*)io.u + at.r * io.u_r + cl;
+  const T* dl = (const T*)io.delta + at.r * io.delta_r + cl;
+  const T* z = io.z && !LOCAL ? (const T*)io.z + at.r * io.z_r + cl : nullptr;
+  T* out = (T*)io.out + at.r * io.out_r + cl;
+  float bias[E], skip[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    bias[e] = io.delta_bias && e < n ? io.delta_bias[cl + e] : 0.0f;
+    skip[e] = io.D && e < n ? io.D[cl + e] : 0.0f;
+  }
+  // this lane's channel in the recurrence
+  const int64_t ch = at.c0 + lane;
+  const bool live = lane < at.nc;
+  const int64_t N = io.states;
+  float A2[NS], h[NS], total = 0.0f;
+  bool was_cut = false;
+  const int64_t slot = (at.r * io.channels + ch) * N;  // (R, D, N)
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int64_t s = w * NS + i;
+    A2[i] = live && s < N ? io.A[ch * N + s] * LOG2E : 0.0f;
+    h[i] = 0.0f;
+    if (!LOCAL && live && s < N) {
+      if (a.p.chunks > 1) h[i] = a.local[at.chunk * io.rows * io.channels * N + slot + s];
+      else if (io.state) h[i] = io.state[slot + s];
+    }
+  }
+  CONSTANT(float)* Bs = (CONSTANT(float)*)(a.Bf + at.r * a.b_r + at.g * a.b_g + w * NS);
+  CONSTANT(float)* Cs = (CONSTANT(float)*)(a.Cf + at.r * a.c_r + at.g * a.c_g + w * NS);
+  typedef typename Vec<T, E>::type V;
+  V vu, vd, vz;
+  auto fetch = [&](int64_t t) __attribute__((always_inline)) {
+    const bool in = t + lt < t_end;
+    vu = load<T, E>(u + (t + lt) * io.u_t, in ? n : 0, a.vec);
+    vd = load<T, E>(dl + (t + lt) * io.delta_t, in ? n : 0, a.vec);
+    if (z) vz = load<T, E>(z + (t + lt) * io.z_t, in ? n : 0, a.vec);
+  };
+  fetch(t_begin);
+  for (int64_t t0 = t_begin; t0 < t_end; t0 += TT) {
+    const V cu = vu, cz = vz;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float rate = rate_of((float)vd[e] + bias[e], io.softplus);
+      sd[lt][lc + e] = make_float2(rate, rate * (float)cu[e]);
+    }
+    const int64_t t1 = t0 + TT < t_end ? t0 + TT : t_end;
+    const uint64_t starts = start_mask(io, at.r, t0, t1);
+    __syncthreads();
+    fetch(t0 + TT);
+    const int steps = (int)(t1 - t0);
+#pragma unroll 4
+    for (int t = 0; t < steps; ++t) {
+      if (!LOCAL && io.checkpoints && ((t0 + t) & (KC - 1)) == 0) {
+        // before step t0 + t: [k][row][tile][wave][NS / 4][64 lanes][4]
+        const int64_t k = (t0 + t) / KC;
+        float* to = io.checkpoints + (((k * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS * 64) + lane * 4;
+#pragma unroll
+        for (int i = 0; i < NS; i += 4) *(float4*)(to + i * 64) = make_float4(h[i], h[i + 1], h[i + 2], h[i + 3]);
+      }
+      const float2 v = sd[t][lane];
+      if (starts >> t & 1) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) h[i] = 0.0f;
+        if (LOCAL) was_cut = true;
+      }
+      CONSTANT(float)* B = Bs + (t0 + t) * a.b_t;
+      CONSTANT(float)* C = Cs + (t0 + t) * a.c_t;
+      float y = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const float decay = __builtin_amdgcn_exp2f(v.x * A2[i]);
+        h[i] = __builtin_fmaf(decay, h[i], v.y * B[i]);
+        if (!LOCAL) y = __builtin_fmaf(C[i], h[i], y);
+      }
+      if (LOCAL) total += v.x;
+      else sy[w][t][lane] = y;
+    }
+    __syncthreads();
+    if (!LOCAL && t0 + lt < t1 && n > 0) {
+      float y[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) s += sy[k][lt][lc + e];
+        y[e] = __builtin_fmaf(skip[e], (float)cu[e], s);
+        if (z) y[e] *= silu((float)cz[e]);
+      }
+      store<T, E>(out + (t0 + lt) * io.out_t, y, n, a.vec);
+    }
+  }
+  if (LOCAL) {
+    const int64_t of = at.chunk * io.rows * io.channels;
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        if (w * NS + i < N) a.local[of * N + slot + w * NS + i] = h[i];
+      if (w == 0) a.rates[of + at.r * io.channels + ch] = total;
+    }
+    if (threadIdx.x == 0 && at.td == 0) a.cut[at.chunk * io.rows + at.r] = was_cut;
+  } else if (io.new_state && live && t_end == io.steps) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+      if (w * NS + i < N) io.new_state[slot + w * NS + i] = h[i];
+  }
+}
+
+// The chunks of a split time axis in turn: what each left from zero becomes the state it starts from.
+// BACK: from the last chunk, with the gradients handed back in place of the states.
+template <bool BACK>
+__global__ __launch_bounds__(256) void join(const Args a) {
+  const ms_scan_io& io = a.io;
+  const int64_t N = io.states, all = io.rows * io.channels * N;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= all) return;
+  const int64_t rc = i / N, r = rc / io.channels, c = rc - r * io.channels;
+  const float A2 = io.A[c * N + (i - rc * N)] * LOG2E;
+  const float* first = BACK ? io.dnew_state : io.state;
+  float h = first ? first[i] : 0.0f;
+  for (int64_t k = 0; k < a.p.chunks; ++k) {
+    const int64_t q = BACK ? a.p.chunks - 1 - k : k;
+    const float mine = a.local[q * all + i];
+    const float decay = __builtin_amdgcn_exp2f(A2 * a.rates[q * io.rows * io.channels + rc]);
+    a.local[q * all + i] = h;
+    h = a.cut[q * io.rows + r] ? mine : __builtin_fmaf(decay, h, mine);
+  }
+}
+
+// ---------------------------------------------------------------- one step
+// The states are read and written once: HBM-bound. Q lanes of four states each share a channel.
+template <typename T, int Q>
+__global__ __launch_bounds__(256) void step4(const ms_scan_io io) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t D = io.channels, rc = i / Q;
+  if (rc >= io.rows * D) return;  // a channel's Q lanes leave together: Q divides the wave
+  const int q = (int)(i % Q) * 4;
+  const int64_t r = rc / D, c = rc - r * D, g = c / (D / io.groups);
+  const float u = (float)((const T*)io.u)[r * io.u_r + c];
+  const float d = (float)((const T*)io.delta)[r * io.delta_r + c] + (io.delta_bias ? io.delta_bias[c] : 0.0f);
+  const float rate = rate_of(d, io.softplus), ru = rate * u;
+  float4 h = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (io.state && !(io.starts && io.starts[r * io.starts_r])) h = *(const float4*)(io.state + rc * (Q * 4) + q);
+  const float4 A = *(const float4*)(io.A + c * (Q * 4) + q);
+  const T* B = (const T*)io.B + r * io.B_r + g * io.B_g + q;
+  const T* C = (const T*)io.C + r * io.C_r + g * io.C_g + q;
+  const float r2 = rate * LOG2E;
+  h.x = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.x), h.x, ru * (float)B[0]);
+  h.y = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.y), h.y, ru * (float)B[1]);
+  h.z = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.z), h.z, ru * (float)B[2]);
+  h.w = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.w), h.w, ru * (float)B[3]);
+  *(float4*)(io.new_state + rc * (Q * 4) + q) = h;
+  float y = (float)C[0] * h.x;
+  y = __builtin_fmaf((float)C[1], h.y, y);
+  y = __builtin_fmaf((float)C[2], h.z, y);
+  y = __builtin_fmaf((float)C[3], h.w, y);
+#pragma unroll
+  for (int m = 1; m < Q; m <<= 1) y += __shfl_xor(y, m);
+  if (q == 0) {
+    if (io.D) y = __builtin_fmaf(io.D[c], u, y);
+    if (io.z) y *= silu((float)((const T*)io.z)[r * io.z_r + c]);
+    ((T*)io.out)[r * io.out_r + c] = (T)y;
+  }
+}
+// any number of states: a thread per channel
+template <typename T>
+__global__ __launch_bounds__(256) void step1(const ms_scan_io io) {
+  const int64_t rc = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t D = io.channels, N = io.states;
+  if (rc >= io.rows * D) return;
+  const int64_t r = rc / D, c = rc - r * D, g = c / (D / io.groups);
+  const float u = (float)((const T*)io.u)[r * io.u_r + c];
+  const float d = (float)((const T*)io.delta)[r * io.delta_r + c] + (io.delta_bias ? io.delta_bias[c] : 0.0f);
+  const float rate = rate_of(d, io.softplus), ru = rate * u, r2 = rate * LOG2E;
+  const bool fresh = !io.state || (io.starts && io.starts[r * io.starts_r]);
+  const T* B = (const T*)io.B + r * io.B_r + g * io.B_g;
+  const T* C = (const T*)io.C + r * io.C_r + g * io.C_g;
+  float y = 0.0f;
+  for (int64_t n = 0; n < N; ++n) {
+    float h = fresh ? 0.0f : io.state[rc * N + n];
+    h = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * io.A[c * N + n]), h, ru * (float)B[n]);
+    io.new_state[rc * N + n] = h;
+    y = __builtin_fmaf((float)C[n], h, y);
+  }
+  if (io.D) y = __builtin_fmaf(io.D[c], u, y);
+  if (io.z) y *= silu((float)((const T*)io.z)[r * io.z_r + c]);
+  ((T*)io.out)[r * io.out_r + c] = (T)y;
+}
+
+// ---------------------------------------------------------------- backward
+// Eight values a lane (8 steps' worth of one folded register each) and eight items a step are summed
+// over the 64 lanes with the total left in one lane each: at every level two registers become one
+// that holds one half of the lanes for each, so 64 sums cost about two operations apiece.
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float fold32(float x0, float x1) {  // lanes 0-31: sum of x0, 32-63: of x1
+  const u32x2 s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x0), __float_as_uint(x1), false, false);
+  const unsigned lo = s.x, hi = s.y;
+  return __uint_as_float(lo) + __uint_as_float(hi);
+}
+__device__ __forceinline__ float fold16(float x0, float x1) {  // even rows of 16 lanes: x0, odd rows: x1
+  const u32x2 s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x0), __float_as_uint(x1), false, false);
+  const unsigned lo = s.x, hi = s.y;
+  return __uint_as_float(lo) + __uint_as_float(hi);
+}
+template <int CTRL>
+__device__ __forceinline__ float moved(float x) {
+  return __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ float fold_dpp(float x0, float x1, bool second) {
+  const float s0 = x0 + moved<CTRL>(x0), s1 = x1 + moved<CTRL>(x1);
+  return second ? s1 : s0;
+}
+constexpr int ROR8 = 0x128, HALF_MIRROR = 0x141, XOR2 = 0x4e, XOR1 = 0xb1;
+
+// items of one step -> a register whose lanes 8 i .. 8 i + 7 hold parts of item i
+__device__ __forceinline__ float fold_items(const float (&x)[8], bool bit3) {
+  float a[4], b[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = fold32(x[i], x[i + 4]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) b[i] = fold16(a[i], a[i + 2]);
+  return fold_dpp<ROR8>(b[0], b[1], bit3);
+}
+// eight steps' registers -> lane 8 i + t holds item i of step t
+__device__ __forceinline__ float fold_steps(const float (&x)[8], int lane) {
+  float a[4], b[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = fold_dpp<HALF_MIRROR>(x[i], x[i + 4], lane & 4);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) b[i] = fold_dpp<XOR2>(a[i], a[i + 2], lane & 2);
+  return fold_dpp<XOR1>(b[0], b[1], lane & 1);
+}
+
+// The first pass of a split time axis: what each chunk hands back from zero.
+template <typename T, int NS, int NW>
+__global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
+  constexpr int TT = 8 * NW, E = 8;
+  __shared__ float2 sd[TT][64];  // rate, dy
+  const ms_scan_io& io = a.io;
+  const Place at = place(a);
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lt = threadIdx.x >> 3, lc = (threadIdx.x & 7) * 8;
+  const int n = at.nc - lc < 0 ? 0 : at.nc - lc;
+  const int64_t t_begin = at.chunk * a.p.chunk;
+  const int64_t t_end = t_begin + a.p.chunk < io.steps ? t_begin + a.p.chunk : io.steps;
+  const int64_t cl = at.c0 + lc;
+  const T* dl = (const T*)io.delta + at.r * io.delta_r + cl;
+  const T* dy = (const T*)io.dout + at.r * io.dout_r + cl;
+  const T* z = io.z ? (const T*)io.z + at.r * io.z_r + cl : nullptr;
+  float bias[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) bias[e] = io.delta_bias && e < n ? io.delta_bias[cl + e] : 0.0f;
+  const int64_t ch = at.c0 + lane, N = io.states;
+  const bool live = lane < at.nc;
+  float A2[NS], carry[NS], total = 0.0f;
+  bool was_cut = false;
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    A2[i] = live && w * NS + i < N ? io.A[ch * N + w * NS + i] * LOG2E : 0.0f;
+    carry[i] = 0.0f;
+  }
+  CONSTANT(float)* Cs = (CONSTANT(float)*)(a.Cf + at.r * a.c_r + at.g * a.c_g + w * NS);
+  const int64_t tiles = (t_end - t_begin + TT - 1) / TT;
+  typedef typename Vec<T, E>::type V;
+  V vd, vy, vz;
+  auto fetch = [&](int64_t t) __attribute__((always_inline)) {
+    const bool in = t >= t_begin && t + lt < t_end;
+    vd = load<T, E>(dl + (t + lt) * io.delta_t, in ? n : 0, a.vec);
+    vy = load<T, E>(dy + (t + lt) * io.dout_t, in ? n : 0, a.vec);
+    if (z) vz = load<T, E>(z + (t + lt) * io.z_t, in ? n : 0, a.vec);
+  };
+  fetch(t_begin + (tiles - 1) * TT);
+  for (int64_t k = tiles - 1; k >= 0; --k) {
+    const int64_t t0 = t_begin + k * TT, t1 = t0 + TT < t_end ? t0 + TT : t_end;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      sd[lt][lc + e] = make_float2(rate_of((float)vd[e] + bias[e], io.softplus),
+                                   z ? (float)vy[e] * silu((float)vz[e]) : (float)vy[e]);
+    const uint64_t starts = start_mask(io, at.r, t0, t1);
+    __syncthreads();
+    fetch(t0 - TT);
+#pragma unroll 4
+    for (int t = (int)(t1 - t0) - 1; t >= 0; --t) {
+      const float2 v = sd[t][lane];
+      CONSTANT(float)* C = Cs + (t0 + t) * a.c_t;
+      total += v.x;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        carry[i] = __builtin_amdgcn_exp2f(v.x * A2[i]) * __builtin_fmaf(C[i], v.y, carry[i]);
+      if (starts >> t & 1) {
+        was_cut = true;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) carry[i] = 0.0f;
+      }
+    }
+    __syncthreads();
+  }
+  const int64_t of = at.chunk * io.rows * io.channels;
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+      if (w * NS + i < N) a.local[(of + at.r * io.channels + ch) * N + w * NS + i] = carry[i];
+    if (w == 0) a.rates[of + at.r * io.channels + ch] = total;
+  }
+  if (threadIdx.x == 0 && at.td == 0) a.cut[at.chunk * io.rows + at.r] = was_cut;
+}
+
+template <typename T, int NS, int NW>
+__global__ __launch_bounds__(64 * NW) void backward(const Args a) {
+  constexpr int E = KC / NW, TPR = 64 / E;  // 1,024 values of a tile over the threads: E channels each
+  __shared__ float s_rate[KC][64], s_ru[KC][64], s_dy[KC][64];
+  __shared__ float s_gb[NW][KC][64], s_ga[NW][KC][64], s_y[NW][KC][64];
+  const ms_scan_io& io = a.io;
+  const Place at = place(a);
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lt = threadIdx.x / TPR, lc = (threadIdx.x % TPR) * E;
+  const int n = at.nc - lc < 0 ? 0 : at.nc - lc;
+  const int64_t t_begin = at.chunk * a.p.chunk;
+  const int64_t t_end = t_begin + a.p.chunk < io.steps ? t_begin + a.p.chunk : io.steps;
+  const int64_t cl = at.c0 + lc;
+  const T* pu = (const T*)io.u + at.r * io.u_r + cl;
+  const T* pd = (const T*)io.delta + at.r * io.delta_r + cl;
+  const T* pz = io.z ? (const T*)io.z + at.r * io.z_r + cl : nullptr;
+  const T* po = (const T*)io.dout + at.r * io.dout_r + cl;
+  T* qu = (T*)io.du + at.r * io.du_r + cl;
+  T* qd = (T*)io.ddelta + at.r * io.ddelta_r + cl;
+  T* qz = io.z ? (T*)io.dz + at.r * io.dz_r + cl : nullptr;
+  float bias[E], skip[E], dskip[E], dbias[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    bias[e] = io.delta_bias && e < n ? io.delta_bias[cl + e] : 0.0f;
+    skip[e] = io.D && e < n ? io.D[cl + e] : 0.0f;
+    dskip[e] = dbias[e] = 0.0f;
+  }
+  const int64_t ch = at.c0 + lane, N = io.states;
+  const bool live = lane < at.nc;
+  const int64_t slot = (at.r * io.channels + ch) * N;
+  float A2[NS], carry[NS], dA[NS];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int64_t s = w * NS + i;
+    A2[i] = live && s < N ? io.A[ch * N + s] * LOG2E : 0.0f;
+    carry[i] = dA[i] = 0.0f;
+    if (live && s < N) {
+      if (a.p.chunks > 1) carry[i] = a.local[at.chunk * io.rows * io.channels * N + slot + s];
+      else if (io.dnew_state) carry[i] = io.dnew_state[slot + s];
+    }
+  }
+  CONSTANT(float)* Bs = (CONSTANT(float)*)(a.Bf + at.r * a.b_r + at.g * a.b_g + w * NS);
+  CONSTANT(float)* Cs = (CONSTANT(float)*)(a.Cf + at.r * a.c_r + at.g * a.c_g + w * NS);
+  const int64_t tiles = (t_end - t_begin + KC - 1) / KC;
+  typedef typename Vec<T, E>::type V;
+  V vu, vd, vz, vo;
+  auto fetch = [&](int64_t t) __attribute__((always_inline)) {
+    const bool in = t >= t_begin && t + lt < t_end;
+    vu = load<T, E>(pu + (t + lt) * io.u_t, in ? n : 0, a.vec);
+    vd = load<T, E>(pd + (t + lt) * io.delta_t, in ? n : 0, a.vec);
+    vo = load<T, E>(po + (t + lt) * io.dout_t, in ? n : 0, a.vec);
+    if (pz) vz = load<T, E>(pz + (t + lt) * io.z_t, in ? n : 0, a.vec);
+  };
+  fetch(t_begin + (tiles - 1) * KC);
+  for (int64_t k = tiles - 1; k >= 0; --k) {
+    const int64_t t0 = t_begin + k * KC, t1 = t0 + KC < t_end ? t0 + KC : t_end;
+    const V cu = vu, cz = vz, co = vo, cd = vd;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {  // a step past the end has rate 0 and dy 0: it changes nothing
+      const bool in = t0 + lt < t1;
+      const float rate = in ? rate_of((float)cd[e] + bias[e], io.softplus) : 0.0f;
+      s_rate[lt][lc + e] = rate;
+      s_ru[lt][lc + e] = rate * (float)cu[e];
+      s_dy[lt][lc + e] = pz ? (float)co[e] * silu((float)cz[e]) : (float)co[e];
+    }
+    const uint64_t starts = start_mask(io, at.r, t0, t1);
+    __syncthreads();
+    fetch(t0 - KC);
+    const int64_t kk = t0 / KC;
+    const float* from = io.checkpoints + (((kk * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS * 64) + lane * 4;
+    float* to = a.parts_bc + ((((kk * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS / 4) * 2) * 64 + lane;
+#pragma unroll
+    for (int nb = 0; nb < NS; nb += 4) {
+      const float4 h0 = *(const float4*)(from + nb * 64);
+      float h[4] = {h0.x, h0.y, h0.z, h0.w};
+      float dec[KC][4], ah[KC][4];  // a[t] and a[t] h[t - 1]
+#pragma unroll
+      for (int t = 0; t < KC; ++t) {
+        const float rate = s_rate[t][lane], ru = s_ru[t][lane];
+        const int64_t tt = t0 + t < t1 ? t0 + t : t1 - 1;
+        CONSTANT(float)* B = Bs + tt * a.b_t + nb;
+        if (starts >> t & 1) h[0] = h[1] = h[2] = h[3] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          dec[t][i] = __builtin_amdgcn_exp2f(rate * A2[nb + i]);
+          ah[t][i] = dec[t][i] * h[i];
+          h[i] = __builtin_fmaf(ru, B[i], ah[t][i]);
+        }
+      }
+      float steps8[8];
+#pragma unroll
+      for (int t = KC - 1; t >= 0; --t) {
+        const float rate = s_rate[t][lane], ru = s_ru[t][lane], dy = s_dy[t][lane];
+        const int64_t tt = t0 + t < t1 ? t0 + t : t1 - 1;
+        CONSTANT(float)* B = Bs + tt * a.b_t + nb;
+        CONSTANT(float)* C = Cs + tt * a.c_t + nb;
+        float gb = 0.0f, ga = 0.0f, y = 0.0f, items[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float g = __builtin_fmaf(C[i], dy, carry[nb + i]);
+          const float hh = __builtin_fmaf(ru, B[i], ah[t][i]);
+          const float q = g * ah[t][i];
+          y = __builtin_fmaf(C[i], hh, y);
+          gb = __builtin_fmaf(g, B[i], gb);
+          ga = __builtin_fmaf(q, A2[nb + i], ga);
+          dA[nb + i] = __builtin_fmaf(q, rate, dA[nb + i]);
+          carry[nb + i] = dec[t][i] * g;
+          items[i] = ru * g;
+          items[4 + i] = dy * hh;
+        }
+        if (starts >> t & 1) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) carry[nb + i] = 0.0f;
+        }
+        if (nb) {
+          gb += s_gb[w][t][lane];
+          ga += s_ga[w][t][lane];
+          y += s_y[w][t][lane];
+        }
+        s_gb[w][t][lane] = gb;
+        s_ga[w][t][lane] = ga;
+        s_y[w][t][lane] = y;
+        steps8[t & 7] = fold_items(items, lane & 8);
+        if ((t & 7) == 0) to[((nb >> 2) * 2 + (t >> 3)) * 64] = fold_steps(steps8, lane);
+      }
+    }
+    __syncthreads();
+    if (t0 + lt < t1 && n > 0) {
+      float du[E], dd[E], dz[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float gb = 0.0f, ga = 0.0f, y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+          gb += s_gb[i][lt][lc + e];
+          ga += s_ga[i][lt][lc + e];
+          y += s_y[i][lt][lc + e];
+        }
+        const float uu = (float)cu[e], rate = s_rate[lt][lc + e], dy = s_dy[lt][lc + e];
+        if (pz) dz[e] = (float)co[e] * __builtin_fmaf(skip[e], uu, y) * silu_slope((float)cz[e]);
+        du[e] = __builtin_fmaf(skip[e], dy, rate * gb);
+        const float raw = (float)cd[e] + bias[e];
+        dd[e] = __builtin_fmaf(gb, uu, ga * LN2) * (io.softplus ? sigmoid(raw) : 1.0f);
+        dskip[e] = __builtin_fmaf(dy, uu, dskip[e]);
+        dbias[e] += dd[e];
+      }
+      store<T, E>(qu + (t0 + lt) * io.du_t, du, n, a.vec);
+      store<T, E>(qd + (t0 + lt) * io.ddelta_t, dd, n, a.vec);
+      if (pz) store<T, E>(qz + (t0 + lt) * io.dz_t, dz, n, a.vec);
+    }
+    __syncthreads();  // the next tile's stores to s_rate .. s_dy
+  }
+  const int64_t part = at.chunk * io.rows + at.r;
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+      if (w * NS + i < N) {
+        a.parts_a[(part * io.channels + ch) * N + w * NS + i] = dA[i];
+        if (io.dstate && t_begin == 0) io.dstate[slot + w * NS + i] = carry[i];
+      }
+  }
+  // dD and ddelta_bias: the threads of the same channels add up through LDS
+  float* red = &s_gb[0][0][0];
+  for (int pass = 0; pass < 2; ++pass) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) red[lt * 64 + lc + e] = pass ? dbias[e] : dskip[e];
+    __syncthreads();
+    if (threadIdx.x < 64 && live) {
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < KC; ++i) s += red[i * 64 + lane];
+      a.parts_d[(part * 2 + pass) * io.channels + ch] = s;
+    }
+  }
+}
+
+// dB, dC: the tiles of a group added and put in place. A thread per (t, r, g, n) and kind.
+template <typename T>
+__global__ __launch_bounds__(256) void finish_bc(const Args a) {
+  const ms_scan_io& io = a.io;
+  const int64_t per = io.steps * io.rows * io.groups * io.states;
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= 2 * per) return;
+  const int kind = i >= per;
+  if (kind) i -= per;
+  const int64_t s = i % io.states;
+  int64_t k = i / io.states;
+  const int64_t g = k % io.groups;
+  k /= io.groups;
+  const int64_t r = k % io.rows, t = k / io.rows;
+  const int64_t ns = a.p.ns, w = s / ns, nb = s % ns / 4;
+  const int64_t lane = (kind * 4 + s % 4) * 8 + t % 8;
+  const int64_t one = a.p.nw * (ns / 4) * 2 * 64;  // a tile's floats
+  const float* p = a.parts_bc + ((t / KC * io.rows + r) * a.p.blocks_d + g * a.p.tiles) * one +
+                   ((w * (ns / 4) + nb) * 2 + t % KC / 8) * 64 + lane;
+  float sum = 0.0f;
+  for (int64_t j = 0; j < a.p.tiles; ++j) sum += p[j * one];
+  ((T*)(kind ? io.dC : io.dB))[i] = (T)sum;
+}
+
+// ---------------------------------------------------------------- the host's side
+
+Plan plan(const ms_scan_io& io, bool back) {
+  Plan p = {};
+  p.ns = io.states <= 16 ? 4 : io.states <= 32 ? 8 : 16;
+  p.nw = io.states <= 4 ? 1 : io.states <= 8 ? 2 : 4;
+  p.tiles = (io.channels / io.groups + 63) / 64;
+  p.blocks_d = p.tiles * io.groups;
+  p.chunks = 1;
+  p.chunk = (io.steps + 31) / 32 * 32;
+  (void)back;
+  p.kc = (io.steps + KC - 1) / KC;
+  return p;
+}
+
+int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
+
+// whether B and C can be read where they are: float32, no padding, dwords
+bool direct(const ms_scan_io& io, const Plan& p) { return io.dtype == 0 && io.states == p.ns * p.nw; }
+
+Work work(const ms_scan_io& io, const Plan& p, bool back) {
+  Work w = {};
+  float* at = (float*)io.workspace;
+  int64_t used = 0;
+  auto take = [&](int64_t n) {
+    float* q = at + used;
+    used += round4(n);
+    return q;
+  };
+  const int64_t rd = io.rows * io.channels, parts = p.chunks * io.rows;
+  if (!direct(io, p)) w.bc = take(2 * io.steps * io.rows * io.groups * p.ns * p.nw);
+  if (p.chunks > 1) {
+    w.local = take(p.chunks * rd * io.states);
+    w.rates = take(p.chunks * rd);
+    w.cut = (int*)take(parts);
+  }
+  if (back) {
+    w.parts_bc = take(p.kc * io.rows * p.blocks_d * p.nw * (p.ns / 4) * 2 * 64);
+    w.parts_a = take(parts * io.channels * io.states);
+    w.parts_d = take(parts * 2 * io.channels);
+    w.sums = take(2 * io.channels);
+  }
+  w.floats = used;
+  return w;
+}
+
+const char* check(const ms_scan_io* io, bool back, bool step) {
+  if (!io) return "no arguments";
+  if (io->dtype < 0 || io->dtype > 2) return "dtype must be 0 (float32), 1 (bfloat16) or 2 (float16)";
+  if (io->steps < 0 || io->rows < 0 || io->channels <= 0) return "steps and rows must be >= 0, channels > 0";
+  if (io->states < 1 || io->states > 64) return "1 to 64 states are supported";
+  if (io->groups < 1 || io->channels % io->groups) return "groups must divide the channels";
+  if (step && io->steps != 1) return "a step has steps = 1";
+  if (!io->A) return "A is NULL";
+  const bool some = io->steps > 0 && io->rows > 0;
+  if (some && (!io->u || !io->delta || !io->B || !io->C)) return "u, delta, B or C is NULL";
+  if (some && !back && !io->out) return "out is NULL";
+  if (step && io->rows > 0 && !io->new_state) return "a step needs new_state";
+  if (back) {
+    if (!io->dA) return "dA is NULL";
+    if (some && (!io->dout || !io->du || !io->ddelta || !io->dB || !io->dC || !io->checkpoints || (io->z && !io->dz)))
+      return "dout, du, ddelta, dz, dB, dC or checkpoints is NULL";
+  }
+  return nullptr;
+}
+
+bool vec_ok(const ms_scan_io& io, bool back) {
+  const int64_t elem = io.dtype == 0 ? 4 : 2, E = 8;
+  if (io.groups > 1 && (io.channels / io.groups) % 8) return false;
+  bool ok = aligned(io.u, io.u_t, io.u_r, elem, E) && aligned(io.delta, io.delta_t, io.delta_r, elem, E) &&
+            (!io.z || aligned(io.z, io.z_t, io.z_r, elem, E));
+  if (!back) return ok && aligned(io.out, io.out_t, io.out_r, elem, E);
+  return ok && aligned(io.dout, io.dout_t, io.dout_r, elem, E) && aligned(io.du, io.du_t, io.du_r, elem, E) &&
+         aligned(io.ddelta, io.ddelta_t, io.ddelta_r, elem, E) && (!io.z || aligned(io.dz, io.dz_t, io.dz_r, elem, E));
+}
+
+// out of 32-bit grids: refused
+bool too_many(int64_t blocks) { return blocks > 0x7fffffff; }
+
+int prepare(const ms_scan_io& io, const Plan& p, const Work& w, bool back, hipStream_t stream, const char* who, Args& a) {
+  a.io = io;
+  a.p = p;
+  a.local = w.local;
+  a.rates = w.rates;
+  a.cut = w.cut;
+  a.parts_bc = w.parts_bc;
+  a.parts_a = w.parts_a;
+  a.parts_d = w.parts_d;
+  a.vec = vec_ok(io, back);
+  if (w.bc) {
+    const int np = p.ns * p.nw;
+    const int64_t per = io.steps * io.rows * io.groups * np, blocks = (per + 255) / 256;
+    if (too_many(blocks)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
+    a.Bf = w.bc;
+    a.Cf = w.bc + per;
+    a.b_t = a.c_t = io.rows * io.groups * np;
+    a.b_r = a.c_r = io.groups * np;
+    a.b_g = a.c_g = np;
+    const dim3 grid((unsigned)blocks), block(256);
+    if (io.dtype == 0) hipLaunchKernelGGL(widen<float>, grid, block, 0, stream, io, np, w.bc);
+    else if (io.dtype == 1) hipLaunchKernelGGL(widen<bf16>, grid, block, 0, stream, io, np, w.bc);
+    else hipLaunchKernelGGL(widen<f16>, grid, block, 0, stream, io, np, w.bc);
+    return launched(who);
+  }
+  a.Bf = (const float*)io.B;
+  a.Cf = (const float*)io.C;
+  a.b_t = io.B_t; a.b_r = io.B_r; a.b_g = io.B_g;
+  a.c_t = io.C_t; a.c_r = io.C_r; a.c_g = io.C_g;
+  return MS_OK;
+}
+
+enum Pass { LOCAL, MAIN, BACK_LOCAL, BACK };
+
+template <typename T, int NS, int NW>
+void launch_as(Pass pass, const Args& a, dim3 grid, hipStream_t stream) {
+  const dim3 block(64 * NW);
+  if (pass == LOCAL) hipLaunchKernelGGL((forward<T, NS, NW, true>), grid, block, 0, stream, a);
+  else if (pass == MAIN) hipLaunchKernelGGL((forward<T, NS, NW, false>), grid, block, 0, stream, a);
+  else if (pass == BACK_LOCAL) hipLaunchKernelGGL((backward_local<T, NS, NW>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((backward<T, NS, NW>), grid, block, 0, stream, a);
+}
+template <typename T>
+void launch_type(Pass pass, const Args& a, dim3 grid, hipStream_t stream) {
+  if (a.p.nw == 1) launch_as<T, 4, 1>(pass, a, grid, stream);
+  else if (a.p.nw == 2) launch_as<T, 4, 2>(pass, a, grid, stream);
+  else if (a.p.ns == 4) launch_as<T, 4, 4>(pass, a, grid, stream);
+  else if (a.p.ns == 8) launch_as<T, 8, 4>(pass, a, grid, stream);
+  else launch_as<T, 16, 4>(pass, a, grid, stream);
+}
+int launch(Pass pass, const Args& a, hipStream_t stream, const char* who) {
+  const int64_t blocks = a.p.blocks_d * a.io.rows * a.p.chunks;
+  if (too_many(blocks)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
+  const dim3 grid((unsigned)blocks);
+  if (a.io.dtype == 0) launch_type<float>(pass, a, grid, stream);
+  else if (a.io.dtype == 1) launch_type<bf16>(pass, a, grid, stream);
+  else launch_type<f16>(pass, a, grid, stream);
+  return launched(who);
+}
+template <bool BACK>
+int launch_join(const Args& a, hipStream_t stream, const char* who) {
+  const int64_t blocks = (a.io.rows * a.io.channels * a.io.states + 255) / 256;
+  if (too_many(blocks)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
+  hipLaunchKernelGGL(join<BACK>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  return launched(who);
+}
+
+__global__ __launch_bounds__(256) void copy_state(const float* __restrict__ from, int64_t n, float* __restrict__ to) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) to[i] = from ? from[i] : 0.0f;
+}
+int copied(const float* from, int64_t n, float* to, hipStream_t stream, const char* who) {
+  if (!to || n == 0 || to == from) return MS_OK;
+  if (too_many((n + 255) / 256)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
+  hipLaunchKernelGGL(copy_state, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, from, n, to);
+  return launched(who);
+}
+
+template <typename T>
+void launch_step(const ms_scan_io& io, hipStream_t stream) {
+  const int64_t rc = io.rows * io.channels;
+  const int q = io.states / 4;
+  const bool four = io.states % 4 == 0 && (q & (q - 1)) == 0 && ((uintptr_t)io.A & 15u) == 0 &&
+                    ((uintptr_t)io.new_state & 15u) == 0 && (!io.state || ((uintptr_t)io.state & 15u) == 0);
+  const dim3 grid((unsigned)((rc * (four ? q : 1) + 255) / 256)), block(256);
+  if (!four) hipLaunchKernelGGL(step1<T>, grid, block, 0, stream, io);
+  else if (q == 1) hipLaunchKernelGGL((step4<T, 1>), grid, block, 0, stream, io);
+  else if (q == 2) hipLaunchKernelGGL((step4<T, 2>), grid, block, 0, stream, io);
+  else if (q == 4) hipLaunchKernelGGL((step4<T, 4>), grid, block, 0, stream, io);
+  else if (q == 8) hipLaunchKernelGGL((step4<T, 8>), grid, block, 0, stream, io);
+  else hipLaunchKernelGGL((step4<T, 16>), grid, block, 0, stream, io);
+}
+
+bool space(const ms_scan_io& io, int64_t bytes) {
+  return bytes == 0 || (io.workspace && ((uintptr_t)io.workspace & 15u) == 0 && io.workspace_bytes >= bytes);
+}
+
+}  // namespace scan
+
+extern "C" {
+
+int64_t ms_scan_checkpoints(const ms_scan_io* io) {
+  if (scan::check(io, false, false) && (!io || io->states < 1 || io->states > 64 || io->groups < 1 || io->channels <= 0)) return 0;
+  const scan::Plan p = scan::plan(*io, false);
+  return p.kc * io->rows * p.blocks_d * p.nw * p.ns * 64 * (int64_t)sizeof(float);
+}
+
+int64_t ms_scan_workspace(const ms_scan_io* io, int backward) {
+  if (!io || io->states < 1 || io->states > 64 || io->groups < 1 || io->channels <= 0 || io->steps < 0 || io->rows < 0) return 0;
+  ms_scan_io none = *io;
+  none.workspace = nullptr;
+  return scan::work(none, scan::plan(*io, backward != 0), backward != 0).floats * (int64_t)sizeof(float);
+}
+
+int ms_scan_forward(const ms_scan_io* io, void* stream) {
+  const char* who = "ms_scan_forward";
+  if (const char* why = scan::check(io, false, false)) return seq::fail(MS_ERR_INVALID_ARGUMENT, who, why);
+  const hipStream_t st = (hipStream_t)stream;
+  if (io->rows == 0) return MS_OK;
+  if (io->steps == 0) return scan::copied(io->state, io->rows * io->channels * io->states, io->new_state, st, who);
+  const scan::Plan p = scan::plan(*io, false);
+  const scan::Work w = scan::work(*io, p, false);
+  if (!scan::space(*io, w.floats * 4))
+    return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "the workspace is missing, misaligned or too small");
+  if (io->checkpoints && ((uintptr_t)io->checkpoints & 15u))
+    return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "checkpoints must be 16-B aligned");
+  scan::Args a = {};
+  if (int rc = scan::prepare(*io, p, w, false, st, who, a)) return rc;
+  if (p.chunks > 1) {
+    if (int rc = scan::launch(scan::LOCAL, a, st, who)) return rc;
+    if (int rc = scan::launch_join<false>(a, st, who)) return rc;
+  }
+  return scan::launch(scan::MAIN, a, st, who);
+}
+
+int ms_scan_step(const ms_scan_io* io, void* stream) {
+  if (const char* why = scan::check(io, false, true)) return seq::fail(MS_ERR_INVALID_ARGUMENT, "ms_scan_step", why);
+  if (io->rows == 0) return MS_OK;
+  if (scan::too_many((io->rows * io->channels * 16 + 255) / 256))
+    return seq::fail(MS_ERR_INVALID_ARGUMENT, "ms_scan_step", "too large");
+  if (io->dtype == 0) scan::launch_step<float>(*io, (hipStream_t)stream);
+  else if (io->dtype == 1) scan::launch_step<seq::bf16>(*io, (hipStream_t)stream);
+  else scan::launch_step<seq::f16>(*io, (hipStream_t)stream);
+  return seq::launched("ms_scan_step");
+}
+
+int ms_scan_backward(const ms_scan_io* io, void* stream) {
+  const char* who = "ms_scan_backward";
+  if (const char* why = scan::check(io, true, false)) return seq::fail(MS_ERR_INVALID_ARGUMENT, who, why);
+  const hipStream_t st = (hipStream_t)stream;
+  const int64_t dn = io->channels * io->states;
+  if (io->rows == 0 || io->steps == 0) {
+    if (int rc = scan::copied(nullptr, dn, io->dA, st, who)) return rc;
+    if (int rc = scan::copied(nullptr, io->channels, io->dD, st, who)) return rc;
+    if (int rc = scan::copied(nullptr, io->channels, io->ddelta_bias, st, who)) return rc;
+    return scan::copied(io->dnew_state, io->rows * dn, io->dstate, st, who);
+  }
+  const scan::Plan p = scan::plan(*io, true);
+  const scan::Work w = scan::work(*io, p, true);
+  if (!scan::space(*io, w.floats * 4) || ((uintptr_t)io->checkpoints & 15u))
+    return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "the workspace or the checkpoints are missing, misaligned or too small");
+  scan::Args a = {};
+  if (int rc = scan::prepare(*io, p, w, true, st, who, a)) return rc;
+  if (p.chunks > 1) {
+    if (int rc = scan::launch(scan::BACK_LOCAL, a, st, who)) return rc;
+    if (int rc = scan::launch_join<true>(a, st, who)) return rc;
+  }
+  if (int rc = scan::launch(scan::BACK, a, st, who)) return rc;
+  const int64_t all = 2 * io->steps * io->rows * io->groups * io->states, blocks = (all + 255) / 256;
+  if (scan::too_many(blocks)) return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
+  if (io->dtype == 0) hipLaunchKernelGGL(scan::finish_bc<float>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  else if (io->dtype == 1) hipLaunchKernelGGL(scan::finish_bc<seq::bf16>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(scan::finish_bc<seq::f16>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  const int64_t parts = p.chunks * io->rows;
+  hipLaunchKernelGGL((seq::sum_parts<8>), dim3((unsigned)((dn + 63) / 64)), dim3(512), 0, st, w.parts_a, parts, dn, io->dA);
+  if (io->dD || io->ddelta_bias) {
+    hipLaunchKernelGGL((seq::sum_parts<8>), dim3((unsigned)((2 * io->channels + 63) / 64)), dim3(512), 0, st, w.parts_d,
+                       parts, 2 * io->channels, w.sums);
+    if (int rc = scan::copied(w.sums, io->dD ? io->channels : 0, io->dD, st, who)) return rc;
+    if (int rc = scan::copied(w.sums + io->channels, io->ddelta_bias ? io->channels : 0, io->ddelta_bias, st, who)) return rc;
+  }
+  return seq::launched(who);
+}
+
+}  // extern "C"

@@ -1,0 +1,116 @@
+// ms_sequence.h — what the sequence kernels (ms_conv.hip, ms_scan.hip) share: element types, vector
+// loads with guarded ends, the activations, and the error text of their entry points.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "../../include/marl_soccer.h"
+
+extern thread_local char g_sequence_error[256];  // ms_conv.hip
+
+namespace seq {
+
+// Element types of the [io] arrays: the value is float32 in registers, rounded to nearest even
+// (v_cvt_pk_bf16_f32, v_cvt_f16_f32) when it is stored.
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+template <typename T, int E>
+struct Vec {
+  // 16 B at most are assumed aligned: wider vectors are moved as several 16-B accesses
+  typedef T type __attribute__((ext_vector_type(E), aligned(sizeof(T) * E < 16 ? sizeof(T) * E : 16)));
+};
+
+// E channels from p, of which the first n (<= E) exist; `vec`: p is aligned for Vec<T, E>
+template <typename T, int E>
+__device__ __forceinline__ typename Vec<T, E>::type load(const T* p, int n, bool vec) {
+  typename Vec<T, E>::type v;
+  if (vec && n >= E) {
+    v = *(const typename Vec<T, E>::type*)p;
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = i < n ? p[i] : (T)0.0f;
+  }
+  return v;
+}
+template <typename T, int E>
+__device__ __forceinline__ void store(T* p, const float (&x)[E], int n, bool vec) {
+  if (vec && n >= E) {
+    typename Vec<T, E>::type v;
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = (T)x[i];
+    *(typename Vec<T, E>::type*)p = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < n) p[i] = (T)x[i];
+  }
+}
+
+// exp(x) with the rounding of x log2(e) carried along: v_exp_f32 alone loses |x| 2^-24 of the value
+__device__ __forceinline__ float exp_f(float x) {
+  const float hi = x * 1.44269504f;
+  const float lo = __builtin_fmaf(x, 1.44269504f, -hi) + x * 1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(hi);
+  // beyond the range of float hi is infinite and lo is not a number: the power alone is the answer
+  return __builtin_fabsf(hi) < 150.0f ? __builtin_fmaf(e * 0.69314718f, lo, e) : e;
+}
+__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_f(-x)); }
+__device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
+__device__ __forceinline__ float silu_slope(float x) {
+  const float s = sigmoid(x);
+  return s * (1.0f + x * (1.0f - s));
+}
+// log(1 + exp(x)); a NaN stays one
+__device__ __forceinline__ float softplus(float x) {
+  return (x > 0.0f ? x : (x < 0.0f ? 0.0f : x)) + log1pf(exp_f(-__builtin_fabsf(x)));
+}
+
+inline bool aligned(const void* p, int64_t a, int64_t b, int64_t elem, int64_t vec) {
+  // every row of an array with element strides a and b starts on a multiple of `vec` elements, 16 B at most
+  const int64_t bytes = vec * elem < 16 ? vec * elem : 16;
+  const int64_t unit = bytes / elem;
+  return ((uintptr_t)p % (uint64_t)bytes) == 0 && a % unit == 0 && b % unit == 0;
+}
+
+inline int fail(int code, const char* who, const char* why) {
+  snprintf(g_sequence_error, sizeof(g_sequence_error), "%s: %s", who, why);
+  return code;
+}
+inline int launched(const char* who) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? MS_OK : fail(MS_ERR_HIP, who, hipGetErrorString(e));
+}
+
+// Row sums of partial results: out[c] = sum over i < parts of in[i * columns + c], in a fixed order.
+// A block owns 64 columns and its waves share the parts; the sum is held in float64, so the number
+// of parts does not cost precision.
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void sum_parts(const float* __restrict__ in, int64_t parts, int64_t columns,
+                                                        float* __restrict__ out) {
+  __shared__ double s[WAVES][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
+  if (c < columns) {
+    int64_t i = w;
+    for (; i + 3 * WAVES < parts; i += 4 * WAVES) {
+      a0 += in[i * columns + c];
+      a1 += in[(i + WAVES) * columns + c];
+      a2 += in[(i + 2 * WAVES) * columns + c];
+      a3 += in[(i + 3 * WAVES) * columns + c];
+    }
+    for (; i < parts; i += WAVES) a0 += in[i * columns + c];
+  }
+  s[w][lane] = (a0 + a1) + (a2 + a3);
+  __syncthreads();
+  if (w == 0 && c < columns) {
+    double a = 0.0;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) a += s[k][lane];
+    out[c] = (float)a;
+  }
+}
+
+}  // namespace seq

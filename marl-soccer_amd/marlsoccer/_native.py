@@ -54,6 +54,46 @@ class MsPolicyIO(C.Structure):
                 ("obs_copy", C.c_void_p), ("env_actions", C.c_void_p), ("red_uniform", C.c_void_p)]
 
 
+class MsConvIO(C.Structure):
+    """ms_conv_io (include/marl_soccer.h): one short convolution, forward or backward."""
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "width", "silu", "pad0")]
+                + [(n, C.c_int64) for n in ("steps", "rows", "channels")]
+                + [("x", C.c_void_p), ("x_t", C.c_int64), ("x_r", C.c_int64), ("weight", C.c_void_p), ("bias", C.c_void_p),
+                   ("state", C.c_void_p), ("starts", C.c_void_p), ("starts_t", C.c_int64), ("starts_r", C.c_int64),
+                   ("out", C.c_void_p), ("out_t", C.c_int64), ("out_r", C.c_int64), ("new_state", C.c_void_p),
+                   ("dout", C.c_void_p), ("dout_t", C.c_int64), ("dout_r", C.c_int64), ("dnew_state", C.c_void_p),
+                   ("dx", C.c_void_p), ("dx_t", C.c_int64), ("dx_r", C.c_int64), ("dstate", C.c_void_p),
+                   ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("workspace", C.c_void_p),
+                   ("workspace_bytes", C.c_int64)])
+
+
+def _strided(*names):
+    return [(n + s, C.c_void_p if not s else C.c_int64) for n in names for s in ("", "_t", "_r")]
+
+
+def _grouped(*names):
+    return [(n + s, C.c_void_p if not s else C.c_int64) for n in names for s in ("", "_t", "_r", "_g")]
+
+
+class MsScanIO(C.Structure):
+    """ms_scan_io (include/marl_soccer.h): one state-space scan, forward, backward or a single step."""
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "softplus", "states", "groups")]
+                + [(n, C.c_int64) for n in ("steps", "rows", "channels")]
+                + _strided("u", "delta", "z") + _grouped("B", "C")
+                + [(n, C.c_void_p) for n in ("A", "D", "delta_bias", "state")]
+                + _strided("starts", "out") + [("new_state", C.c_void_p), ("checkpoints", C.c_void_p)]
+                + _strided("dout") + [("dnew_state", C.c_void_p)] + _strided("du", "ddelta", "dz")
+                + [(n, C.c_void_p) for n in ("dB", "dC", "dA", "dD", "ddelta_bias", "dstate", "workspace")]
+                + [("workspace_bytes", C.c_int64)])
+
+
+class MsOptimTensor(C.Structure):
+    """ms_optim_tensor (include/marl_soccer.h): one parameter of an optimiser step."""
+    _fields_ = ([(n, C.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale",
+                                           "step")]
+                + [("numel", C.c_int64), ("dtype", C.c_int32), ("pad0", C.c_int32)])
+
+
 # numpy view of ms_env_state (include/marl_soccer.h), for export/import
 BODY_DTYPE = np.dtype([(n, "<f4") for n in ("px", "py", "vx", "vy", "angle", "w", "vbx", "vby", "wb")])
 ARB_DTYPE = np.dtype([("pair", "u1"), ("count", "u1"), ("idle", "u1"), ("pad0", "u1"),
@@ -74,6 +114,9 @@ EXPORTED = (
     "ms_config_specialised", "ms_step_ring", "ms_reset_ring", "ms_step_n",
     "ms_set_lane_group", "ms_get_lane_group", "ms_set_group_solve", "ms_get_group_solve", "ms_step_kernel_name",
     "ms_policy_forward", "ms_policy_last_error", "ms_policy_run", "ms_rollout_record",
+    "ms_conv_forward", "ms_conv_workspace", "ms_conv_backward", "ms_scan_forward", "ms_scan_step", "ms_scan_checkpoints",
+    "ms_scan_workspace", "ms_scan_backward", "ms_sequence_last_error", "ms_grad_clip", "ms_adamw_step",
+    "ms_optim_last_error",
 )
 
 _lib = None
@@ -149,6 +192,23 @@ def lib():
         L.ms_policy_run.restype = C.c_int
         L.ms_rollout_record.argtypes = [I64, P, P, P, P, P, P, P, P, P, P]
         L.ms_rollout_record.restype = C.c_int
+    if hasattr(L, "ms_scan_forward"):  # likewise
+        for fn, io in (("ms_conv_forward", MsConvIO), ("ms_conv_backward", MsConvIO), ("ms_scan_forward", MsScanIO),
+                       ("ms_scan_step", MsScanIO), ("ms_scan_backward", MsScanIO)):
+            getattr(L, fn).argtypes = [C.POINTER(io), P]
+            getattr(L, fn).restype = C.c_int
+        L.ms_conv_workspace.argtypes = [C.POINTER(MsConvIO)]
+        L.ms_scan_checkpoints.argtypes = [C.POINTER(MsScanIO)]
+        L.ms_scan_workspace.argtypes = [C.POINTER(MsScanIO), C.c_int]
+        for fn in ("ms_conv_workspace", "ms_scan_checkpoints", "ms_scan_workspace"):
+            getattr(L, fn).restype = I64
+        L.ms_sequence_last_error.restype = C.c_char_p
+        L.ms_grad_clip.argtypes = [P, I64, C.c_double, P, P, P]
+        L.ms_grad_clip.restype = C.c_int
+        L.ms_adamw_step.argtypes = [P, I64, C.c_int, C.c_double, P, C.c_double, C.c_double, C.c_double, C.c_double,
+                                    C.c_int, P, P]
+        L.ms_adamw_step.restype = C.c_int
+        L.ms_optim_last_error.restype = C.c_char_p
     for fn in ("ms_create", "ms_destroy", "ms_set_stream", "ms_seed_pcg64", "ms_seed_pcg64_range", "ms_reset",
                "ms_step", "ms_observe", "ms_export_state", "ms_import_state", "ms_debug_rewards",
                "ms_get_stats", "ms_reset_stats"):

@@ -1,0 +1,242 @@
+"""AdamW over many tensors in one launch (csrc/ms_optim.hip), for the PPO update of a policy.
+
+The reference's update (marl-soccer.ipynb train cell) is clip_grad_norm_ and Adam over the Agent's 21
+tensors, small ones: a launch an operation and tensor. Here the norm is one launch and the step
+another, for any list; parameters change in place, so a captured rollout graph (DeviceRollout) goes on
+reading them, and step counts, clip factor and, if wanted, the learning rate stay on the device, so
+the step itself may be captured.
+
+    opt = AdamW(agent.parameters(), lr=2.5e-4, eps=1e-5, weight_decay=0.0, max_grad_norm=0.5)
+    loss.backward(); opt.step(); opt.zero_grad()
+
+state_bits=8 holds both moments as OCP e4m3 bytes with a float32 scale for every 256 values: 2 B a
+value instead of 8. The second moment is held as its root. Rounding is to nearest: against moments in
+32 bits a value is off by up to 2^-4 of itself down to 2^-15 of its block's largest (by 2^-19 of the
+largest below that), and a change of less than half a step waits until it is more, so use it where
+memory counts.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _native as N
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+WORKSPACE = 4096   # MS_OPTIM_WORKSPACE, floats
+BLOCK = 256        # MS_ADAMW_BLOCK: values that share a scale
+F8 = torch.float8_e4m3fn
+
+
+def scales_for(numel: int) -> int:
+    """How many scales an 8-bit moment of numel values has."""
+    return -(-numel // BLOCK)
+
+
+def moment_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The float32 values that an 8-bit moment holds (for exp_avg_sq: their squares are the second
+    moment)."""
+    flat = codes.reshape(-1).to(torch.float32)
+    return (flat * scales.repeat_interleave(BLOCK)[: flat.numel()]).view(codes.shape)
+
+
+def _raise(rc: int) -> None:
+    raise (ValueError if rc == N.MS_ERR_INVALID_ARGUMENT else N.NativeError)(
+        N.lib().ms_optim_last_error().decode(errors="replace"))
+
+
+def _bad(name, want):
+    raise ValueError(f"adamw_step: {name} must be {want}")
+
+
+def _entries(params, grads, exp_avg, exp_avg_sq, steps, scales, sq_scales):
+    """The checked list as ms_optim_tensor rows."""
+    bits8 = scales is not None
+    n, device = len(params), None
+    for name, ts in (("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq), ("steps", steps),
+                     ("exp_avg_scales", scales), ("exp_avg_sq_scales", sq_scales)):
+        if ts is not None and len(ts) != n:
+            _bad(name, f"a list of {n} tensors, one for every parameter")
+    rows = (N.MsOptimTensor * n)()
+    moment = F8 if bits8 else torch.float32
+    for i, p in enumerate(params):
+        g, m, v, s = grads[i], exp_avg[i], exp_avg_sq[i], steps[i]
+        if device is None:
+            device = p.device
+        dt = _DTYPES.get(p.dtype)
+        if dt is None:
+            _bad("a parameter", f"float32, bfloat16 or float16, got {p.dtype}")
+        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+            _bad("every tensor", "contiguous")
+        if g.dtype != p.dtype or g.shape != p.shape:
+            _bad("a gradient", "of its parameter's type and shape")
+        if m.dtype != moment or v.dtype != moment or m.shape != p.shape or v.shape != p.shape:
+            _bad("a moment", f"{moment} of its parameter's shape")
+        if s.dtype != torch.int64 or s.numel() != 1:
+            _bad("a step count", "one int64")
+        k = p.numel()
+        row = rows[i]
+        if bits8:
+            a, b = scales[i], sq_scales[i]
+            want = scales_for(k)
+            for t in (a, b):
+                if t.dtype != torch.float32 or t.numel() != want or not t.is_contiguous() or t.device != device:
+                    _bad("scales", f"contiguous float32 of {want} values on {device} (one for every {BLOCK} values)")
+            row.exp_avg_scale, row.exp_avg_sq_scale = a.data_ptr(), b.data_ptr()
+        if p.device != device or g.device != device or m.device != device or v.device != device or s.device != device:
+            _bad("every tensor", f"on one device ({device})")
+        row.param, row.grad, row.exp_avg, row.exp_avg_sq = p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr()
+        row.step, row.numel, row.dtype = s.data_ptr(), k, dt
+    return rows, device
+
+
+def _check_workspace(workspace, device):
+    if workspace.dtype != torch.float32 or workspace.numel() < WORKSPACE or not workspace.is_contiguous() or workspace.device != device:
+        _bad("workspace", f"{WORKSPACE} contiguous float32 on {device}, zeroed when made")
+
+
+def _launch(device, calls):
+    if device.type != "cuda":
+        raise ValueError(f"adamw_step: tensors must be on a HIP device, got {device}")
+    stream = torch.cuda.current_stream(device).cuda_stream
+    with torch.cuda.device(device):
+        for fn, *args in calls:
+            rc = fn(*args, stream)
+            if rc:
+                _raise(rc)
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avg, exp_avg_sq, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               max_grad_norm=None, exp_avg_scales=None, exp_avg_sq_scales=None, workspace=None, grad_norm=None):
+    """One AdamW step over a list of tensors, in place (see ms_adamw_step in include/marl_soccer.h):
+    parameters and gradients float32, bfloat16 or float16, contiguous; moments float32, or float8_e4m3fn
+    with scales; steps: one int64 on the device for each. lr: a float, or one float32 on the device.
+    max_grad_norm: clip all gradients together by their norm (the gradients themselves stay as they
+    are); grad_norm: one float32 on the device that receives the norm. workspace: WORKSPACE zeroed
+    floats, kept by a caller that steps often (None: made here); one step at a time may use it."""
+    if not len(params):
+        return
+    if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
+        _bad("exp_avg_scales and exp_avg_sq_scales", "both given or both None")
+    rows, device = _entries(params, grads, exp_avg, exp_avg_sq, steps, exp_avg_scales, exp_avg_sq_scales)
+    if max_grad_norm is not None and not max_grad_norm > 0:
+        _bad("max_grad_norm", "positive")
+    if grad_norm is not None and (grad_norm.dtype != torch.float32 or grad_norm.numel() != 1 or grad_norm.device != device):
+        _bad("grad_norm", f"one float32 on {device}")
+    if device.type == "cuda" and workspace is None:
+        workspace = torch.zeros(WORKSPACE, dtype=torch.float32, device=device)
+    if workspace is not None:
+        _check_workspace(workspace, device)
+    calls = []
+    if max_grad_norm is not None:
+        calls.append(_clip_call(rows, max_grad_norm, grad_norm, workspace))
+    calls.append(_step_call(rows, 8 if exp_avg_scales is not None else 32, lr, betas, eps, weight_decay,
+                            max_grad_norm is not None, workspace, device))
+    _launch(device, calls)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _clip_call(rows, max_norm, grad_norm, workspace):
+    return N.lib().ms_grad_clip, rows, len(rows), float(max_norm), _ptr(grad_norm), _ptr(workspace)
+
+
+def _step_call(rows, bits, lr, betas, eps, weight_decay, clip, workspace, device):
+    lr_device = None
+    if isinstance(lr, torch.Tensor):
+        if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
+            _bad("lr", f"a float or one float32 on {device}")
+        lr, lr_device = 0.0, lr.data_ptr()
+    return (N.lib().ms_adamw_step, rows, len(rows), bits, float(lr), lr_device, float(betas[0]), float(betas[1]),
+            float(eps), float(weight_decay), int(clip), _ptr(workspace))
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's update (decoupled weight decay, no amsgrad) with every tensor of a group in
+    one launch; weight_decay=0 is the notebook's Adam. max_grad_norm clips the gradients of all groups
+    together inside the step (.grad stays unclipped; `last_grad_norm`, on the device, holds the norm).
+    A parameter without a gradient is left alone, its step count too. state_bits: 32 or 8 (the
+    module's comment). lr may be one float32 on the device, which a captured step reads anew. State:
+    step, exp_avg, exp_avg_sq and, with 8 bits, their scales; state_dict() carries all of it."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None, state_bits=32):
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"lr must be >= 0, got {lr}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
+            raise ValueError("betas must be in [0, 1), eps and weight_decay >= 0")
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError(f"max_grad_norm must be positive, got {max_grad_norm}")
+        self.max_grad_norm, self.state_bits = max_grad_norm, state_bits
+        self._work = {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    @property
+    def last_grad_norm(self):
+        """The norm of the last clipped step, one float32 on the device (None before it)."""
+        return next((w[1] for w in self._work.values()), None)
+
+    def _state_of(self, p):
+        s = self.state[p]
+        if not s:
+            dt = F8 if self.state_bits == 8 else torch.float32
+            s["step"] = torch.zeros((), dtype=torch.int64, device=p.device)
+            s["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device).to(dt)
+            s["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device).to(dt)
+            if self.state_bits == 8:
+                for k in ("exp_avg_scale", "exp_avg_sq_scale"):
+                    s[k] = torch.zeros(scales_for(p.numel()), dtype=torch.float32, device=p.device)
+        return s
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # Optimizer.load_state_dict casts floating-point state to the parameter's type: take it as it was saved
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        own = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, own):
+            if i in state_dict["state"]:
+                self.state[p] = {k: v.to(device=p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                                 for k, v in state_dict["state"][i].items()}
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        groups, device = [], None
+        for group in self.param_groups:
+            ps = [p for p in group["params"] if p.grad is not None]
+            if not ps:
+                continue
+            if any(p.grad.is_sparse for p in ps):
+                raise ValueError("adamw_step: sparse gradients are not supported")
+            ss = [self._state_of(p) for p in ps]
+            get = lambda k: [s[k] for s in ss]  # noqa: E731
+            eight = self.state_bits == 8
+            grads = [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p in ps]
+            rows, dev = _entries(ps, grads, get("exp_avg"), get("exp_avg_sq"), get("step"),
+                                 get("exp_avg_scale") if eight else None, get("exp_avg_sq_scale") if eight else None)
+            if device is not None and dev != device:
+                _bad("every tensor", f"on one device ({device})")
+            device = dev
+            groups.append((group, rows, grads))  # copies among them live until the launches are in the stream
+        if not groups:
+            return loss
+        if device.type == "cuda" and device not in self._work:
+            self._work[device] = (torch.zeros(WORKSPACE, dtype=torch.float32, device=device),
+                                  torch.zeros((), dtype=torch.float32, device=device))
+        work, norm = self._work.get(device, (None, None))
+        calls = []
+        if self.max_grad_norm is not None:
+            every = groups[0][1] if len(groups) == 1 else (N.MsOptimTensor * sum(len(r) for _, r, _ in groups))(
+                *[t for _, r, _ in groups for t in r])
+            calls.append(_clip_call(every, self.max_grad_norm, norm, work))
+        for group, rows, _ in groups:
+            calls.append(_step_call(rows, self.state_bits, group["lr"], group["betas"], group["eps"], group["weight_decay"],
+                                    self.max_grad_norm is not None, work, device))
+        _launch(device, calls)
+        return loss
