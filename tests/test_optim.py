@@ -1,0 +1,343 @@
+"""marlsoccer.optim (ms_adamw_step, ms_grad_clip) against a 64-bit AdamW, and what it refuses.
+
+Bounds: with u = 2^-24, m = b1 m + c1 g rounds three times and its constants once each, so it is off by
+at most 6 u (|b1 m| + |c1 g|); v likewise by 8 u v, its root by 5 u of itself. The update's factors
+(the bias corrections, computed in float64 and rounded, the quotient, the products) add 8 roundings to
+the 6 and 5, the clip factor 3 more with its own in g: 24 u of (|b1 m| + |c1 g|) lr / denominator, and
+p itself rounds 3 times. A 16-bit parameter is rounded once more, to half a step. A moment of 8 bits is
+off by half a step of e4m3: 2^-4 of its value among the normal ones, half of 2^-9 scales below 2^-6
+scales (the scale itself is max / 448 within 2 u)."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from marlsoccer import optim  # noqa: E402
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a HIP device")
+
+
+SHAPES = [(1,), (3,), (64, 66), (512,), (7, 5), (255,), (256,), (257,), (1000, 13), (0,), (4099,), (1, 3)]
+
+
+def make(shapes, dtype, seed, device="cuda"):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    ps = [torch.randn(s, generator=g).mul_(0.1).to(dtype).to(device) for s in shapes]
+    gs = [(torch.randn(s, generator=g) * math.exp(torch.randn((), generator=g).item())).to(dtype).to(device) for s in shapes]
+    return ps, gs
+
+
+class Exact:
+    """AdamW in 64 bits; with 8 bits the caller puts the held moments back after every step."""
+
+    def __init__(self, ps, lr, betas, eps, decay, clip):
+        self.p = [p.double().cpu() for p in ps]
+        self.m = [torch.zeros_like(p) for p in self.p]
+        self.v = [torch.zeros_like(p) for p in self.p]
+        self.t = [0] * len(self.p)
+        self.hp = lr, betas, eps, decay, clip
+
+    def step(self, gs):
+        lr, (b1, b2), eps, decay, clip = self.hp
+        gs = [None if g is None else g.double().cpu() for g in gs]
+        self.norm = math.sqrt(sum(float(g.square().sum()) for g in gs if g is not None))
+        c = min(1.0, clip / (self.norm + 1e-6)) if clip else 1.0
+        self.size, self.msize = [0.0] * len(gs), [0.0] * len(gs)
+        for i, g in enumerate(gs):
+            if g is None:
+                continue
+            self.t[i] += 1
+            t, g = self.t[i], g * c
+            self.msize[i] = b1 * self.m[i].abs() + (1 - b1) * g.abs()
+            self.m[i] = b1 * self.m[i] + (1 - b1) * g
+            self.v[i] = b2 * self.v[i] + (1 - b2) * g * g
+            den = torch.sqrt(self.v[i] / (1 - b2 ** t)) + eps
+            f = lr / (1 - b1 ** t)
+            self.size[i] = f * self.msize[i] / den
+            self.p[i] = self.p[i] * (1 - lr * decay) - f * self.m[i] / den
+
+
+def within(name, got, want, bound):
+    off = (got.double().cpu() - want).abs()
+    assert bool((off <= bound).all()), f"{name}: worst excess {float((off - bound).max()):.3g}"
+
+
+def check(ref, ps, moments, dtype, bits):
+    eps = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    tiny = 2.0 ** -126
+    for i, p in enumerate(ps):
+        raw = 24 * U * ref.size[i] + 3 * U * ref.p[i].abs() + tiny
+        sub = 2.0 ** -25 if dtype == torch.float16 else 0.0  # half a step among float16's subnormals
+        within(f"p{i}", p, ref.p[i], raw + eps * (ref.p[i].abs() + raw) + sub)
+        m, v = moments(i)
+        if bits == 32:
+            within(f"m{i}", m, ref.m[i], 9 * U * ref.msize[i] + tiny)
+            within(f"v{i}", v, ref.v[i], 12 * U * ref.v[i] + tiny)
+        elif p.numel():
+            for name, got, want, err in (("m", m, ref.m[i], 9 * U * ref.msize[i]), ("r", v, ref.v[i].sqrt(), 8 * U * ref.v[i].sqrt())):
+                n = want.numel()
+                top = torch.nn.functional.pad(want.abs().reshape(-1), (0, -n % optim.BLOCK)).view(-1, optim.BLOCK).amax(1)
+                scale = (top / 448).repeat_interleave(optim.BLOCK)[:n].view(want.shape)
+                err = torch.as_tensor(err) + 4 * U * top.repeat_interleave(optim.BLOCK)[:n].view(want.shape)
+                within(f"{name}{i}", got, want, (want.abs() + err) * 2.0 ** -4 + scale * 2.0 ** -10 * (1 + 8 * U) + err + 2.0 ** -99)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("clip", [None, 0.5, 1e9])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_steps_match_64_bits(dtype, clip, bits):
+    need_gpu()
+    lr, betas, eps, decay = 3e-3, (0.9, 0.99), 1e-5, 0.05
+    ps, _ = make(SHAPES, dtype, 1)
+    opt = optim.AdamW([torch.nn.Parameter(p) for p in ps], lr=lr, betas=betas, eps=eps, weight_decay=decay, max_grad_norm=clip, state_bits=bits)
+    params = opt.param_groups[0]["params"]
+    ref = Exact(ps, lr, betas, eps, decay, clip)
+    for step in range(5):
+        _, gs = make(SHAPES, dtype, 10 + step)
+        ref.p = [p.detach().double().cpu() for p in params]  # each step is held to its own bound
+        if step:
+            held = [moments(i) for i in range(len(ps))]
+            ref.m = [m.double().cpu() for m, _ in held]
+            ref.v = [(v.double() ** (2 if bits == 8 else 1)).cpu() for _, v in held]
+        for p, g in zip(params, gs):
+            p.grad = g.clone()
+        opt.step()
+        ref.step(gs)
+
+        def moments(i):
+            s = opt.state[params[i]]
+            if bits == 32:
+                return s["exp_avg"], s["exp_avg_sq"]
+            return (optim.moment_values(s["exp_avg"], s["exp_avg_scale"]), optim.moment_values(s["exp_avg_sq"], s["exp_avg_sq_scale"]))
+
+        check(ref, [p.detach() for p in params], moments, dtype, bits)
+        assert all(int(opt.state[p]["step"]) == step + 1 for p in params)
+        assert all(torch.equal(p.grad, g) for p, g in zip(params, gs))
+        if clip:
+            assert abs(float(opt.last_grad_norm) - ref.norm) <= 2 * U * ref.norm
+
+
+@gpu
+def test_many_tensors_over_several_launches():
+    """More tensors than one launch takes, groups with their own settings, a parameter without a
+    gradient, and one norm over all of them."""
+    need_gpu()
+    shapes = [(5 + i % 37, 1 + i % 11) for i in range(131)]
+    ps, gs = make(shapes, torch.float32, 3)
+    params = [torch.nn.Parameter(p.clone()) for p in ps]
+    opt = optim.AdamW([dict(params=params[:100]), dict(params=params[100:], lr=1e-2, weight_decay=0.0)], lr=1e-3, weight_decay=0.1, max_grad_norm=2.0)
+    a, b = Exact(ps[:100], 1e-3, (0.9, 0.999), 1e-8, 0.1, None), Exact(ps[100:], 1e-2, (0.9, 0.999), 1e-8, 0.0, None)
+    skip = 57
+    norm = math.sqrt(sum(float(g.double().square().sum()) for i, g in enumerate(gs) if i != skip))
+    scale = min(1.0, 2.0 / (norm + 1e-6))
+    for p, g, i in zip(params, gs, range(131)):
+        p.grad = None if i == skip else g
+    opt.step()
+    clipped = [None if i == skip else g.double() * scale for i, g in enumerate(gs)]
+    a.step(clipped[:100])
+    b.step(clipped[100:])
+    assert abs(float(opt.last_grad_norm) - norm) <= 2 * U * norm
+    for i, p in enumerate(params):
+        if i == skip:
+            assert torch.equal(p.detach(), ps[i]) and not opt.state[p]
+            continue
+        ref, j = (a, i) if i < 100 else (b, i - 100)
+        within(f"p{i}", p.detach(), ref.p[j], 24 * U * ref.size[j] + 3 * U * ref.p[j].abs() + 2.0 ** -126)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_unaligned_views_and_the_functional_form(bits):
+    """Tensors cut out of one buffer at odd offsets; values around them stay as they were; the same
+    bits as the aligned ones."""
+    need_gpu()
+    shapes = [(33,), (256,), (700,), (1025,)]
+    ps, gs = make(shapes, torch.float32, 5)
+    outs = []
+    for off in (0, 1):
+        lists = dict(p=[], g=[], m=[], v=[], s=[], ms=[], vs=[])
+        pads = []
+        for p, g in zip(ps, gs):
+            for key, src, dt in (("p", p, torch.float32), ("g", g, torch.float32), ("m", torch.zeros_like(p), None), ("v", torch.zeros_like(p), None)):
+                dt = dt or (optim.F8 if bits == 8 else torch.float32)
+                buf = torch.full((p.numel() + 2 * off + 2,), 7.0, device="cuda").to(dt)
+                buf[off:off + p.numel()] = src.to(dt)
+                lists[key].append(buf[off:off + p.numel()])
+                pads.append((buf, off, p.numel()))
+            lists["s"].append(torch.zeros(1, dtype=torch.int64, device="cuda"))
+            for key in ("ms", "vs"):
+                lists[key].append(torch.zeros(optim.scales_for(p.numel()), device="cuda"))
+        for _ in range(3):
+            optim.adamw_step(lists["p"], lists["g"], lists["m"], lists["v"], lists["s"], lr=1e-2, max_grad_norm=1.0,
+                             exp_avg_scales=lists["ms"] if bits == 8 else None, exp_avg_sq_scales=lists["vs"] if bits == 8 else None)
+        for buf, o, n in pads:
+            assert bool((buf[:o].float() == 7.0).all()) and bool((buf[o + n:].float() == 7.0).all())
+        outs.append([t.float() for k in ("p", "m", "v", "ms", "vs") for t in lists[k]])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_non_finite_gradients_pass_into_the_update():
+    """As clip_grad_norm_ and AdamW have it: an infinite norm makes the factor 0 (0 times the infinite
+    gradient is no number, the others' 0), a NaN reaches every parameter."""
+    need_gpu()
+    for bad, others_nan in ((float("inf"), False), (float("nan"), True)):
+        ps, gs = make([(300,), (10,)], torch.float32, 6)
+        params = [torch.nn.Parameter(p.clone()) for p in ps]
+        opt = optim.AdamW(params, max_grad_norm=1.0, weight_decay=0.0)
+        gs[0][7] = bad
+        for p, g in zip(params, gs):
+            p.grad = g
+        opt.step()
+        got = torch.isnan(params[0].detach()).cpu()
+        assert got[7] and bool(got.all()) == others_nan and bool(torch.isnan(params[1]).all()) == others_nan
+    # with 8 bits a NaN is held as one, and the rest of its block goes on
+    ps, gs = make([(300,)], torch.float32, 7)
+    p = torch.nn.Parameter(ps[0].clone())
+    opt = optim.AdamW([p], state_bits=8)
+    gs[0][7] = float("nan")
+    p.grad = gs[0]
+    opt.step()
+    held = optim.moment_values(opt.state[p]["exp_avg"], opt.state[p]["exp_avg_scale"])
+    assert int(torch.isnan(held).sum()) == 1 and int(torch.isnan(p.detach()).sum()) == 1
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict_round_trip(bits):
+    need_gpu()
+    ps, _ = make([(40, 9), (17,)], torch.bfloat16, 8)
+    runs = []
+    for reload in (False, True):
+        params = [torch.nn.Parameter(p.clone()) for p in ps]
+        opt = optim.AdamW(params, lr=1e-2, max_grad_norm=1.0, state_bits=bits)
+        for step in range(4):
+            _, gs = make([(40, 9), (17,)], torch.bfloat16, 20 + step)
+            for p, g in zip(params, gs):
+                p.grad = g
+            if reload and step == 2:
+                saved = opt.state_dict()
+                opt = optim.AdamW(params, lr=1e-2, max_grad_norm=1.0, state_bits=bits)
+                opt.load_state_dict(saved)
+            opt.step()
+        runs.append([p.detach().clone() for p in params] + [opt.state[p]["exp_avg"].float() for p in params])
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_replays(bits):
+    """A step in a graph counts its steps and reads the learning rate and the gradients anew; eager
+    steps may come between."""
+    need_gpu()
+    shapes = [(66, 64), (64,), (3,)]
+    ps, gs = make(shapes, torch.float32, 9)
+    runs = []
+    for graph in (False, True):
+        params = [torch.nn.Parameter(p.clone()) for p in ps]
+        lr = torch.full((), 1e-2, device="cuda")
+        opt = optim.AdamW(params, lr=lr, max_grad_norm=0.5, state_bits=bits)
+        for p, g in zip(params, gs):
+            p.grad = g.clone()
+        opt.step()
+        if graph:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                opt.step()
+        for k in range(5):
+            lr.mul_(0.8)
+            for p in params:
+                p.grad.mul_(-0.9)
+            if graph and k != 2:
+                g.replay()
+            else:
+                opt.step()
+            torch.cuda.synchronize()
+        assert all(int(opt.state[p]["step"]) == 6 for p in params)
+        runs.append([p.detach().clone() for p in params] + [opt.state[p]["exp_avg_sq"].float() for p in params])
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_agrees_with_torch_adamw():
+    need_gpu()
+    ps, _ = make([(64, 66), (64,)], torch.float32, 30)
+    a, b = [[torch.nn.Parameter(p.clone()) for p in ps] for _ in range(2)]
+    mine, theirs = optim.AdamW(a, lr=1e-3, weight_decay=0.02, max_grad_norm=0.5), torch.optim.AdamW(b, lr=1e-3, weight_decay=0.02)
+    for k in range(20):
+        _, gs = make([(64, 66), (64,)], torch.float32, 40 + k)
+        for p, q, g in zip(a, b, gs):
+            p.grad, q.grad = g.clone(), g.clone()
+        mine.step()
+        torch.nn.utils.clip_grad_norm_(b, 0.5)
+        theirs.step()
+    for p, q in zip(a, b):  # each of 20 steps moves a parameter by about lr, each within 24 u and some for theirs
+        assert float((p - q).abs().max()) <= 20 * (48 * U * 10 * 1e-3 + 6 * U)
+
+
+# ---------------------------------------------------------------- refusals (CPU)
+
+def test_refusals():
+    p = torch.nn.Parameter(torch.zeros(4))
+    for kw in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-0.1), dict(max_grad_norm=0.0),
+               dict(lr=float("nan"))):
+        with pytest.raises(ValueError):
+            optim.AdamW([p], **kw)
+    p.grad = torch.zeros(4)
+    with pytest.raises(ValueError, match="HIP device"):
+        optim.AdamW([p]).step()
+    z = lambda n=4, dt=torch.float32: torch.zeros(n, dtype=dt)  # noqa: E731
+    good = dict(params=[z()], grads=[z()], exp_avg=[z()], exp_avg_sq=[z()], steps=[z(1, torch.int64)], lr=1e-3)
+
+    def refuses(match, **kw):
+        with pytest.raises(ValueError, match=match):
+            optim.adamw_step(**{**good, **kw})
+
+    refuses("HIP device")
+    refuses("one for every parameter", grads=[])
+    refuses("float32, bfloat16 or float16", params=[z(4, torch.float64)])
+    refuses("of its parameter's type", grads=[z(4, torch.float16)])
+    refuses("of its parameter's type", grads=[z(5)])
+    refuses("contiguous", params=[torch.zeros(2, 8)[:, ::2]], grads=[torch.zeros(2, 4)])
+    refuses("a moment", exp_avg=[z(3)])
+    refuses("a moment", exp_avg_sq=[z(4, torch.float16)])
+    refuses("one int64", steps=[z(1)])
+    refuses("both given", exp_avg_scales=[z(1)])
+    refuses("a moment", exp_avg_scales=[z(1)], exp_avg_sq_scales=[z(1)])
+    f8 = dict(exp_avg=[z(4, optim.F8)], exp_avg_sq=[z(4, optim.F8)])
+    refuses("scales", **f8, exp_avg_scales=[z(2)], exp_avg_sq_scales=[z(1)])
+    refuses("positive", max_grad_norm=-1.0)
+    refuses("workspace", workspace=z(7))
+    refuses("grad_norm", grad_norm=z(2))
+    refuses("lr must be", lr=z(2))
+
+
+def test_c_entries_refuse_bad_arguments():
+    from marlsoccer import _native as N
+    L = N.lib()
+    rows = (N.MsOptimTensor * 1)(N.MsOptimTensor(numel=4))
+    step = lambda rows, bits=32, lr=1e-3, b1=0.9, work=16: L.ms_adamw_step(rows, 1, bits, lr, None, b1, 0.99, 1e-8, 0.0, 0, work, None)  # noqa: E731
+    assert step(rows) == N.MS_ERR_INVALID_ARGUMENT and b"gradient" in L.ms_optim_last_error()
+    rows[0].grad = 16
+    assert step(rows) == N.MS_ERR_INVALID_ARGUMENT and b"step count" in L.ms_optim_last_error()
+    rows[0].step = 16
+    assert step(rows) == N.MS_ERR_INVALID_ARGUMENT and b"param" in L.ms_optim_last_error()
+    assert step(rows, work=None) == N.MS_ERR_INVALID_ARGUMENT and b"workspace" in L.ms_optim_last_error()
+    assert step(rows, bits=4) == N.MS_ERR_INVALID_ARGUMENT
+    assert step(rows, lr=float("nan")) == N.MS_ERR_INVALID_ARGUMENT
+    assert step(rows, b1=1.0) == N.MS_ERR_INVALID_ARGUMENT
+    assert L.ms_grad_clip(rows, 1, 0.0, None, 16, None) == N.MS_ERR_INVALID_ARGUMENT
+    rows[0].dtype = 5
+    assert L.ms_grad_clip(rows, 1, 1.0, None, 16, None) == N.MS_ERR_INVALID_ARGUMENT
