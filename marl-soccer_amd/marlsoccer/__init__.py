@@ -12,3 +12,4 @@ from . import _native  # noqa: F401
 
 __all__ = ["SoccerBatch", "FrameRingBatch", "StepOutput", "spawn_mode", "load_config", "to_ms_config"]
 # marlsoccer.rollout (Agent, RunningMeanStd, DeviceRollout): the device-resident policy loop
+# marlsoccer.sequence (short_conv, ssm_scan and their steps), marlsoccer.memory (SequenceMemory), marlsoccer.optim (AdamW)

@@ -54,8 +54,13 @@ def evaluate(agent: Agent, normalizer: RunningMeanStd, num_episodes: int, seed=N
             from .render import render_batch
         blue = torch.tensor(TRAINABLE, dtype=torch.int64, device=dev)  # on the device: a host index would copy per step
 
+        memory = getattr(agent, "memory", None)
+        memory_state = None if memory is None else memory.init_state(2 * n, dev)
+
         def body():
             x = normalizer.normalize(batch.obs.index_select(1, blue).reshape(-1, OBS_DIM))
+            if memory is not None:
+                x = memory.step(x, memory_state)  # every env plays one episode, from zeros
             acts[:, :2] = agent.get_deterministic_action(x).reshape(n, 2, ACT_DIM)
             if red == "uniform":
                 acts[:, 2:] = torch.rand((n, 2, ACT_DIM), generator=gen, device=dev) * 2.0 - 1.0

@@ -83,9 +83,13 @@ def layer_init(layer: nn.Linear, std=np.sqrt(2), bias_const=0.0) -> nn.Linear:
 
 class Agent(nn.Module):
     """The reference's actor-critic (notebook `Agent`, eval.py:17-47): two tanh MLPs
-    66-512-256-128-64-{1, 3} and a state-independent log-std."""
+    66-512-256-128-64-{1, 3} and a state-independent log-std.
+    memory (opt-in, no counterpart in the reference; None keeps its checkpoints' layout): a
+    marlsoccer.memory.SequenceMemory whose output the actor and critic take in place of the
+    normalised observations. DeviceRollout and evaluate step it; an update runs
+    agent.memory(x, starts, state) over the stored sequences first."""
 
-    def __init__(self, obs_dim: int = OBS_DIM, act_dim: int = ACT_DIM, rpo_alpha: float = 0.0):
+    def __init__(self, obs_dim: int = OBS_DIM, act_dim: int = ACT_DIM, rpo_alpha: float = 0.0, memory: nn.Module | None = None):
         super().__init__()
         self.critic = nn.Sequential(
             layer_init(nn.Linear(obs_dim, 512)), nn.Tanh(),
@@ -99,6 +103,7 @@ class Agent(nn.Module):
         )
         self.actor_logstd = nn.Parameter(torch.zeros(1, act_dim))
         self.rpo_alpha = rpo_alpha
+        self.memory = memory
 
     def get_value(self, x: torch.Tensor) -> torch.Tensor:
         return self.critic(x)
@@ -163,6 +168,10 @@ class DeviceRollout:
     (the notebook's) starts its first epoch with exp(new - old) within 1e-4 of 1, not exactly 1
     (tests/test_policy.py::test_fused_rollout_ppo_first_epoch_ratio_near_one). policy="torch"
     keeps the notebook's bit-for-bit first-epoch ratio of 1.
+    An agent with a memory (Agent(memory=...)) runs with policy="torch" (its default then): every
+    step the memory of all 2 N rows is stepped in place, from zeros where an episode ended before it.
+    collect() then also returns "memory_state", the state before the rollout's first step, with which
+    agent.memory(x, dones.reshape(T, -1).bool(), memory_state) replays the rollout for the update.
     """
 
     def __init__(self, batch, agent: Agent, normalizer: RunningMeanStd, num_steps: int, seed: int = 0,
@@ -176,10 +185,13 @@ class DeviceRollout:
         if policy_dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"policy_dtype must be torch.float32 or torch.bfloat16, got {policy_dtype}")
         self.policy_dtype = policy_dtype
+        memory = getattr(agent, "memory", None)
         if policy is None:
-            policy = "fused" if policy_dtype == torch.float32 else "torch"
+            policy = "fused" if policy_dtype == torch.float32 and memory is None else "torch"
         if policy not in ("fused", "torch") or (policy == "fused" and policy_dtype != torch.float32):
             raise ValueError(f"policy must be 'fused' (fp32) or 'torch', got {policy!r} with {policy_dtype}")
+        if policy == "fused" and memory is not None:
+            raise ValueError("policy='fused' has no memory: use policy='torch' for an agent with one")
         self.policy = policy
         self._fused = None
         if policy == "fused":
@@ -204,6 +216,10 @@ class DeviceRollout:
         self.next_done = torch.zeros((N, 2), dtype=torch.float32, device=dev)
         self.episodes = torch.zeros((), dtype=torch.int64, device=dev)  # finished env episodes
         self.score_sum = torch.zeros((2,), dtype=torch.int64, device=dev)
+        self.memory_state = self.memory_start = None
+        if memory is not None:
+            self.memory_state = memory.init_state(2 * N, dev, policy_dtype)
+            self.memory_start = memory.init_state(2 * N, dev, policy_dtype)
 
     @torch.no_grad()
     def step(self, t: int) -> None:
@@ -232,6 +248,8 @@ class DeviceRollout:
             # capture (the casts of ~0.4 M parameters per step are negligible)
             with torch.autocast("cuda", dtype=torch.bfloat16, enabled=self.policy_dtype == torch.bfloat16,
                                 cache_enabled=False):
+                if self.memory_state is not None:
+                    x = self.agent.memory.step(x, self.memory_state, self.next_done.reshape(-1) != 0)
                 if self.deterministic:
                     action = self.agent.get_deterministic_action(x)
                     value = self.agent.get_value(x)
@@ -261,6 +279,9 @@ class DeviceRollout:
         if self._fused is not None:  # the parameters and the normaliser as they are now
             self._fused.pack()
             torch.add(self.normalizer.std, 1e-8, out=self._den)
+        if self.memory_state is not None:
+            for start, now in zip(self.memory_start, self.memory_state):
+                start.copy_(now)
         for t in range(self.T):
             self.step(t)
         if self._fused is not None:  # the fused step reads the env's obs rows directly
@@ -303,6 +324,9 @@ class DeviceRollout:
         self.batch.raise_if_nonfinite()
         if self.update_normalizer:  # notebook L347: after the rollout, from the raw observations
             self.normalizer.update(self.obs.reshape(-1, OBS_DIM))
-        return {"obs": self.obs, "actions": self.actions, "logprobs": self.logprobs, "rewards": self.rewards,
-                "dones": self.dones, "values": self.values, "next_obs": self.next_obs, "next_done": self.next_done,
-                "episodes": self.episodes, "score_sum": self.score_sum}
+        out = {"obs": self.obs, "actions": self.actions, "logprobs": self.logprobs, "rewards": self.rewards,
+               "dones": self.dones, "values": self.values, "next_obs": self.next_obs, "next_done": self.next_done,
+               "episodes": self.episodes, "score_sum": self.score_sum}
+        if self.memory_start is not None:
+            out["memory_state"] = self.memory_start
+        return out

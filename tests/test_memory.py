@@ -1,0 +1,160 @@
+"""Agents with a sequence memory: the rollout, its replay by the update, evaluation, and the whole
+loop with the optimiser."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import sequence_reference as ref  # noqa: E402
+
+from marlsoccer.memory import SequenceMemory  # noqa: E402
+from marlsoccer.rollout import Agent, DeviceRollout, RunningMeanStd  # noqa: E402
+
+gpu = pytest.mark.gpu
+
+
+def need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a HIP device")
+
+
+def test_an_agent_without_memory_keeps_its_checkpoint_layout():
+    assert not any(k.startswith("memory") for k in Agent().state_dict())
+    keys = Agent(memory=SequenceMemory()).state_dict()
+    assert {"memory.in_proj.weight", "memory.A_log", "memory.conv_weight"} <= set(keys)
+
+
+def plain_memory(m, x, starts, state):
+    """SequenceMemory.forward in 64 bits on the CPU."""
+    d = lambda t: t.detach().double().cpu()  # noqa: E731
+    xz = d(x) @ d(m.in_proj.weight).t()
+    u, z = xz.chunk(2, -1)
+    u, conv, _ = ref.conv(u, m.conv_weight, m.conv_bias, state[0], starts)
+    r, B, C = (u @ d(m.x_proj.weight).t()).split((m.rank, m.states, m.states), -1)
+    y, h, _ = ref.scan(u, r @ d(m.rate_proj.weight).t(), -torch.exp(d(m.A_log)), B, C, m.skip, z, m.rate_bias, state[1], starts)
+    return d(x) + y @ d(m.out_proj.weight).t(), conv, h
+
+
+@gpu
+def test_steps_and_sequences_match_the_plain_form():
+    """Both forms against 64 bits. The projections are products of at most 128 terms in float32 (an error
+    of 128 u of their size) and feed the recurrences, whose outputs are held to 1e-4 here; each operator's
+    own bound is tests/test_sequence.py's."""
+    need_gpu()
+    torch.manual_seed(0)
+    T, R = 20, 6
+    m = SequenceMemory(channels=96).cuda()
+    x = torch.randn(T, R, 66).cuda()
+    starts = torch.rand(T, R).cuda() < 0.1
+    state = tuple(torch.randn_like(s) for s in m.init_state(R, "cuda"))
+    want, conv, h = plain_memory(m, x, starts, state)
+    y, (c1, h1) = m(x, starts, state)
+    stepped = tuple(s.clone() for s in state)
+    ys = torch.stack([m.step(x[t], stepped, starts[t]) for t in range(T)])
+    for got, c, s in ((y, c1, h1), (ys, *stepped)):
+        for a, b in ((got, want), (c, conv), (s, h)):
+            assert float((a.detach().double().cpu() - b).abs().max()) <= 1e-4 * (1 + float(b.abs().max()))
+
+
+def make(N, T, graph=False, config=None, **kw):
+    from marlsoccer import SoccerBatch
+    torch.manual_seed(0)
+    agent = Agent(memory=SequenceMemory()).cuda()
+    b = SoccerBatch(N, config=config)
+    b.reset(seed=19)
+    return agent, b, DeviceRollout(b, agent, RunningMeanStd((66,), device="cuda"), T, seed=5, graph=graph, update_normalizer=False, **kw)
+
+
+def short_config(steps):
+    from marlsoccer.config import load_config
+    cfg = load_config()
+    cfg["simulation"]["max_steps"] = steps
+    return cfg
+
+
+@gpu
+def test_rollout_replays_as_one_sequence():
+    """What the rollout's single steps stored is what the update computes from the stored sequences and
+    the state before them, across episode ends."""
+    need_gpu()
+    N, T = 24, 30
+    agent, b, ro = make(N, T, config=short_config(13))
+    assert ro.policy == "torch"
+    with pytest.raises(ValueError, match="memory"):
+        DeviceRollout(b, agent, ro.normalizer, T, policy="fused")
+    for _ in range(2):
+        out = ro.collect()
+        assert out["dones"].any()
+        x = ro.normalizer.normalize(out["obs"].reshape(-1, 66)).view(T, 2 * N, 66)
+        y, state = agent.memory(x, out["dones"].reshape(T, -1).bool(), out["memory_state"])
+        value = agent.get_value(y.reshape(-1, 66)).view(T, N, 2)
+        assert float((value - out["values"]).abs().max()) <= 1e-4  # float32 products in another order
+        for a, c in zip(state, ro.memory_state):
+            assert float((a - c).abs().max()) <= 1e-4 * (1 + float(c.abs().max()))
+        plain = agent.get_value(x.reshape(-1, 66)).view(T, N, 2)
+        assert float((plain - out["values"]).abs().max()) > 1e-3  # the memory does something
+    b.close()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_graph_rollout_matches_eager(dtype):
+    need_gpu()
+    runs = []
+    for graph in (False, True):
+        agent, b, ro = make(32, 9, graph, short_config(7), policy_dtype=dtype)
+        outs = []
+        for _ in range(4):
+            out = ro.collect()
+            outs += [out[k].clone() for k in ("obs", "actions", "values", "dones", "rewards")] + [s.clone() for s in ro.memory_state + out["memory_state"]]
+        runs.append(outs)
+        b.close()
+    for a, c in zip(*runs):
+        assert torch.equal(a, c)
+
+
+@gpu
+def test_evaluate_with_memory():
+    need_gpu()
+    from marlsoccer.evaluate import evaluate
+    torch.manual_seed(0)
+    agent = Agent(memory=SequenceMemory()).cuda()
+    rms = RunningMeanStd(device="cuda")
+    a = evaluate(agent, rms, 8, seed=3, config=short_config(40))
+    g = evaluate(agent, rms, 8, seed=3, config=short_config(40), graph=True)
+    assert (a["returns"] == g["returns"]).all() and (a["score"] == g["score"]).all()
+    agent.memory = None
+    plain = evaluate(agent, rms, 8, seed=3, config=short_config(40))
+    assert (a["returns"] != plain["returns"]).any()
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_collect_update_loop(bits):
+    """Rollout (a replayed graph from the third on), replay through the memory, gradients to every
+    parameter, the optimiser's step in place: the graph goes on reading the parameters."""
+    need_gpu()
+    from marlsoccer.optim import AdamW
+    N, T = 16, 12
+    agent, b, ro = make(N, T, True, short_config(9))
+    opt = AdamW(agent.parameters(), lr=2.5e-4, eps=1e-5, weight_decay=0.0, max_grad_norm=0.5, state_bits=bits)
+    at = None
+    for it in range(4):
+        out = ro.collect()
+        if it > 1:
+            assert ro._graph is at  # not captured again
+        at = ro._graph
+        x = ro.normalizer.normalize(out["obs"].reshape(-1, 66)).view(T, 2 * N, 66)
+        y, _ = agent.memory(x, out["dones"].reshape(T, -1).bool(), out["memory_state"])
+        _, logprob, entropy, value = agent.get_action_and_value(y.reshape(-1, 66), out["actions"].reshape(-1, 3))
+        ratio = (logprob - out["logprobs"].reshape(-1)).exp()
+        assert float((ratio - 1).abs().max()) <= 1e-3
+        loss = -(ratio * out["rewards"].reshape(-1)).mean() + (value.squeeze(-1) - 1.0).square().mean() - 0.01 * entropy.mean()
+        loss.backward()
+        before = [p.detach().clone() for p in agent.parameters()]
+        assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in agent.parameters())
+        assert all(bool(p.grad.any()) for n, p in agent.named_parameters() if n.startswith("memory"))
+        opt.step()
+        opt.zero_grad()
+        assert all(bool(torch.isfinite(p).all()) for p in agent.parameters())
+        assert any(not torch.equal(p, q) for p, q in zip(before, agent.parameters()))
+    b.close()
