@@ -312,7 +312,7 @@ int run_backward(const ms_conv_io& io, const Shape& s, bool vec, hipStream_t str
   if (int rc = launched("ms_conv_backward")) return rc;
   if (!io.dweight && !io.dbias) return MS_OK;
   hipLaunchKernelGGL((sum_parts<8>), dim3((unsigned)((columns + 63) / 64)), dim3(512), 0, stream, parts, s.blocks_p,
-                     columns, sums);
+                     s.blocks_p, columns, sums);
   hipLaunchKernelGGL(finish, dim3((unsigned)((columns + 255) / 256)), dim3(256), 0, stream, sums, io.channels, io.width,
                      io.dweight, io.dbias);
   return launched("ms_conv_backward");

@@ -19,6 +19,8 @@
 // Backward runs the same tiles from the end: g[t] = C dy + a[t+1] g[t+1]. The states it needs are
 // rebuilt from checkpoints of every KC = 16 steps; dB and dC are sums over channels, folded over the
 // wave's lanes with v_permlane swaps and DPP, and over the channel blocks by a last kernel.
+#include <type_traits>
+
 #include "ms_sequence.h"
 
 namespace scan {
@@ -32,13 +34,15 @@ constexpr float LOG2E = 1.44269504f, LN2 = 0.69314718f;
 // How a call is cut. NW waves hold NS states each; `tiles` blocks of 64 channels a group.
 struct Plan {
   int ns, nw;               // states per wave, waves per block
+  int unit;                 // states of a scalar unit: 16 / unit steps of `unit` states
+  int64_t units;            // scalar units along time (of all steps, and one more that is only fetched)
   int64_t tiles, blocks_d;  // tiles per group, tiles * groups
   int64_t chunks, chunk;    // over time; steps per chunk (a multiple of 32)
   int64_t kc;               // checkpoints
 };
 
 struct Work {  // the workspace, in floats
-  float *bc, *local, *rates, *parts_bc, *parts_a, *parts_d, *sums;
+  float *bc, *local, *rates, *parts_bc, *parts, *sums;
   int* cut;
   int64_t floats;
 };
@@ -47,29 +51,48 @@ struct Work {  // the workspace, in floats
 struct Args {
   ms_scan_io io;
   Plan p;
-  const float *Bf, *Cf;  // float32, padded to ns * nw states
-  int64_t b_t, b_r, b_g, c_t, c_r, c_g;
-  float *local, *rates, *parts_bc, *parts_a, *parts_d;
+  float *bc, *local, *rates, *parts_bc, *parts;
   int* cut;
   int vec;
 };
 
-__device__ __forceinline__ float rate_of(float x, int soft) { return soft ? softplus(x) : x; }
-
-// B and C (T, R, G, N) of any strides and type -> float32 [T][R][G][NP], zeros past N
+// B and C (T, R, G, N) of any strides and type -> float32 in the order that the scans' scalar loads
+// want: [row][group][states / unit][16 / unit steps][B, C][16], zeros past the last step and state
 template <typename T>
-__global__ __launch_bounds__(256) void widen(const ms_scan_io io, int np, float* __restrict__ to) {
-  const int64_t per = io.steps * io.rows * io.groups * np;
+__global__ __launch_bounds__(256) void widen(const ms_scan_io io, int unit, int shares, int64_t units, float* __restrict__ to) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= per) return;
-  const int n = (int)(i % np);
-  int64_t k = i / np;
-  const int64_t g = k % io.groups;
-  k /= io.groups;
-  const int64_t r = k % io.rows, t = k / io.rows;
-  const bool in = n < io.states;
-  to[i] = in ? (float)((const T*)io.B)[t * io.B_t + r * io.B_r + g * io.B_g + n] : 0.0f;
-  to[per + i] = in ? (float)((const T*)io.C)[t * io.C_t + r * io.C_r + g * io.C_g + n] : 0.0f;
+  const int e = (int)(i & 15), kind = (int)(i >> 4 & 1);
+  int64_t k = i >> 5;
+  const int64_t v = k % units;
+  k /= units;
+  const int share = (int)(k % shares);
+  k /= shares;
+  const int64_t g = k % io.groups, r = k / io.groups;
+  if (r >= io.rows) return;
+  const int n = share * unit + e % unit;
+  const int64_t t = v * (16 / unit) + e / unit;
+  const bool in = n < io.states && t < io.steps;
+  const T* p = kind ? (const T*)io.C + t * io.C_t + r * io.C_r + g * io.C_g : (const T*)io.B + t * io.B_t + r * io.B_r + g * io.B_g;
+  to[i] = in ? (float)p[n] : 0.0f;
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+struct Scalars {  // a unit's B and C, in SGPRs
+  f32x16 b, c;
+};
+__device__ __forceinline__ Scalars scalars(CONSTANT(f32x16)* p) {
+  Scalars s;
+  s.b = p[0];
+  s.c = p[1];
+  return s;
+}
+__device__ __forceinline__ CONSTANT(f32x16)* scalars_at(const Args& a, int64_t r, int64_t g, int share) {
+  const int shares = a.p.ns * a.p.nw / a.p.unit;
+  return (CONSTANT(f32x16)*)(a.bc + ((r * a.io.groups + g) * shares + share) * a.p.units * 32);
+}
+// the checkpoint of step 16 k: [k][row][tile][states / 4][64 channels][4]
+__device__ __forceinline__ int64_t checkpoint_at(const Args& a, int64_t k, int64_t r, int64_t td, int state, int lane) {
+  return (((k * a.io.rows + r) * a.p.blocks_d + td) * (a.p.ns * a.p.nw / 4) + state / 4) * 256 + lane * 4;
 }
 
 // Which steps of a tile begin an episode, as a mask the whole wave shares
@@ -101,11 +124,16 @@ __device__ __forceinline__ Place place(const Args& a) {
 
 // ---------------------------------------------------------------- forward
 // LOCAL: the first pass of a split time axis (states from zero, no outputs).
+// The loop over a tile goes by units of 16 / NS steps: 32 scalars (one s_load_dwordx16 for B and one
+// for C) and the unit's rates from LDS are fetched a unit ahead, both before the work of the present
+// one, since scalar loads return in no order and one wait covers them all.
 template <typename T, int NS, int NW, bool LOCAL>
 __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
   constexpr int TT = 8 * NW, E = 8;  // a tile: TT steps x 64 channels, 8 channels of one step a thread
-  __shared__ float2 sd[TT][64];
-  __shared__ float sy[LOCAL ? 1 : NW][LOCAL ? 1 : TT][64];
+  constexpr int G = 16 / NS;         // steps of a unit
+  static_assert(TT % G == 0 && TT % 8 == 0, "tiles are whole units");
+  __shared__ float s_rate[TT + G][64], s_ru[TT + G][64];  // the last unit is only fetched
+  __shared__ float s_y[LOCAL ? 1 : NW][LOCAL ? 1 : TT][64];
   const ms_scan_io& io = a.io;
   const Place at = place(a);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -114,10 +142,11 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
   const int64_t t_begin = at.chunk * a.p.chunk;
   const int64_t t_end = t_begin + a.p.chunk < io.steps ? t_begin + a.p.chunk : io.steps;
   const int64_t cl = at.c0 + lc;
-  const T* u = (const T*)io.u + at.r * io.u_r + cl;
-  const T* dl = (const T*)io.delta + at.r * io.delta_r + cl;
-  const T* z = io.z && !LOCAL ? (const T*)io.z + at.r * io.z_r + cl : nullptr;
-  T* out = (T*)io.out + at.r * io.out_r + cl;
+  const T* u = (const T*)io.u + at.r * io.u_r + cl + (t_begin + lt) * io.u_t;
+  const T* dl = (const T*)io.delta + at.r * io.delta_r + cl + (t_begin + lt) * io.delta_t;
+  const T* z = io.z && !LOCAL ? (const T*)io.z + at.r * io.z_r + cl + (t_begin + lt) * io.z_t : nullptr;
+  T* out = (T*)io.out + at.r * io.out_r + cl + (t_begin + lt) * io.out_t;
+  const int64_t u_step = io.u_t * TT, d_step = io.delta_t * TT, z_step = io.z_t * TT, o_step = io.out_t * TT;
   float bias[E], skip[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -127,13 +156,13 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
   // this lane's channel in the recurrence
   const int64_t ch = at.c0 + lane;
   const bool live = lane < at.nc;
-  const int64_t N = io.states;
+  const int N = io.states;
   float A2[NS], h[NS], total = 0.0f;
   bool was_cut = false;
   const int64_t slot = (at.r * io.channels + ch) * N;  // (R, D, N)
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    const int64_t s = w * NS + i;
+    const int s = w * NS + i;
     A2[i] = live && s < N ? io.A[ch * N + s] * LOG2E : 0.0f;
     h[i] = 0.0f;
     if (!LOCAL && live && s < N) {
@@ -141,68 +170,104 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
       else if (io.state) h[i] = io.state[slot + s];
     }
   }
-  CONSTANT(float)* Bs = (CONSTANT(float)*)(a.Bf + at.r * a.b_r + at.g * a.b_g + w * NS);
-  CONSTANT(float)* Cs = (CONSTANT(float)*)(a.Cf + at.r * a.c_r + at.g * a.c_g + w * NS);
+  CONSTANT(f32x16)* next = scalars_at(a, at.r, at.g, w) + t_begin / G * 2;
+  float* ckpt = !LOCAL && io.checkpoints ? io.checkpoints + checkpoint_at(a, t_begin / KC, at.r, at.td, w * NS, lane) : nullptr;
+  const int64_t ckpt_step = io.rows * a.p.blocks_d * (a.p.ns * a.p.nw / 4) * 256;
+  const int soft = io.softplus;
+  const bool vec = a.vec;
   typedef typename Vec<T, E>::type V;
   V vu, vd, vz;
-  auto fetch = [&](int64_t t) __attribute__((always_inline)) {
-    const bool in = t + lt < t_end;
-    vu = load<T, E>(u + (t + lt) * io.u_t, in ? n : 0, a.vec);
-    vd = load<T, E>(dl + (t + lt) * io.delta_t, in ? n : 0, a.vec);
-    if (z) vz = load<T, E>(z + (t + lt) * io.z_t, in ? n : 0, a.vec);
+  auto fetch = [&](bool in) __attribute__((always_inline)) {
+    vu = load<T, E>(u, in ? n : 0, vec);
+    vd = load<T, E>(dl, in ? n : 0, vec);
+    if (z) vz = load<T, E>(z, in ? n : 0, vec);
+    u += u_step;
+    dl += d_step;
+    if (z) z += z_step;
   };
-  fetch(t_begin);
-  for (int64_t t0 = t_begin; t0 < t_end; t0 += TT) {
+  int left = (int)(t_end - t_begin);  // steps of the chunk not done yet
+  fetch(lt < left);
+  Scalars s = scalars(next);
+  for (int64_t t0 = t_begin; left > 0; t0 += TT, left -= TT) {
     const V cu = vu, cz = vz;
+    const bool mine = lt < left;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float rate = rate_of((float)vd[e] + bias[e], io.softplus);
-      sd[lt][lc + e] = make_float2(rate, rate * (float)cu[e]);
+    for (int e = 0; e < E; ++e) {  // a step past the end has rate 0: it changes nothing
+      float slope, rate = (float)vd[e] + bias[e];
+      if (soft) rate = softplus(rate, slope);
+      rate = mine ? rate : 0.0f;
+      s_rate[lt][lc + e] = rate;
+      s_ru[lt][lc + e] = rate * (float)cu[e];
     }
-    const int64_t t1 = t0 + TT < t_end ? t0 + TT : t_end;
-    const uint64_t starts = start_mask(io, at.r, t0, t1);
+    const uint64_t starts = start_mask(io, at.r, t0, t0 + (left < TT ? left : TT));
     __syncthreads();
-    fetch(t0 + TT);
-    const int steps = (int)(t1 - t0);
-#pragma unroll 4
-    for (int t = 0; t < steps; ++t) {
-      if (!LOCAL && io.checkpoints && ((t0 + t) & (KC - 1)) == 0) {
-        // before step t0 + t: [k][row][tile][wave][NS / 4][64 lanes][4]
-        const int64_t k = (t0 + t) / KC;
-        float* to = io.checkpoints + (((k * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS * 64) + lane * 4;
+    fetch(lt + TT < left);
+    float rate[G], ru[G];
 #pragma unroll
-        for (int i = 0; i < NS; i += 4) *(float4*)(to + i * 64) = make_float4(h[i], h[i + 1], h[i + 2], h[i + 3]);
-      }
-      const float2 v = sd[t][lane];
-      if (starts >> t & 1) {
+    for (int j = 0; j < G; ++j) {
+      rate[j] = s_rate[j][lane];
+      ru[j] = s_ru[j][lane];
+    }
+    const int steps = left < TT ? (left + G - 1) / G * G : TT;
+    for (int t = 0; t < steps; t += G) {
+      if (!LOCAL && ckpt && ((t0 + t) & (KC - 1)) == 0) {  // the states before step t0 + t
 #pragma unroll
-        for (int i = 0; i < NS; ++i) h[i] = 0.0f;
-        if (LOCAL) was_cut = true;
+        for (int i = 0; i < NS; i += 4) *(float4*)(ckpt + i * 64) = make_float4(h[i], h[i + 1], h[i + 2], h[i + 3]);
+        ckpt += ckpt_step;
       }
-      CONSTANT(float)* B = Bs + (t0 + t) * a.b_t;
-      CONSTANT(float)* C = Cs + (t0 + t) * a.c_t;
-      float y = 0.0f;
+      next += 2;
+      const Scalars ns = scalars(next);
+      float nrate[G], nru[G];
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const float decay = __builtin_amdgcn_exp2f(v.x * A2[i]);
-        h[i] = __builtin_fmaf(decay, h[i], v.y * B[i]);
-        if (!LOCAL) y = __builtin_fmaf(C[i], h[i], y);
+      for (int j = 0; j < G; ++j) {
+        nrate[j] = s_rate[t + G + j][lane];
+        nru[j] = s_ru[t + G + j][lane];
       }
-      if (LOCAL) total += v.x;
-      else sy[w][t][lane] = y;
+      __builtin_amdgcn_sched_barrier(0);
+      const unsigned cut = (unsigned)(starts >> t) & ((1u << G) - 1);
+      auto work = [&](auto any) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+          if (decltype(any)::value && (cut >> j & 1)) {
+#pragma unroll
+            for (int i = 0; i < NS; ++i) h[i] = 0.0f;
+            if (LOCAL) was_cut = true;
+          }
+          float y = 0.0f;
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(rate[j] * A2[i]), h[i], ru[j] * s.b[j * NS + i]);
+            if (!LOCAL) y = i ? __builtin_fmaf(s.c[j * NS + i], h[i], y) : s.c[j * NS] * h[0];
+          }
+          if (LOCAL) total += rate[j];
+          else s_y[w][t + j][lane] = y;
+        }
+      };
+      if (cut) work(std::true_type{});
+      else work(std::false_type{});
+      __builtin_amdgcn_sched_barrier(0);
+      s = ns;
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        rate[j] = nrate[j];
+        ru[j] = nru[j];
+      }
     }
     __syncthreads();
-    if (!LOCAL && t0 + lt < t1 && n > 0) {
-      float y[E];
+    if (!LOCAL) {
+      if (mine && n > 0) {
+        float y[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float s = 0.0f;
+        for (int e = 0; e < E; ++e) {
+          float v = s_y[0][lt][lc + e];
 #pragma unroll
-        for (int k = 0; k < NW; ++k) s += sy[k][lt][lc + e];
-        y[e] = __builtin_fmaf(skip[e], (float)cu[e], s);
-        if (z) y[e] *= silu((float)cz[e]);
+          for (int k = 1; k < NW; ++k) v += s_y[k][lt][lc + e];
+          y[e] = __builtin_fmaf(skip[e], (float)cu[e], v);
+          if (z) y[e] *= silu((float)cz[e]);
+        }
+        store<T, E>(out, y, n, vec);
       }
-      store<T, E>(out + (t0 + lt) * io.out_t, y, n, a.vec);
+      out += o_step;
     }
   }
   if (LOCAL) {
@@ -253,7 +318,8 @@ __global__ __launch_bounds__(256) void step4(const ms_scan_io io) {
   const int64_t r = rc / D, c = rc - r * D, g = c / (D / io.groups);
   const float u = (float)((const T*)io.u)[r * io.u_r + c];
   const float d = (float)((const T*)io.delta)[r * io.delta_r + c] + (io.delta_bias ? io.delta_bias[c] : 0.0f);
-  const float rate = rate_of(d, io.softplus), ru = rate * u;
+  float slope;
+  const float rate = io.softplus ? softplus(d, slope) : d, ru = rate * u;
   float4 h = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (io.state && !(io.starts && io.starts[r * io.starts_r])) h = *(const float4*)(io.state + rc * (Q * 4) + q);
   const float4 A = *(const float4*)(io.A + c * (Q * 4) + q);
@@ -286,7 +352,8 @@ __global__ __launch_bounds__(256) void step1(const ms_scan_io io) {
   const int64_t r = rc / D, c = rc - r * D, g = c / (D / io.groups);
   const float u = (float)((const T*)io.u)[r * io.u_r + c];
   const float d = (float)((const T*)io.delta)[r * io.delta_r + c] + (io.delta_bias ? io.delta_bias[c] : 0.0f);
-  const float rate = rate_of(d, io.softplus), ru = rate * u, r2 = rate * LOG2E;
+  float slope;
+  const float rate = io.softplus ? softplus(d, slope) : d, ru = rate * u, r2 = rate * LOG2E;
   const bool fresh = !io.state || (io.starts && io.starts[r * io.starts_r]);
   const T* B = (const T*)io.B + r * io.B_r + g * io.B_g;
   const T* C = (const T*)io.C + r * io.C_r + g * io.C_g;
@@ -350,8 +417,8 @@ __device__ __forceinline__ float fold_steps(const float (&x)[8], int lane) {
 // The first pass of a split time axis: what each chunk hands back from zero.
 template <typename T, int NS, int NW>
 __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
-  constexpr int TT = 8 * NW, E = 8;
-  __shared__ float2 sd[TT][64];  // rate, dy
+  constexpr int TT = 8 * NW, E = 8, G = 4;  // units as the main pass has them: 4 steps of 4 states
+  __shared__ float s_rate[TT][64], s_dy[TT][64];
   const ms_scan_io& io = a.io;
   const Place at = place(a);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -366,7 +433,8 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
   float bias[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) bias[e] = io.delta_bias && e < n ? io.delta_bias[cl + e] : 0.0f;
-  const int64_t ch = at.c0 + lane, N = io.states;
+  const int64_t ch = at.c0 + lane;
+  const int N = io.states;
   const bool live = lane < at.nc;
   float A2[NS], carry[NS], total = 0.0f;
   bool was_cut = false;
@@ -375,38 +443,50 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
     A2[i] = live && w * NS + i < N ? io.A[ch * N + w * NS + i] * LOG2E : 0.0f;
     carry[i] = 0.0f;
   }
-  CONSTANT(float)* Cs = (CONSTANT(float)*)(a.Cf + at.r * a.c_r + at.g * a.c_g + w * NS);
+  CONSTANT(f32x16)* base[NS / 4];
+#pragma unroll
+  for (int q = 0; q < NS / 4; ++q) base[q] = scalars_at(a, at.r, at.g, w * (NS / 4) + q);
   const int64_t tiles = (t_end - t_begin + TT - 1) / TT;
+  const bool vec = a.vec;
   typedef typename Vec<T, E>::type V;
   V vd, vy, vz;
   auto fetch = [&](int64_t t) __attribute__((always_inline)) {
     const bool in = t >= t_begin && t + lt < t_end;
-    vd = load<T, E>(dl + (t + lt) * io.delta_t, in ? n : 0, a.vec);
-    vy = load<T, E>(dy + (t + lt) * io.dout_t, in ? n : 0, a.vec);
-    if (z) vz = load<T, E>(z + (t + lt) * io.z_t, in ? n : 0, a.vec);
+    vd = load<T, E>(dl + (t + lt) * io.delta_t, in ? n : 0, vec);
+    vy = load<T, E>(dy + (t + lt) * io.dout_t, in ? n : 0, vec);
+    if (z) vz = load<T, E>(z + (t + lt) * io.z_t, in ? n : 0, vec);
   };
   fetch(t_begin + (tiles - 1) * TT);
   for (int64_t k = tiles - 1; k >= 0; --k) {
     const int64_t t0 = t_begin + k * TT, t1 = t0 + TT < t_end ? t0 + TT : t_end;
+    const bool mine = t0 + lt < t1;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      sd[lt][lc + e] = make_float2(rate_of((float)vd[e] + bias[e], io.softplus),
-                                   z ? (float)vy[e] * silu((float)vz[e]) : (float)vy[e]);
+    for (int e = 0; e < E; ++e) {
+      float slope, rate = (float)vd[e] + bias[e];
+      if (io.softplus) rate = softplus(rate, slope);
+      s_rate[lt][lc + e] = mine ? rate : 0.0f;
+      s_dy[lt][lc + e] = z ? (float)vy[e] * silu((float)vz[e]) : (float)vy[e];
+    }
     const uint64_t starts = start_mask(io, at.r, t0, t1);
     __syncthreads();
     fetch(t0 - TT);
-#pragma unroll 4
-    for (int t = (int)(t1 - t0) - 1; t >= 0; --t) {
-      const float2 v = sd[t][lane];
-      CONSTANT(float)* C = Cs + (t0 + t) * a.c_t;
-      total += v.x;
+    for (int t = TT - G; t >= 0; t -= G) {
+      f32x16 c[NS / 4];
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
-        carry[i] = __builtin_amdgcn_exp2f(v.x * A2[i]) * __builtin_fmaf(C[i], v.y, carry[i]);
-      if (starts >> t & 1) {
-        was_cut = true;
+      for (int q = 0; q < NS / 4; ++q) c[q] = base[q][(t0 + t) / G * 2 + 1];
+      const unsigned cut = (unsigned)(starts >> t) & 15u;
 #pragma unroll
-        for (int i = 0; i < NS; ++i) carry[i] = 0.0f;
+      for (int j = G - 1; j >= 0; --j) {
+        const float rate = s_rate[t + j][lane], d = s_dy[t + j][lane];
+        total += rate;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+          carry[i] = __builtin_amdgcn_exp2f(rate * A2[i]) * __builtin_fmaf(c[i / 4][j * 4 + i % 4], d, carry[i]);
+        if (cut >> j & 1) {
+          was_cut = true;
+#pragma unroll
+          for (int i = 0; i < NS; ++i) carry[i] = 0.0f;
+        }
       }
     }
     __syncthreads();
@@ -421,8 +501,10 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
   if (threadIdx.x == 0 && at.td == 0) a.cut[at.chunk * io.rows + at.r] = was_cut;
 }
 
+// A tile of 16 steps at a time, four states at a time: first forwards from the checkpoint, keeping
+// a[t] and a[t] h[t - 1] in registers (128 of them), then backwards through them.
 template <typename T, int NS, int NW>
-__global__ __launch_bounds__(64 * NW) void backward(const Args a) {
+__global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
   constexpr int E = KC / NW, TPR = 64 / E;  // 1,024 values of a tile over the threads: E channels each
   __shared__ float s_rate[KC][64], s_ru[KC][64], s_dy[KC][64];
   __shared__ float s_gb[NW][KC][64], s_ga[NW][KC][64], s_y[NW][KC][64];
@@ -433,14 +515,15 @@ __global__ __launch_bounds__(64 * NW) void backward(const Args a) {
   const int n = at.nc - lc < 0 ? 0 : at.nc - lc;
   const int64_t t_begin = at.chunk * a.p.chunk;
   const int64_t t_end = t_begin + a.p.chunk < io.steps ? t_begin + a.p.chunk : io.steps;
-  const int64_t cl = at.c0 + lc;
-  const T* pu = (const T*)io.u + at.r * io.u_r + cl;
-  const T* pd = (const T*)io.delta + at.r * io.delta_r + cl;
-  const T* pz = io.z ? (const T*)io.z + at.r * io.z_r + cl : nullptr;
-  const T* po = (const T*)io.dout + at.r * io.dout_r + cl;
-  T* qu = (T*)io.du + at.r * io.du_r + cl;
-  T* qd = (T*)io.ddelta + at.r * io.ddelta_r + cl;
-  T* qz = io.z ? (T*)io.dz + at.r * io.dz_r + cl : nullptr;
+  const int64_t cl = at.c0 + lc, tiles = (t_end - t_begin + KC - 1) / KC;
+  const int64_t last = t_begin + (tiles - 1) * KC + lt;
+  const T* pu = (const T*)io.u + at.r * io.u_r + cl + last * io.u_t;
+  const T* pd = (const T*)io.delta + at.r * io.delta_r + cl + last * io.delta_t;
+  const T* pz = io.z ? (const T*)io.z + at.r * io.z_r + cl + last * io.z_t : nullptr;
+  const T* po = (const T*)io.dout + at.r * io.dout_r + cl + last * io.dout_t;
+  T* qu = (T*)io.du + at.r * io.du_r + cl + last * io.du_t;
+  T* qd = (T*)io.ddelta + at.r * io.ddelta_r + cl + last * io.ddelta_t;
+  T* qz = io.z ? (T*)io.dz + at.r * io.dz_r + cl + last * io.dz_t : nullptr;
   float bias[E], skip[E], dskip[E], dbias[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -448,13 +531,14 @@ __global__ __launch_bounds__(64 * NW) void backward(const Args a) {
     skip[e] = io.D && e < n ? io.D[cl + e] : 0.0f;
     dskip[e] = dbias[e] = 0.0f;
   }
-  const int64_t ch = at.c0 + lane, N = io.states;
+  const int64_t ch = at.c0 + lane;
+  const int N = io.states;
   const bool live = lane < at.nc;
   const int64_t slot = (at.r * io.channels + ch) * N;
   float A2[NS], carry[NS], dA[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    const int64_t s = w * NS + i;
+    const int s = w * NS + i;
     A2[i] = live && s < N ? io.A[ch * N + s] * LOG2E : 0.0f;
     carry[i] = dA[i] = 0.0f;
     if (live && s < N) {
@@ -462,93 +546,155 @@ __global__ __launch_bounds__(64 * NW) void backward(const Args a) {
       else if (io.dnew_state) carry[i] = io.dnew_state[slot + s];
     }
   }
-  CONSTANT(float)* Bs = (CONSTANT(float)*)(a.Bf + at.r * a.b_r + at.g * a.b_g + w * NS);
-  CONSTANT(float)* Cs = (CONSTANT(float)*)(a.Cf + at.r * a.c_r + at.g * a.c_g + w * NS);
-  const int64_t tiles = (t_end - t_begin + KC - 1) / KC;
+  CONSTANT(f32x16)* base = scalars_at(a, at.r, at.g, w * (NS / 4)) + (t_begin / 4 + (tiles - 1) * 4) * 2;
+  const int64_t share = a.p.units * 2;
+  const int soft = io.softplus;
+  const bool vec = a.vec;
   typedef typename Vec<T, E>::type V;
   V vu, vd, vz, vo;
-  auto fetch = [&](int64_t t) __attribute__((always_inline)) {
-    const bool in = t >= t_begin && t + lt < t_end;
-    vu = load<T, E>(pu + (t + lt) * io.u_t, in ? n : 0, a.vec);
-    vd = load<T, E>(pd + (t + lt) * io.delta_t, in ? n : 0, a.vec);
-    vo = load<T, E>(po + (t + lt) * io.dout_t, in ? n : 0, a.vec);
-    if (pz) vz = load<T, E>(pz + (t + lt) * io.z_t, in ? n : 0, a.vec);
+  auto fetch = [&](bool in) __attribute__((always_inline)) {
+    vu = load<T, E>(pu, in ? n : 0, vec);
+    vd = load<T, E>(pd, in ? n : 0, vec);
+    vo = load<T, E>(po, in ? n : 0, vec);
+    if (pz) vz = load<T, E>(pz, in ? n : 0, vec);
   };
-  fetch(t_begin + (tiles - 1) * KC);
+  fetch(last < t_end);
   for (int64_t k = tiles - 1; k >= 0; --k) {
     const int64_t t0 = t_begin + k * KC, t1 = t0 + KC < t_end ? t0 + KC : t_end;
-    const V cu = vu, cz = vz, co = vo, cd = vd;
+    const V cu = vu, cz = vz, co = vo;
+    const bool mine = t0 + lt < t1;
+    float sig[E], gate[E];  // the slope of the rate, the logistic function of z
 #pragma unroll
     for (int e = 0; e < E; ++e) {  // a step past the end has rate 0 and dy 0: it changes nothing
-      const bool in = t0 + lt < t1;
-      const float rate = in ? rate_of((float)cd[e] + bias[e], io.softplus) : 0.0f;
+      float rate = (float)vd[e] + bias[e];
+      sig[e] = 1.0f;
+      if (soft) rate = softplus(rate, sig[e]);
+      rate = mine ? rate : 0.0f;
+      gate[e] = pz ? sigmoid((float)cz[e]) : 1.0f;
       s_rate[lt][lc + e] = rate;
       s_ru[lt][lc + e] = rate * (float)cu[e];
-      s_dy[lt][lc + e] = pz ? (float)co[e] * silu((float)cz[e]) : (float)co[e];
+      s_dy[lt][lc + e] = pz ? (float)co[e] * ((float)cz[e] * gate[e]) : (float)co[e];
     }
     const uint64_t starts = start_mask(io, at.r, t0, t1);
     __syncthreads();
-    fetch(t0 - KC);
+    pu -= KC * io.u_t;
+    pd -= KC * io.delta_t;
+    po -= KC * io.dout_t;
+    if (pz) pz -= KC * io.z_t;
+    fetch(k > 0);
     const int64_t kk = t0 / KC;
-    const float* from = io.checkpoints + (((kk * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS * 64) + lane * 4;
+    const float* from = io.checkpoints + checkpoint_at(a, kk, at.r, at.td, w * NS, lane);
     float* to = a.parts_bc + ((((kk * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS / 4) * 2) * 64 + lane;
+    auto tile = [&](auto any) __attribute__((always_inline)) {
+      constexpr bool CUTS = decltype(any)::value;
 #pragma unroll
-    for (int nb = 0; nb < NS; nb += 4) {
-      const float4 h0 = *(const float4*)(from + nb * 64);
-      float h[4] = {h0.x, h0.y, h0.z, h0.w};
-      float dec[KC][4], ah[KC][4];  // a[t] and a[t] h[t - 1]
+      for (int nb = 0; nb < NS; nb += 4) {
+        const float4 h0 = *(const float4*)(from + nb * 64);
+        CONSTANT(f32x16)* p = base + (nb >> 2) * share;
+        float h[4] = {h0.x, h0.y, h0.z, h0.w};
+        float dec[KC][4], ah[KC][4];  // a[t] and a[t] h[t - 1]
+        f32x16 b = p[0];
+        float rate[4], ru[4];
 #pragma unroll
-      for (int t = 0; t < KC; ++t) {
-        const float rate = s_rate[t][lane], ru = s_ru[t][lane];
-        const int64_t tt = t0 + t < t1 ? t0 + t : t1 - 1;
-        CONSTANT(float)* B = Bs + tt * a.b_t + nb;
-        if (starts >> t & 1) h[0] = h[1] = h[2] = h[3] = 0.0f;
+        for (int j = 0; j < 4; ++j) {
+          rate[j] = s_rate[j][lane];
+          ru[j] = s_ru[j][lane];
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          dec[t][i] = __builtin_amdgcn_exp2f(rate * A2[nb + i]);
-          ah[t][i] = dec[t][i] * h[i];
-          h[i] = __builtin_fmaf(ru, B[i], ah[t][i]);
+        for (int t4 = 0; t4 < KC; t4 += 4) {
+          const int tn = t4 + 4 < KC ? t4 + 4 : KC - 4;
+          const f32x16 b_next = p[tn / 4 * 2];
+          float rate_next[4], ru_next[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            rate_next[j] = s_rate[tn + j][lane];
+            ru_next[j] = s_ru[tn + j][lane];
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int t = t4 + j;
+            if (CUTS && (starts >> t & 1)) h[0] = h[1] = h[2] = h[3] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              dec[t][i] = __builtin_amdgcn_exp2f(rate[j] * A2[nb + i]);
+              ah[t][i] = dec[t][i] * h[i];
+              h[i] = __builtin_fmaf(ru[j], b[j * 4 + i], ah[t][i]);
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          b = b_next;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            rate[j] = rate_next[j];
+            ru[j] = ru_next[j];
+          }
+        }
+        float steps8[8];
+        Scalars s;
+        s.b = b;
+        s.c = p[7];
+        float dy[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dy[j] = s_dy[KC - 4 + j][lane];
+#pragma unroll
+        for (int t4 = KC - 4; t4 >= 0; t4 -= 4) {
+          const int tp = t4 ? t4 - 4 : 0;
+          const Scalars prev = scalars(p + tp / 4 * 2);
+          float dy_prev[4], rate_prev[4], ru_prev[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            dy_prev[j] = s_dy[tp + j][lane];
+            rate_prev[j] = s_rate[tp + j][lane];
+            ru_prev[j] = s_ru[tp + j][lane];
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 3; j >= 0; --j) {
+            const int t = t4 + j;
+            float gb = 0.0f, ga = 0.0f, y = 0.0f, items[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float B = s.b[j * 4 + i], C = s.c[j * 4 + i];
+              const float g = __builtin_fmaf(C, dy[j], carry[nb + i]);
+              const float hh = __builtin_fmaf(ru[j], B, ah[t][i]);
+              const float q = g * ah[t][i];
+              y = __builtin_fmaf(C, hh, y);
+              gb = __builtin_fmaf(B, g, gb);
+              ga = __builtin_fmaf(q, A2[nb + i], ga);
+              dA[nb + i] = __builtin_fmaf(q, rate[j], dA[nb + i]);
+              carry[nb + i] = dec[t][i] * g;
+              items[i] = ru[j] * g;
+              items[4 + i] = dy[j] * hh;
+            }
+            if (CUTS && (starts >> t & 1)) carry[nb] = carry[nb + 1] = carry[nb + 2] = carry[nb + 3] = 0.0f;
+            if (nb) {
+              gb += s_gb[w][t][lane];
+              ga += s_ga[w][t][lane];
+              y += s_y[w][t][lane];
+            }
+            s_gb[w][t][lane] = gb;
+            s_ga[w][t][lane] = ga;
+            s_y[w][t][lane] = y;
+            steps8[t & 7] = fold_items(items, lane & 8);
+            if ((t & 7) == 0) to[((nb >> 2) * 2 + (t >> 3)) * 64] = fold_steps(steps8, lane);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          s = prev;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            dy[j] = dy_prev[j];
+            rate[j] = rate_prev[j];
+            ru[j] = ru_prev[j];
+          }
         }
       }
-      float steps8[8];
-#pragma unroll
-      for (int t = KC - 1; t >= 0; --t) {
-        const float rate = s_rate[t][lane], ru = s_ru[t][lane], dy = s_dy[t][lane];
-        const int64_t tt = t0 + t < t1 ? t0 + t : t1 - 1;
-        CONSTANT(float)* B = Bs + tt * a.b_t + nb;
-        CONSTANT(float)* C = Cs + tt * a.c_t + nb;
-        float gb = 0.0f, ga = 0.0f, y = 0.0f, items[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float g = __builtin_fmaf(C[i], dy, carry[nb + i]);
-          const float hh = __builtin_fmaf(ru, B[i], ah[t][i]);
-          const float q = g * ah[t][i];
-          y = __builtin_fmaf(C[i], hh, y);
-          gb = __builtin_fmaf(g, B[i], gb);
-          ga = __builtin_fmaf(q, A2[nb + i], ga);
-          dA[nb + i] = __builtin_fmaf(q, rate, dA[nb + i]);
-          carry[nb + i] = dec[t][i] * g;
-          items[i] = ru * g;
-          items[4 + i] = dy * hh;
-        }
-        if (starts >> t & 1) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) carry[nb + i] = 0.0f;
-        }
-        if (nb) {
-          gb += s_gb[w][t][lane];
-          ga += s_ga[w][t][lane];
-          y += s_y[w][t][lane];
-        }
-        s_gb[w][t][lane] = gb;
-        s_ga[w][t][lane] = ga;
-        s_y[w][t][lane] = y;
-        steps8[t & 7] = fold_items(items, lane & 8);
-        if ((t & 7) == 0) to[((nb >> 2) * 2 + (t >> 3)) * 64] = fold_steps(steps8, lane);
-      }
-    }
+    };
+    if (starts) tile(std::true_type{});
+    else tile(std::false_type{});
+    base -= 8;
     __syncthreads();
-    if (t0 + lt < t1 && n > 0) {
+    if (mine && n > 0) {
       float du[E], dd[E], dz[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -559,26 +705,33 @@ __global__ __launch_bounds__(64 * NW) void backward(const Args a) {
           ga += s_ga[i][lt][lc + e];
           y += s_y[i][lt][lc + e];
         }
-        const float uu = (float)cu[e], rate = s_rate[lt][lc + e], dy = s_dy[lt][lc + e];
-        if (pz) dz[e] = (float)co[e] * __builtin_fmaf(skip[e], uu, y) * silu_slope((float)cz[e]);
-        du[e] = __builtin_fmaf(skip[e], dy, rate * gb);
-        const float raw = (float)cd[e] + bias[e];
-        dd[e] = __builtin_fmaf(gb, uu, ga * LN2) * (io.softplus ? sigmoid(raw) : 1.0f);
+        const float uu = (float)cu[e], rt = s_rate[lt][lc + e], dy = s_dy[lt][lc + e];
+        if (pz) {
+          const float zz = (float)cz[e];
+          dz[e] = (float)co[e] * __builtin_fmaf(skip[e], uu, y) * (gate[e] * (1.0f + zz * (1.0f - gate[e])));
+        }
+        du[e] = __builtin_fmaf(skip[e], dy, rt * gb);
+        dd[e] = __builtin_fmaf(gb, uu, ga * LN2) * sig[e];
         dskip[e] = __builtin_fmaf(dy, uu, dskip[e]);
         dbias[e] += dd[e];
       }
-      store<T, E>(qu + (t0 + lt) * io.du_t, du, n, a.vec);
-      store<T, E>(qd + (t0 + lt) * io.ddelta_t, dd, n, a.vec);
-      if (pz) store<T, E>(qz + (t0 + lt) * io.dz_t, dz, n, a.vec);
+      store<T, E>(qu, du, n, vec);
+      store<T, E>(qd, dd, n, vec);
+      if (pz) store<T, E>(qz, dz, n, vec);
     }
+    qu -= KC * io.du_t;
+    qd -= KC * io.ddelta_t;
+    if (pz) qz -= KC * io.dz_t;
     __syncthreads();  // the next tile's stores to s_rate .. s_dy
   }
-  const int64_t part = at.chunk * io.rows + at.r;
+  // this chunk's parts of dA (D, N), dD (D) and ddelta_bias (D), in one row
+  const int64_t D = io.channels;
+  float* part = a.parts + (at.chunk * io.rows + at.r) * D * (N + 2);
   if (live) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
       if (w * NS + i < N) {
-        a.parts_a[(part * io.channels + ch) * N + w * NS + i] = dA[i];
+        part[ch * N + w * NS + i] = dA[i];
         if (io.dstate && t_begin == 0) io.dstate[slot + w * NS + i] = carry[i];
       }
   }
@@ -590,12 +743,24 @@ __global__ __launch_bounds__(64 * NW) void backward(const Args a) {
     for (int e = 0; e < E; ++e) red[lt * 64 + lc + e] = pass ? dbias[e] : dskip[e];
     __syncthreads();
     if (threadIdx.x < 64 && live) {
-      float s = 0.0f;
+      float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < KC; ++i) s += red[i * 64 + lane];
-      a.parts_d[(part * 2 + pass) * io.channels + ch] = s;
+      for (int i = 0; i < KC; ++i) sum += red[i * 64 + lane];
+      part[D * (N + pass) + ch] = sum;
     }
   }
+}
+
+// The second stage of the sums over rows and chunks, put in place: dA, dD, ddelta_bias
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void finish_weights(const float* __restrict__ in, int64_t parts, ms_scan_io io) {
+  __shared__ double s[WAVES][64];
+  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63), D = io.channels, dn = D * io.states;
+  const float sum = (float)sum_share<WAVES>(in, 0, parts, dn + 2 * D, c, s);
+  if (threadIdx.x >= 64) return;
+  if (c < dn) io.dA[c] = sum;
+  else if (c < dn + D) { if (io.dD) io.dD[c - dn] = sum; }
+  else if (c < dn + 2 * D) { if (io.ddelta_bias) io.ddelta_bias[c - dn - D] = sum; }
 }
 
 // dB, dC: the tiles of a group added and put in place. A thread per (t, r, g, n) and kind.
@@ -632,15 +797,17 @@ Plan plan(const ms_scan_io& io, bool back) {
   p.blocks_d = p.tiles * io.groups;
   p.chunks = 1;
   p.chunk = (io.steps + 31) / 32 * 32;
-  (void)back;
   p.kc = (io.steps + KC - 1) / KC;
+  p.unit = back ? 4 : p.ns;
+  // whole tiles of 32 steps, and a unit past the end
+  p.units = (io.steps + 31) / 32 * 32 * p.unit / 16 + 1;
   return p;
 }
 
 int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
 
-// whether B and C can be read where they are: float32, no padding, dwords
-bool direct(const ms_scan_io& io, const Plan& p) { return io.dtype == 0 && io.states == p.ns * p.nw; }
+// how many parts the sums over rows and chunks add in the first of their two stages
+int64_t share_of(int64_t parts) { return parts <= 64 ? parts : parts <= 4096 ? 64 : (parts + 63) / 64; }
 
 Work work(const ms_scan_io& io, const Plan& p, bool back) {
   Work w = {};
@@ -651,8 +818,8 @@ Work work(const ms_scan_io& io, const Plan& p, bool back) {
     used += round4(n);
     return q;
   };
-  const int64_t rd = io.rows * io.channels, parts = p.chunks * io.rows;
-  if (!direct(io, p)) w.bc = take(2 * io.steps * io.rows * io.groups * p.ns * p.nw);
+  const int64_t rd = io.rows * io.channels, parts = p.chunks * io.rows, row = io.channels * (io.states + 2);
+  w.bc = take(io.rows * io.groups * (p.ns * p.nw / p.unit) * p.units * 32);
   if (p.chunks > 1) {
     w.local = take(p.chunks * rd * io.states);
     w.rates = take(p.chunks * rd);
@@ -660,9 +827,9 @@ Work work(const ms_scan_io& io, const Plan& p, bool back) {
   }
   if (back) {
     w.parts_bc = take(p.kc * io.rows * p.blocks_d * p.nw * (p.ns / 4) * 2 * 64);
-    w.parts_a = take(parts * io.channels * io.states);
-    w.parts_d = take(parts * 2 * io.channels);
-    w.sums = take(2 * io.channels);
+    w.parts = take(parts * row);
+    const int64_t share = share_of(parts);
+    w.sums = share ? take((parts + share - 1) / share * row) : nullptr;
   }
   w.floats = used;
   return w;
@@ -704,33 +871,21 @@ bool too_many(int64_t blocks) { return blocks > 0x7fffffff; }
 int prepare(const ms_scan_io& io, const Plan& p, const Work& w, bool back, hipStream_t stream, const char* who, Args& a) {
   a.io = io;
   a.p = p;
+  a.bc = w.bc;
   a.local = w.local;
   a.rates = w.rates;
   a.cut = w.cut;
   a.parts_bc = w.parts_bc;
-  a.parts_a = w.parts_a;
-  a.parts_d = w.parts_d;
+  a.parts = w.parts;
   a.vec = vec_ok(io, back);
-  if (w.bc) {
-    const int np = p.ns * p.nw;
-    const int64_t per = io.steps * io.rows * io.groups * np, blocks = (per + 255) / 256;
-    if (too_many(blocks)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
-    a.Bf = w.bc;
-    a.Cf = w.bc + per;
-    a.b_t = a.c_t = io.rows * io.groups * np;
-    a.b_r = a.c_r = io.groups * np;
-    a.b_g = a.c_g = np;
-    const dim3 grid((unsigned)blocks), block(256);
-    if (io.dtype == 0) hipLaunchKernelGGL(widen<float>, grid, block, 0, stream, io, np, w.bc);
-    else if (io.dtype == 1) hipLaunchKernelGGL(widen<bf16>, grid, block, 0, stream, io, np, w.bc);
-    else hipLaunchKernelGGL(widen<f16>, grid, block, 0, stream, io, np, w.bc);
-    return launched(who);
-  }
-  a.Bf = (const float*)io.B;
-  a.Cf = (const float*)io.C;
-  a.b_t = io.B_t; a.b_r = io.B_r; a.b_g = io.B_g;
-  a.c_t = io.C_t; a.c_r = io.C_r; a.c_g = io.C_g;
-  return MS_OK;
+  const int shares = p.ns * p.nw / p.unit;
+  const int64_t blocks = (io.rows * io.groups * shares * p.units * 32 + 255) / 256;
+  if (too_many(blocks)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
+  const dim3 grid((unsigned)blocks), block(256);
+  if (io.dtype == 0) hipLaunchKernelGGL(widen<float>, grid, block, 0, stream, io, p.unit, shares, p.units, w.bc);
+  else if (io.dtype == 1) hipLaunchKernelGGL(widen<bf16>, grid, block, 0, stream, io, p.unit, shares, p.units, w.bc);
+  else hipLaunchKernelGGL(widen<f16>, grid, block, 0, stream, io, p.unit, shares, p.units, w.bc);
+  return launched(who);
 }
 
 enum Pass { LOCAL, MAIN, BACK_LOCAL, BACK };
@@ -874,14 +1029,11 @@ int ms_scan_backward(const ms_scan_io* io, void* stream) {
   if (io->dtype == 0) hipLaunchKernelGGL(scan::finish_bc<float>, dim3((unsigned)blocks), dim3(256), 0, st, a);
   else if (io->dtype == 1) hipLaunchKernelGGL(scan::finish_bc<seq::bf16>, dim3((unsigned)blocks), dim3(256), 0, st, a);
   else hipLaunchKernelGGL(scan::finish_bc<seq::f16>, dim3((unsigned)blocks), dim3(256), 0, st, a);
-  const int64_t parts = p.chunks * io->rows;
-  hipLaunchKernelGGL((seq::sum_parts<8>), dim3((unsigned)((dn + 63) / 64)), dim3(512), 0, st, w.parts_a, parts, dn, io->dA);
-  if (io->dD || io->ddelta_bias) {
-    hipLaunchKernelGGL((seq::sum_parts<8>), dim3((unsigned)((2 * io->channels + 63) / 64)), dim3(512), 0, st, w.parts_d,
-                       parts, 2 * io->channels, w.sums);
-    if (int rc = scan::copied(w.sums, io->dD ? io->channels : 0, io->dD, st, who)) return rc;
-    if (int rc = scan::copied(w.sums + io->channels, io->ddelta_bias ? io->channels : 0, io->ddelta_bias, st, who)) return rc;
-  }
+  const int64_t parts = p.chunks * io->rows, share = scan::share_of(parts), row = io->channels * (io->states + 2);
+  const unsigned columns = (unsigned)((row + 63) / 64), shares = (unsigned)((parts + share - 1) / share);
+  if (shares > 1)
+    hipLaunchKernelGGL(seq::sum_parts<4>, dim3(columns, shares), dim3(256), 0, st, w.parts, parts, share, row, w.sums);
+  hipLaunchKernelGGL(scan::finish_weights<4>, dim3(columns), dim3(256), 0, st, shares > 1 ? w.sums : w.parts, shares > 1 ? shares : parts, *io);
   return seq::launched(who);
 }
 

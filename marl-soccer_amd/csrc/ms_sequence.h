@@ -62,9 +62,22 @@ __device__ __forceinline__ float silu_slope(float x) {
   const float s = sigmoid(x);
   return s * (1.0f + x * (1.0f - s));
 }
-// log(1 + exp(x)); a NaN stays one
-__device__ __forceinline__ float softplus(float x) {
-  return (x > 0.0f ? x : (x < 0.0f ? 0.0f : x)) + log1pf(exp_f(-__builtin_fabsf(x)));
+// log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|), and its slope, the logistic function of x.
+// log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3: the odd series to s^13 is exact to 2^-25 of the value,
+// for small e too, where log(1 + e) would lose e's digits. A NaN stays one.
+__device__ __forceinline__ float softplus(float x, float& slope) {
+  const float e = exp_f(-__builtin_fabsf(x));
+  const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
+  float p = 1.0f / 13.0f;
+  p = __builtin_fmaf(p, q, 1.0f / 11.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 9.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 7.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 5.0f);
+  p = __builtin_fmaf(p, q, 1.0f / 3.0f);
+  p = __builtin_fmaf(p * q, s, s);
+  const float r = __builtin_amdgcn_rcpf(1.0f + e);
+  slope = x < 0.0f ? e * r : r;
+  return __builtin_fmaf(2.0f, p, x < 0.0f ? 0.0f : x);
 }
 
 inline bool aligned(const void* p, int64_t a, int64_t b, int64_t elem, int64_t vec) {
@@ -83,34 +96,39 @@ inline int launched(const char* who) {
   return e == hipSuccess ? MS_OK : fail(MS_ERR_HIP, who, hipGetErrorString(e));
 }
 
-// Row sums of partial results: out[c] = sum over i < parts of in[i * columns + c], in a fixed order.
-// A block owns 64 columns and its waves share the parts; the sum is held in float64, so the number
-// of parts does not cost precision.
+// Row sums of partial results: out[y][c] = sum of in[i][c] over the y-th share of the parts, in a fixed
+// order. A block owns 64 columns and its waves share the parts of its share; the sum is held in
+// float64, so the number of parts does not cost precision.
 template <int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void sum_parts(const float* __restrict__ in, int64_t parts, int64_t columns,
-                                                        float* __restrict__ out) {
-  __shared__ double s[WAVES][64];
+__device__ __forceinline__ double sum_share(const float* __restrict__ in, int64_t first, int64_t last, int64_t columns,
+                                            int64_t c, double (&s)[WAVES][64]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
   double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
   if (c < columns) {
-    int64_t i = w;
-    for (; i + 3 * WAVES < parts; i += 4 * WAVES) {
+    int64_t i = first + w;
+    for (; i + 3 * WAVES < last; i += 4 * WAVES) {
       a0 += in[i * columns + c];
       a1 += in[(i + WAVES) * columns + c];
       a2 += in[(i + 2 * WAVES) * columns + c];
       a3 += in[(i + 3 * WAVES) * columns + c];
     }
-    for (; i < parts; i += WAVES) a0 += in[i * columns + c];
+    for (; i < last; i += WAVES) a0 += in[i * columns + c];
   }
   s[w][lane] = (a0 + a1) + (a2 + a3);
   __syncthreads();
-  if (w == 0 && c < columns) {
-    double a = 0.0;
+  double a = 0.0;
+  if (w == 0)
 #pragma unroll
     for (int k = 0; k < WAVES; ++k) a += s[k][lane];
-    out[c] = (float)a;
-  }
+  return a;  // the first wave's lanes hold the sums
+}
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void sum_parts(const float* __restrict__ in, int64_t parts, int64_t share,
+                                                        int64_t columns, float* __restrict__ out) {
+  __shared__ double s[WAVES][64];
+  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63), first = blockIdx.y * share;
+  const double a = sum_share<WAVES>(in, first, first + share < parts ? first + share : parts, columns, c, s);
+  if (threadIdx.x < 64 && c < columns) out[blockIdx.y * columns + c] = (float)a;
 }
 
 }  // namespace seq
