@@ -17,7 +17,7 @@
 //     exp(A sum rate)), a small kernel joins the chunks, and the scan proper starts each chunk from
 //     its state. The first pass costs another N exponentials, so chunks are used only then.
 // Backward runs the same tiles from the end: g[t] = C dy + a[t+1] g[t+1]. The states it needs are
-// rebuilt from checkpoints of every KC = 16 steps; dB and dC are sums over channels, folded over the
+// rebuilt from checkpoints of every KC = 8 steps; dB and dC are sums over channels, folded over the
 // wave's lanes with v_permlane swaps and DPP, and over the channel blocks by a last kernel.
 #include <type_traits>
 
@@ -26,7 +26,18 @@
 namespace scan {
 using namespace seq;
 
-constexpr int KC = 16;     // steps between checkpoints, and a tile of the backward pass
+constexpr int KC = 8;  // steps between checkpoints
+#ifdef MS_TUNE
+#include <stdlib.h>
+static int64_t tune(const char* n, int64_t d) { const char* v = getenv(n); return v ? atoll(v) : d; }
+#define TUNE_SPLIT tune(back ? "T_BSPLIT" : "T_SPLIT", 192)
+#define TUNE_TARGET tune(back ? "T_BTARGET" : "T_TARGET", 768)
+#define TUNE_MINP tune("T_MINP", 4)
+#else
+#define TUNE_SPLIT 192
+#define TUNE_TARGET 768
+#define TUNE_MINP 4
+#endif
 constexpr float LOG2E = 1.44269504f, LN2 = 0.69314718f;
 
 #define CONSTANT(T) const __attribute__((address_space(4))) T
@@ -38,7 +49,7 @@ struct Plan {
   int64_t units;            // scalar units along time (of all steps, and one more that is only fetched)
   int64_t tiles, blocks_d;  // tiles per group, tiles * groups
   int64_t chunks, chunk;    // over time; steps per chunk (a multiple of 32)
-  int64_t kc;               // checkpoints
+  int64_t kc, bt;           // checkpoints; tiles of 16 steps of the backward pass
 };
 
 struct Work {  // the workspace, in floats
@@ -90,9 +101,17 @@ __device__ __forceinline__ CONSTANT(f32x16)* scalars_at(const Args& a, int64_t r
   const int shares = a.p.ns * a.p.nw / a.p.unit;
   return (CONSTANT(f32x16)*)(a.bc + ((r * a.io.groups + g) * shares + share) * a.p.units * 32);
 }
-// the checkpoint of step 16 k: [k][row][tile][states / 4][64 channels][4]
+// Every LDS and scalar load issued so far has returned. Scalar loads return in no order, so a wait for
+// any of them is a wait for all: the one for a unit's operands has to stand before the next unit's
+// loads are issued, or it would wait for those too.
+__device__ __forceinline__ void loads_done() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0), the others unbounded
+  __builtin_amdgcn_sched_barrier(0);
+}
+// the checkpoint of step KC k: [k][row][tile][states / 4][64 channels][4]
 __device__ __forceinline__ int64_t checkpoint_at(const Args& a, int64_t k, int64_t r, int64_t td, int state, int lane) {
-  return (((k * a.io.rows + r) * a.p.blocks_d + td) * (a.p.ns * a.p.nw / 4) + state / 4) * 256 + lane * 4;
+  return (((k * a.io.rows + r) * a.p.blocks_d + td) * (a.p.ns * a.p.nw / 4) + state / 4) * 256 + lane * 4 + state % 4;
 }
 
 // Which steps of a tile begin an episode, as a mask the whole wave shares
@@ -129,15 +148,15 @@ __device__ __forceinline__ Place place(const Args& a) {
 // one, since scalar loads return in no order and one wait covers them all.
 template <typename T, int NS, int NW, bool LOCAL>
 __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
-  constexpr int TT = 8 * NW, E = 8;  // a tile: TT steps x 64 channels, 8 channels of one step a thread
-  constexpr int G = 16 / NS;         // steps of a unit
+  constexpr int TT = NW < 4 ? 8 * NW : 32, E = TT / NW, TPR = 64 / E;  // a tile: TT steps x 64 channels, E channels of one step a thread
+  constexpr int G = 16 / NS;                                          // steps of a unit
   static_assert(TT % G == 0 && TT % 8 == 0, "tiles are whole units");
   __shared__ float s_rate[TT + G][64], s_ru[TT + G][64];  // the last unit is only fetched
   __shared__ float s_y[LOCAL ? 1 : NW][LOCAL ? 1 : TT][64];
   const ms_scan_io& io = a.io;
   const Place at = place(a);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lt = threadIdx.x >> 3, lc = (threadIdx.x & 7) * 8;  // this thread's step and channels in loads
+  const int lt = threadIdx.x / TPR, lc = threadIdx.x % TPR * E;  // this thread's step and channels in loads
   const int n = at.nc - lc < 0 ? 0 : at.nc - lc;
   const int64_t t_begin = at.chunk * a.p.chunk;
   const int64_t t_end = t_begin + a.p.chunk < io.steps ? t_begin + a.p.chunk : io.steps;
@@ -171,7 +190,8 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
     }
   }
   CONSTANT(f32x16)* next = scalars_at(a, at.r, at.g, w) + t_begin / G * 2;
-  float* ckpt = !LOCAL && io.checkpoints ? io.checkpoints + checkpoint_at(a, t_begin / KC, at.r, at.td, w * NS, lane) : nullptr;
+  const bool keep = !LOCAL && io.checkpoints;
+  float* ckpt = io.checkpoints + (keep ? checkpoint_at(a, t_begin / KC, at.r, at.td, w * NS, lane) : 0);
   const int64_t ckpt_step = io.rows * a.p.blocks_d * (a.p.ns * a.p.nw / 4) * 256;
   const int soft = io.softplus;
   const bool vec = a.vec;
@@ -210,11 +230,16 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
     }
     const int steps = left < TT ? (left + G - 1) / G * G : TT;
     for (int t = 0; t < steps; t += G) {
-      if (!LOCAL && ckpt && ((t0 + t) & (KC - 1)) == 0) {  // the states before step t0 + t
+      if (keep && (((int)t0 + t) & (KC - 1)) == 0) {  // the states before step t0 + t
+        if constexpr (NS == 2) {
+          *(float2*)ckpt = make_float2(h[0], h[1]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < NS; i += 4) *(float4*)(ckpt + i * 64) = make_float4(h[i], h[i + 1], h[i + 2], h[i + 3]);
+          for (int i = 0; i < NS; i += 4) *(float4*)(ckpt + i * 64) = make_float4(h[i], h[i + 1], h[i + 2], h[i + 3]);
+        }
         ckpt += ckpt_step;
       }
+      loads_done();
       next += 2;
       const Scalars ns = scalars(next);
       float nrate[G], nru[G];
@@ -298,12 +323,24 @@ __global__ __launch_bounds__(256) void join(const Args a) {
   const float A2 = io.A[c * N + (i - rc * N)] * LOG2E;
   const float* first = BACK ? io.dnew_state : io.state;
   float h = first ? first[i] : 0.0f;
-  for (int64_t k = 0; k < a.p.chunks; ++k) {
-    const int64_t q = BACK ? a.p.chunks - 1 - k : k;
-    const float mine = a.local[q * all + i];
-    const float decay = __builtin_amdgcn_exp2f(A2 * a.rates[q * io.rows * io.channels + rc]);
-    a.local[q * all + i] = h;
-    h = a.cut[q * io.rows + r] ? mine : __builtin_fmaf(decay, h, mine);
+  const int64_t chunks = a.p.chunks, rd = io.rows * io.channels;
+  for (int64_t k0 = 0; k0 < chunks; k0 += 8) {  // eight chunks' loads in flight
+    float mine[8], rate[8];
+    int cut[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t k = k0 + j < chunks ? k0 + j : chunks - 1, q = BACK ? chunks - 1 - k : k;
+      mine[j] = a.local[q * all + i];
+      rate[j] = a.rates[q * rd + rc];
+      cut[j] = a.cut[q * io.rows + r];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (k0 + j >= chunks) break;
+      const int64_t q = BACK ? chunks - 1 - (k0 + j) : k0 + j;
+      a.local[q * all + i] = h;
+      h = cut[j] ? mine[j] : __builtin_fmaf(__builtin_amdgcn_exp2f(A2 * rate[j]), h, mine[j]);
+    }
   }
 }
 
@@ -501,13 +538,14 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
   if (threadIdx.x == 0 && at.td == 0) a.cut[at.chunk * io.rows + at.r] = was_cut;
 }
 
-// A tile of 16 steps at a time, four states at a time: first forwards from the checkpoint, keeping
-// a[t] and a[t] h[t - 1] in registers (128 of them), then backwards through them.
+// A tile of 16 steps at a time, in it the KC steps from a checkpoint and four states at a time: first
+// forwards, keeping a[t] and a[t] h[t - 1] in registers (64 of them), then backwards through them. With
+// 16 steps between checkpoints they would be 128, and the kernel would spill.
 template <typename T, int NS, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
-  constexpr int E = KC / NW, TPR = 64 / E;  // 1,024 values of a tile over the threads: E channels each
-  __shared__ float s_rate[KC][64], s_ru[KC][64], s_dy[KC][64];
-  __shared__ float s_gb[NW][KC][64], s_ga[NW][KC][64], s_y[NW][KC][64];
+  constexpr int TT = NW == 1 ? 8 : 16, E = TT / NW, TPR = 64 / E;  // a tile's values over the threads: E channels each
+  __shared__ float s_rate[TT][64], s_ru[TT][64], s_dy[TT][64];
+  __shared__ float s_gb[NW][TT][64], s_ga[NW][TT][64], s_y[NW][TT][64];
   const ms_scan_io& io = a.io;
   const Place at = place(a);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -515,8 +553,8 @@ __global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
   const int n = at.nc - lc < 0 ? 0 : at.nc - lc;
   const int64_t t_begin = at.chunk * a.p.chunk;
   const int64_t t_end = t_begin + a.p.chunk < io.steps ? t_begin + a.p.chunk : io.steps;
-  const int64_t cl = at.c0 + lc, tiles = (t_end - t_begin + KC - 1) / KC;
-  const int64_t last = t_begin + (tiles - 1) * KC + lt;
+  const int64_t cl = at.c0 + lc, tiles = (t_end - t_begin + TT - 1) / TT;
+  const int64_t last = t_begin + (tiles - 1) * TT + lt;
   const T* pu = (const T*)io.u + at.r * io.u_r + cl + last * io.u_t;
   const T* pd = (const T*)io.delta + at.r * io.delta_r + cl + last * io.delta_t;
   const T* pz = io.z ? (const T*)io.z + at.r * io.z_r + cl + last * io.z_t : nullptr;
@@ -546,7 +584,7 @@ __global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
       else if (io.dnew_state) carry[i] = io.dnew_state[slot + s];
     }
   }
-  CONSTANT(f32x16)* base = scalars_at(a, at.r, at.g, w * (NS / 4)) + (t_begin / 4 + (tiles - 1) * 4) * 2;
+  CONSTANT(f32x16)* base = scalars_at(a, at.r, at.g, w * (NS / 4)) + (t_begin + (tiles - 1) * TT) / 4 * 2;
   const int64_t share = a.p.units * 2;
   const int soft = io.softplus;
   const bool vec = a.vec;
@@ -560,7 +598,7 @@ __global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
   };
   fetch(last < t_end);
   for (int64_t k = tiles - 1; k >= 0; --k) {
-    const int64_t t0 = t_begin + k * KC, t1 = t0 + KC < t_end ? t0 + KC : t_end;
+    const int64_t t0 = t_begin + k * TT, t1 = t0 + TT < t_end ? t0 + TT : t_end;
     const V cu = vu, cz = vz, co = vo;
     const bool mine = t0 + lt < t1;
     float sig[E], gate[E];  // the slope of the rate, the logistic function of z
@@ -577,122 +615,132 @@ __global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
     }
     const uint64_t starts = start_mask(io, at.r, t0, t1);
     __syncthreads();
-    pu -= KC * io.u_t;
-    pd -= KC * io.delta_t;
-    po -= KC * io.dout_t;
-    if (pz) pz -= KC * io.z_t;
+    pu -= TT * io.u_t;
+    pd -= TT * io.delta_t;
+    po -= TT * io.dout_t;
+    if (pz) pz -= TT * io.z_t;
     fetch(k > 0);
-    const int64_t kk = t0 / KC;
-    const float* from = io.checkpoints + checkpoint_at(a, kk, at.r, at.td, w * NS, lane);
-    float* to = a.parts_bc + ((((kk * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS / 4) * 2) * 64 + lane;
+    const int64_t ckpt_step = io.rows * a.p.blocks_d * (NS * NW / 4) * 256;
+    const float* from = io.checkpoints + checkpoint_at(a, t0 / KC, at.r, at.td, w * NS, lane);
+    float* to = a.parts_bc + ((((t0 / 16 * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS / 4) * 2 + (t0 / 8 & 1)) * 64 + lane;
     auto tile = [&](auto any) __attribute__((always_inline)) {
       constexpr bool CUTS = decltype(any)::value;
 #pragma unroll
       for (int nb = 0; nb < NS; nb += 4) {
-        const float4 h0 = *(const float4*)(from + nb * 64);
-        CONSTANT(f32x16)* p = base + (nb >> 2) * share;
-        float h[4] = {h0.x, h0.y, h0.z, h0.w};
-        float dec[KC][4], ah[KC][4];  // a[t] and a[t] h[t - 1]
-        f32x16 b = p[0];
-        float rate[4], ru[4];
+        for (int half = TT / KC - 1; half >= 0; --half) {
+          const int t0h = half * KC;
+          if (t0 + t0h >= t1) {  // no steps there, and no checkpoint
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          rate[j] = s_rate[j][lane];
-          ru[j] = s_ru[j][lane];
-        }
-#pragma unroll
-        for (int t4 = 0; t4 < KC; t4 += 4) {
-          const int tn = t4 + 4 < KC ? t4 + 4 : KC - 4;
-          const f32x16 b_next = p[tn / 4 * 2];
-          float rate_next[4], ru_next[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            rate_next[j] = s_rate[tn + j][lane];
-            ru_next[j] = s_ru[tn + j][lane];
+            for (int j = 0; j < KC; ++j) s_gb[w][t0h + j][lane] = s_ga[w][t0h + j][lane] = s_y[w][t0h + j][lane] = 0.0f;
+            continue;
           }
-          __builtin_amdgcn_sched_barrier(0);
+          const float4 h0 = *(const float4*)(from + half * ckpt_step + nb * 64);
+          CONSTANT(f32x16)* p = base + (nb >> 2) * share + half * (KC / 4 * 2);
+          float h[4] = {h0.x, h0.y, h0.z, h0.w};
+          float dec[KC][4], ah[KC][4];  // a[t] and a[t] h[t - 1]
+          f32x16 b = p[0];
+          float rate[4], ru[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int t = t4 + j;
-            if (CUTS && (starts >> t & 1)) h[0] = h[1] = h[2] = h[3] = 0.0f;
+            rate[j] = s_rate[t0h + j][lane];
+            ru[j] = s_ru[t0h + j][lane];
+          }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              dec[t][i] = __builtin_amdgcn_exp2f(rate[j] * A2[nb + i]);
-              ah[t][i] = dec[t][i] * h[i];
-              h[i] = __builtin_fmaf(ru[j], b[j * 4 + i], ah[t][i]);
+          for (int t4 = 0; t4 < KC; t4 += 4) {
+            loads_done();
+            const int tn = t4 + 4 < KC ? t4 + 4 : KC - 4;
+            const f32x16 b_next = p[tn / 4 * 2];
+            float rate_next[4], ru_next[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              rate_next[j] = s_rate[t0h + tn + j][lane];
+              ru_next[j] = s_ru[t0h + tn + j][lane];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int t = t4 + j;
+              if (CUTS && (starts >> (t0h + t) & 1)) h[0] = h[1] = h[2] = h[3] = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                dec[t][i] = __builtin_amdgcn_exp2f(rate[j] * A2[nb + i]);
+                ah[t][i] = dec[t][i] * h[i];
+                h[i] = __builtin_fmaf(ru[j], b[j * 4 + i], ah[t][i]);
+              }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            b = b_next;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              rate[j] = rate_next[j];
+              ru[j] = ru_next[j];
             }
           }
-          __builtin_amdgcn_sched_barrier(0);
-          b = b_next;
+          float steps8[8];
+          Scalars s;
+          s.b = b;
+          s.c = p[KC / 4 * 2 - 1];
+          float dy[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            rate[j] = rate_next[j];
-            ru[j] = ru_next[j];
-          }
-        }
-        float steps8[8];
-        Scalars s;
-        s.b = b;
-        s.c = p[7];
-        float dy[4];
+          for (int j = 0; j < 4; ++j) dy[j] = s_dy[t0h + KC - 4 + j][lane];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dy[j] = s_dy[KC - 4 + j][lane];
+          for (int t4 = KC - 4; t4 >= 0; t4 -= 4) {
+            loads_done();
+            const int tp = t4 ? t4 - 4 : 0;
+            const Scalars prev = scalars(p + tp / 4 * 2);
+            float dy_prev[4], rate_prev[4], ru_prev[4];
 #pragma unroll
-        for (int t4 = KC - 4; t4 >= 0; t4 -= 4) {
-          const int tp = t4 ? t4 - 4 : 0;
-          const Scalars prev = scalars(p + tp / 4 * 2);
-          float dy_prev[4], rate_prev[4], ru_prev[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            dy_prev[j] = s_dy[tp + j][lane];
-            rate_prev[j] = s_rate[tp + j][lane];
-            ru_prev[j] = s_ru[tp + j][lane];
-          }
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int j = 3; j >= 0; --j) {
-            const int t = t4 + j;
-            float gb = 0.0f, ga = 0.0f, y = 0.0f, items[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float B = s.b[j * 4 + i], C = s.c[j * 4 + i];
-              const float g = __builtin_fmaf(C, dy[j], carry[nb + i]);
-              const float hh = __builtin_fmaf(ru[j], B, ah[t][i]);
-              const float q = g * ah[t][i];
-              y = __builtin_fmaf(C, hh, y);
-              gb = __builtin_fmaf(B, g, gb);
-              ga = __builtin_fmaf(q, A2[nb + i], ga);
-              dA[nb + i] = __builtin_fmaf(q, rate[j], dA[nb + i]);
-              carry[nb + i] = dec[t][i] * g;
-              items[i] = ru[j] * g;
-              items[4 + i] = dy[j] * hh;
+            for (int j = 0; j < 4; ++j) {
+              dy_prev[j] = s_dy[t0h + tp + j][lane];
+              rate_prev[j] = s_rate[t0h + tp + j][lane];
+              ru_prev[j] = s_ru[t0h + tp + j][lane];
             }
-            if (CUTS && (starts >> t & 1)) carry[nb] = carry[nb + 1] = carry[nb + 2] = carry[nb + 3] = 0.0f;
-            if (nb) {
-              gb += s_gb[w][t][lane];
-              ga += s_ga[w][t][lane];
-              y += s_y[w][t][lane];
-            }
-            s_gb[w][t][lane] = gb;
-            s_ga[w][t][lane] = ga;
-            s_y[w][t][lane] = y;
-            steps8[t & 7] = fold_items(items, lane & 8);
-            if ((t & 7) == 0) to[((nb >> 2) * 2 + (t >> 3)) * 64] = fold_steps(steps8, lane);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          s = prev;
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            dy[j] = dy_prev[j];
-            rate[j] = rate_prev[j];
-            ru[j] = ru_prev[j];
+            for (int j = 3; j >= 0; --j) {
+              const int t = t4 + j;
+              float gb = 0.0f, ga = 0.0f, y = 0.0f, items[8];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float B = s.b[j * 4 + i], C = s.c[j * 4 + i];
+                const float g = __builtin_fmaf(C, dy[j], carry[nb + i]);
+                const float hh = __builtin_fmaf(ru[j], B, ah[t][i]);
+                const float q = g * ah[t][i];
+                y = i ? __builtin_fmaf(C, hh, y) : C * hh;
+                gb = i ? __builtin_fmaf(B, g, gb) : B * g;
+                ga = i ? __builtin_fmaf(q, A2[nb + i], ga) : q * A2[nb];
+                dA[nb + i] = __builtin_fmaf(q, rate[j], dA[nb + i]);
+                carry[nb + i] = dec[t][i] * g;
+                items[i] = ru[j] * g;
+                items[4 + i] = dy[j] * hh;
+              }
+              if (CUTS && (starts >> (t0h + t) & 1)) carry[nb] = carry[nb + 1] = carry[nb + 2] = carry[nb + 3] = 0.0f;
+              if (nb) {
+                gb += s_gb[w][t0h + t][lane];
+                ga += s_ga[w][t0h + t][lane];
+                y += s_y[w][t0h + t][lane];
+              }
+              s_gb[w][t0h + t][lane] = gb;
+              s_ga[w][t0h + t][lane] = ga;
+              s_y[w][t0h + t][lane] = y;
+              steps8[t] = fold_items(items, lane & 8);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            s = prev;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              dy[j] = dy_prev[j];
+              rate[j] = rate_prev[j];
+              ru[j] = ru_prev[j];
+            }
           }
+          to[((nb >> 2) * 2 + half) * 64] = fold_steps(steps8, lane);
         }
       }
     };
     if (starts) tile(std::true_type{});
     else tile(std::false_type{});
-    base -= 8;
+    base -= TT / 4 * 2;
     __syncthreads();
     if (mine && n > 0) {
       float du[E], dd[E], dz[E];
@@ -719,9 +767,9 @@ __global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
       store<T, E>(qd, dd, n, vec);
       if (pz) store<T, E>(qz, dz, n, vec);
     }
-    qu -= KC * io.du_t;
-    qd -= KC * io.ddelta_t;
-    if (pz) qz -= KC * io.dz_t;
+    qu -= TT * io.du_t;
+    qd -= TT * io.ddelta_t;
+    if (pz) qz -= TT * io.dz_t;
     __syncthreads();  // the next tile's stores to s_rate .. s_dy
   }
   // this chunk's parts of dA (D, N), dD (D) and ddelta_bias (D), in one row
@@ -745,7 +793,7 @@ __global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
     if (threadIdx.x < 64 && live) {
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < KC; ++i) sum += red[i * 64 + lane];
+      for (int i = 0; i < TT; ++i) sum += red[i * 64 + lane];
       part[D * (N + pass) + ch] = sum;
     }
   }
@@ -780,8 +828,8 @@ __global__ __launch_bounds__(256) void finish_bc(const Args a) {
   const int64_t ns = a.p.ns, w = s / ns, nb = s % ns / 4;
   const int64_t lane = (kind * 4 + s % 4) * 8 + t % 8;
   const int64_t one = a.p.nw * (ns / 4) * 2 * 64;  // a tile's floats
-  const float* p = a.parts_bc + ((t / KC * io.rows + r) * a.p.blocks_d + g * a.p.tiles) * one +
-                   ((w * (ns / 4) + nb) * 2 + t % KC / 8) * 64 + lane;
+  const float* p = a.parts_bc + ((t / 16 * io.rows + r) * a.p.blocks_d + g * a.p.tiles) * one +
+                   ((w * (ns / 4) + nb) * 2 + t % 16 / 8) * 64 + lane;
   float sum = 0.0f;
   for (int64_t j = 0; j < a.p.tiles; ++j) sum += p[j * one];
   ((T*)(kind ? io.dC : io.dB))[i] = (T)sum;
@@ -791,13 +839,22 @@ __global__ __launch_bounds__(256) void finish_bc(const Args a) {
 
 Plan plan(const ms_scan_io& io, bool back) {
   Plan p = {};
-  p.ns = io.states <= 16 ? 4 : io.states <= 32 ? 8 : 16;
-  p.nw = io.states <= 4 ? 1 : io.states <= 8 ? 2 : 4;
   p.tiles = (io.channels / io.groups + 63) / 64;
   p.blocks_d = p.tiles * io.groups;
-  p.chunks = 1;
-  p.chunk = (io.steps + 31) / 32 * 32;
+  const int64_t blocks = p.blocks_d * io.rows;
+  const int np = io.states <= 4 ? 4 : io.states <= 8 ? 8 : io.states <= 16 ? 16 : io.states <= 32 ? 32 : 64;
+  p.ns = np <= 16 ? 4 : np / 4;
+  if (!back && np == 16 && blocks > 192 && blocks <= 256) p.ns = 2;
+  p.nw = np / p.ns;
+  const int64_t pieces = (io.steps + 31) / 32;
+  int64_t chunks = blocks > 0 && blocks <= TUNE_SPLIT ? (TUNE_TARGET + blocks - 1) / blocks : 1;
+  if (chunks > pieces / TUNE_MINP) chunks = pieces / TUNE_MINP;
+  if (chunks < 1) chunks = 1;
+  p.chunk = (pieces + chunks - 1) / chunks * 32;
+  p.chunk = p.chunk < 32 ? 32 : p.chunk;
+  p.chunks = io.steps > 0 ? (io.steps + p.chunk - 1) / p.chunk : 1;
   p.kc = (io.steps + KC - 1) / KC;
+  p.bt = (io.steps + 15) / 16;
   p.unit = back ? 4 : p.ns;
   // whole tiles of 32 steps, and a unit past the end
   p.units = (io.steps + 31) / 32 * 32 * p.unit / 16 + 1;
@@ -826,7 +883,7 @@ Work work(const ms_scan_io& io, const Plan& p, bool back) {
     w.cut = (int*)take(parts);
   }
   if (back) {
-    w.parts_bc = take(p.kc * io.rows * p.blocks_d * p.nw * (p.ns / 4) * 2 * 64);
+    w.parts_bc = take(p.bt * io.rows * p.blocks_d * p.nw * (p.ns / 4) * 2 * 64);
     w.parts = take(parts * row);
     const int64_t share = share_of(parts);
     w.sums = share ? take((parts + share - 1) / share * row) : nullptr;
@@ -900,7 +957,8 @@ void launch_as(Pass pass, const Args& a, dim3 grid, hipStream_t stream) {
 }
 template <typename T>
 void launch_type(Pass pass, const Args& a, dim3 grid, hipStream_t stream) {
-  if (a.p.nw == 1) launch_as<T, 4, 1>(pass, a, grid, stream);
+  if (a.p.nw == 8) hipLaunchKernelGGL((forward<T, 2, 8, false>), grid, dim3(512), 0, stream, a);  // never split
+  else if (a.p.nw == 1) launch_as<T, 4, 1>(pass, a, grid, stream);
   else if (a.p.nw == 2) launch_as<T, 4, 2>(pass, a, grid, stream);
   else if (a.p.ns == 4) launch_as<T, 4, 4>(pass, a, grid, stream);
   else if (a.p.ns == 8) launch_as<T, 8, 4>(pass, a, grid, stream);

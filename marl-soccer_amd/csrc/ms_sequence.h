@@ -48,32 +48,32 @@ __device__ __forceinline__ void store(T* p, const float (&x)[E], int n, bool vec
   }
 }
 
-// exp(x) with the rounding of x log2(e) carried along: v_exp_f32 alone loses |x| 2^-24 of the value
-__device__ __forceinline__ float exp_f(float x) {
-  const float hi = x * 1.44269504f;
-  const float lo = __builtin_fmaf(x, 1.44269504f, -hi) + x * 1.92596299e-8f;
-  const float e = __builtin_amdgcn_exp2f(hi);
-  // beyond the range of float hi is infinite and lo is not a number: the power alone is the answer
-  return __builtin_fabsf(hi) < 150.0f ? __builtin_fmaf(e * 0.69314718f, lo, e) : e;
+// 1 / (1 + exp(-x)) and its product with x. The argument is held where exp is finite; a NaN is lost
+// here and comes back with x in every use. v_exp_f32's argument is rounded, which costs |x| 2^-24 of
+// exp: less than a unit in the last place of the result where it is not small.
+__device__ __forceinline__ float sigmoid(float x) {
+  const float t = __builtin_amdgcn_fmed3f(x * -1.44269504f, -126.0f, 126.0f);
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
 }
-__device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_f(-x)); }
 __device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
 __device__ __forceinline__ float silu_slope(float x) {
   const float s = sigmoid(x);
   return s * (1.0f + x * (1.0f - s));
 }
 // log(1 + exp(x)) = max(x, 0) + log1p(e), e = exp(-|x|), and its slope, the logistic function of x.
-// log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3: the odd series to s^13 is exact to 2^-25 of the value,
-// for small e too, where log(1 + e) would lose e's digits. A NaN stays one.
+// exp carries the rounding of its argument along (a state's decay feels it at every step). log1p(e) =
+// 2 atanh(s), s = e / (2 + e) <= 1/3, by a polynomial in s^2 fitted on Chebyshev nodes, exact to
+// 2^-25 of the value for small e too, where log(1 + e) would lose e's digits. A NaN stays one.
 __device__ __forceinline__ float softplus(float x, float& slope) {
-  const float e = exp_f(-__builtin_fabsf(x));
+  const float y = fminf(__builtin_fabsf(x), 87.0f), hi = y * -1.44269504f;
+  const float lo = __builtin_fmaf(y, -1.92596299e-8f, __builtin_fmaf(y, -1.44269504f, -hi));
+  float e = __builtin_amdgcn_exp2f(hi);
+  e = __builtin_fmaf(e * 0.69314718f, lo, e);
   const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
-  float p = 1.0f / 13.0f;
-  p = __builtin_fmaf(p, q, 1.0f / 11.0f);
-  p = __builtin_fmaf(p, q, 1.0f / 9.0f);
-  p = __builtin_fmaf(p, q, 1.0f / 7.0f);
-  p = __builtin_fmaf(p, q, 1.0f / 5.0f);
-  p = __builtin_fmaf(p, q, 1.0f / 3.0f);
+  float p = 0.134337768f;
+  p = __builtin_fmaf(p, q, 0.141169772f);
+  p = __builtin_fmaf(p, q, 0.200038359f);
+  p = __builtin_fmaf(p, q, 0.333333194f);
   p = __builtin_fmaf(p * q, s, s);
   const float r = __builtin_amdgcn_rcpf(1.0f + e);
   slope = x < 0.0f ? e * r : r;
