@@ -25,14 +25,18 @@ struct Shape {  // the launch: a block covers `cols` groups of E channels and `s
   int64_t groups, spans, span, items, blocks_c, blocks_p;
 };
 
-template <typename T, int E, int W>
-__global__ __launch_bounds__(THREADS) void forward(const ms_conv_io io, const Shape sh, bool vec) {
+// FULL: every access is E aligned channels, so the loads of BATCH steps are issued together without a
+// branch between them; otherwise they are guarded value by value.
+constexpr int BATCH = 4;
+template <typename T, int E, int W, bool FULL>
+__global__ __launch_bounds__(THREADS) void forward(const ms_conv_io io, const Shape sh) {
   const int cols = 1 << sh.cols_log2, slots = THREADS >> sh.cols_log2;
   const int64_t group = (int64_t)(blockIdx.x % sh.blocks_c) * cols + (threadIdx.x & (cols - 1));
   const int64_t item = (int64_t)(blockIdx.x / sh.blocks_c) * slots + (threadIdx.x >> sh.cols_log2);
   if (group >= sh.groups || item >= sh.items) return;
   const int64_t c = group * E, D = io.channels;
-  const int n = (int)(D - c < E ? D - c : E);
+  constexpr bool vec = FULL;
+  const int n = FULL ? E : (int)(D - c < E ? D - c : E);
   const int64_t r = item % io.rows, t0 = item / io.rows * sh.span;
   const int64_t t1 = t0 + sh.span < io.steps ? t0 + sh.span : io.steps;
   const T* x = (const T*)io.x + r * io.x_r + c;
@@ -66,10 +70,12 @@ __global__ __launch_bounds__(THREADS) void forward(const ms_conv_io io, const Sh
 #pragma unroll
     for (int e = 0; e < E; ++e) win[k][e] = (float)v[e];
   }
-#pragma unroll 4
-  for (int64_t t = t0; t < t1; ++t) {
-    const typename Vec<T, E>::type v = load<T, E>(x + t * io.x_t, n, vec);
-    if (starts && starts[t * io.starts_t]) {
+  const T* px = x + t0 * io.x_t;
+  T* po = out + t0 * io.out_t;
+  const uint8_t* ps = starts ? starts + t0 * io.starts_t : nullptr;
+  const bool act = io.silu;
+  auto step = [&](const typename Vec<T, E>::type& v, bool cut) __attribute__((always_inline)) {
+    if (cut) {
 #pragma unroll
       for (int j = 0; j < W - 1; ++j)
 #pragma unroll
@@ -82,12 +88,33 @@ __global__ __launch_bounds__(THREADS) void forward(const ms_conv_io io, const Sh
 #pragma unroll
       for (int k = 0; k < W - 1; ++k) a = __builtin_fmaf(w[k][e], win[k][e], a);
       a = __builtin_fmaf(w[W - 1][e], (float)v[e], a);
-      y[e] = io.silu ? silu(a) : a;
+      y[e] = act ? silu(a) : a;
 #pragma unroll
       for (int k = 0; k < W - 2; ++k) win[k][e] = win[k + 1][e];
       win[W - 2][e] = (float)v[e];
     }
-    store<T, E>(out + t * io.out_t, y, n, vec);
+    store<T, E>(po, y, n, vec);
+    po += io.out_t;
+  };
+  int64_t t = t0;
+  for (; t + BATCH <= t1; t += BATCH) {
+    typename Vec<T, E>::type v[BATCH];
+    bool cut[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      v[k] = load<T, E>(px, n, vec);
+      px += io.x_t;
+      cut[k] = ps && ps[k * io.starts_t];
+    }
+    if (ps) ps += BATCH * io.starts_t;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) step(v[k], cut[k]);
+  }
+  for (; t < t1; ++t) {
+    const typename Vec<T, E>::type v = load<T, E>(px, n, vec);
+    px += io.x_t;
+    step(v, ps && ps[0]);
+    if (ps) ps += io.starts_t;
   }
   if (io.new_state && t1 == io.steps) {
     T* ns = (T*)io.new_state + r * (W - 1) * D + c;
@@ -99,15 +126,15 @@ __global__ __launch_bounds__(THREADS) void forward(const ms_conv_io io, const Sh
 // p[t] reaches dx of steps t - W + 1 .. t: pend[j] collects dx[t - j], complete (and stored) when it
 // falls out of the window. reach: how many steps back belong to step t's episode. A span stores the
 // steps of its own and runs W - 1 steps past them, whose p counts for dx but not for dw and db.
-template <typename T, int E, int W>
-__global__ __launch_bounds__(THREADS) void backward(const ms_conv_io io, const Shape sh, bool vec,
-                                                    float* __restrict__ parts) {
+template <typename T, int E, int W, bool FULL>
+__global__ __launch_bounds__(THREADS) void backward(const ms_conv_io io, const Shape sh, float* __restrict__ parts) {
+  constexpr bool vec = FULL;
   __shared__ float red[THREADS];
   const int cols = 1 << sh.cols_log2, slots = THREADS >> sh.cols_log2;
   const int64_t bc = blockIdx.x % sh.blocks_c, bp = blockIdx.x / sh.blocks_c;
   const int col = threadIdx.x & (cols - 1), slot = threadIdx.x >> sh.cols_log2;
   const int64_t group = bc * cols + col, D = io.channels, c = group * E;
-  const int n = group < sh.groups ? (int)(D - c < E ? D - c : E) : 0;
+  const int n = group >= sh.groups ? 0 : FULL ? E : (int)(D - c < E ? D - c : E);
   float w[W][E], b[E], dw[W][E], db[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -154,24 +181,24 @@ __global__ __launch_bounds__(THREADS) void backward(const ms_conv_io io, const S
         pend[k][e] = 0.0f;
       }
     }
+    const bool act = io.silu;
     // after the W - 1 steps before t0, reach counts how many of the steps t0 - 1, t0 - 2, ... belong
     // to step t0 - 1's episode (that step itself not counted)
     auto flush = [&](int64_t t, const float (&g)[E]) __attribute__((always_inline)) {  // dx[t] is complete
       if (t >= t0 && t < t1) store<T, E>(dx + t * io.dx_t, g, n, vec);
       if (t < 0 && t0 == 0 && io.dstate) store<T, E>((T*)io.dstate + row + (W - 1 + t) * D, g, n, vec);
     };
-#pragma unroll 2
-    for (int64_t t = t0; t < t2; ++t) {
-      const typename Vec<T, E>::type v = load<T, E>(x + t * io.x_t, n, vec);
-      const typename Vec<T, E>::type d = load<T, E>(dout + t * io.dout_t, n, vec);
+    const int m = FULL ? E : n;
+    auto step = [&](int64_t t, const typename Vec<T, E>::type& v, const typename Vec<T, E>::type& d, bool cut) __attribute__((always_inline)) {
       reach = reach < W - 1 ? reach + 1 : W - 1;
-      if (starts && starts[t * io.starts_t]) {
+      if (cut) {
         reach = 0;
 #pragma unroll
         for (int j = 0; j < W - 1; ++j)
 #pragma unroll
           for (int e = 0; e < E; ++e) win[j][e] = 0.0f;
       }
+      const bool own = t < t1;
       float done[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -179,8 +206,8 @@ __global__ __launch_bounds__(THREADS) void backward(const ms_conv_io io, const S
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) a = __builtin_fmaf(w[k][e], win[k][e], a);
         a = __builtin_fmaf(w[W - 1][e], (float)v[e], a);
-        const float p = io.silu ? (float)d[e] * silu_slope(a) : (float)d[e];
-        if (t < t1) {
+        const float p = act ? (float)d[e] * silu_slope(a) : (float)d[e];
+        if (own) {
           db[e] += p;
 #pragma unroll
           for (int k = 0; k < W - 1; ++k) dw[k][e] = __builtin_fmaf(p, win[k][e], dw[k][e]);
@@ -198,6 +225,32 @@ __global__ __launch_bounds__(THREADS) void backward(const ms_conv_io io, const S
         win[W - 2][e] = (float)v[e];
       }
       flush(t - (W - 1), done);
+    };
+    const T* px = x + t0 * io.x_t;
+    const T* pd = dout + t0 * io.dout_t;
+    const uint8_t* ps = starts ? starts + t0 * io.starts_t : nullptr;
+    int64_t t = t0;
+    for (; t + BATCH <= t2; t += BATCH) {
+      typename Vec<T, E>::type v[BATCH], d[BATCH];
+      bool cut[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        v[k] = load<T, E>(px, m, vec);
+        d[k] = load<T, E>(pd, m, vec);
+        px += io.x_t;
+        pd += io.dout_t;
+        cut[k] = ps && ps[k * io.starts_t];
+      }
+      if (ps) ps += BATCH * io.starts_t;
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) step(t + k, v[k], d[k], cut[k]);
+    }
+    for (; t < t2; ++t) {
+      const typename Vec<T, E>::type v = load<T, E>(px, m, vec), d = load<T, E>(pd, m, vec);
+      px += io.x_t;
+      pd += io.dout_t;
+      step(t, v, d, ps && ps[0]);
+      if (ps) ps += io.starts_t;
     }
     if (t2 == io.steps) {  // the last steps, and the gradient of the state handed on
 #pragma unroll
@@ -228,17 +281,20 @@ __global__ __launch_bounds__(THREADS) void backward(const ms_conv_io io, const S
     }
 }
 
-// parts (P, D, W + 1) -> dweight (D, W), dbias (D)
-__global__ __launch_bounds__(256) void finish(const float* __restrict__ sums, int64_t D, int W, float* __restrict__ dweight,
-                                              float* __restrict__ dbias) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= D * (W + 1)) return;
-  const int64_t d = i / (W + 1);
-  const int k = (int)(i - d * (W + 1));
+// parts (P, D, W + 1) added up -> dweight (D, W), dbias (D)
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void finish(const float* __restrict__ in, int64_t parts, int64_t D, int W,
+                                                     float* __restrict__ dweight, float* __restrict__ dbias) {
+  __shared__ double s[WAVES][64];
+  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const float sum = (float)sum_share<WAVES>(in, 0, parts, D * (W + 1), c, s);
+  if (threadIdx.x >= 64 || c >= D * (W + 1)) return;
+  const int64_t d = c / (W + 1);
+  const int k = (int)(c - d * (W + 1));
   if (k < W) {
-    if (dweight) dweight[d * W + k] = sums[i];
+    if (dweight) dweight[d * W + k] = sum;
   } else if (dbias) {
-    dbias[d] = sums[i];
+    dbias[d] = sum;
   }
 }
 
@@ -286,35 +342,32 @@ const char* check(const ms_conv_io* io, bool back) {
   return nullptr;
 }
 
-template <typename T, int E>
-int run_forward(const ms_conv_io& io, const Shape& s, bool vec, hipStream_t stream) {
+template <typename T, int E, bool FULL>
+int run_forward(const ms_conv_io& io, const Shape& s, hipStream_t stream) {
   const int64_t blocks = s.blocks_c * s.blocks_p;
   if (blocks > 0x7fffffff) return fail(MS_ERR_INVALID_ARGUMENT, "ms_conv_forward", "too large");
   const dim3 grid((unsigned)blocks), block(THREADS);
   switch (io.width) {
-    case 2: hipLaunchKernelGGL((forward<T, E, 2>), grid, block, 0, stream, io, s, vec); break;
-    case 3: hipLaunchKernelGGL((forward<T, E, 3>), grid, block, 0, stream, io, s, vec); break;
-    default: hipLaunchKernelGGL((forward<T, E, 4>), grid, block, 0, stream, io, s, vec); break;
+    case 2: hipLaunchKernelGGL((forward<T, E, 2, FULL>), grid, block, 0, stream, io, s); break;
+    case 3: hipLaunchKernelGGL((forward<T, E, 3, FULL>), grid, block, 0, stream, io, s); break;
+    default: hipLaunchKernelGGL((forward<T, E, 4, FULL>), grid, block, 0, stream, io, s); break;
   }
   return launched("ms_conv_forward");
 }
-template <typename T, int E>
-int run_backward(const ms_conv_io& io, const Shape& s, bool vec, hipStream_t stream) {
+template <typename T, int E, bool FULL>
+int run_backward(const ms_conv_io& io, const Shape& s, hipStream_t stream) {
   const dim3 grid((unsigned)(s.blocks_c * s.blocks_p)), block(THREADS);
   float* parts = (float*)io.workspace;
   const int64_t columns = io.channels * (io.width + 1);
-  float* sums = parts + s.blocks_p * columns;
   switch (io.width) {
-    case 2: hipLaunchKernelGGL((backward<T, E, 2>), grid, block, 0, stream, io, s, vec, parts); break;
-    case 3: hipLaunchKernelGGL((backward<T, E, 3>), grid, block, 0, stream, io, s, vec, parts); break;
-    default: hipLaunchKernelGGL((backward<T, E, 4>), grid, block, 0, stream, io, s, vec, parts); break;
+    case 2: hipLaunchKernelGGL((backward<T, E, 2, FULL>), grid, block, 0, stream, io, s, parts); break;
+    case 3: hipLaunchKernelGGL((backward<T, E, 3, FULL>), grid, block, 0, stream, io, s, parts); break;
+    default: hipLaunchKernelGGL((backward<T, E, 4, FULL>), grid, block, 0, stream, io, s, parts); break;
   }
   if (int rc = launched("ms_conv_backward")) return rc;
   if (!io.dweight && !io.dbias) return MS_OK;
-  hipLaunchKernelGGL((sum_parts<8>), dim3((unsigned)((columns + 63) / 64)), dim3(512), 0, stream, parts, s.blocks_p,
-                     s.blocks_p, columns, sums);
-  hipLaunchKernelGGL(finish, dim3((unsigned)((columns + 255) / 256)), dim3(256), 0, stream, sums, io.channels, io.width,
-                     io.dweight, io.dbias);
+  hipLaunchKernelGGL(finish<16>, dim3((unsigned)((columns + 63) / 64)), dim3(1024), 0, stream, parts, s.blocks_p, io.channels,
+                     io.width, io.dweight, io.dbias);
   return launched("ms_conv_backward");
 }
 
@@ -337,15 +390,16 @@ int ms_conv_forward(const ms_conv_io* io, void* stream) {
   const bool vec = seq::aligned(io->x, io->x_t, io->x_r, elem, E) && seq::aligned(io->out, io->out_t, io->out_r, elem, E) &&
                    conv::state_aligned(*io, elem, E);
   const hipStream_t st = (hipStream_t)stream;
-  if (io->dtype == 0) return conv::run_forward<float, 4>(*io, s, vec, st);
-  if (io->dtype == 1) return conv::run_forward<seq::bf16, 8>(*io, s, vec, st);
-  return conv::run_forward<seq::f16, 8>(*io, s, vec, st);
+  const bool full = vec && io->channels % E == 0;
+  if (io->dtype == 0) return full ? conv::run_forward<float, 4, true>(*io, s, st) : conv::run_forward<float, 4, false>(*io, s, st);
+  if (io->dtype == 1) return full ? conv::run_forward<seq::bf16, 8, true>(*io, s, st) : conv::run_forward<seq::bf16, 8, false>(*io, s, st);
+  return full ? conv::run_forward<seq::f16, 8, true>(*io, s, st) : conv::run_forward<seq::f16, 8, false>(*io, s, st);
 }
 
 int64_t ms_conv_workspace(const ms_conv_io* io) {
   if (conv::check(io, true)) return 0;
   const conv::Shape s = conv::shape(*io, true);
-  return (s.blocks_p + 1) * io->channels * (io->width + 1) * (int64_t)sizeof(float);
+  return s.blocks_p * io->channels * (io->width + 1) * (int64_t)sizeof(float);
 }
 
 int ms_conv_backward(const ms_conv_io* io, void* stream) {
@@ -358,9 +412,10 @@ int ms_conv_backward(const ms_conv_io* io, void* stream) {
   const bool vec = seq::aligned(io->x, io->x_t, io->x_r, elem, E) && seq::aligned(io->dout, io->dout_t, io->dout_r, elem, E) &&
                    seq::aligned(io->dx, io->dx_t, io->dx_r, elem, E) && conv::state_aligned(*io, elem, E);
   const hipStream_t st = (hipStream_t)stream;
-  if (io->dtype == 0) return conv::run_backward<float, 4>(*io, s, vec, st);
-  if (io->dtype == 1) return conv::run_backward<seq::bf16, 8>(*io, s, vec, st);
-  return conv::run_backward<seq::f16, 8>(*io, s, vec, st);
+  const bool full = vec && io->channels % E == 0;
+  if (io->dtype == 0) return full ? conv::run_backward<float, 4, true>(*io, s, st) : conv::run_backward<float, 4, false>(*io, s, st);
+  if (io->dtype == 1) return full ? conv::run_backward<seq::bf16, 8, true>(*io, s, st) : conv::run_backward<seq::bf16, 8, false>(*io, s, st);
+  return full ? conv::run_backward<seq::f16, 8, true>(*io, s, st) : conv::run_backward<seq::f16, 8, false>(*io, s, st);
 }
 
 }  // extern "C"

@@ -13,6 +13,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
+#ifdef MS_TUNE
+#include <stdlib.h>
+#endif
 
 #include "../../include/marl_soccer.h"
 
@@ -22,7 +25,10 @@ namespace opt {
 
 constexpr int THREADS = 256, E = 4, ROUND = THREADS * E;  // values a block handles at a time
 constexpr int LIST = MS_OPTIM_TENSORS;
-constexpr int64_t NORM_BLOCKS = 1024;
+#ifndef MS_NB
+#define MS_NB 1024
+#endif
+constexpr int64_t NORM_BLOCKS = MS_NB;
 static_assert(ROUND % MS_ADAMW_BLOCK == 0 && MS_ADAMW_BLOCK == 64 * E, "a wave's round is one scale block");
 
 typedef __bf16 bf16;
@@ -124,6 +130,25 @@ __device__ __forceinline__ void put_codes(uint8_t* p, int64_t i, int64_t n, bool
     if (i + k < n) p[i + k] = (uint8_t)(c >> (8 * k));
 }
 
+// the largest of the wave's values, in every lane: within rows of 16 by DPP, across them by swaps
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+template <int CTRL>
+__device__ __forceinline__ float max_dpp(float x) {
+  return fmaxf(x, __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = max_dpp<0x128>(x);  // row_ror:8, 4, 2, 1
+  x = max_dpp<0x124>(x);
+  x = max_dpp<0x122>(x);
+  x = max_dpp<0x121>(x);
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const unsigned a0 = a.x, a1 = a.y;
+  x = fmaxf(__uint_as_float(a0), __uint_as_float(a1));
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const unsigned b0 = b.x, b1 = b.y;
+  return fmaxf(__uint_as_float(b0), __uint_as_float(b1));
+}
+
 // Eight bits for a moment: a wave's 256 values share the scale max|.| / 448, so the largest is held
 // to a unit in the last place of float32 and the others to e4m3's half step, 2^-4 of the value, down
 // to 2^-16 of the largest. The second moment is held as its root, which halves the range it spans. A
@@ -133,8 +158,7 @@ __device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_l
   float top = 0.0f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) top = fmaxf(top, __builtin_fabsf(v[k]));
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
+  top = wave_max(top);
   const bool some = top >= 7.8886090522101181e-31f;
   const float inv = some ? 448.0f / top : 0.0f;
   if (first_lane) *scale = some ? top / 448.0f : 0.0f;
@@ -145,88 +169,152 @@ __device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_l
 
 __device__ __forceinline__ bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 
+// b^t by squaring, in float64: off by about t 2^-53 of itself, far below the float32 it ends in
+__device__ __forceinline__ double power(double b, int64_t t) {
+  double p = 1.0;
+  for (; t > 0; t >>= 1) {
+    if (t & 1) p *= b;
+    b *= b;
+  }
+  return p;
+}
+
+// What all of a tensor's blocks share: the step size and the root's factor of step t
+struct Factors {
+  float fix1, fix2, keep, clip;
+};
+
+struct Moments {
+  f32x4 m, v;
+};
+
 template <int BITS>
 __global__ __launch_bounds__(THREADS) void adamw(const List list, const Hyper hp, const Ws ws) {
-  int k = 0;
-  while (blockIdx.x >= list.end[k]) ++k;  // the last end is the grid's size
+  __shared__ Factors shared;
+  // this block's tensor: as many as end at or before it come before it (the last end is the grid's size)
+  const int lane = threadIdx.x & 63;
+  const int k = __popcll(__ballot(lane < list.count && blockIdx.x >= list.end[lane]));
   const ms_optim_tensor& a = list.t[k];
   const int64_t block = blockIdx.x - (k ? list.end[k - 1] : 0), n = a.numel;
-  const int64_t t = *(volatile int64_t*)a.step + 1;
-  const double lr = hp.lr_device ? (double)*hp.lr_device : hp.lr;
-  const float fix1 = (float)(lr / (1.0 - pow(hp.beta1, (double)t)));
-  const float fix2 = (float)(1.0 / sqrt(1.0 - pow(hp.beta2, (double)t)));
-  const float keep = (float)(1.0 - lr * hp.weight_decay);
-  const float clip = hp.use_clip ? ws.f[0] : 1.0f;
-  const int size = a.dtype == 0 ? 16 : 8;
+  const int dtype = a.dtype, size = dtype == 0 ? 16 : 8;
   const bool vp = aligned(a.param, size), vg = aligned(a.grad, size);
   const bool vs = BITS == 32 ? aligned(a.exp_avg, 16) && aligned(a.exp_avg_sq, 16)
                              : aligned(a.exp_avg, 4) && aligned(a.exp_avg_sq, 4);
-  const int64_t begin = block * list.rounds * ROUND;
-  for (int j = 0; j < list.rounds; ++j) {
-    const int64_t i = begin + (int64_t)j * ROUND + threadIdx.x * E;
-    // whole waves leave together: the 64 lanes of a wave take one scale block
-    if (begin + (int64_t)j * ROUND + (threadIdx.x & ~63) * E >= n) break;
-    const f32x4 p = get_any(a.param, a.dtype, i, n, vp);
-    f32x4 g = get_any(a.grad, a.dtype, i, n, vg), m, v, r;
-    const int64_t q = i / MS_ADAMW_BLOCK;
-    if (BITS == 32) {
-      m = get4<f32x4>((const float*)a.exp_avg, i, n, vs);
-      v = get4<f32x4>((const float*)a.exp_avg_sq, i, n, vs);
+  const int64_t begin = block * list.rounds * ROUND + threadIdx.x * E;
+  f32x4 p, g;
+  Moments s;
+  float ms = 0.0f, vs8 = 0.0f;
+  uint32_t mc = 0, vc = 0;
+  auto fetch = [&](int64_t i) __attribute__((always_inline)) {
+    p = get_any(a.param, dtype, i, n, vp);
+    g = get_any(a.grad, dtype, i, n, vg);
+    if constexpr (BITS == 32) {
+      s.m = get4<f32x4>((const float*)a.exp_avg, i, n, vs);
+      s.v = get4<f32x4>((const float*)a.exp_avg_sq, i, n, vs);
     } else {
-      m = decode(get_codes((const uint8_t*)a.exp_avg, i, n, vs)) * a.exp_avg_scale[q];
-      r = decode(get_codes((const uint8_t*)a.exp_avg_sq, i, n, vs)) * a.exp_avg_sq_scale[q];
+      mc = get_codes((const uint8_t*)a.exp_avg, i, n, vs);
+      vc = get_codes((const uint8_t*)a.exp_avg_sq, i, n, vs);
+      const int64_t q = i / MS_ADAMW_BLOCK;
+      ms = a.exp_avg_scale[q];
+      vs8 = a.exp_avg_sq_scale[q];
+    }
+  };
+  // whole waves work or leave: the 64 lanes of a wave take one scale block
+  const bool some = begin - lane * E < n;
+  if (some) fetch(begin);
+  if (threadIdx.x < 64) {  // one wave's float64 arithmetic, under the first loads
+    const int64_t t = *(volatile int64_t*)a.step + 1;
+    const double lr = hp.lr_device ? (double)*hp.lr_device : hp.lr;
+    Factors f;
+    f.fix1 = (float)(lr / (1.0 - power(hp.beta1, t)));
+    f.fix2 = (float)(1.0 / sqrt(1.0 - power(hp.beta2, t)));
+    f.keep = (float)(1.0 - lr * hp.weight_decay);
+    f.clip = hp.use_clip ? ws.f[0] : 1.0f;
+    if (threadIdx.x == 0) shared = f;
+  }
+  __syncthreads();
+  const Factors f = shared;
+  for (int j = 0; some && j < list.rounds; ++j) {
+    const int64_t i = begin + (int64_t)j * ROUND;
+    if (i - lane * E >= n) break;
+    const f32x4 p0 = p;
+    f32x4 g0 = g, m, v, r;
+    if constexpr (BITS == 32) {
+      m = s.m;
+      v = s.v;
+    } else {
+      m = decode(mc) * ms;
+      r = decode(vc) * vs8;
       v = r * r;
     }
-    if (hp.use_clip) g = g * clip;
-    m = m * hp.b1 + g * hp.c1;
-    v = v * hp.b2 + g * g * hp.c2;
+    if (j + 1 < list.rounds && i + ROUND - lane * E < n) fetch(i + ROUND);  // the next round's loads under this one's arithmetic
+    if (hp.use_clip) g0 = g0 * f.clip;
+    m = m * hp.b1 + g0 * hp.c1;
+    v = v * hp.b2 + g0 * g0 * hp.c2;
     f32x4 to;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       r[e] = sqrtf(v[e]);
-      to[e] = p[e] * keep - fix1 * m[e] / (r[e] * fix2 + hp.eps);
+      to[e] = p0[e] * f.keep - f.fix1 * m[e] / (r[e] * f.fix2 + hp.eps);
     }
-    put_any(a.param, a.dtype, i, n, vp, to);
-    if (BITS == 32) {
+    put_any(a.param, dtype, i, n, vp, to);
+    if constexpr (BITS == 32) {
       put4<f32x4>((float*)a.exp_avg, i, n, vs, m);
       put4<f32x4>((float*)a.exp_avg_sq, i, n, vs, v);
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e)
         if (i + e >= n) m[e] = r[e] = 0.0f;  // values past the end count for no scale
-      const bool lane0 = (threadIdx.x & 63) == 0;
-      put_codes((uint8_t*)a.exp_avg, i, n, vs, quantise(m, a.exp_avg_scale + q, lane0));
-      put_codes((uint8_t*)a.exp_avg_sq, i, n, vs, quantise(r, a.exp_avg_sq_scale + q, lane0));
+      const int64_t q = i / MS_ADAMW_BLOCK;
+      put_codes((uint8_t*)a.exp_avg, i, n, vs, quantise(m, a.exp_avg_scale + q, lane == 0));
+      put_codes((uint8_t*)a.exp_avg_sq, i, n, vs, quantise(r, a.exp_avg_sq_scale + q, lane == 0));
     }
   }
-  // every block has read its count by its ticket; the last one raises them all
+  // every block has read its count (and used it) by its ticket; the last one raises them all. The ticket
+  // orders nothing else, so it is relaxed: with release and acquire each block would write back and
+  // invalidate its XCD's L2, 60 ns a block one after the other.
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const unsigned got = __hip_atomic_fetch_add(ws.ticket(), 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    if (got == gridDim.x - 1) {
-      for (int i = 0; i < list.count; ++i) *list.t[i].step += 1;
-      __hip_atomic_store(ws.ticket(), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (threadIdx.x < 64) {
+    unsigned got = 0;
+    if (lane == 0) got = __hip_atomic_fetch_add(ws.ticket(), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__builtin_amdgcn_readfirstlane((int)got) == (int)gridDim.x - 1) {
+      if (lane < list.count) *list.t[lane].step += 1;
+      if (lane == 0) __hip_atomic_store(ws.ticket(), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
+}
+
+// four rounds' loads in flight at a time
+template <typename T4, typename T>
+__device__ __forceinline__ double squares(const T* p, int64_t i, int64_t n, int rounds, bool vec) {
+  double sum = 0.0;
+  for (int j = 0; j < rounds; j += 4) {
+    f32x4 g[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) g[k] = get4<T4>(p, i + (int64_t)(j + k) * ROUND, j + k < rounds ? n : 0, vec);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += (double)g[k][e] * (double)g[k][e];
+  }
+  return sum;
 }
 
 __global__ __launch_bounds__(THREADS) void norm(const NormList list, double max_norm, float* grad_norm, const Ws ws) {
   __shared__ double s[THREADS];
   __shared__ bool last;
   double sum = 0.0;
-  int k = 0;
+  const int lane = threadIdx.x & 63;
   for (uint32_t b = blockIdx.x; b < list.blocks; b += gridDim.x) {
-    while (b >= list.end[k]) ++k;
+    const int k = __popcll(__ballot(lane < list.count && b >= list.end[lane]));
     const int64_t n = list.numel[k];
-    const bool vec = aligned(list.grad[k], list.dtype[k] == 0 ? 16 : 8);
-    const int64_t begin = (int64_t)(b - (k ? list.end[k - 1] : 0)) * list.rounds * ROUND;
-    for (int j = 0; j < list.rounds; ++j) {
-      const int64_t i = begin + (int64_t)j * ROUND + threadIdx.x * E;
-      if (i >= n) break;
-      const f32x4 g = get_any(list.grad[k], list.dtype[k], i, n, vec);
-#pragma unroll
-      for (int e = 0; e < E; ++e) sum += (double)g[e] * (double)g[e];
-    }
+    const int dtype = list.dtype[k];
+    const void* g = list.grad[k];
+    const bool vec = aligned(g, dtype == 0 ? 16 : 8);
+    const int64_t i = (int64_t)(b - (k ? list.end[k - 1] : 0)) * list.rounds * ROUND + threadIdx.x * E;
+    if (dtype == 0) sum += squares<f32x4>((const float*)g, i, n, list.rounds, vec);
+    else if (dtype == 1) sum += squares<bf16x4>((const bf16*)g, i, n, list.rounds, vec);
+    else sum += squares<f16x4>((const f16*)g, i, n, list.rounds, vec);
   }
   s[threadIdx.x] = sum;
   __syncthreads();
@@ -235,8 +323,12 @@ __global__ __launch_bounds__(THREADS) void norm(const NormList list, double max_
     __syncthreads();
   }
   if (threadIdx.x == 0) {
+    // the part goes through to where every XCD sees it (an agent-scope store) and has arrived (the wait)
+    // before the ticket is taken; the last block reads the parts the same way. Release and acquire on
+    // the ticket would write back and invalidate the L2 for every block, for nothing else's sake.
     __hip_atomic_store(ws.parts() + blockIdx.x, s[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last = __hip_atomic_fetch_add(ws.norm_ticket(), 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    last = __hip_atomic_fetch_add(ws.norm_ticket(), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
   }
   __syncthreads();
   if (!last) return;
@@ -285,7 +377,10 @@ const char* check(const ms_optim_tensor* t, int64_t count, const float* workspac
 int rounds(const ms_optim_tensor* t, int64_t count) {
   int64_t all = 0;
   for (int64_t i = 0; i < count; ++i) all += t[i].numel;
-  return all > (int64_t)ROUND * 4096 ? 4 : 1;
+#ifdef MS_TUNE
+  if (const char* v = getenv("T_ROUNDS")) return atoi(v);
+#endif
+  return all > (int64_t)ROUND * 16384 ? 8 : all > (int64_t)ROUND * 4096 ? 4 : 1;
 }
 
 }  // namespace opt

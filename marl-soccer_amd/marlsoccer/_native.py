@@ -193,13 +193,12 @@ def lib():
         L.ms_rollout_record.argtypes = [I64, P, P, P, P, P, P, P, P, P, P]
         L.ms_rollout_record.restype = C.c_int
     if hasattr(L, "ms_scan_forward"):  # likewise
-        for fn, io in (("ms_conv_forward", MsConvIO), ("ms_conv_backward", MsConvIO), ("ms_scan_forward", MsScanIO),
-                       ("ms_scan_step", MsScanIO), ("ms_scan_backward", MsScanIO)):
-            getattr(L, fn).argtypes = [C.POINTER(io), P]
+        for fn in ("ms_conv_forward", "ms_conv_backward", "ms_scan_forward", "ms_scan_step", "ms_scan_backward"):
+            getattr(L, fn).argtypes = [P, P]  # an ms_*_io: a reference to the Structure, or its packed bytes
             getattr(L, fn).restype = C.c_int
-        L.ms_conv_workspace.argtypes = [C.POINTER(MsConvIO)]
-        L.ms_scan_checkpoints.argtypes = [C.POINTER(MsScanIO)]
-        L.ms_scan_workspace.argtypes = [C.POINTER(MsScanIO), C.c_int]
+        L.ms_conv_workspace.argtypes = [P]
+        L.ms_scan_checkpoints.argtypes = [P]
+        L.ms_scan_workspace.argtypes = [P, C.c_int]
         for fn in ("ms_conv_workspace", "ms_scan_checkpoints", "ms_scan_workspace"):
             getattr(L, fn).restype = I64
         L.ms_sequence_last_error.restype = C.c_char_p
@@ -215,6 +214,17 @@ def lib():
         getattr(L, fn).restype = C.c_int
     _lib = L
     return L
+
+
+def on_current_stream(index: int, fn, *args) -> int:
+    """fn(*args, the current stream of device `index`) with that device current: its status."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    stream = raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
+    if torch.cuda.current_device() == index:
+        return fn(*args, stream)
+    with torch.cuda.device(index):
+        return fn(*args, stream)
 
 
 def check(rc: int, what: str = "") -> None:

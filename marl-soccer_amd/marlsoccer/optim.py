@@ -17,6 +17,10 @@ memory counts.
 """
 from __future__ import annotations
 
+import struct
+from itertools import chain, repeat
+from operator import attrgetter
+
 import torch
 
 from . import _native as N
@@ -48,45 +52,60 @@ def _bad(name, want):
     raise ValueError(f"adamw_step: {name} must be {want}")
 
 
+_ROW = "6QQq2i"  # ms_optim_tensor
+_ROW_BYTES = struct.calcsize("<" + _ROW)
+_KIND, _DTYPE = attrgetter("dtype", "shape"), attrgetter("dtype")
+_where, _ptr_of, _numel, _packed = (getattr(torch.Tensor, k) for k in ("get_device", "data_ptr", "numel", "is_contiguous"))
+
+
 def _entries(params, grads, exp_avg, exp_avg_sq, steps, scales, sq_scales):
-    """The checked list as ms_optim_tensor rows."""
-    bits8 = scales is not None
-    n, device = len(params), None
+    """The checked list as ms_optim_tensor rows (bytes), and its device. The lists are gone through
+    attribute by attribute: a short list of small tensors takes longer on the host than on the GPU."""
+    n, bits8 = len(params), scales is not None
     for name, ts in (("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq), ("steps", steps),
                      ("exp_avg_scales", scales), ("exp_avg_sq_scales", sq_scales)):
         if ts is not None and len(ts) != n:
             _bad(name, f"a list of {n} tensors, one for every parameter")
-    rows = (N.MsOptimTensor * n)()
-    moment = F8 if bits8 else torch.float32
-    for i, p in enumerate(params):
-        g, m, v, s = grads[i], exp_avg[i], exp_avg_sq[i], steps[i]
-        if device is None:
-            device = p.device
-        dt = _DTYPES.get(p.dtype)
-        if dt is None:
-            _bad("a parameter", f"float32, bfloat16 or float16, got {p.dtype}")
-        if not (p.is_contiguous() and g.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
-            _bad("every tensor", "contiguous")
-        if g.dtype != p.dtype or g.shape != p.shape:
-            _bad("a gradient", "of its parameter's type and shape")
-        if m.dtype != moment or v.dtype != moment or m.shape != p.shape or v.shape != p.shape:
-            _bad("a moment", f"{moment} of its parameter's shape")
-        if s.dtype != torch.int64 or s.numel() != 1:
-            _bad("a step count", "one int64")
-        k = p.numel()
-        row = rows[i]
-        if bits8:
-            a, b = scales[i], sq_scales[i]
-            want = scales_for(k)
-            for t in (a, b):
-                if t.dtype != torch.float32 or t.numel() != want or not t.is_contiguous() or t.device != device:
-                    _bad("scales", f"contiguous float32 of {want} values on {device} (one for every {BLOCK} values)")
-            row.exp_avg_scale, row.exp_avg_sq_scale = a.data_ptr(), b.data_ptr()
-        if p.device != device or g.device != device or m.device != device or v.device != device or s.device != device:
-            _bad("every tensor", f"on one device ({device})")
-        row.param, row.grad, row.exp_avg, row.exp_avg_sq = p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr()
-        row.step, row.numel, row.dtype = s.data_ptr(), k, dt
-    return rows, device
+    every = [*params, *grads, *exp_avg, *exp_avg_sq]
+    kinds = list(map(_KIND, every))
+    of_params, moment = kinds[:n], F8 if bits8 else torch.float32
+    moments = [(moment, shape) for _, shape in of_params]
+    if not (kinds[n:2 * n] == of_params and kinds[2 * n:3 * n] == moments and kinds[3 * n:] == moments
+            and all(map(_packed, every)) and all(dt in _DTYPES for dt, _ in of_params)
+            and all(dt is torch.int64 for dt in map(_DTYPE, steps)) and all(k == 1 for k in map(_numel, steps))
+            and len({*map(_where, every), *map(_where, steps)}) == 1):
+        for p, g, m, v, s in zip(params, grads, exp_avg, exp_avg_sq, steps):
+            _explain(p, g, m, v, s, moment, params[0].device)
+    sizes = list(map(_numel, params))
+    if bits8:
+        where = params[0].get_device()
+        for k, *pair in zip(sizes, scales, sq_scales):
+            for t in pair:
+                if t.dtype != torch.float32 or t.numel() != scales_for(k) or not t.is_contiguous() or t.get_device() != where:
+                    _bad("scales", f"contiguous float32 of {scales_for(k)} values on {params[0].device} (one for every {BLOCK} values)")
+        a, b = map(_ptr_of, scales), map(_ptr_of, sq_scales)
+    else:
+        a = b = repeat(0)
+    at = list(map(_ptr_of, every))
+    rows = zip(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], a, b, map(_ptr_of, steps), sizes,
+               (_DTYPES[dt] for dt, _ in of_params), repeat(0))
+    return struct.pack("<" + _ROW * n, *chain.from_iterable(rows)), params[0].device
+
+
+def _explain(p, g, m, v, s, moment, device):
+    """Raises for the first thing that is wrong with a parameter's tensors."""
+    if p.dtype not in _DTYPES:
+        _bad("a parameter", f"float32, bfloat16 or float16, got {p.dtype}")
+    if not all(t.is_contiguous() for t in (p, g, m, v)):
+        _bad("every tensor", "contiguous")
+    if g.dtype != p.dtype or g.shape != p.shape:
+        _bad("a gradient", "of its parameter's type and shape")
+    if any(t.dtype != moment or t.shape != p.shape for t in (m, v)):
+        _bad("a moment", f"{moment} of its parameter's shape")
+    if s.dtype != torch.int64 or s.numel() != 1:
+        _bad("a step count", "one int64")
+    if any(t.device != device for t in (p, g, m, v, s)):
+        _bad("every tensor", f"on one device ({device})")
 
 
 def _check_workspace(workspace, device):
@@ -94,18 +113,16 @@ def _check_workspace(workspace, device):
         _bad("workspace", f"{WORKSPACE} contiguous float32 on {device}, zeroed when made")
 
 
-def _launch(device, calls):
+def _launch(device, params, calls):
     if device.type != "cuda":
         raise ValueError(f"adamw_step: tensors must be on a HIP device, got {device}")
-    stream = torch.cuda.current_stream(device).cuda_stream
-    with torch.cuda.device(device):
-        for fn, *args in calls:
-            rc = fn(*args, stream)
-            if rc:
-                _raise(rc)
+    for fn, *args in calls:
+        rc = N.on_current_stream(device.index, fn, *args)
+        if rc:
+            _raise(rc)
+    torch.autograd.graph.increment_version(params)  # a graph that saved a parameter refuses its backward
 
 
-@torch.no_grad()
 def adamw_step(params, grads, exp_avg, exp_avg_sq, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                max_grad_norm=None, exp_avg_scales=None, exp_avg_sq_scales=None, workspace=None, grad_norm=None):
     """One AdamW step over a list of tensors, in place (see ms_adamw_step in include/marl_soccer.h):
@@ -132,7 +149,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, steps, *, lr, betas=(0.9, 0.9
         calls.append(_clip_call(rows, max_grad_norm, grad_norm, workspace))
     calls.append(_step_call(rows, 8 if exp_avg_scales is not None else 32, lr, betas, eps, weight_decay,
                             max_grad_norm is not None, workspace, device))
-    _launch(device, calls)
+    _launch(device, params, calls)
 
 
 def _ptr(t):
@@ -140,7 +157,7 @@ def _ptr(t):
 
 
 def _clip_call(rows, max_norm, grad_norm, workspace):
-    return N.lib().ms_grad_clip, rows, len(rows), float(max_norm), _ptr(grad_norm), _ptr(workspace)
+    return N.lib().ms_grad_clip, rows, len(rows) // _ROW_BYTES, float(max_norm), _ptr(grad_norm), _ptr(workspace)
 
 
 def _step_call(rows, bits, lr, betas, eps, weight_decay, clip, workspace, device):
@@ -149,7 +166,7 @@ def _step_call(rows, bits, lr, betas, eps, weight_decay, clip, workspace, device
         if lr.dtype != torch.float32 or lr.numel() != 1 or lr.device != device:
             _bad("lr", f"a float or one float32 on {device}")
         lr, lr_device = 0.0, lr.data_ptr()
-    return (N.lib().ms_adamw_step, rows, len(rows), bits, float(lr), lr_device, float(betas[0]), float(betas[1]),
+    return (N.lib().ms_adamw_step, rows, len(rows) // _ROW_BYTES, bits, float(lr), lr_device, float(betas[0]), float(betas[1]),
             float(eps), float(weight_decay), int(clip), _ptr(workspace))
 
 
@@ -207,7 +224,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        groups, device = [], None
+        groups, device, every_param = [], None, []
         for group in self.param_groups:
             ps = [p for p in group["params"] if p.grad is not None]
             if not ps:
@@ -223,6 +240,7 @@ class AdamW(torch.optim.Optimizer):
             if device is not None and dev != device:
                 _bad("every tensor", f"on one device ({device})")
             device = dev
+            every_param += ps
             groups.append((group, rows, grads))  # copies among them live until the launches are in the stream
         if not groups:
             return loss
@@ -232,11 +250,10 @@ class AdamW(torch.optim.Optimizer):
         work, norm = self._work.get(device, (None, None))
         calls = []
         if self.max_grad_norm is not None:
-            every = groups[0][1] if len(groups) == 1 else (N.MsOptimTensor * sum(len(r) for _, r, _ in groups))(
-                *[t for _, r, _ in groups for t in r])
+            every = b"".join(rows for _, rows, _ in groups)
             calls.append(_clip_call(every, self.max_grad_norm, norm, work))
         for group, rows, _ in groups:
             calls.append(_step_call(rows, self.state_bits, group["lr"], group["betas"], group["eps"], group["weight_decay"],
                                     self.max_grad_norm is not None, work, device))
-        _launch(device, calls)
+        _launch(device, every_param, calls)
         return loss

@@ -23,7 +23,7 @@ asynchronous on the current stream of the tensors' device and may be captured in
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 
 import torch
 
@@ -33,24 +33,47 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_STATES = 64
 
 
+# ms_conv_io and ms_scan_io (include/marl_soccer.h), packed in one go: a step's latency is the host's
+_CONV = struct.Struct("<4i3q" + "Qqq" + "QQQ" + "Qqq" + "Qqq" + "Q" + "Qqq" + "Q" + "Qqq" + "QQQ" + "Qq")
+_SCAN = struct.Struct("<4i3q" + "Qqq" * 3 + "Qqqq" * 2 + "QQQQ" + "Qqq" * 2 + "QQ" + "Qqq" + "Q" + "Qqq" * 3 + "Q" * 7 + "q")
+assert _CONV.size == N.C.sizeof(N.MsConvIO) and _SCAN.size == N.C.sizeof(N.MsScanIO)
+_NONE3 = (0, 0, 0)
+_NO_GRADS = (0,) * 12  # ms_conv_io from dout on
+_NO_SCAN_GRADS = (0,) * 22  # ms_scan_io from checkpoints on
+
+
 def _fail(rc: int) -> None:
     raise (ValueError if rc == N.MS_ERR_INVALID_ARGUMENT else N.NativeError)(
         N.lib().ms_sequence_last_error().decode(errors="replace"))
 
 
-def _call(fn, io, device) -> None:
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        rc = fn(C.byref(io), stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(C.byref(io), stream)
+def _call(fn, io, index) -> None:
+    rc = N.on_current_stream(index, fn, io)
     if rc:
         _fail(rc)
 
 
+# a tensor written behind autograd's back: a graph that saved it refuses its backward
+_renewed = torch.autograd.graph.increment_version
+
+
 def _p(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
+
+
+def _p3(t):
+    """Pointer, step stride, row stride of (T, R, ...)."""
+    return _NONE3 if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _g4(t):
+    """The same with the group's stride, of (T, R, [G,] N)."""
+    return (t.data_ptr(), t.stride(0), t.stride(1), t.stride(2) if t.dim() == 4 else 0)
+
+
+def _row3(t):
+    """Pointer, no step stride, row stride of (R, ...)."""
+    return _NONE3 if t is None else (t.data_ptr(), 0, t.stride(0))
 
 
 def _check(who, name, t, shape, dtype, device, rows_contiguous=False):
@@ -68,6 +91,19 @@ def _check(who, name, t, shape, dtype, device, rows_contiguous=False):
             raise ValueError(f"{who}: {name} must be contiguous")
     elif t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{who}: {name}'s last dimension must be contiguous (stride 1)")
+
+
+def _right(t, shape, dtype, index):
+    """Whether a time-dependent argument is right as it stands, without saying what is wrong."""
+    return t.shape == shape and t.dtype is dtype and t.get_device() == index and t.stride(-1) == 1
+
+
+def _right_weight(t, shape, index):
+    return t is None or (t.shape == shape and t.dtype is torch.float32 and t.get_device() == index and t.is_contiguous())
+
+
+def _right_starts(t, shape, index):
+    return t is None or (t.shape == shape and (t.dtype is torch.bool or t.dtype is torch.uint8) and t.get_device() == index)
 
 
 def _check_starts(who, starts, shape, device):
@@ -108,16 +144,30 @@ def _rows(t):
 
 # ---------------------------------------------------------------- short convolution
 
-def _conv_io(x, weight, bias, state, starts, silu):
+def _conv_io(x, weight, bias, state, starts, silu, out=None, new=None, dout=None, dnew=None, dx=None, dstate=None,
+             dweight=None, dbias=None, work=0, work_bytes=0):
     T, R, D = x.shape
-    io = N.MsConvIO(dtype=_DTYPES[x.dtype], width=weight.shape[1], silu=silu, steps=T, rows=R, channels=D, x=_p(x),
-                    x_t=x.stride(0), x_r=x.stride(1), weight=_p(weight), bias=_p(bias), state=_p(state))
-    if starts is not None:
-        io.starts, io.starts_t, io.starts_r = starts.data_ptr(), starts.stride(0), starts.stride(1)
-    return io
+    return _CONV.pack(_DTYPES[x.dtype], weight.shape[1], silu, 0, T, R, D, *_p3(x), weight.data_ptr(), _p(bias), _p(state),
+                      *_p3(starts), *_p3(out), _p(new), *_p3(dout), _p(dnew), *_p3(dx), _p(dstate), _p(dweight), _p(dbias),
+                      work, work_bytes)
+
+
+def _conv_right(x, weight, bias, state, starts, activation, dims):
+    """Everything that _conv_check looks for, in one go."""
+    try:
+        shape, i = x.shape, x.get_device()
+        D, W = shape[-1], weight.shape[1]
+        return (i >= 0 and len(shape) == dims and x.dtype in _DTYPES and D > 0 and x.stride(-1) == 1 and 2 <= W <= 4
+                and (activation is None or activation == "silu") and _right_weight(weight, (D, W), i) and _right_weight(bias, (D,), i)
+                and (state is None or (_right(state, (shape[-2], W - 1, D), x.dtype, i) and state.is_contiguous()))
+                and _right_starts(starts, shape[:-1], i))
+    except (AttributeError, IndexError):
+        return False
 
 
 def _conv_check(who, x, weight, bias, state, starts, activation, dims):
+    if _conv_right(x, weight, bias, state, starts, activation, dims):
+        return
     _sequence(who, "x", x, dims)
     device, D = x.device, x.shape[-1]
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 2 <= weight.shape[1] <= 4:
@@ -140,9 +190,7 @@ class _ShortConv(torch.autograd.Function):
     def forward(ctx, x, weight, bias, state, starts, silu, want_state):
         out = _like(x)
         new = torch.empty((x.shape[1], weight.shape[1] - 1, x.shape[2]), dtype=x.dtype, device=x.device) if want_state else None
-        io = _conv_io(x, weight, bias, state, starts, silu)
-        io.out, io.out_t, io.out_r, io.new_state = _p(out), out.stride(0), out.stride(1), _p(new)
-        _call(N.lib().ms_conv_forward, io, x.device)
+        _call(N.lib().ms_conv_forward, _conv_io(x, weight, bias, state, starts, silu, out, new), x.get_device())
         ctx.save_for_backward(x, weight, bias, state, starts)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
@@ -161,14 +209,11 @@ class _ShortConv(torch.autograd.Function):
         dbias = torch.empty_like(bias) if bias is not None and need[2] else None
         dstate = torch.empty_like(state) if state is not None and need[3] else None
         dnew = None if dnew is None else dnew.contiguous()
-        io = _conv_io(x, weight, bias, state, starts, ctx.silu)
-        io.dout, io.dout_t, io.dout_r, io.dnew_state = _p(dout), dout.stride(0), dout.stride(1), _p(dnew)
-        io.dx, io.dx_t, io.dx_r, io.dstate, io.dweight, io.dbias = _p(dx), dx.stride(0), dx.stride(1), _p(dstate), _p(dweight), _p(dbias)
         L = N.lib()
-        io.workspace_bytes = L.ms_conv_workspace(C.byref(io))
-        work = torch.empty((io.workspace_bytes,), dtype=torch.uint8, device=x.device)
-        io.workspace = work.data_ptr()
-        _call(L.ms_conv_backward, io, x.device)
+        args = (x, weight, bias, state, starts, ctx.silu, None, None, dout, dnew, dx, dstate, dweight, dbias)
+        size = L.ms_conv_workspace(_conv_io(*args))
+        work = torch.empty((size,), dtype=torch.uint8, device=x.device)
+        _call(L.ms_conv_backward, _conv_io(*args, work.data_ptr(), size), x.get_device())
         return dx if need[0] else None, dweight, dbias, dstate, None, None, None
 
 
@@ -185,7 +230,6 @@ def short_conv(x, weight, bias=None, state=None, starts=None, activation=None, r
     return (out, new) if return_state else out
 
 
-@torch.no_grad()
 def short_conv_step(x, state, weight, bias=None, starts=None, activation=None):
     """One step of short_conv for every row: x (R, D), starts (R,); state (R, W - 1, D) is renewed in
     place. Returns y (R, D). No gradients."""
@@ -193,18 +237,42 @@ def short_conv_step(x, state, weight, bias=None, starts=None, activation=None):
     if not isinstance(state, torch.Tensor):
         raise ValueError(f"{who}: state must be a tensor")
     _conv_check(who, x, weight, bias, state, starts, activation, 2)
-    out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    io = N.MsConvIO(dtype=_DTYPES[x.dtype], width=weight.shape[1], silu=activation == "silu", steps=1, rows=x.shape[0],
-                    channels=x.shape[1], x=x.data_ptr(), x_r=x.stride(0), weight=weight.data_ptr(), bias=_p(bias),
-                    state=state.data_ptr(), starts=_p(starts), starts_r=0 if starts is None else starts.stride(0),
-                    out=out.data_ptr(), out_r=out.stride(0), new_state=state.data_ptr())
-    _call(N.lib().ms_conv_forward, io, x.device)
+    R, D = x.shape
+    out = torch.empty((R, D), dtype=x.dtype, device=x.device)
+    at = state.data_ptr()
+    _call(N.lib().ms_conv_forward,
+          _CONV.pack(_DTYPES[x.dtype], weight.shape[1], activation == "silu", 0, 1, R, D, *_row3(x), weight.data_ptr(), _p(bias),
+                     at, *_row3(starts), out.data_ptr(), 0, D, at, *_NO_GRADS), x.get_device())
+    _renewed(state)
     return out
 
 
 # ---------------------------------------------------------------- state-space scan
 
+def _scan_right(u, delta, A, B, Cm, D, z, delta_bias, state, starts, dims):
+    """Everything that _scan_check looks for, in one go."""
+    try:
+        shape, dt, i = u.shape, u.dtype, u.get_device()
+        ch, (_, n), given = shape[-1], A.shape, B.shape
+        if not (i >= 0 and len(shape) == dims and dt in _DTYPES and ch > 0 and u.stride(-1) == 1 and 1 <= n <= MAX_STATES):
+            return False
+        lead = shape[:-1]
+        if len(given) > dims:
+            if given[-2] < 1 or ch % given[-2] or given != (*lead, given[-2], n):
+                return False
+        elif given != (*lead, n):
+            return False
+        return (_right(delta, shape, dt, i) and _right(B, given, dt, i) and _right(Cm, given, dt, i)
+                and (z is None or _right(z, shape, dt, i)) and _right_weight(A, (ch, n), i) and _right_weight(D, (ch,), i)
+                and _right_weight(delta_bias, (ch,), i) and _right_weight(state, (shape[-2], ch, n), i)
+                and _right_starts(starts, lead, i))
+    except (AttributeError, IndexError, ValueError):
+        return False
+
+
 def _scan_check(who, u, delta, A, B, Cm, D, z, delta_bias, state, starts, dims):
+    if _scan_right(u, delta, A, B, Cm, D, z, delta_bias, state, starts, dims):
+        return
     _sequence(who, "u", u, dims)
     device, dt, ch = u.device, u.dtype, u.shape[-1]
     lead = u.shape[:-1]
@@ -235,20 +303,13 @@ def _scan_check(who, u, delta, A, B, Cm, D, z, delta_bias, state, starts, dims):
     _on_gpu(who, device)
 
 
-def _scan_io(u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft):
+def _scan_io(u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft, out=None, new=None, keep=None, dout=None, dnew=None,
+             du=None, ddelta=None, dz=None, dB=None, dC=None, dA=None, dD=None, dbias=None, dstate=None, work=0, work_bytes=0):
     T, R, ch = u.shape
-    io = N.MsScanIO(dtype=_DTYPES[u.dtype], softplus=soft, states=A.shape[1], groups=B.shape[2] if B.dim() == 4 else 1,
-                    steps=T, rows=R, channels=ch, u=_p(u), u_t=u.stride(0), u_r=u.stride(1), delta=_p(delta),
-                    delta_t=delta.stride(0), delta_r=delta.stride(1), B=_p(B), B_t=B.stride(0), B_r=B.stride(1),
-                    C=_p(Cm), C_t=Cm.stride(0), C_r=Cm.stride(1), A=_p(A), D=_p(D), delta_bias=_p(delta_bias),
-                    state=_p(state))
-    if B.dim() == 4:
-        io.B_g, io.C_g = B.stride(2), Cm.stride(2)
-    if z is not None:
-        io.z, io.z_t, io.z_r = z.data_ptr(), z.stride(0), z.stride(1)
-    if starts is not None:
-        io.starts, io.starts_t, io.starts_r = starts.data_ptr(), starts.stride(0), starts.stride(1)
-    return io
+    return _SCAN.pack(_DTYPES[u.dtype], soft, A.shape[1], B.shape[2] if B.dim() == 4 else 1, T, R, ch, *_p3(u), *_p3(delta),
+                      *_p3(z), *_g4(B), *_g4(Cm), A.data_ptr(), _p(D), _p(delta_bias), _p(state), *_p3(starts), *_p3(out),
+                      _p(new), _p(keep), *_p3(dout), _p(dnew), *_p3(du), *_p3(ddelta), *_p3(dz), _p(dB), _p(dC), _p(dA), _p(dD),
+                      _p(dbias), _p(dstate), work, work_bytes)
 
 
 class _Scan(torch.autograd.Function):
@@ -257,18 +318,12 @@ class _Scan(torch.autograd.Function):
         L = N.lib()
         out = _like(u)
         new = torch.empty((u.shape[1], *A.shape), dtype=torch.float32, device=u.device) if want_state else None
-        io = _scan_io(u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft)
-        io.out, io.out_t, io.out_r, io.new_state = _p(out), out.stride(0), out.stride(1), _p(new)
-        keep = None
-        if want_grad:
-            keep = torch.empty((L.ms_scan_checkpoints(C.byref(io)),), dtype=torch.uint8, device=u.device)
-            io.checkpoints = keep.data_ptr()
-        io.workspace_bytes = L.ms_scan_workspace(C.byref(io), 0)
-        work = None
-        if io.workspace_bytes:
-            work = torch.empty((io.workspace_bytes,), dtype=torch.uint8, device=u.device)
-            io.workspace = work.data_ptr()
-        _call(L.ms_scan_forward, io, u.device)
+        args = (u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft, out, new)
+        io = _scan_io(*args)
+        keep = torch.empty((L.ms_scan_checkpoints(io),), dtype=torch.uint8, device=u.device) if want_grad else None
+        size = L.ms_scan_workspace(io, 0)
+        work = torch.empty((size,), dtype=torch.uint8, device=u.device)
+        _call(L.ms_scan_forward, _scan_io(*args, keep, work=work.data_ptr(), work_bytes=size), u.get_device())
         ctx.save_for_backward(u, delta, A, B, Cm, D, z, delta_bias, state, starts, keep)
         ctx.soft = soft
         ctx.set_materialize_grads(False)
@@ -284,8 +339,6 @@ class _Scan(torch.autograd.Function):
         L = N.lib()
         dout = torch.zeros_like(u) if dout is None else _rows(dout)
         dnew = None if dnew is None else dnew.contiguous()
-        io = _scan_io(u, delta, A, B, Cm, D, z, delta_bias, state, starts, ctx.soft)
-        io.checkpoints = keep.data_ptr()
         du, ddelta, dz = _like(u), _like(u), _like(u) if z is not None else None
         dB = torch.empty_like(B, memory_format=torch.contiguous_format)
         dC = torch.empty_like(Cm, memory_format=torch.contiguous_format)
@@ -293,16 +346,11 @@ class _Scan(torch.autograd.Function):
         dD = torch.empty_like(D) if D is not None and need[5] else None
         dbias = torch.empty_like(delta_bias) if delta_bias is not None and need[7] else None
         dstate = torch.empty_like(state) if state is not None and need[8] else None
-        io.dout, io.dout_t, io.dout_r, io.dnew_state = _p(dout), dout.stride(0), dout.stride(1), _p(dnew)
-        io.du, io.du_t, io.du_r = _p(du), du.stride(0), du.stride(1)
-        io.ddelta, io.ddelta_t, io.ddelta_r = _p(ddelta), ddelta.stride(0), ddelta.stride(1)
-        if dz is not None:
-            io.dz, io.dz_t, io.dz_r = _p(dz), dz.stride(0), dz.stride(1)
-        io.dB, io.dC, io.dA, io.dD, io.ddelta_bias, io.dstate = _p(dB), _p(dC), _p(dA), _p(dD), _p(dbias), _p(dstate)
-        io.workspace_bytes = L.ms_scan_workspace(C.byref(io), 1)
-        work = torch.empty((io.workspace_bytes,), dtype=torch.uint8, device=u.device)
-        io.workspace = work.data_ptr()
-        _call(L.ms_scan_backward, io, u.device)
+        args = (u, delta, A, B, Cm, D, z, delta_bias, state, starts, ctx.soft, None, None, keep, dout, dnew, du, ddelta, dz, dB,
+                dC, dA, dD, dbias, dstate)
+        size = L.ms_scan_workspace(_scan_io(*args), 1)
+        work = torch.empty((size,), dtype=torch.uint8, device=u.device)
+        _call(L.ms_scan_backward, _scan_io(*args, work.data_ptr(), size), u.get_device())
         grads = (du, ddelta, dA, dB, dC, dD, dz, dbias, dstate)
         return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * 4
 
@@ -325,7 +373,6 @@ def ssm_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, state=None, sta
     return (out, new) if return_state else out
 
 
-@torch.no_grad()
 def ssm_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=None, starts=None, delta_softplus=True):
     """One step of ssm_scan for every row: u, delta, z (R, D), B, C (R, N) or (R, G, N), starts (R,);
     state (R, D, N) is renewed in place. Returns y (R, D). No gradients."""
@@ -333,14 +380,13 @@ def ssm_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=None, starts=N
     if not isinstance(state, torch.Tensor):
         raise ValueError(f"{who}: state must be a tensor")
     _scan_check(who, u, delta, A, B, C, D, z, delta_bias, state, starts, 2)
-    out = torch.empty_like(u, memory_format=torch.contiguous_format)
-    io = N.MsScanIO(dtype=_DTYPES[u.dtype], softplus=bool(delta_softplus), states=A.shape[1],
-                    groups=B.shape[1] if B.dim() == 3 else 1, steps=1, rows=u.shape[0], channels=u.shape[1],
-                    u=u.data_ptr(), u_r=u.stride(0), delta=delta.data_ptr(), delta_r=delta.stride(0), B=B.data_ptr(),
-                    B_r=B.stride(0), B_g=B.stride(1) if B.dim() == 3 else 0, C=C.data_ptr(), C_r=C.stride(0),
-                    C_g=C.stride(1) if B.dim() == 3 else 0, z=_p(z), z_r=0 if z is None else z.stride(0), A=A.data_ptr(),
-                    D=_p(D), delta_bias=_p(delta_bias), state=state.data_ptr(), starts=_p(starts),
-                    starts_r=0 if starts is None else starts.stride(0), out=out.data_ptr(), out_r=out.stride(0),
-                    new_state=state.data_ptr())
-    _call(N.lib().ms_scan_step, io, u.device)
+    R, ch = u.shape
+    out = torch.empty((R, ch), dtype=u.dtype, device=u.device)
+    grouped, at = B.dim() == 3, state.data_ptr()
+    _call(N.lib().ms_scan_step,
+          _SCAN.pack(_DTYPES[u.dtype], bool(delta_softplus), A.shape[1], B.shape[1] if grouped else 1, 1, R, ch, *_row3(u),
+                     *_row3(delta), *_row3(z), *_row3(B), B.stride(1) if grouped else 0, *_row3(C), C.stride(1) if grouped else 0,
+                     A.data_ptr(), _p(D), _p(delta_bias), at, *_row3(starts), out.data_ptr(), 0, ch, at, *_NO_SCAN_GRADS),
+          u.get_device())
+    _renewed(state)
     return out
