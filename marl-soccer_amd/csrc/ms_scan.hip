@@ -441,15 +441,9 @@ __device__ __forceinline__ float fold_items(const float (&x)[8], bool bit3) {
   for (int i = 0; i < 2; ++i) b[i] = fold16(a[i], a[i + 2]);
   return fold_dpp<ROR8>(b[0], b[1], bit3);
 }
-// eight steps' registers -> lane 8 i + t holds item i of step t
-__device__ __forceinline__ float fold_steps(const float (&x)[8], int lane) {
-  float a[4], b[2];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) a[i] = fold_dpp<HALF_MIRROR>(x[i], x[i + 4], lane & 4);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) b[i] = fold_dpp<XOR2>(a[i], a[i + 2], lane & 2);
-  return fold_dpp<XOR1>(b[0], b[1], lane & 1);
-}
+// eight steps' registers, folded two by two as they come: lane 8 i + l then holds item i of the step
+// whose three bits are l's in reverse order
+__device__ __forceinline__ int lane_of_step(int t) { return (t & 1) << 2 | (t & 2) | (t & 4) >> 2; }
 
 // The first pass of a split time axis: what each chunk hands back from zero.
 template <typename T, int NS, int NW>
@@ -538,12 +532,12 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
   if (threadIdx.x == 0 && at.td == 0) a.cut[at.chunk * io.rows + at.r] = was_cut;
 }
 
-// A tile of 16 steps at a time, in it the KC steps from a checkpoint and four states at a time: first
-// forwards, keeping a[t] and a[t] h[t - 1] in registers (64 of them), then backwards through them. With
-// 16 steps between checkpoints they would be 128, and the kernel would spill.
+// The KC steps from a checkpoint at a time, and of them four states at a time: first forwards, keeping
+// a[t] and a[t] h[t - 1] in registers (64 of them), then backwards through them. With 16 steps between
+// checkpoints they would be 128, and two waves a SIMD would spill.
 template <typename T, int NS, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
-  constexpr int TT = NW == 1 ? 8 : 16, E = TT / NW, TPR = 64 / E;  // a tile's values over the threads: E channels each
+__global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : 2) void backward(const Args a) {
+  constexpr int TT = KC, E = TT / NW, TPR = 64 / E;  // a tile's values over the threads: E channels each
   __shared__ float s_rate[TT][64], s_ru[TT][64], s_dy[TT][64];
   __shared__ float s_gb[NW][TT][64], s_ga[NW][TT][64], s_y[NW][TT][64];
   const ms_scan_io& io = a.io;
@@ -620,47 +614,33 @@ __global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
     po -= TT * io.dout_t;
     if (pz) pz -= TT * io.z_t;
     fetch(k > 0);
-    const int64_t ckpt_step = io.rows * a.p.blocks_d * (NS * NW / 4) * 256;
     const float* from = io.checkpoints + checkpoint_at(a, t0 / KC, at.r, at.td, w * NS, lane);
     float* to = a.parts_bc + ((((t0 / 16 * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS / 4) * 2 + (t0 / 8 & 1)) * 64 + lane;
     auto tile = [&](auto any) __attribute__((always_inline)) {
       constexpr bool CUTS = decltype(any)::value;
 #pragma unroll
       for (int nb = 0; nb < NS; nb += 4) {
-        for (int half = TT / KC - 1; half >= 0; --half) {
-          const int t0h = half * KC;
-          if (t0 + t0h >= t1) {  // no steps there, and no checkpoint
-#pragma unroll
-            for (int j = 0; j < KC; ++j) s_gb[w][t0h + j][lane] = s_ga[w][t0h + j][lane] = s_y[w][t0h + j][lane] = 0.0f;
-            continue;
-          }
-          const float4 h0 = *(const float4*)(from + half * ckpt_step + nb * 64);
-          CONSTANT(f32x16)* p = base + (nb >> 2) * share + half * (KC / 4 * 2);
+        {
+          const float4 h0 = *(const float4*)(from + nb * 64);
+          CONSTANT(f32x16)* p = base + (nb >> 2) * share;
           float h[4] = {h0.x, h0.y, h0.z, h0.w};
           float dec[KC][4], ah[KC][4];  // a[t] and a[t] h[t - 1]
           f32x16 b = p[0];
-          float rate[4], ru[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            rate[j] = s_rate[t0h + j][lane];
-            ru[j] = s_ru[t0h + j][lane];
-          }
 #pragma unroll
           for (int t4 = 0; t4 < KC; t4 += 4) {
-            loads_done();
-            const int tn = t4 + 4 < KC ? t4 + 4 : KC - 4;
-            const f32x16 b_next = p[tn / 4 * 2];
-            float rate_next[4], ru_next[4];
+            float rate[4], ru[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              rate_next[j] = s_rate[t0h + tn + j][lane];
-              ru_next[j] = s_ru[t0h + tn + j][lane];
+              rate[j] = s_rate[t4 + j][lane];
+              ru[j] = s_ru[t4 + j][lane];
             }
+            loads_done();
+            const f32x16 b_next = p[(t4 + 4 < KC ? t4 + 4 : KC - 4) / 4 * 2];
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int t = t4 + j;
-              if (CUTS && (starts >> (t0h + t) & 1)) h[0] = h[1] = h[2] = h[3] = 0.0f;
+              if (CUTS && (starts >> t & 1)) h[0] = h[1] = h[2] = h[3] = 0.0f;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 dec[t][i] = __builtin_amdgcn_exp2f(rate[j] * A2[nb + i]);
@@ -670,31 +650,22 @@ __global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
             }
             __builtin_amdgcn_sched_barrier(0);
             b = b_next;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              rate[j] = rate_next[j];
-              ru[j] = ru_next[j];
-            }
           }
-          float steps8[8];
           Scalars s;
           s.b = b;
           s.c = p[KC / 4 * 2 - 1];
-          float dy[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) dy[j] = s_dy[t0h + KC - 4 + j][lane];
+          float pair = 0.0f, four = 0.0f, eight = 0.0f;  // folded registers of 1, 2 and 4 steps that wait for their other half
 #pragma unroll
           for (int t4 = KC - 4; t4 >= 0; t4 -= 4) {
-            loads_done();
-            const int tp = t4 ? t4 - 4 : 0;
-            const Scalars prev = scalars(p + tp / 4 * 2);
-            float dy_prev[4], rate_prev[4], ru_prev[4];
+            float rate[4], ru[4], dy[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              dy_prev[j] = s_dy[t0h + tp + j][lane];
-              rate_prev[j] = s_rate[t0h + tp + j][lane];
-              ru_prev[j] = s_ru[t0h + tp + j][lane];
+              dy[j] = s_dy[t4 + j][lane];
+              rate[j] = s_rate[t4 + j][lane];
+              ru[j] = s_ru[t4 + j][lane];
             }
+            loads_done();
+            const Scalars prev = scalars(p + (t4 ? t4 - 4 : 0) / 4 * 2);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 3; j >= 0; --j) {
@@ -714,27 +685,32 @@ __global__ __launch_bounds__(64 * NW, 2) void backward(const Args a) {
                 items[i] = ru[j] * g;
                 items[4 + i] = dy[j] * hh;
               }
-              if (CUTS && (starts >> (t0h + t) & 1)) carry[nb] = carry[nb + 1] = carry[nb + 2] = carry[nb + 3] = 0.0f;
+              if (CUTS && (starts >> t & 1)) carry[nb] = carry[nb + 1] = carry[nb + 2] = carry[nb + 3] = 0.0f;
               if (nb) {
-                gb += s_gb[w][t0h + t][lane];
-                ga += s_ga[w][t0h + t][lane];
-                y += s_y[w][t0h + t][lane];
+                gb += s_gb[w][t][lane];
+                ga += s_ga[w][t][lane];
+                y += s_y[w][t][lane];
               }
-              s_gb[w][t0h + t][lane] = gb;
-              s_ga[w][t0h + t][lane] = ga;
-              s_y[w][t0h + t][lane] = y;
-              steps8[t] = fold_items(items, lane & 8);
+              s_gb[w][t][lane] = gb;
+              s_ga[w][t][lane] = ga;
+              s_y[w][t][lane] = y;
+              float x = fold_items(items, lane & 8);
+              if (t & 1) {
+                pair = x;
+              } else {
+                x = fold_dpp<HALF_MIRROR>(x, pair, lane & 4);
+                if (t & 2) {
+                  four = x;
+                } else {
+                  x = fold_dpp<XOR2>(x, four, lane & 2);
+                  if (t & 4) eight = x;
+                  else to[(nb >> 2) * 2 * 64] = fold_dpp<XOR1>(x, eight, lane & 1);
+                }
+              }
             }
             __builtin_amdgcn_sched_barrier(0);
             s = prev;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              dy[j] = dy_prev[j];
-              rate[j] = rate_prev[j];
-              ru[j] = ru_prev[j];
-            }
           }
-          to[((nb >> 2) * 2 + half) * 64] = fold_steps(steps8, lane);
         }
       }
     };
@@ -826,7 +802,7 @@ __global__ __launch_bounds__(256) void finish_bc(const Args a) {
   k /= io.groups;
   const int64_t r = k % io.rows, t = k / io.rows;
   const int64_t ns = a.p.ns, w = s / ns, nb = s % ns / 4;
-  const int64_t lane = (kind * 4 + s % 4) * 8 + t % 8;
+  const int64_t lane = (kind * 4 + s % 4) * 8 + lane_of_step((int)(t & 7));
   const int64_t one = a.p.nw * (ns / 4) * 2 * 64;  // a tile's floats
   const float* p = a.parts_bc + ((t / 16 * io.rows + r) * a.p.blocks_d + g * a.p.tiles) * one +
                    ((w * (ns / 4) + nb) * 2 + t % 16 / 8) * 64 + lane;
