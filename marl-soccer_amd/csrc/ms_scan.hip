@@ -141,6 +141,14 @@ __device__ __forceinline__ Place place(const Args& a) {
   return p;
 }
 
+// Where channel c of step t lies in its row of LDS. Threads that move 8 neighbouring values reach every
+// other 16 B of a row; odd rows are shifted by 16 B, so that the two rows a 16-lane access covers use
+// all banks and not half of them twice.
+template <int E>
+__device__ __forceinline__ int column(int c, int t) {
+  return E == 8 ? c ^ (t & 1) << 2 : c;
+}
+
 // ---------------------------------------------------------------- forward
 // LOCAL: the first pass of a split time axis (states from zero, no outputs).
 // The loop over a tile goes by units of 16 / NS steps: 32 scalars (one s_load_dwordx16 for B and one
@@ -216,8 +224,8 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
       float slope, rate = (float)vd[e] + bias[e];
       if (soft) rate = softplus(rate, slope);
       rate = mine ? rate : 0.0f;
-      s_rate[lt][lc + e] = rate;
-      s_ru[lt][lc + e] = rate * (float)cu[e];
+      s_rate[lt][column<E>(lc + e, lt)] = rate;
+      s_ru[lt][column<E>(lc + e, lt)] = rate * (float)cu[e];
     }
     const uint64_t starts = start_mask(io, at.r, t0, t0 + (left < TT ? left : TT));
     __syncthreads();
@@ -225,8 +233,8 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
     float rate[G], ru[G];
 #pragma unroll
     for (int j = 0; j < G; ++j) {
-      rate[j] = s_rate[j][lane];
-      ru[j] = s_ru[j][lane];
+      rate[j] = s_rate[j][column<E>(lane, j)];
+      ru[j] = s_ru[j][column<E>(lane, j)];
     }
     const int steps = left < TT ? (left + G - 1) / G * G : TT;
     for (int t = 0; t < steps; t += G) {
@@ -245,8 +253,9 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
       float nrate[G], nru[G];
 #pragma unroll
       for (int j = 0; j < G; ++j) {
-        nrate[j] = s_rate[t + G + j][lane];
-        nru[j] = s_ru[t + G + j][lane];
+        const int c = column<E>(lane, G > 1 ? j : t + 1);
+        nrate[j] = s_rate[t + G + j][c];
+        nru[j] = s_ru[t + G + j][c];
       }
       __builtin_amdgcn_sched_barrier(0);
       const unsigned cut = (unsigned)(starts >> t) & ((1u << G) - 1);
@@ -265,7 +274,7 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
             if (!LOCAL) y = i ? __builtin_fmaf(s.c[j * NS + i], h[i], y) : s.c[j * NS] * h[0];
           }
           if (LOCAL) total += rate[j];
-          else s_y[w][t + j][lane] = y;
+          else s_y[w][t + j][column<E>(lane, G > 1 ? j : t)] = y;
         }
       };
       if (cut) work(std::true_type{});
@@ -284,9 +293,9 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
         float y[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          float v = s_y[0][lt][lc + e];
+          float v = s_y[0][lt][column<E>(lc + e, lt)];
 #pragma unroll
-          for (int k = 1; k < NW; ++k) v += s_y[k][lt][lc + e];
+          for (int k = 1; k < NW; ++k) v += s_y[k][lt][column<E>(lc + e, lt)];
           y[e] = __builtin_fmaf(skip[e], (float)cu[e], v);
           if (z) y[e] *= silu((float)cz[e]);
         }
@@ -495,8 +504,8 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
     for (int e = 0; e < E; ++e) {
       float slope, rate = (float)vd[e] + bias[e];
       if (io.softplus) rate = softplus(rate, slope);
-      s_rate[lt][lc + e] = mine ? rate : 0.0f;
-      s_dy[lt][lc + e] = z ? (float)vy[e] * silu((float)vz[e]) : (float)vy[e];
+      s_rate[lt][column<E>(lc + e, lt)] = mine ? rate : 0.0f;
+      s_dy[lt][column<E>(lc + e, lt)] = z ? (float)vy[e] * silu((float)vz[e]) : (float)vy[e];
     }
     const uint64_t starts = start_mask(io, at.r, t0, t1);
     __syncthreads();
@@ -508,7 +517,7 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
       const unsigned cut = (unsigned)(starts >> t) & 15u;
 #pragma unroll
       for (int j = G - 1; j >= 0; --j) {
-        const float rate = s_rate[t + j][lane], d = s_dy[t + j][lane];
+        const float rate = s_rate[t + j][column<E>(lane, j)], d = s_dy[t + j][column<E>(lane, j)];
         total += rate;
 #pragma unroll
         for (int i = 0; i < NS; ++i)
@@ -536,9 +545,12 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
 // a[t] and a[t] h[t - 1] in registers (64 of them), then backwards through them. With 16 steps between
 // checkpoints they would be 128, and two waves a SIMD would spill.
 template <typename T, int NS, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : 2) void backward(const Args a) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) void backward(const Args a) {
   constexpr int TT = KC, E = TT / NW, TPR = 64 / E;  // a tile's values over the threads: E channels each
-  __shared__ float s_rate[TT][64], s_ru[TT][64], s_dy[TT][64];
+  __shared__ float s_in[2][3][TT][64];  // rate, rate u and dy of this tile and, while it is finished, the next
+  // what a thread needs of its own values again after the recurrence: kept here, 168 registers are few
+  enum { U, Z, DOUT, SLOPE, GATE, DSKIP, DBIAS, KEPT };
+  __shared__ float s_kept[KEPT][TT][64], s_bias[64], s_skip[64];
   __shared__ float s_gb[NW][TT][64], s_ga[NW][TT][64], s_y[NW][TT][64];
   const ms_scan_io& io = a.io;
   const Place at = place(a);
@@ -556,13 +568,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : 2) void backward(
   T* qu = (T*)io.du + at.r * io.du_r + cl + last * io.du_t;
   T* qd = (T*)io.ddelta + at.r * io.ddelta_r + cl + last * io.ddelta_t;
   T* qz = io.z ? (T*)io.dz + at.r * io.dz_r + cl + last * io.dz_t : nullptr;
-  float bias[E], skip[E], dskip[E], dbias[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    bias[e] = io.delta_bias && e < n ? io.delta_bias[cl + e] : 0.0f;
-    skip[e] = io.D && e < n ? io.D[cl + e] : 0.0f;
-    dskip[e] = dbias[e] = 0.0f;
+  if (threadIdx.x < 64) {
+    const bool in = lane < at.nc;
+    s_bias[lane] = in && io.delta_bias ? io.delta_bias[at.c0 + lane] : 0.0f;
+    s_skip[lane] = in && io.D ? io.D[at.c0 + lane] : 0.0f;
   }
+#pragma unroll
+  for (int e = 0; e < E; ++e) s_kept[DSKIP][lt][lc + e] = s_kept[DBIAS][lt][lc + e] = 0.0f;
+  __syncthreads();
   const int64_t ch = at.c0 + lane;
   const int N = io.states;
   const bool live = lane < at.nc;
@@ -584,6 +597,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : 2) void backward(
   const bool vec = a.vec;
   typedef typename Vec<T, E>::type V;
   V vu, vd, vz, vo;
+  float4 start[NS / 4];  // the checkpoint, a tile ahead as the rest
+  const int64_t ckpt_step = io.rows * a.p.blocks_d * (NS * NW / 4) * 256;
+  const float* from = io.checkpoints + checkpoint_at(a, t_begin / KC + tiles - 1, at.r, at.td, w * NS, lane);
   auto fetch = [&](bool in) __attribute__((always_inline)) {
     vu = load<T, E>(pu, in ? n : 0, vec);
     vd = load<T, E>(pd, in ? n : 0, vec);
@@ -591,21 +607,31 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : 2) void backward(
     if (pz) vz = load<T, E>(pz, in ? n : 0, vec);
   };
   fetch(last < t_end);
+#pragma unroll
+  for (int q = 0; q < NS / 4; ++q) start[q] = *(const float4*)(from + q * 256);
   for (int64_t k = tiles - 1; k >= 0; --k) {
     const int64_t t0 = t_begin + k * TT, t1 = t0 + TT < t_end ? t0 + TT : t_end;
-    const V cu = vu, cz = vz, co = vo;
+    float4 h_start[NS / 4];
+#pragma unroll
+    for (int q = 0; q < NS / 4; ++q) h_start[q] = start[q];
+    float(&s_rate)[TT][64] = s_in[k & 1][0], (&s_ru)[TT][64] = s_in[k & 1][1], (&s_dy)[TT][64] = s_in[k & 1][2];
     const bool mine = t0 + lt < t1;
-    float sig[E], gate[E];  // the slope of the rate, the logistic function of z
 #pragma unroll
     for (int e = 0; e < E; ++e) {  // a step past the end has rate 0 and dy 0: it changes nothing
-      float rate = (float)vd[e] + bias[e];
-      sig[e] = 1.0f;
-      if (soft) rate = softplus(rate, sig[e]);
+      const int c = lc + e;
+      const float u = (float)vu[e], z = pz ? (float)vz[e] : 0.0f, d = (float)vo[e];
+      float rate = (float)vd[e] + s_bias[c], slope = 1.0f;
+      if (soft) rate = softplus(rate, slope);
       rate = mine ? rate : 0.0f;
-      gate[e] = pz ? sigmoid((float)cz[e]) : 1.0f;
-      s_rate[lt][lc + e] = rate;
-      s_ru[lt][lc + e] = rate * (float)cu[e];
-      s_dy[lt][lc + e] = pz ? (float)co[e] * ((float)cz[e] * gate[e]) : (float)co[e];
+      const float gate = pz ? sigmoid(z) : 1.0f;
+      s_rate[lt][c] = rate;
+      s_ru[lt][c] = rate * u;
+      s_dy[lt][c] = pz ? d * (z * gate) : d;
+      s_kept[U][lt][c] = u;
+      s_kept[Z][lt][c] = z;
+      s_kept[DOUT][lt][c] = d;
+      s_kept[SLOPE][lt][c] = slope;
+      s_kept[GATE][lt][c] = gate;
     }
     const uint64_t starts = start_mask(io, at.r, t0, t1);
     __syncthreads();
@@ -614,14 +640,18 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : 2) void backward(
     po -= TT * io.dout_t;
     if (pz) pz -= TT * io.z_t;
     fetch(k > 0);
-    const float* from = io.checkpoints + checkpoint_at(a, t0 / KC, at.r, at.td, w * NS, lane);
+    if (k > 0) {
+      from -= ckpt_step;
+#pragma unroll
+      for (int q = 0; q < NS / 4; ++q) start[q] = *(const float4*)(from + q * 256);
+    }
     float* to = a.parts_bc + ((((t0 / 16 * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS / 4) * 2 + (t0 / 8 & 1)) * 64 + lane;
     auto tile = [&](auto any) __attribute__((always_inline)) {
       constexpr bool CUTS = decltype(any)::value;
 #pragma unroll
       for (int nb = 0; nb < NS; nb += 4) {
         {
-          const float4 h0 = *(const float4*)(from + nb * 64);
+          const float4 h0 = h_start[nb >> 2];
           CONSTANT(f32x16)* p = base + (nb >> 2) * share;
           float h[4] = {h0.x, h0.y, h0.z, h0.w};
           float dec[KC][4], ah[KC][4];  // a[t] and a[t] h[t - 1]
@@ -729,15 +759,16 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : 2) void backward(
           ga += s_ga[i][lt][lc + e];
           y += s_y[i][lt][lc + e];
         }
-        const float uu = (float)cu[e], rt = s_rate[lt][lc + e], dy = s_dy[lt][lc + e];
+        const int c = lc + e;
+        const float u = s_kept[U][lt][c], rt = s_rate[lt][c], dy = s_dy[lt][c], skip = s_skip[c];
         if (pz) {
-          const float zz = (float)cz[e];
-          dz[e] = (float)co[e] * __builtin_fmaf(skip[e], uu, y) * (gate[e] * (1.0f + zz * (1.0f - gate[e])));
+          const float z = s_kept[Z][lt][c], gate = s_kept[GATE][lt][c];
+          dz[e] = s_kept[DOUT][lt][c] * __builtin_fmaf(skip, u, y) * (gate * (1.0f + z * (1.0f - gate)));
         }
-        du[e] = __builtin_fmaf(skip[e], dy, rt * gb);
-        dd[e] = __builtin_fmaf(gb, uu, ga * LN2) * sig[e];
-        dskip[e] = __builtin_fmaf(dy, uu, dskip[e]);
-        dbias[e] += dd[e];
+        du[e] = __builtin_fmaf(skip, dy, rt * gb);
+        dd[e] = __builtin_fmaf(gb, u, ga * LN2) * s_kept[SLOPE][lt][c];
+        s_kept[DSKIP][lt][c] += dy * u;
+        s_kept[DBIAS][lt][c] += dd[e];
       }
       store<T, E>(qu, du, n, vec);
       store<T, E>(qd, dd, n, vec);
@@ -746,7 +777,6 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : 2) void backward(
     qu -= TT * io.du_t;
     qd -= TT * io.ddelta_t;
     if (pz) qz -= TT * io.dz_t;
-    __syncthreads();  // the next tile's stores to s_rate .. s_dy
   }
   // this chunk's parts of dA (D, N), dD (D) and ddelta_bias (D), in one row
   const int64_t D = io.channels;
@@ -759,19 +789,17 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : 2) void backward(
         if (io.dstate && t_begin == 0) io.dstate[slot + w * NS + i] = carry[i];
       }
   }
-  // dD and ddelta_bias: the threads of the same channels add up through LDS
-  float* red = &s_gb[0][0][0];
-  for (int pass = 0; pass < 2; ++pass) {
-    __syncthreads();
+  // dD and ddelta_bias: the threads of the same channels add up
+  __syncthreads();
+  if (threadIdx.x < 64 && live) {
+    float dskip = 0.0f, dbias = 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) red[lt * 64 + lc + e] = pass ? dbias[e] : dskip[e];
-    __syncthreads();
-    if (threadIdx.x < 64 && live) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < TT; ++i) sum += red[i * 64 + lane];
-      part[D * (N + pass) + ch] = sum;
+    for (int i = 0; i < TT; ++i) {
+      dskip += s_kept[DSKIP][i][lane];
+      dbias += s_kept[DBIAS][i][lane];
     }
+    part[D * N + ch] = dskip;
+    part[D * (N + 1) + ch] = dbias;
   }
 }
 
