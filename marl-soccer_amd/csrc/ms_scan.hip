@@ -49,7 +49,7 @@ struct Plan {
   int64_t units;            // scalar units along time (of all steps, and one more that is only fetched)
   int64_t tiles, blocks_d;  // tiles per group, tiles * groups
   int64_t chunks, chunk;    // over time; steps per chunk (a multiple of 32)
-  int64_t kc, bt;           // checkpoints; tiles of 16 steps of the backward pass
+  int64_t kc;               // checkpoints, tiles of the backward pass
 };
 
 struct Work {  // the workspace, in floats
@@ -68,23 +68,34 @@ struct Args {
 };
 
 // B and C (T, R, G, N) of any strides and type -> float32 in the order that the scans' scalar loads
-// want: [row][group][states / unit][16 / unit steps][B, C][16], zeros past the last step and state
+// want: [row][group][states / unit][16 / unit steps][B, C][16], zeros past the last step and state. A
+// block takes a unit's steps of some neighbouring rows, so that it reads runs of rows and writes whole
+// units: wave c writes the c-th 16 B of each, its lanes the shares of the states, then the rows.
 template <typename T>
 __global__ __launch_bounds__(256) void widen(const ms_scan_io io, int unit, int shares, int64_t units, float* __restrict__ to) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int e = (int)(i & 15), kind = (int)(i >> 4 & 1);
-  int64_t k = i >> 5;
-  const int64_t v = k % units;
-  k /= units;
-  const int share = (int)(k % shares);
-  k /= shares;
-  const int64_t g = k % io.groups, r = k / io.groups;
-  if (r >= io.rows) return;
-  const int n = share * unit + e % unit;
-  const int64_t t = v * (16 / unit) + e / unit;
-  const bool in = n < io.states && t < io.steps;
-  const T* p = kind ? (const T*)io.C + t * io.C_t + r * io.C_r + g * io.C_g : (const T*)io.B + t * io.B_t + r * io.B_r + g * io.B_g;
-  to[i] = in ? (float)p[n] : 0.0f;
+  const int lane = threadIdx.x & 63, c = threadIdx.x >> 6;
+  const unsigned per_wave = 64 / shares, rgs = (unsigned)(io.rows * io.groups);
+  const int64_t first = (int64_t)blockIdx.x * per_wave, v0 = first / rgs;
+  const unsigned i = (unsigned)(first - v0 * rgs) + lane / shares;
+  const int share = lane % shares;
+  const int64_t v = v0 + i / rgs;
+  const unsigned rg = i % rgs, r = rg / (unsigned)io.groups, g = rg - r * (unsigned)io.groups;
+  if (v >= units) return;
+  const int log = 31 - __builtin_clz(unit);
+  float* q = to + (((int64_t)rg * shares + share) * units + v) * 32 + c * 4;
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind) {
+    const T* p = kind ? (const T*)io.C + r * io.C_r + g * io.C_g : (const T*)io.B + r * io.B_r + g * io.B_g;
+    const int64_t step = kind ? io.C_t : io.B_t;
+    float x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int e = c * 4 + k, n = share * unit + (e & (unit - 1));
+      const int64_t t = v * (16 / unit) + (e >> log);
+      x[k] = n < io.states && t < io.steps ? (float)p[t * step + n] : 0.0f;
+    }
+    *(float4*)(q + kind * 16) = make_float4(x[0], x[1], x[2], x[3]);
+  }
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -114,12 +125,19 @@ __device__ __forceinline__ int64_t checkpoint_at(const Args& a, int64_t k, int64
   return (((k * a.io.rows + r) * a.p.blocks_d + td) * (a.p.ns * a.p.nw / 4) + state / 4) * 256 + lane * 4 + state % 4;
 }
 
-// Which steps of a tile begin an episode, as a mask the whole wave shares
-__device__ __forceinline__ uint64_t start_mask(const ms_scan_io& io, int64_t r, int64_t t0, int64_t t1) {
-  if (!io.starts) return 0;
-  const int64_t t = t0 + (threadIdx.x & 63);
-  return __ballot(t < t1 && io.starts[t * io.starts_t + r * io.starts_r] != 0);
-}
+// Which steps of a tile begin an episode, as a mask the whole wave shares: lane l looks at step l
+struct Starts {
+  const uint8_t* p;
+  int64_t by;
+  __device__ __forceinline__ Starts(const ms_scan_io& io, int64_t r, int64_t t0, int64_t steps)
+      : p(io.starts ? io.starts + r * io.starts_r + (t0 + (threadIdx.x & 63)) * io.starts_t : nullptr), by(steps * io.starts_t) {}
+  __device__ __forceinline__ uint64_t mask(int steps) const {  // of the tile's first `steps` steps
+    return p ? __ballot((int)(threadIdx.x & 63) < steps && *p != 0) : 0;
+  }
+  __device__ __forceinline__ void move() {
+    if (p) p += by;
+  }
+};
 
 struct Place {  // a block's channels
   int64_t r, chunk, g, c0;  // row, chunk, group, first channel
@@ -216,7 +234,8 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
   int left = (int)(t_end - t_begin);  // steps of the chunk not done yet
   fetch(lt < left);
   Scalars s = scalars(next);
-  for (int64_t t0 = t_begin; left > 0; t0 += TT, left -= TT) {
+  Starts flags(io, at.r, t_begin, TT);
+  for (; left > 0; left -= TT) {
     const V cu = vu, cz = vz;
     const bool mine = lt < left;
 #pragma unroll
@@ -227,7 +246,8 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
       s_rate[lt][column<E>(lc + e, lt)] = rate;
       s_ru[lt][column<E>(lc + e, lt)] = rate * (float)cu[e];
     }
-    const uint64_t starts = start_mask(io, at.r, t0, t0 + (left < TT ? left : TT));
+    const uint64_t starts = flags.mask(left < TT ? left : TT);
+    flags.move();
     __syncthreads();
     fetch(lt + TT < left);
     float rate[G], ru[G];
@@ -238,7 +258,7 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
     }
     const int steps = left < TT ? (left + G - 1) / G * G : TT;
     for (int t = 0; t < steps; t += G) {
-      if (keep && (((int)t0 + t) & (KC - 1)) == 0) {  // the states before step t0 + t
+      if (keep && (G >= KC || (t & (KC - 1)) == 0)) {  // the states before this step: tiles are multiples of KC
         if constexpr (NS == 2) {
           *(float2*)ckpt = make_float2(h[0], h[1]);
         } else {
@@ -497,6 +517,7 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
     if (z) vz = load<T, E>(z + (t + lt) * io.z_t, in ? n : 0, vec);
   };
   fetch(t_begin + (tiles - 1) * TT);
+  Starts flags(io, at.r, t_begin + (tiles - 1) * TT, -TT);
   for (int64_t k = tiles - 1; k >= 0; --k) {
     const int64_t t0 = t_begin + k * TT, t1 = t0 + TT < t_end ? t0 + TT : t_end;
     const bool mine = t0 + lt < t1;
@@ -507,7 +528,8 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
       s_rate[lt][column<E>(lc + e, lt)] = mine ? rate : 0.0f;
       s_dy[lt][column<E>(lc + e, lt)] = z ? (float)vy[e] * silu((float)vz[e]) : (float)vy[e];
     }
-    const uint64_t starts = start_mask(io, at.r, t0, t1);
+    const uint64_t starts = flags.mask((int)(t1 - t0));
+    flags.move();
     __syncthreads();
     fetch(t0 - TT);
     for (int t = TT - G; t >= 0; t -= G) {
@@ -559,8 +581,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
   const int n = at.nc - lc < 0 ? 0 : at.nc - lc;
   const int64_t t_begin = at.chunk * a.p.chunk;
   const int64_t t_end = t_begin + a.p.chunk < io.steps ? t_begin + a.p.chunk : io.steps;
-  const int64_t cl = at.c0 + lc, tiles = (t_end - t_begin + TT - 1) / TT;
-  const int64_t last = t_begin + (tiles - 1) * TT + lt;
+  const int len = (int)(t_end - t_begin), tiles = (len + TT - 1) / TT;
+  const int64_t cl = at.c0 + lc, last = t_begin + (tiles - 1) * TT + lt;
   const T* pu = (const T*)io.u + at.r * io.u_r + cl + last * io.u_t;
   const T* pd = (const T*)io.delta + at.r * io.delta_r + cl + last * io.delta_t;
   const T* pz = io.z ? (const T*)io.z + at.r * io.z_r + cl + last * io.z_t : nullptr;
@@ -599,23 +621,22 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
   V vu, vd, vz, vo;
   float4 start[NS / 4];  // the checkpoint, a tile ahead as the rest
   const int64_t ckpt_step = io.rows * a.p.blocks_d * (NS * NW / 4) * 256;
-  const float* from = io.checkpoints + checkpoint_at(a, t_begin / KC + tiles - 1, at.r, at.td, w * NS, lane);
+  const float* from = io.checkpoints + checkpoint_at(a, t_begin / KC + tiles - 1, at.r, at.td, w * NS, 0);
+  const int64_t to_step = io.rows * a.p.blocks_d * (NS * NW / 4) * 64;
+  float* to = a.parts_bc + (((t_begin / KC + tiles - 1) * io.rows + at.r) * a.p.blocks_d + at.td) * (NS * NW / 4) * 64 + w * (NS / 4) * 64;
+  Starts flags(io, at.r, t_begin + (tiles - 1) * TT, -TT);
   auto fetch = [&](bool in) __attribute__((always_inline)) {
     vu = load<T, E>(pu, in ? n : 0, vec);
     vd = load<T, E>(pd, in ? n : 0, vec);
     vo = load<T, E>(po, in ? n : 0, vec);
     if (pz) vz = load<T, E>(pz, in ? n : 0, vec);
   };
-  fetch(last < t_end);
+  fetch((tiles - 1) * TT + lt < len);
 #pragma unroll
-  for (int q = 0; q < NS / 4; ++q) start[q] = *(const float4*)(from + q * 256);
-  for (int64_t k = tiles - 1; k >= 0; --k) {
-    const int64_t t0 = t_begin + k * TT, t1 = t0 + TT < t_end ? t0 + TT : t_end;
-    float4 h_start[NS / 4];
-#pragma unroll
-    for (int q = 0; q < NS / 4; ++q) h_start[q] = start[q];
+  for (int q = 0; q < NS / 4; ++q) start[q] = *(const float4*)(from + q * 256 + lane * 4);
+  for (int k = tiles - 1; k >= 0; --k) {
     float(&s_rate)[TT][64] = s_in[k & 1][0], (&s_ru)[TT][64] = s_in[k & 1][1], (&s_dy)[TT][64] = s_in[k & 1][2];
-    const bool mine = t0 + lt < t1;
+    const bool mine = k * TT + lt < len;
 #pragma unroll
     for (int e = 0; e < E; ++e) {  // a step past the end has rate 0 and dy 0: it changes nothing
       const int c = lc + e;
@@ -633,29 +654,25 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
       s_kept[SLOPE][lt][c] = slope;
       s_kept[GATE][lt][c] = gate;
     }
-    const uint64_t starts = start_mask(io, at.r, t0, t1);
+    const uint64_t starts = flags.mask(len - k * TT < TT ? len - k * TT : TT);
+    flags.move();
     __syncthreads();
     pu -= TT * io.u_t;
     pd -= TT * io.delta_t;
     po -= TT * io.dout_t;
     if (pz) pz -= TT * io.z_t;
     fetch(k > 0);
-    if (k > 0) {
-      from -= ckpt_step;
-#pragma unroll
-      for (int q = 0; q < NS / 4; ++q) start[q] = *(const float4*)(from + q * 256);
-    }
-    float* to = a.parts_bc + ((((t0 / 16 * io.rows + at.r) * a.p.blocks_d + at.td) * NW + w) * (NS / 4) * 2 + (t0 / 8 & 1)) * 64 + lane;
+    if (k > 0) from -= ckpt_step;
     auto tile = [&](auto any) __attribute__((always_inline)) {
       constexpr bool CUTS = decltype(any)::value;
 #pragma unroll
       for (int nb = 0; nb < NS; nb += 4) {
         {
-          const float4 h0 = h_start[nb >> 2];
+          const float4 h0 = start[nb >> 2];
           CONSTANT(f32x16)* p = base + (nb >> 2) * share;
           float h[4] = {h0.x, h0.y, h0.z, h0.w};
           float dec[KC][4], ah[KC][4];  // a[t] and a[t] h[t - 1]
-          f32x16 b = p[0];
+          f32x16 b = p[0], c_last;
 #pragma unroll
           for (int t4 = 0; t4 < KC; t4 += 4) {
             float rate[4], ru[4];
@@ -665,7 +682,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
               ru[j] = s_ru[t4 + j][lane];
             }
             loads_done();
-            const f32x16 b_next = p[(t4 + 4 < KC ? t4 + 4 : KC - 4) / 4 * 2];
+            f32x16 b_next = b;
+            if (t4 + 4 < KC) b_next = p[(t4 + 4) / 4 * 2];
+            else c_last = p[KC / 4 * 2 - 1];
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -681,9 +700,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
             __builtin_amdgcn_sched_barrier(0);
             b = b_next;
           }
+          start[nb >> 2] = *(const float4*)(from + nb * 64 + lane * 4);  // the next tile's
           Scalars s;
           s.b = b;
-          s.c = p[KC / 4 * 2 - 1];
+          s.c = c_last;
           float pair = 0.0f, four = 0.0f, eight = 0.0f;  // folded registers of 1, 2 and 4 steps that wait for their other half
 #pragma unroll
           for (int t4 = KC - 4; t4 >= 0; t4 -= 4) {
@@ -695,7 +715,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
               ru[j] = s_ru[t4 + j][lane];
             }
             loads_done();
-            const Scalars prev = scalars(p + (t4 ? t4 - 4 : 0) / 4 * 2);
+            Scalars prev = s;
+            if (t4) prev = scalars(p + (t4 - 4) / 4 * 2);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 3; j >= 0; --j) {
@@ -734,7 +755,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
                 } else {
                   x = fold_dpp<XOR2>(x, four, lane & 2);
                   if (t & 4) eight = x;
-                  else to[(nb >> 2) * 2 * 64] = fold_dpp<XOR1>(x, eight, lane & 1);
+                  else to[(nb >> 2) * 64 + lane] = fold_dpp<XOR1>(x, eight, lane & 1);
                 }
               }
             }
@@ -747,6 +768,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
     if (starts) tile(std::true_type{});
     else tile(std::false_type{});
     base -= TT / 4 * 2;
+    to -= to_step;
     __syncthreads();
     if (mine && n > 0) {
       float du[E], dd[E], dz[E];
@@ -815,28 +837,35 @@ __global__ __launch_bounds__(64 * WAVES) void finish_weights(const float* __rest
   else if (c < dn + 2 * D) { if (io.ddelta_bias) io.ddelta_bias[c - dn - D] = sum; }
 }
 
-// dB, dC: the tiles of a group added and put in place. A thread per (t, r, g, n) and kind.
+// dB, dC: the tiles of a group added and put in place. A wave takes 8 steps of a row's group, 64 sums
+// (4 states of both, one a lane as the folds left them) at a time; `split` waves share a row's states
+// where rows and steps alone are too few waves.
 template <typename T>
-__global__ __launch_bounds__(256) void finish_bc(const Args a) {
+__global__ __launch_bounds__(256) void finish_bc(const Args a, int split) {
   const ms_scan_io& io = a.io;
-  const int64_t per = io.steps * io.rows * io.groups * io.states;
-  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= 2 * per) return;
-  const int kind = i >= per;
-  if (kind) i -= per;
-  const int64_t s = i % io.states;
-  int64_t k = i / io.states;
-  const int64_t g = k % io.groups;
-  k /= io.groups;
-  const int64_t r = k % io.rows, t = k / io.rows;
-  const int64_t ns = a.p.ns, w = s / ns, nb = s % ns / 4;
-  const int64_t lane = (kind * 4 + s % 4) * 8 + lane_of_step((int)(t & 7));
-  const int64_t one = a.p.nw * (ns / 4) * 2 * 64;  // a tile's floats
-  const float* p = a.parts_bc + ((t / 16 * io.rows + r) * a.p.blocks_d + g * a.p.tiles) * one +
-                   ((w * (ns / 4) + nb) * 2 + t % 16 / 8) * 64 + lane;
-  float sum = 0.0f;
-  for (int64_t j = 0; j < a.p.tiles; ++j) sum += p[j * one];
-  ((T*)(kind ? io.dC : io.dB))[i] = (T)sum;
+  const int lane = threadIdx.x & 63, n4 = a.p.ns * a.p.nw / 4;
+  const unsigned wave = blockIdx.x * 4 + (unsigned)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned k = wave / (unsigned)split, first = wave - k * (unsigned)split;
+  const unsigned rgs = (unsigned)(io.rows * io.groups), t8 = k / rgs, rg = k - t8 * rgs;
+  if (t8 >= (io.steps + 7) / 8) return;
+  const unsigned r = rg / (unsigned)io.groups, g = rg - r * (unsigned)io.groups;
+  const int64_t one = n4 * 64, tiles = a.p.tiles;  // a tile's floats
+  const float* p = a.parts_bc + ((t8 * io.rows + r) * a.p.blocks_d + g * tiles) * one + lane;
+  const int item = lane >> 3;
+  const int64_t t = (int64_t)t8 * 8 + lane_of_step(lane & 7);  // its own inverse
+  T* out = (T*)(item & 4 ? io.dC : io.dB) + ((t * io.rows + r) * io.groups + g) * io.states;
+  for (int q = (int)first; q < n4; q += split) {
+    float sum = 0.0f;
+    int64_t j = 0;
+    for (; j + 4 <= tiles; j += 4) {
+      const float x0 = p[j * one + q * 64], x1 = p[(j + 1) * one + q * 64], x2 = p[(j + 2) * one + q * 64],
+                  x3 = p[(j + 3) * one + q * 64];
+      sum += (x0 + x1) + (x2 + x3);
+    }
+    for (; j < tiles; ++j) sum += p[j * one + q * 64];
+    const int s = q * 4 + (item & 3);
+    if (s < io.states && t < io.steps) out[s] = (T)sum;
+  }
 }
 
 // ---------------------------------------------------------------- the host's side
@@ -858,7 +887,6 @@ Plan plan(const ms_scan_io& io, bool back) {
   p.chunk = p.chunk < 32 ? 32 : p.chunk;
   p.chunks = io.steps > 0 ? (io.steps + p.chunk - 1) / p.chunk : 1;
   p.kc = (io.steps + KC - 1) / KC;
-  p.bt = (io.steps + 15) / 16;
   p.unit = back ? 4 : p.ns;
   // whole tiles of 32 steps, and a unit past the end
   p.units = (io.steps + 31) / 32 * 32 * p.unit / 16 + 1;
@@ -887,7 +915,7 @@ Work work(const ms_scan_io& io, const Plan& p, bool back) {
     w.cut = (int*)take(parts);
   }
   if (back) {
-    w.parts_bc = take(p.bt * io.rows * p.blocks_d * p.nw * (p.ns / 4) * 2 * 64);
+    w.parts_bc = take(p.kc * io.rows * p.blocks_d * (p.ns * p.nw / 4) * 64);
     w.parts = take(parts * row);
     const int64_t share = share_of(parts);
     w.sums = share ? take((parts + share - 1) / share * row) : nullptr;
@@ -900,6 +928,7 @@ const char* check(const ms_scan_io* io, bool back, bool step) {
   if (!io) return "no arguments";
   if (io->dtype < 0 || io->dtype > 2) return "dtype must be 0 (float32), 1 (bfloat16) or 2 (float16)";
   if (io->steps < 0 || io->rows < 0 || io->channels <= 0) return "steps and rows must be >= 0, channels > 0";
+  if (io->steps > 0x7fffff00) return "too many steps";
   if (io->states < 1 || io->states > 64) return "1 to 64 states are supported";
   if (io->groups < 1 || io->channels % io->groups) return "groups must divide the channels";
   if (step && io->steps != 1) return "a step has steps = 1";
@@ -940,8 +969,8 @@ int prepare(const ms_scan_io& io, const Plan& p, const Work& w, bool back, hipSt
   a.parts = w.parts;
   a.vec = vec_ok(io, back);
   const int shares = p.ns * p.nw / p.unit;
-  const int64_t blocks = (io.rows * io.groups * shares * p.units * 32 + 255) / 256;
-  if (too_many(blocks)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
+  const int64_t each = 64 / shares, blocks = (p.units * io.rows * io.groups + each - 1) / each;
+  if (too_many(blocks) || too_many(io.rows * io.groups)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
   const dim3 grid((unsigned)blocks), block(256);
   if (io.dtype == 0) hipLaunchKernelGGL(widen<float>, grid, block, 0, stream, io, p.unit, shares, p.units, w.bc);
   else if (io.dtype == 1) hipLaunchKernelGGL(widen<bf16>, grid, block, 0, stream, io, p.unit, shares, p.units, w.bc);
@@ -1086,11 +1115,14 @@ int ms_scan_backward(const ms_scan_io* io, void* stream) {
     if (int rc = scan::launch_join<true>(a, st, who)) return rc;
   }
   if (int rc = scan::launch(scan::BACK, a, st, who)) return rc;
-  const int64_t all = 2 * io->steps * io->rows * io->groups * io->states, blocks = (all + 255) / 256;
-  if (scan::too_many(blocks)) return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
-  if (io->dtype == 0) hipLaunchKernelGGL(scan::finish_bc<float>, dim3((unsigned)blocks), dim3(256), 0, st, a);
-  else if (io->dtype == 1) hipLaunchKernelGGL(scan::finish_bc<seq::bf16>, dim3((unsigned)blocks), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(scan::finish_bc<seq::f16>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  int64_t waves = (io->steps + 7) / 8 * io->rows * io->groups;
+  const int split = waves < 32768 ? p.ns * p.nw / 4 : 1;
+  waves *= split;
+  if (scan::too_many(waves + 4)) return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
+  const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
+  if (io->dtype == 0) hipLaunchKernelGGL(scan::finish_bc<float>, grid, block, 0, st, a, split);
+  else if (io->dtype == 1) hipLaunchKernelGGL(scan::finish_bc<seq::bf16>, grid, block, 0, st, a, split);
+  else hipLaunchKernelGGL(scan::finish_bc<seq::f16>, grid, block, 0, st, a, split);
   const int64_t parts = p.chunks * io->rows, share = scan::share_of(parts), row = io->channels * (io->states + 2);
   const unsigned columns = (unsigned)((row + 63) / 64), shares = (unsigned)((parts + share - 1) / share);
   if (shares > 1)
