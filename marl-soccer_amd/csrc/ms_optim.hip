@@ -13,9 +13,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
-#ifdef MS_TUNE
-#include <stdlib.h>
-#endif
 
 #include "../../include/marl_soccer.h"
 
@@ -25,10 +22,7 @@ namespace opt {
 
 constexpr int THREADS = 256, E = 4, ROUND = THREADS * E;  // values a block handles at a time
 constexpr int LIST = MS_OPTIM_TENSORS;
-#ifndef MS_NB
-#define MS_NB 1024
-#endif
-constexpr int64_t NORM_BLOCKS = MS_NB;
+constexpr int64_t NORM_BLOCKS = 1024;
 static_assert(ROUND % MS_ADAMW_BLOCK == 0 && MS_ADAMW_BLOCK == 64 * E, "a wave's round is one scale block");
 
 typedef __bf16 bf16;
@@ -377,9 +371,6 @@ const char* check(const ms_optim_tensor* t, int64_t count, const float* workspac
 int rounds(const ms_optim_tensor* t, int64_t count) {
   int64_t all = 0;
   for (int64_t i = 0; i < count; ++i) all += t[i].numel;
-#ifdef MS_TUNE
-  if (const char* v = getenv("T_ROUNDS")) return atoi(v);
-#endif
   return all > (int64_t)ROUND * 16384 ? 8 : all > (int64_t)ROUND * 4096 ? 4 : 1;
 }
 

@@ -27,17 +27,6 @@ namespace scan {
 using namespace seq;
 
 constexpr int KC = 8;  // steps between checkpoints
-#ifdef MS_TUNE
-#include <stdlib.h>
-static int64_t tune(const char* n, int64_t d) { const char* v = getenv(n); return v ? atoll(v) : d; }
-#define TUNE_SPLIT tune(back ? "T_BSPLIT" : "T_SPLIT", 192)
-#define TUNE_TARGET tune(back ? "T_BTARGET" : "T_TARGET", 768)
-#define TUNE_MINP tune("T_MINP", 4)
-#else
-#define TUNE_SPLIT 192
-#define TUNE_TARGET 768
-#define TUNE_MINP 4
-#endif
 constexpr float LOG2E = 1.44269504f, LN2 = 0.69314718f;
 
 #define CONSTANT(T) const __attribute__((address_space(4))) T
@@ -374,39 +363,51 @@ __global__ __launch_bounds__(256) void join(const Args a) {
 }
 
 // ---------------------------------------------------------------- one step
-// The states are read and written once: HBM-bound. Q lanes of four states each share a channel.
+// The states are read and written once: HBM-bound (16,384 x 128 x 16 states: 304 MB in 68 us). Q lanes of
+// four states each share a channel. Every load is issued before the first is used, the state's too: an
+// episode's start is selected after it, where waiting for the flag first took 86 us. Two or four of
+// these a thread took longer (73, 94 us).
 template <typename T, int Q>
 __global__ __launch_bounds__(256) void step4(const ms_scan_io io) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t D = io.channels, rc = i / Q;
   if (rc >= io.rows * D) return;  // a channel's Q lanes leave together: Q divides the wave
-  const int q = (int)(i % Q) * 4;
-  const int64_t r = rc / D, c = rc - r * D, g = c / (D / io.groups);
-  const float u = (float)((const T*)io.u)[r * io.u_r + c];
-  const float d = (float)((const T*)io.delta)[r * io.delta_r + c] + (io.delta_bias ? io.delta_bias[c] : 0.0f);
-  float slope;
-  const float rate = io.softplus ? softplus(d, slope) : d, ru = rate * u;
+  const int q = (int)(threadIdx.x % Q) * 4;
+  const int64_t r = rc / D, ch = rc - r * D, g = ch / (D / io.groups);
   float4 h = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (io.state && !(io.starts && io.starts[r * io.starts_r])) h = *(const float4*)(io.state + rc * (Q * 4) + q);
-  const float4 A = *(const float4*)(io.A + c * (Q * 4) + q);
+  if (io.state) h = *(const float4*)(io.state + rc * (Q * 4) + q);
+  const bool cut = io.starts && io.starts[r * io.starts_r];
+  const float u = (float)((const T*)io.u)[r * io.u_r + ch];
+  const float d = (float)((const T*)io.delta)[r * io.delta_r + ch] + (io.delta_bias ? io.delta_bias[ch] : 0.0f);
+  const float z = io.z ? (float)((const T*)io.z)[r * io.z_r + ch] : 0.0f;
+  const float skip = io.D ? io.D[ch] : 0.0f;
+  const float4 A = *(const float4*)(io.A + ch * (Q * 4) + q);
   const T* B = (const T*)io.B + r * io.B_r + g * io.B_g + q;
   const T* C = (const T*)io.C + r * io.C_r + g * io.C_g + q;
-  const float r2 = rate * LOG2E;
-  h.x = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.x), h.x, ru * (float)B[0]);
-  h.y = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.y), h.y, ru * (float)B[1]);
-  h.z = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.z), h.z, ru * (float)B[2]);
-  h.w = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.w), h.w, ru * (float)B[3]);
+  float b[4], c[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    b[j] = (float)B[j];
+    c[j] = (float)C[j];
+  }
+  float slope;
+  const float rate = io.softplus ? softplus(d, slope) : d, ru = rate * u, r2 = rate * LOG2E;
+  if (cut) h = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  h.x = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.x), h.x, ru * b[0]);
+  h.y = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.y), h.y, ru * b[1]);
+  h.z = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.z), h.z, ru * b[2]);
+  h.w = __builtin_fmaf(__builtin_amdgcn_exp2f(r2 * A.w), h.w, ru * b[3]);
   *(float4*)(io.new_state + rc * (Q * 4) + q) = h;
-  float y = (float)C[0] * h.x;
-  y = __builtin_fmaf((float)C[1], h.y, y);
-  y = __builtin_fmaf((float)C[2], h.z, y);
-  y = __builtin_fmaf((float)C[3], h.w, y);
+  float y = c[0] * h.x;
+  y = __builtin_fmaf(c[1], h.y, y);
+  y = __builtin_fmaf(c[2], h.z, y);
+  y = __builtin_fmaf(c[3], h.w, y);
 #pragma unroll
   for (int m = 1; m < Q; m <<= 1) y += __shfl_xor(y, m);
   if (q == 0) {
-    if (io.D) y = __builtin_fmaf(io.D[c], u, y);
-    if (io.z) y *= silu((float)((const T*)io.z)[r * io.z_r + c]);
-    ((T*)io.out)[r * io.out_r + c] = (T)y;
+    y = __builtin_fmaf(skip, u, y);
+    if (io.z) y *= silu(z);
+    ((T*)io.out)[r * io.out_r + ch] = (T)y;
   }
 }
 // any number of states: a thread per channel
@@ -870,18 +871,30 @@ __global__ __launch_bounds__(256) void finish_bc(const Args a, int split) {
 
 // ---------------------------------------------------------------- the host's side
 
+// How many states a wave holds, and whether the time axis is split. Measured at 16 states, bf16, T x D =
+// 2,048 x 2,048 a row unless stated (forward alone; forward with backward for the backward's rule):
+//   * four states a wave, four waves a block. One wave with all 16 has less to add up but leaves the
+//     SIMDs idle: 64 rows of 256 steps 259 us against 181, 8 rows 996 against 310.
+//   * forward with one block a CU (193 to 256 blocks, 8 rows): two states a wave and eight waves, 254 us
+//     against 310; with more blocks the four have it (12 rows of 1,024 steps: 204 against 253).
+//   * fewer blocks: chunks of time, 768 blocks in all. 4 rows 180 us against 301 unsplit, 6 rows (192
+//     blocks) 247 against 303, one row of 16,411 steps x 1,536 241 against 2,300.
+//   * backward: chunks up to 511 blocks, 1,536 blocks in all. 6 rows of 1,024 steps 406 us against 581,
+//     12 rows 714 against 805; 16 rows (512 blocks) 872 against 825, so not there.
+//   * chunks of 64 steps at least: 512 steps x 256 channels 39 us, 128 steps 50, 32 steps 41.
 Plan plan(const ms_scan_io& io, bool back) {
   Plan p = {};
   p.tiles = (io.channels / io.groups + 63) / 64;
   p.blocks_d = p.tiles * io.groups;
   const int64_t blocks = p.blocks_d * io.rows;
   const int np = io.states <= 4 ? 4 : io.states <= 8 ? 8 : io.states <= 16 ? 16 : io.states <= 32 ? 32 : 64;
+  const bool split = blocks > 0 && blocks <= (back ? 511 : 192);
   p.ns = np <= 16 ? 4 : np / 4;
-  if (!back && np == 16 && blocks > 192 && blocks <= 256) p.ns = 2;
+  if (!back && np == 16 && !split && blocks <= 256) p.ns = 2;
   p.nw = np / p.ns;
   const int64_t pieces = (io.steps + 31) / 32;
-  int64_t chunks = blocks > 0 && blocks <= TUNE_SPLIT ? (TUNE_TARGET + blocks - 1) / blocks : 1;
-  if (chunks > pieces / TUNE_MINP) chunks = pieces / TUNE_MINP;
+  int64_t chunks = split ? ((back ? 1536 : 768) + blocks - 1) / blocks : 1;
+  if (chunks > pieces / 2) chunks = pieces / 2;
   if (chunks < 1) chunks = 1;
   p.chunk = (pieces + chunks - 1) / chunks * 32;
   p.chunk = p.chunk < 32 ? 32 : p.chunk;

@@ -487,3 +487,26 @@ def test_a_chain_of_both_matches_the_references():
         ref.assert_close("out", out, want, size, k)
         ref.assert_close("state", s, h, hs, k)
         assert torch.equal(cs.double().cpu(), cnew)
+
+
+@gpu
+@pytest.mark.parametrize("R,D,N,G", [(70, 130, 16, 1), (100, 130, 12, 1), (200, 80, 16, 2), (260, 64, 5, 1)])
+def test_ssm_scan_many_rows(R, D, N, G):
+    """Row counts on both sides of the launch's choices: one block a compute unit and more."""
+    need_gpu()
+    T = 21
+    v = scan_inputs(T, R, D, N, G, torch.float32, 91, "cuda", starts=True, state=True)
+    g = gen(92)
+    check_scan(v, True, torch.randn((T, R, D), generator=g).cuda(), torch.randn((R, D, N), generator=g).cuda())
+
+
+@gpu
+@pytest.mark.parametrize("N", [3, 8, 12, 16, 17, 40, 64])
+@pytest.mark.parametrize("T", [63, 64, 65, 129, 300])
+def test_ssm_scan_chunk_edges(T, N):
+    """Lengths around the chunks and tiles a split time axis has, for every way the states are shared."""
+    need_gpu()
+    v = scan_inputs(T, 2, 70, N, 1, torch.float32, 93, "cuda", state=True)
+    v["starts"] = (torch.rand((T, 2), generator=gen(94)) < 0.02).cuda()
+    g = gen(95)
+    check_scan(v, True, torch.randn((T, 2, 70), generator=g).cuda(), torch.randn((2, 70, N), generator=g).cuda())
