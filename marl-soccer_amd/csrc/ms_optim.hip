@@ -145,7 +145,7 @@ __device__ __forceinline__ float wave_max(float x) {
 
 // Eight bits for a moment: a wave's 256 values share the scale max|.| / 448, so the largest is held
 // to a unit in the last place of float32 and the others to e4m3's half step, 2^-4 of the value, down
-// to 2^-16 of the largest. The second moment is held as its root, which halves the range it spans. A
+// to 2^-15 of the largest. The second moment is held as its root, which halves the range it spans. A
 // change of less than half a step is not kept, except by the largest, through the scale. Blocks under
 // 2^-100 are held as zeros, where the scale's inverse would overflow.
 __device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_lane) {

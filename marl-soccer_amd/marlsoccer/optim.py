@@ -191,6 +191,13 @@ class AdamW(torch.optim.Optimizer):
         self._work = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "state_bits": self.state_bits}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._work = {}  # a copy's own
+
     @property
     def last_grad_norm(self):
         """The norm of the last clipped step, one float32 on the device (None before it)."""
@@ -199,6 +206,7 @@ class AdamW(torch.optim.Optimizer):
     def _state_of(self, p):
         s = self.state[p]
         if not s:
+            self._refuse_capture(p)
             dt = F8 if self.state_bits == 8 else torch.float32
             s["step"] = torch.zeros((), dtype=torch.int64, device=p.device)
             s["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device).to(dt)
@@ -207,6 +215,11 @@ class AdamW(torch.optim.Optimizer):
                 for k in ("exp_avg_scale", "exp_avg_sq_scale"):
                     s[k] = torch.zeros(scales_for(p.numel()), dtype=torch.float32, device=p.device)
         return s
+
+    @staticmethod
+    def _refuse_capture(p):
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: take one step before the capture: a graph that made the moments would zero them at every replay")
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
@@ -217,6 +230,9 @@ class AdamW(torch.optim.Optimizer):
             if i in state_dict["state"]:
                 self.state[p] = {k: v.to(device=p.device, copy=True) if isinstance(v, torch.Tensor) else v
                                  for k, v in state_dict["state"][i].items()}
+                step = self.state[p].get("step")
+                if isinstance(step, (int, float, torch.Tensor)):  # torch's own AdamW counts in float32, on the host
+                    self.state[p]["step"] = torch.as_tensor(step).to(device=p.device, dtype=torch.int64)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -245,6 +261,7 @@ class AdamW(torch.optim.Optimizer):
         if not groups:
             return loss
         if device.type == "cuda" and device not in self._work:
+            self._refuse_capture(every_param[0])
             self._work[device] = (torch.zeros(WORKSPACE, dtype=torch.float32, device=device),
                                   torch.zeros((), dtype=torch.float32, device=device))
         work, norm = self._work.get(device, (None, None))

@@ -171,7 +171,8 @@ class DeviceRollout:
     An agent with a memory (Agent(memory=...)) runs with policy="torch" (its default then): every
     step the memory of all 2 N rows is stepped in place, from zeros where an episode ended before it.
     collect() then also returns "memory_state", the state before the rollout's first step, with which
-    agent.memory(x, dones.reshape(T, -1).bool(), memory_state) replays the rollout for the update.
+    agent.memory(x, dones.reshape(T, -1).bool(), memory_state) replays the rollout for the update. A
+    caller that resets the batch between rollouts zeroes the tensors of `memory_state` too.
     """
 
     def __init__(self, batch, agent: Agent, normalizer: RunningMeanStd, num_steps: int, seed: int = 0,

@@ -19,7 +19,8 @@ and for one step, with the states renewed in place:
 Everything that varies in time has one type (float32, bfloat16 or float16); weights, A, D, biases and
 the scan's states are float32. Results are rounded once, and repeat bit for bit (no atomics). The
 sequence forms carry gradients to every input but `starts` (once: no double backward). Calls are
-asynchronous on the current stream of the tensors' device and may be captured into a HIP graph.
+asynchronous on the current stream of the tensors' device and may be captured into a HIP graph; a
+captured forward and backward need leaves that no eager autograd graph holds any more.
 """
 from __future__ import annotations
 
@@ -53,8 +54,28 @@ def _call(fn, io, index) -> None:
         _fail(rc)
 
 
-# a tensor written behind autograd's back: a graph that saved it refuses its backward
-_renewed = torch.autograd.graph.increment_version
+def _renewed(t):
+    """t was written behind autograd's back: a graph that saved it refuses its backward."""
+    if not t.is_inference():  # those carry no version, and no graph saves them
+        torch.autograd.graph.increment_version(t)
+
+
+def _mark(*inputs):
+    """Refuses a forward under graph capture whose leaves are held by a living eager graph: their
+    gradient accumulators belong to that graph's stream, and the captured backward would have to wait
+    for it, at which torch ends the process. An eager forward leaves its stream on the accumulators,
+    which live as long as a graph holds them: the caller keeps what is returned until its own does."""
+    leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
+    if not leaves:
+        return leaves
+    here, capturing = torch.cuda.current_stream(leaves[0].device).cuda_stream, torch.cuda.is_current_stream_capturing()
+    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves]
+    for node in nodes:
+        if capturing and node.metadata.get("marlsoccer.stream", here) != here:
+            raise RuntimeError("a graph capture needs leaves that no eager autograd graph holds: drop the outputs and losses "
+                               "of earlier forward passes before capturing")
+        node.metadata["marlsoccer.stream"] = here
+    return nodes
 
 
 def _p(t):
@@ -226,7 +247,9 @@ def short_conv(x, weight, bias=None, state=None, starts=None, activation=None, r
     and with return_state the state after the last step (inputs from before the last start as
     zeros). Gradients flow to x, weight, bias, state and back from the returned state."""
     _conv_check("short_conv", x, weight, bias, state, starts, activation, 3)
+    held = _mark(x, weight, bias, state) if torch.is_grad_enabled() else None
     out, new = _ShortConv.apply(x, weight, bias, state, starts, activation == "silu", return_state)
+    del held  # now the graph holds them
     return (out, new) if return_state else out
 
 
@@ -368,8 +391,10 @@ def ssm_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, state=None, sta
     input but starts, and back from the returned state; with them the forward also keeps the states
     of every 16th step (4 N bytes a channel) until the backward."""
     _scan_check("ssm_scan", u, delta, A, B, C, D, z, delta_bias, state, starts, 3)
+    held = _mark(u, delta, A, B, C, D, z, delta_bias, state) if torch.is_grad_enabled() else None
     grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (u, delta, A, B, C, D, z, delta_bias, state))
     out, new = _Scan.apply(u, delta, A, B, C, D, z, delta_bias, state, starts, bool(delta_softplus), return_state, grad)
+    del held
     return (out, new) if return_state else out
 
 

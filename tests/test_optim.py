@@ -341,3 +341,67 @@ def test_c_entries_refuse_bad_arguments():
     assert L.ms_grad_clip(rows, 1, 0.0, None, 16, None) == N.MS_ERR_INVALID_ARGUMENT
     rows[0].dtype = 5
     assert L.ms_grad_clip(rows, 1, 1.0, None, 16, None) == N.MS_ERR_INVALID_ARGUMENT
+
+
+@gpu
+def test_copies_and_torchs_own_state():
+    """A deep copy goes on like the original; torch.optim.AdamW's state_dict is taken over."""
+    import copy
+    need_gpu()
+    ps, _ = make([(20, 5), (7,)], torch.float32, 50)
+    params = [torch.nn.Parameter(p.clone()) for p in ps]
+    theirs = torch.optim.AdamW(params, lr=1e-3, weight_decay=0.02)
+
+    def grads(k):
+        for p, g in zip(params, make([(20, 5), (7,)], torch.float32, 60 + k)[1]):
+            p.grad = g
+
+    for k in range(3):
+        grads(k)
+        theirs.step()
+    mine = optim.AdamW(params, lr=1e-3, weight_decay=0.02)
+    mine.load_state_dict(theirs.state_dict())
+    assert all(int(mine.state[p]["step"]) == 3 for p in params)
+    grads(3)
+    before = [p.detach().clone() for p in params]
+    mine.step()
+    mine_after = [p.detach().clone() for p in params]
+    for p, b in zip(params, before):
+        p.data.copy_(b)
+    theirs.step()
+    for p, a in zip(params, mine_after):
+        assert float((p.detach() - a).abs().max()) <= 48 * U * 10 * 1e-3 + 6 * U  # one step's worth of both's roundings
+    twin = copy.deepcopy(mine)
+    assert twin.state_bits == 32 and twin.max_grad_norm is None
+    twin.step()  # its parameters have no gradients' history of their own, but deep copies of them
+
+
+@gpu
+def test_a_first_step_is_not_captured():
+    need_gpu()
+    ps, gs = make([(8, 3)], torch.float32, 70)
+    p = torch.nn.Parameter(ps[0].clone())
+    p.grad = gs[0]
+    opt = optim.AdamW([p], max_grad_norm=1.0)
+    torch.cuda.synchronize()
+    count = torch.zeros(1, device="cuda")
+    refused = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(refused):
+        count.add_(1)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            opt.step()
+    assert torch.equal(p.detach(), ps[0])
+    opt.step()
+    assert int(opt.state[p]["step"]) == 1
+
+
+@gpu
+def test_a_saved_parameter_that_was_stepped_refuses_its_backward():
+    need_gpu()
+    p = torch.nn.Parameter(torch.ones(4, device="cuda"))
+    opt = optim.AdamW([p])
+    loss = (p * p).sum()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

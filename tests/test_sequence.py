@@ -510,3 +510,106 @@ def test_ssm_scan_chunk_edges(T, N):
     v["starts"] = (torch.rand((T, 2), generator=gen(94)) < 0.02).cuda()
     g = gen(95)
     check_scan(v, True, torch.randn((T, 2, 70), generator=g).cuda(), torch.randn((2, 70, N), generator=g).cuda())
+
+
+@gpu
+def test_strides_past_32_bits():
+    """Steps that lie more than 2^31 elements apart."""
+    need_gpu()
+    far = 2 ** 31 + 64
+    T, R, D, N = 3, 2, 64, 16
+    big = torch.empty(2 * far + 8 * R * (D + N), dtype=torch.bfloat16, device="cuda")
+
+    def place(t, at):
+        view = big.as_strided((T, *t.shape[1:]), (far, *t[0].stride()), at)
+        view.copy_(t)
+        return view
+
+    v = scan_inputs(T, R, D, N, 1, torch.bfloat16, 101, "cuda", state=True, starts=True)
+    c = conv_inputs(T, R, D, 4, torch.bfloat16, 102, "cuda", state=True, starts=True)
+    dout = torch.randn((T, R, D), generator=gen(103)).bfloat16().cuda()
+    w, at = dict(v), 0
+    for k in ("u", "delta", "z", "B", "C"):
+        w[k] = place(v[k], at)
+        at += v[k][0].numel()
+    cw = dict(c, x=place(c["x"], at))
+    for fn, a, b, kw in ((seq.ssm_scan, v, w, {}), (seq.short_conv, c, cw, dict(activation="silu"))):
+        got = []
+        for args in (a, b):
+            leaves = {k: t.detach().requires_grad_() if k != "starts" else t for k, t in args.items()}
+            out, new = fn(**leaves, **kw, return_state=True)
+            got.append([out, new, *torch.autograd.grad(out, [leaves[k] for k in leaves if k != "starts"], dout)])
+        for x, y in zip(*got):
+            assert torch.equal(x, y)
+
+
+@gpu
+def test_steps_in_inference_mode_and_a_saved_state_that_was_renewed():
+    need_gpu()
+    v = scan_inputs(1, 2, 16, 4, 1, torch.float32, 111, "cuda", state=True)
+    at = {k: (t[0] if t is not None and k in ("u", "delta", "B", "C", "z") else t) for k, t in v.items()}
+    c = conv_inputs(1, 2, 16, 4, torch.float32, 112, "cuda", state=True)
+    with torch.inference_mode():
+        state, cstate = v["state"].clone(), c["state"].clone()
+        y = seq.ssm_step(**{**at, "state": state})
+        seq.short_conv_step(c["x"][0], cstate, c["weight"], c["bias"])
+    assert torch.isfinite(y).all() and not torch.equal(state, v["state"])
+    u = v["u"].clone().requires_grad_()
+    out = seq.ssm_scan(**{**v, "u": u})
+    seq.ssm_step(**at)  # renews the state that the scan saved
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_marks_live_with_the_graph_that_holds_a_leaf(monkeypatch):
+    """The bookkeeping behind the refusal below, without a device: the mark of an eager forward stays on a
+    leaf while a graph holds it, is seen from another stream's capture, and goes with the graph."""
+    stream, capturing = [1], [False]
+    monkeypatch.setattr(seq.torch.cuda, "current_stream", lambda device=None: type("S", (), {"cuda_stream": stream[0]}))
+    monkeypatch.setattr(seq.torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    leaf = torch.ones(3, requires_grad=True)
+    other = leaf * 2  # not a leaf: nothing to mark
+    assert seq._mark(None, other, torch.ones(3)) == []
+    del other
+    held = seq._mark(leaf)
+    out = leaf * 3
+    del held
+    stream[0], capturing[0] = 2, True
+    with pytest.raises(RuntimeError, match="no eager autograd graph"):
+        seq._mark(leaf)
+    stream[0] = 1  # captured on the stream it was marked on
+    assert len(seq._mark(leaf)) == 1
+    stream[0] = 2
+    del out
+    assert len(seq._mark(leaf)) == 1  # the graph is gone, and the mark with it
+
+
+@gpu
+def test_capture_refuses_leaves_that_an_eager_graph_holds():
+    need_gpu()
+    v = scan_inputs(5, 2, 16, 4, 1, torch.float32, 121, "cuda")
+    leaves = {k: t.detach().requires_grad_() if t is not None and k != "starts" else t for k, t in v.items()}
+    dout = torch.ones((5, 2, 16), device="cuda")
+
+    def train():
+        out = seq.ssm_scan(**leaves)
+        return torch.autograd.grad(out, [t for t in leaves.values() if t is not None], dout)
+
+    held = seq.ssm_scan(**leaves)  # an eager graph that goes on living
+    torch.cuda.synchronize()
+    count = torch.zeros(1, device="cuda")
+    refused = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(refused):
+        count.add_(1)
+        with pytest.raises(RuntimeError, match="no eager autograd graph"):
+            seq.ssm_scan(**leaves)
+    del held
+    want = train()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = train()
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
