@@ -216,15 +216,21 @@ def lib():
     return L
 
 
+_cuda = None  # (torch.cuda, the current raw stream of a device), looked up at the first launch
+
+
 def on_current_stream(index: int, fn, *args) -> int:
     """fn(*args, the current stream of device `index`) with that device current: its status."""
-    import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    stream = raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
-    if torch.cuda.current_device() == index:
-        return fn(*args, stream)
-    with torch.cuda.device(index):
-        return fn(*args, stream)
+    global _cuda
+    if _cuda is None:
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _cuda = torch.cuda, raw or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    cuda, raw_stream = _cuda
+    if cuda.current_device() == index:
+        return fn(*args, raw_stream(index))
+    with cuda.device(index):
+        return fn(*args, raw_stream(index))
 
 
 def check(rc: int, what: str = "") -> None:

@@ -54,7 +54,7 @@ def _bad(name, want):
 
 _ROW = "6QQq2i"  # ms_optim_tensor
 _ROW_BYTES = struct.calcsize("<" + _ROW)
-_KIND, _DTYPE = attrgetter("dtype", "shape"), attrgetter("dtype")
+_DTYPE, _SHAPE = attrgetter("dtype"), attrgetter("shape")
 _where, _ptr_of, _numel, _packed = (getattr(torch.Tensor, k) for k in ("get_device", "data_ptr", "numel", "is_contiguous"))
 
 
@@ -67,11 +67,10 @@ def _entries(params, grads, exp_avg, exp_avg_sq, steps, scales, sq_scales):
         if ts is not None and len(ts) != n:
             _bad(name, f"a list of {n} tensors, one for every parameter")
     every = [*params, *grads, *exp_avg, *exp_avg_sq]
-    kinds = list(map(_KIND, every))
-    of_params, moment = kinds[:n], F8 if bits8 else torch.float32
-    moments = [(moment, shape) for _, shape in of_params]
-    if not (kinds[n:2 * n] == of_params and kinds[2 * n:3 * n] == moments and kinds[3 * n:] == moments
-            and all(map(_packed, every)) and all(dt in _DTYPES for dt, _ in of_params)
+    dts, shapes, moment = list(map(_DTYPE, every)), list(map(_SHAPE, every)), F8 if bits8 else torch.float32
+    of_params = dts[:n]
+    if not (dts[n:2 * n] == of_params and dts[2 * n:] == [moment] * (2 * n) and all(dt in _DTYPES for dt in set(of_params))
+            and shapes[:n] == shapes[n:2 * n] == shapes[2 * n:3 * n] == shapes[3 * n:] and all(map(_packed, every))
             and all(dt is torch.int64 for dt in map(_DTYPE, steps)) and all(k == 1 for k in map(_numel, steps))
             and len({*map(_where, every), *map(_where, steps)}) == 1):
         for p, g, m, v, s in zip(params, grads, exp_avg, exp_avg_sq, steps):
@@ -88,7 +87,7 @@ def _entries(params, grads, exp_avg, exp_avg_sq, steps, scales, sq_scales):
         a = b = repeat(0)
     at = list(map(_ptr_of, every))
     rows = zip(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], a, b, map(_ptr_of, steps), sizes,
-               (_DTYPES[dt] for dt, _ in of_params), repeat(0))
+               [_DTYPES[dt] for dt in of_params], repeat(0))
     return struct.pack("<" + _ROW * n, *chain.from_iterable(rows)), params[0].device
 
 

@@ -35,12 +35,15 @@ MAX_STATES = 64
 
 
 # ms_conv_io and ms_scan_io (include/marl_soccer.h), packed in one go: a step's latency is the host's
-_CONV = struct.Struct("<4i3q" + "Qqq" + "QQQ" + "Qqq" + "Qqq" + "Q" + "Qqq" + "Q" + "Qqq" + "QQQ" + "Qq")
-_SCAN = struct.Struct("<4i3q" + "Qqq" * 3 + "Qqqq" * 2 + "QQQQ" + "Qqq" * 2 + "QQ" + "Qqq" + "Q" + "Qqq" * 3 + "Q" * 7 + "q")
+_CONV_HEAD, _CONV_TAIL = "<4i3q" + "Qqq" + "QQQ" + "Qqq" + "Qqq" + "Q", "Qqq" + "Q" + "Qqq" + "QQQ" + "Qq"
+_CONV = struct.Struct(_CONV_HEAD + _CONV_TAIL)
+_SCAN_HEAD, _SCAN_TAIL = "<4i3q" + "Qqq" * 3 + "Qqqq" * 2 + "QQQQ" + "Qqq" * 2 + "Q", "Q" + "Qqq" + "Q" + "Qqq" * 3 + "Q" * 7 + "q"
+_SCAN = struct.Struct(_SCAN_HEAD + _SCAN_TAIL)
 assert _CONV.size == N.C.sizeof(N.MsConvIO) and _SCAN.size == N.C.sizeof(N.MsScanIO)
 _NONE3 = (0, 0, 0)
-_NO_GRADS = (0,) * 12  # ms_conv_io from dout on
-_NO_SCAN_GRADS = (0,) * 22  # ms_scan_io from checkpoints on
+# a step's: the head alone, and zeros from dout (ms_conv_io) or checkpoints (ms_scan_io) on
+_CONV_STEP, _CONV_ZEROS = struct.Struct(_CONV_HEAD), bytes(struct.calcsize("<" + _CONV_TAIL))
+_SCAN_STEP, _SCAN_ZEROS = struct.Struct(_SCAN_HEAD), bytes(struct.calcsize("<" + _SCAN_TAIL))
 
 
 def _fail(rc: int) -> None:
@@ -264,8 +267,8 @@ def short_conv_step(x, state, weight, bias=None, starts=None, activation=None):
     out = torch.empty((R, D), dtype=x.dtype, device=x.device)
     at = state.data_ptr()
     _call(N.lib().ms_conv_forward,
-          _CONV.pack(_DTYPES[x.dtype], weight.shape[1], activation == "silu", 0, 1, R, D, *_row3(x), weight.data_ptr(), _p(bias),
-                     at, *_row3(starts), out.data_ptr(), 0, D, at, *_NO_GRADS), x.get_device())
+          _CONV_STEP.pack(_DTYPES[x.dtype], weight.shape[1], activation == "silu", 0, 1, R, D, x.data_ptr(), 0, x.stride(0),
+                          weight.data_ptr(), _p(bias), at, *_row3(starts), out.data_ptr(), 0, D, at) + _CONV_ZEROS, x.get_device())
     _renewed(state)
     return out
 
@@ -409,9 +412,9 @@ def ssm_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=None, starts=N
     out = torch.empty((R, ch), dtype=u.dtype, device=u.device)
     grouped, at = B.dim() == 3, state.data_ptr()
     _call(N.lib().ms_scan_step,
-          _SCAN.pack(_DTYPES[u.dtype], bool(delta_softplus), A.shape[1], B.shape[1] if grouped else 1, 1, R, ch, *_row3(u),
-                     *_row3(delta), *_row3(z), *_row3(B), B.stride(1) if grouped else 0, *_row3(C), C.stride(1) if grouped else 0,
-                     A.data_ptr(), _p(D), _p(delta_bias), at, *_row3(starts), out.data_ptr(), 0, ch, at, *_NO_SCAN_GRADS),
-          u.get_device())
+          _SCAN_STEP.pack(_DTYPES[u.dtype], bool(delta_softplus), A.shape[1], B.shape[1] if grouped else 1, 1, R, ch, u.data_ptr(),
+                          0, u.stride(0), delta.data_ptr(), 0, delta.stride(0), *_row3(z), B.data_ptr(), 0, B.stride(0),
+                          B.stride(1) if grouped else 0, C.data_ptr(), 0, C.stride(0), C.stride(1) if grouped else 0, A.data_ptr(),
+                          _p(D), _p(delta_bias), at, *_row3(starts), out.data_ptr(), 0, ch, at) + _SCAN_ZEROS, u.get_device())
     _renewed(state)
     return out
