@@ -25,6 +25,7 @@ captured forward and backward need leaves that no eager autograd graph holds any
 from __future__ import annotations
 
 import struct
+import weakref
 
 import torch
 
@@ -39,6 +40,7 @@ _CONV_HEAD, _CONV_TAIL = "<4i3q" + "Qqq" + "QQQ" + "Qqq" + "Qqq" + "Q", "Qqq" + 
 _CONV = struct.Struct(_CONV_HEAD + _CONV_TAIL)
 _SCAN_HEAD, _SCAN_TAIL = "<4i3q" + "Qqq" * 3 + "Qqqq" * 2 + "QQQQ" + "Qqq" * 2 + "Q", "Q" + "Qqq" + "Q" + "Qqq" * 3 + "Q" * 7 + "q"
 _SCAN = struct.Struct(_SCAN_HEAD + _SCAN_TAIL)
+_POINTER, _WORKSPACE, _KEEP_AT = struct.Struct("<Q"), struct.Struct("<Qq"), struct.calcsize("<" + _SCAN_HEAD.lstrip("<"))
 assert _CONV.size == N.C.sizeof(N.MsConvIO) and _SCAN.size == N.C.sizeof(N.MsScanIO)
 _NONE3 = (0, 0, 0)
 # a step's: the head alone, and zeros from dout (ms_conv_io) or checkpoints (ms_scan_io) on
@@ -63,22 +65,31 @@ def _renewed(t):
         torch.autograd.graph.increment_version(t)
 
 
-def _mark(*inputs):
-    """Refuses a forward under graph capture whose leaves are held by a living eager graph: their
-    gradient accumulators belong to that graph's stream, and the captured backward would have to wait
-    for it, at which torch ends the process. An eager forward leaves its stream on the accumulators,
-    which live as long as a graph holds them: the caller keeps what is returned until its own does."""
-    leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf]
-    if not leaves:
-        return leaves
-    here, capturing = torch.cuda.current_stream(leaves[0].device).cuda_stream, torch.cuda.is_current_stream_capturing()
-    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves]
-    for node in nodes:
-        if capturing and node.metadata.get("marlsoccer.stream", here) != here:
+# the autograd nodes of eager forwards that some graph still holds
+_living = weakref.WeakSet()
+
+
+def _refuse_held(*inputs):
+    """Refuses a forward under graph capture whose leaves an eager graph still holds: their gradient
+    accumulators belong to that graph's stream, and the captured backward would have to wait for it,
+    at which torch ends the process."""
+    here = torch.cuda.current_stream().cuda_stream
+    for node in list(_living):
+        if node.stream != here and any(getattr(f, "variable", None) is t for f, _ in node.next_functions for t in inputs
+                                       if t is not None and t.requires_grad):
             raise RuntimeError("a graph capture needs leaves that no eager autograd graph holds: drop the outputs and losses "
                                "of earlier forward passes before capturing")
-        node.metadata["marlsoccer.stream"] = here
-    return nodes
+
+
+def _lives(ctx):
+    """A forward's node, noted with its stream for as long as a graph holds it."""
+    ctx.stream = torch.cuda.current_stream().cuda_stream
+    _living.add(ctx)
+
+
+def _with_workspace(io, work):
+    """The packed arguments with their last two, the workspace and its size, filled in."""
+    return io[:-_WORKSPACE.size] + _WORKSPACE.pack(work.data_ptr(), work.numel())
 
 
 def _p(t):
@@ -169,11 +180,11 @@ def _rows(t):
 # ---------------------------------------------------------------- short convolution
 
 def _conv_io(x, weight, bias, state, starts, silu, out=None, new=None, dout=None, dnew=None, dx=None, dstate=None,
-             dweight=None, dbias=None, work=0, work_bytes=0):
+             dweight=None, dbias=None):
     T, R, D = x.shape
     return _CONV.pack(_DTYPES[x.dtype], weight.shape[1], silu, 0, T, R, D, *_p3(x), weight.data_ptr(), _p(bias), _p(state),
                       *_p3(starts), *_p3(out), _p(new), *_p3(dout), _p(dnew), *_p3(dx), _p(dstate), _p(dweight), _p(dbias),
-                      work, work_bytes)
+                      0, 0)
 
 
 def _conv_right(x, weight, bias, state, starts, activation, dims):
@@ -209,15 +220,21 @@ def _conv_check(who, x, weight, bias, state, starts, activation, dims):
     _on_gpu(who, device)
 
 
+def _conv_forward(x, weight, bias, state, starts, silu, want_state):
+    out = _like(x)
+    new = torch.empty((x.shape[1], weight.shape[1] - 1, x.shape[2]), dtype=x.dtype, device=x.device) if want_state else None
+    _call(N.lib().ms_conv_forward, _conv_io(x, weight, bias, state, starts, silu, out, new), x.get_device())
+    return out, new
+
+
 class _ShortConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, state, starts, silu, want_state):
-        out = _like(x)
-        new = torch.empty((x.shape[1], weight.shape[1] - 1, x.shape[2]), dtype=x.dtype, device=x.device) if want_state else None
-        _call(N.lib().ms_conv_forward, _conv_io(x, weight, bias, state, starts, silu, out, new), x.get_device())
+        out, new = _conv_forward(x, weight, bias, state, starts, silu, want_state)
         ctx.save_for_backward(x, weight, bias, state, starts)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
+        _lives(ctx)
         return out, new
 
     @staticmethod
@@ -234,10 +251,9 @@ class _ShortConv(torch.autograd.Function):
         dstate = torch.empty_like(state) if state is not None and need[3] else None
         dnew = None if dnew is None else dnew.contiguous()
         L = N.lib()
-        args = (x, weight, bias, state, starts, ctx.silu, None, None, dout, dnew, dx, dstate, dweight, dbias)
-        size = L.ms_conv_workspace(_conv_io(*args))
-        work = torch.empty((size,), dtype=torch.uint8, device=x.device)
-        _call(L.ms_conv_backward, _conv_io(*args, work.data_ptr(), size), x.get_device())
+        io = _conv_io(x, weight, bias, state, starts, ctx.silu, None, None, dout, dnew, dx, dstate, dweight, dbias)
+        work = torch.empty((L.ms_conv_workspace(io),), dtype=torch.uint8, device=x.device)
+        _call(L.ms_conv_backward, _with_workspace(io, work), x.get_device())
         return dx if need[0] else None, dweight, dbias, dstate, None, None, None
 
 
@@ -250,9 +266,12 @@ def short_conv(x, weight, bias=None, state=None, starts=None, activation=None, r
     and with return_state the state after the last step (inputs from before the last start as
     zeros). Gradients flow to x, weight, bias, state and back from the returned state."""
     _conv_check("short_conv", x, weight, bias, state, starts, activation, 3)
-    held = _mark(x, weight, bias, state) if torch.is_grad_enabled() else None
-    out, new = _ShortConv.apply(x, weight, bias, state, starts, activation == "silu", return_state)
-    del held  # now the graph holds them
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, state)):
+        if torch.cuda.is_current_stream_capturing():
+            _refuse_held(x, weight, bias, state)
+        out, new = _ShortConv.apply(x, weight, bias, state, starts, activation == "silu", return_state)
+    else:
+        out, new = _conv_forward(x, weight, bias, state, starts, activation == "silu", return_state)
     return (out, new) if return_state else out
 
 
@@ -330,34 +349,40 @@ def _scan_check(who, u, delta, A, B, Cm, D, z, delta_bias, state, starts, dims):
 
 
 def _scan_io(u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft, out=None, new=None, keep=None, dout=None, dnew=None,
-             du=None, ddelta=None, dz=None, dB=None, dC=None, dA=None, dD=None, dbias=None, dstate=None, work=0, work_bytes=0):
+             du=None, ddelta=None, dz=None, dB=None, dC=None, dA=None, dD=None, dbias=None, dstate=None):
     T, R, ch = u.shape
     return _SCAN.pack(_DTYPES[u.dtype], soft, A.shape[1], B.shape[2] if B.dim() == 4 else 1, T, R, ch, *_p3(u), *_p3(delta),
                       *_p3(z), *_g4(B), *_g4(Cm), A.data_ptr(), _p(D), _p(delta_bias), _p(state), *_p3(starts), *_p3(out),
                       _p(new), _p(keep), *_p3(dout), _p(dnew), *_p3(du), *_p3(ddelta), *_p3(dz), _p(dB), _p(dC), _p(dA), _p(dD),
-                      _p(dbias), _p(dstate), work, work_bytes)
+                      _p(dbias), _p(dstate), 0, 0)
+
+
+def _scan_forward(u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft, want_state, want_grad):
+    """The outputs, the last states, and what the backward reads beside the inputs."""
+    L = N.lib()
+    out = _like(u)
+    new = torch.empty((u.shape[1], *A.shape), dtype=torch.float32, device=u.device) if want_state else None
+    io = _scan_io(u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft, out, new)
+    keep = None
+    if want_grad:
+        keep = torch.empty((L.ms_scan_checkpoints(io),), dtype=torch.uint8, device=u.device)
+        io = io[:_KEEP_AT] + _POINTER.pack(keep.data_ptr()) + io[_KEEP_AT + _POINTER.size:]
+    size = L.ms_scan_workspace(io, 0)
+    if size:
+        work = torch.empty((size,), dtype=torch.uint8, device=u.device)
+        io = _with_workspace(io, work)
+    _call(L.ms_scan_forward, io, u.get_device())
+    return out, new, keep
 
 
 class _Scan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft, want_state, want_grad):
-        L = N.lib()
-        out = _like(u)
-        new = torch.empty((u.shape[1], *A.shape), dtype=torch.float32, device=u.device) if want_state else None
-        args = (u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft, out, new)
-        io = _scan_io(*args)
-        keep = None
-        if want_grad:
-            keep = torch.empty((L.ms_scan_checkpoints(io),), dtype=torch.uint8, device=u.device)
-            io = _scan_io(*args, keep)
-        size = L.ms_scan_workspace(io, 0)
-        if size:
-            work = torch.empty((size,), dtype=torch.uint8, device=u.device)
-            io = _scan_io(*args, keep, work=work.data_ptr(), work_bytes=size)
-        _call(L.ms_scan_forward, io, u.get_device())
+    def forward(ctx, u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft, want_state):
+        out, new, keep = _scan_forward(u, delta, A, B, Cm, D, z, delta_bias, state, starts, soft, want_state, True)
         ctx.save_for_backward(u, delta, A, B, Cm, D, z, delta_bias, state, starts, keep)
         ctx.soft = soft
         ctx.set_materialize_grads(False)
+        _lives(ctx)
         return out, new
 
     @staticmethod
@@ -365,7 +390,7 @@ class _Scan(torch.autograd.Function):
     def backward(ctx, dout, dnew):
         u, delta, A, B, Cm, D, z, delta_bias, state, starts, keep = ctx.saved_tensors
         if dout is None and dnew is None:
-            return (None,) * 13
+            return (None,) * 12
         need = ctx.needs_input_grad
         L = N.lib()
         dout = torch.zeros_like(u) if dout is None else _rows(dout)
@@ -377,13 +402,12 @@ class _Scan(torch.autograd.Function):
         dD = torch.empty_like(D) if D is not None and need[5] else None
         dbias = torch.empty_like(delta_bias) if delta_bias is not None and need[7] else None
         dstate = torch.empty_like(state) if state is not None and need[8] else None
-        args = (u, delta, A, B, Cm, D, z, delta_bias, state, starts, ctx.soft, None, None, keep, dout, dnew, du, ddelta, dz, dB,
-                dC, dA, dD, dbias, dstate)
-        size = L.ms_scan_workspace(_scan_io(*args), 1)
-        work = torch.empty((size,), dtype=torch.uint8, device=u.device)
-        _call(L.ms_scan_backward, _scan_io(*args, work.data_ptr(), size), u.get_device())
+        io = _scan_io(u, delta, A, B, Cm, D, z, delta_bias, state, starts, ctx.soft, None, None, keep, dout, dnew, du, ddelta,
+                      dz, dB, dC, dA, dD, dbias, dstate)
+        work = torch.empty((L.ms_scan_workspace(io, 1),), dtype=torch.uint8, device=u.device)
+        _call(L.ms_scan_backward, _with_workspace(io, work), u.get_device())
         grads = (du, ddelta, dA, dB, dC, dD, dz, dbias, dstate)
-        return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * 4
+        return tuple(g if n else None for g, n in zip(grads, need)) + (None,) * 3
 
 
 def ssm_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, state=None, starts=None, delta_softplus=True,
@@ -399,10 +423,12 @@ def ssm_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, state=None, sta
     input but starts, and back from the returned state; with them the forward also keeps the states
     of every 16th step (4 N bytes a channel) until the backward."""
     _scan_check("ssm_scan", u, delta, A, B, C, D, z, delta_bias, state, starts, 3)
-    held = _mark(u, delta, A, B, C, D, z, delta_bias, state) if torch.is_grad_enabled() else None
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (u, delta, A, B, C, D, z, delta_bias, state))
-    out, new = _Scan.apply(u, delta, A, B, C, D, z, delta_bias, state, starts, bool(delta_softplus), return_state, grad)
-    del held
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (u, delta, A, B, C, D, z, delta_bias, state)):
+        if torch.cuda.is_current_stream_capturing():
+            _refuse_held(u, delta, A, B, C, D, z, delta_bias, state)
+        out, new = _Scan.apply(u, delta, A, B, C, D, z, delta_bias, state, starts, bool(delta_softplus), return_state)
+    else:
+        out, new, _ = _scan_forward(u, delta, A, B, C, D, z, delta_bias, state, starts, bool(delta_softplus), return_state, False)
     return (out, new) if return_state else out
 
 

@@ -561,27 +561,37 @@ def test_steps_in_inference_mode_and_a_saved_state_that_was_renewed():
         out.sum().backward()
 
 
-def test_marks_live_with_the_graph_that_holds_a_leaf(monkeypatch):
-    """The bookkeeping behind the refusal below, without a device: the mark of an eager forward stays on a
-    leaf while a graph holds it, is seen from another stream's capture, and goes with the graph."""
-    stream, capturing = [1], [False]
+def test_nodes_are_noted_while_a_graph_holds_them(monkeypatch):
+    """The bookkeeping behind the refusal below, without a device: an eager forward's node is seen from
+    another stream's capture while its graph lives, and goes with it."""
+    stream = [1]
     monkeypatch.setattr(seq.torch.cuda, "current_stream", lambda device=None: type("S", (), {"cuda_stream": stream[0]}))
-    monkeypatch.setattr(seq.torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
-    leaf = torch.ones(3, requires_grad=True)
-    other = leaf * 2  # not a leaf: nothing to mark
-    assert seq._mark(None, other, torch.ones(3)) == []
-    del other
-    held = seq._mark(leaf)
-    out = leaf * 3
-    del held
-    stream[0], capturing[0] = 2, True
-    with pytest.raises(RuntimeError, match="no eager autograd graph"):
-        seq._mark(leaf)
-    stream[0] = 1  # captured on the stream it was marked on
-    assert len(seq._mark(leaf)) == 1
+
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            seq._lives(ctx)
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            return g * 2, None
+
+    leaf, other = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    out = Twice.apply(leaf, torch.ones(3))
+    seq._refuse_held(leaf)  # the same stream
     stream[0] = 2
+    seq._refuse_held(None, other, torch.ones(3), other * 2)
+    with pytest.raises(RuntimeError, match="no eager autograd graph"):
+        seq._refuse_held(other, leaf)
+    out = (out * 3).sum()
+    with pytest.raises(RuntimeError, match="no eager autograd graph"):
+        seq._refuse_held(leaf)
+    out.backward()
+    with pytest.raises(RuntimeError, match="no eager autograd graph"):
+        seq._refuse_held(leaf)  # a graph that has run its backward still holds the leaf
     del out
-    assert len(seq._mark(leaf)) == 1  # the graph is gone, and the mark with it
+    seq._refuse_held(leaf)
 
 
 @gpu
