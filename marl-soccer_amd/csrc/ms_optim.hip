@@ -367,7 +367,9 @@ const char* check(const ms_optim_tensor* t, int64_t count, const float* workspac
   return nullptr;
 }
 
-// rounds a block: one for lists that would otherwise leave CUs idle, four for long ones
+// Rounds a block: one for lists that would otherwise leave CUs idle (the Agent's 423 k values, step 10 us
+// and norm 10), more for long ones, so that each block's loads run ahead under its arithmetic and fewer
+// tickets are taken (201 M values in 8 bits: 0.59-0.68 ms).
 int rounds(const ms_optim_tensor* t, int64_t count) {
   int64_t all = 0;
   for (int64_t i = 0; i < count; ++i) all += t[i].numel;

@@ -324,6 +324,23 @@ def test_refusals():
     refuses("lr must be", lr=z(2))
 
 
+def test_a_tensor_given_twice_is_refused():
+    """Two blocks would race on it (a shared count would rise once for all of a launch's tensors)."""
+    def two(dt=torch.float32, n=4):
+        return [torch.zeros(n, dtype=dt), torch.zeros(n, dtype=dt)]
+
+    good = dict(params=two(), grads=two(), exp_avg=two(), exp_avg_sq=two(), steps=two(torch.int64, 1), lr=1e-3)
+    for name in ("params", "exp_avg", "exp_avg_sq", "steps"):
+        with pytest.raises(ValueError, match="given twice"):
+            optim.adamw_step(**{**good, name: [good[name][0]] * 2})
+    with pytest.raises(ValueError, match="given twice"):
+        optim.adamw_step(**{**good, "exp_avg": good["exp_avg_sq"]})
+    with pytest.raises(ValueError, match="HIP device"):  # a gradient is only read, and empty tensors have no address
+        optim.adamw_step(**{**good, "grads": [good["grads"][0]] * 2})
+    with pytest.raises(ValueError, match="HIP device"):
+        optim.adamw_step(two(n=0), two(n=0), two(n=0), two(n=0), two(torch.int64, 1), lr=1e-3)
+
+
 def test_c_entries_refuse_bad_arguments():
     from marlsoccer import _native as N
     L = N.lib()
