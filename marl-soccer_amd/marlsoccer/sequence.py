@@ -20,7 +20,8 @@ Everything that varies in time has one type (float32, bfloat16 or float16); weig
 the scan's states are float32. Results are rounded once, and repeat bit for bit (no atomics). The
 sequence forms carry gradients to every input but `starts` (once: no double backward). Calls are
 asynchronous on the current stream of the tensors' device and may be captured into a HIP graph; a
-captured forward and backward need leaves that no eager autograd graph holds any more.
+captured backward needs its forward in the same capture, and leaves (the inputs', or those they were
+computed from) that no eager autograd graph of these operators holds any more.
 """
 from __future__ import annotations
 
@@ -69,16 +70,34 @@ def _renewed(t):
 _living = weakref.WeakSet()
 
 
+def _leaves(nodes):
+    """The leaves whose gradient accumulators lie behind these autograd nodes (their ids)."""
+    found, seen, todo = set(), set(), list(nodes)
+    while todo:
+        node = todo.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        leaf = getattr(node, "variable", None)
+        if isinstance(leaf, torch.Tensor):
+            found.add(id(leaf))
+        todo.extend(f for f, _ in node.next_functions)
+    return found
+
+
 def _refuse_held(*inputs):
-    """Refuses a forward under graph capture whose leaves an eager graph still holds: their gradient
-    accumulators belong to that graph's stream, and the captured backward would have to wait for it,
-    at which torch ends the process."""
+    """Refuses a forward under graph capture whose leaves, or those its inputs were computed from, an
+    eager graph still holds: their gradient accumulators belong to that graph's stream, and the captured
+    backward would have to wait for it, at which torch ends the process."""
     here = torch.cuda.current_stream().cuda_stream
-    for node in list(_living):
-        if node.stream != here and any(getattr(f, "variable", None) is t for f, _ in node.next_functions for t in inputs
-                                       if t is not None and t.requires_grad):
-            raise RuntimeError("a graph capture needs leaves that no eager autograd graph holds: drop the outputs and losses "
-                               "of earlier forward passes before capturing")
+    others = [node for node in list(_living) if node.stream != here]
+    if not others:
+        return
+    grad = [t for t in inputs if t is not None and t.requires_grad]
+    mine = {id(t) for t in grad if t.is_leaf} | _leaves(t.grad_fn for t in grad if not t.is_leaf)
+    if mine & _leaves(others):
+        raise RuntimeError("a graph capture needs leaves that no eager autograd graph holds: drop the outputs and losses "
+                           "of earlier forward passes before capturing")
 
 
 def _lives(ctx):
@@ -421,7 +440,7 @@ def ssm_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, state=None, sta
     N 1 to 64; state (R, D, N) float32 before step 0 (None: zeros); starts (T, R); z None: no gate.
     Returns y like u, and with return_state the states after the last step. Gradients flow to every
     input but starts, and back from the returned state; with them the forward also keeps the states
-    of every 16th step (4 N bytes a channel) until the backward."""
+    of every 8th step (4 N bytes a channel), and B and C in float32, until the backward."""
     _scan_check("ssm_scan", u, delta, A, B, C, D, z, delta_bias, state, starts, 3)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (u, delta, A, B, C, D, z, delta_bias, state)):
         if torch.cuda.is_current_stream_capturing():

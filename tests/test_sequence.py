@@ -594,6 +594,32 @@ def test_nodes_are_noted_while_a_graph_holds_them(monkeypatch):
     seq._refuse_held(leaf)
 
 
+def test_nodes_are_found_behind_other_operations(monkeypatch):
+    """The same where the leaves feed the operators through torch's own: A = -exp(A_log), a projection."""
+    stream = [1]
+    monkeypatch.setattr(seq.torch.cuda, "current_stream", lambda device=None: type("S", (), {"cuda_stream": stream[0]}))
+
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            seq._lives(ctx)
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            return g * 2, None
+
+    a_log, other = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    out = Twice.apply(-torch.exp(a_log), other.detach())
+    stream[0] = 2
+    seq._refuse_held(other, -torch.exp(other))
+    for t in (a_log, -torch.exp(a_log), (other * a_log).sum()):
+        with pytest.raises(RuntimeError, match="no eager autograd graph"):
+            seq._refuse_held(other, t)
+    del out
+    seq._refuse_held(a_log, -torch.exp(a_log))
+
+
 @gpu
 def test_capture_refuses_leaves_that_an_eager_graph_holds():
     need_gpu()
