@@ -5,6 +5,8 @@
 // so a step is one launch whatever the tensors' sizes, needs no table in memory, and a captured graph
 // holds its own copy. A block finds its tensor from the running block counts, 4 values a thread and
 // round. A short list of small tensors (a policy's) is cut finer than a long one, to fill the chip.
+// 201 M values in 8 bits, clipped: 0.78 ms a call, 5.2 TB/s with the norm's read of g; the Agent's 423 k
+// values: 10 us for the norm and 10 for the step, which is a launch and a chain of two dependent reads.
 //
 // Step counts stay on the device, one a tensor: every block reads its tensor's count before it takes
 // a ticket, and the block with the last ticket raises the counts, so no second launch is needed.

@@ -15,10 +15,15 @@
 //   * where rows and channels do not fill the chip, the time axis is split into chunks: one pass
 //     leaves each chunk's end state from zero and its summed rate (the decay over a chunk is
 //     exp(A sum rate)), a small kernel joins the chunks, and the scan proper starts each chunk from
-//     its state. The first pass costs another N exponentials, so chunks are used only then.
+//     its state. The first pass costs another N exponentials, so only few rows are split.
 // Backward runs the same tiles from the end: g[t] = C dy + a[t+1] g[t+1]. The states it needs are
-// rebuilt from checkpoints of every KC = 8 steps (and B and C kept as scalars, 30 us of 950 saved); dB and dC are sums over channels, folded over the
-// wave's lanes with v_permlane swaps and DPP, and over the channel blocks by a last kernel.
+// rebuilt from checkpoints of every KC = 8 steps, B and C read as the forward left them; dB and dC are
+// sums over channels, folded over the wave's lanes with v_permlane swaps and DPP, and over the channel
+// blocks by a last kernel.
+// Measured at 16 states (time; share of the vector units' cycles that issue): forward 8 rows of 2,048
+// steps x 2,048 channels bf16 260 us, 58 %; one row of 16,411 x 1,536 bf16 in 31 chunks 106 + 133 us,
+// 77 and 72 %; with gradients 2,048 rows of 128 x 128 f32 243 us forward, 59 %, and 600 us backward,
+// 67 % (107 vector instructions a wave, step and four states).
 #include <type_traits>
 
 #include "ms_sequence.h"
@@ -59,9 +64,10 @@ struct Args {
 // B and C (T, R, G, N) of any strides and type -> float32 in the order that the scans' scalar loads
 // want: [row][group][states / unit][16 / unit steps][B, C][16], zeros past the last step and state. A
 // block takes a unit's steps of some neighbouring rows, so that it reads runs of rows and writes whole
-// units: wave c writes the c-th 16 B of each, its lanes the shares of the states, then the rows.
+// units: wave c writes the c-th 16 B of each, its lanes the shares of the states, then the rows. vec: units
+// of four states and more, whose four neighbours are read in one access.
 template <typename T>
-__global__ __launch_bounds__(256) void widen(const ms_scan_io io, int unit, int shares, int64_t units, float* __restrict__ to) {
+__global__ __launch_bounds__(256) void widen(const ms_scan_io io, int unit, int shares, int64_t units, bool vec, float* __restrict__ to) {
   const int lane = threadIdx.x & 63, c = threadIdx.x >> 6;
   const unsigned per_wave = 64 / shares, rgs = (unsigned)(io.rows * io.groups);
   const int64_t first = (int64_t)blockIdx.x * per_wave, v0 = first / rgs;
@@ -77,11 +83,20 @@ __global__ __launch_bounds__(256) void widen(const ms_scan_io io, int unit, int 
     const T* p = kind ? (const T*)io.C + r * io.C_r + g * io.C_g : (const T*)io.B + r * io.B_r + g * io.B_g;
     const int64_t step = kind ? io.C_t : io.B_t;
     float x[4];
+    const int n0 = share * unit + (c * 4 & (unit - 1));
+    const int64_t t0 = v * (16 / unit) + (c * 4 >> log);
+    if (vec && n0 + 4 <= io.states && t0 < io.steps) {  // four states of one step
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      const T4 four = *(const T4*)(p + t0 * step + n0);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int e = c * 4 + k, n = share * unit + (e & (unit - 1));
-      const int64_t t = v * (16 / unit) + (e >> log);
-      x[k] = n < io.states && t < io.steps ? (float)p[t * step + n] : 0.0f;
+      for (int k = 0; k < 4; ++k) x[k] = (float)four[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int e = c * 4 + k, n = share * unit + (e & (unit - 1));
+        const int64_t t = v * (16 / unit) + (e >> log);
+        x[k] = n < io.states && t < io.steps ? (float)p[t * step + n] : 0.0f;
+      }
     }
     *(float4*)(q + kind * 16) = make_float4(x[0], x[1], x[2], x[3]);
   }
@@ -363,7 +378,8 @@ __global__ __launch_bounds__(256) void join(const Args a) {
 }
 
 // ---------------------------------------------------------------- one step
-// The states are read and written once: HBM-bound (16,384 x 128 x 16 states: 304 MB in 68 us). Q lanes of
+// The states are read and written once: HBM-bound (16,384 x 128 x 16 states: 304 MB in
+// 63 us a call, 4.8 TB/s; 250 x 4,096, bf16: 140 MB in 28 us, 5.0 TB/s). Q lanes of
 // four states each share a channel. Every load is issued before the first is used, the state's too: an
 // episode's start is selected after it, where waiting for the flag first took 86 us. Two or four of
 // these a thread took longer (73, 94 us).
@@ -840,7 +856,8 @@ __global__ __launch_bounds__(64 * WAVES) void finish_weights(const float* __rest
 
 // dB, dC: the tiles of a group added and put in place. A wave takes 8 steps of a row's group, 64 sums
 // (4 states of both, one a lane as the folds left them) at a time; `split` waves share a row's states
-// where rows and steps alone are too few waves.
+// where rows and steps alone are too few waves. 128 steps x 2,048 rows x 128, f32: 26 us, 3.9 TB/s (37 with
+// one quad of states at a time).
 template <typename T>
 __global__ __launch_bounds__(256) void finish_bc(const Args a, int split) {
   const ms_scan_io& io = a.io;
@@ -855,18 +872,33 @@ __global__ __launch_bounds__(256) void finish_bc(const Args a, int split) {
   const int item = lane >> 3;
   const int64_t t = (int64_t)t8 * 8 + lane_of_step(lane & 7);  // its own inverse
   T* out = (T*)(item & 4 ? io.dC : io.dB) + ((t * io.rows + r) * io.groups + g) * io.states;
-  for (int q = (int)first; q < n4; q += split) {
-    float sum = 0.0f;
+  auto sums = [&](int q, auto many) __attribute__((always_inline)) {  // quads q, q + split, ...: their loads together
+    constexpr int K = decltype(many)::value, U = K == 1 ? 4 : 2;
+    float sum[K] = {};
     int64_t j = 0;
-    for (; j + 4 <= tiles; j += 4) {
-      const float x0 = p[j * one + q * 64], x1 = p[(j + 1) * one + q * 64], x2 = p[(j + 2) * one + q * 64],
-                  x3 = p[(j + 3) * one + q * 64];
-      sum += (x0 + x1) + (x2 + x3);
+    for (; j + U <= tiles; j += U) {
+      float x[K][U];
+#pragma unroll
+      for (int i = 0; i < K; ++i)
+#pragma unroll
+        for (int m = 0; m < U; ++m) x[i][m] = p[(j + m) * one + (q + i * split) * 64];
+#pragma unroll
+      for (int i = 0; i < K; ++i)
+#pragma unroll
+        for (int m = 0; m < U; m += 2) sum[i] += x[i][m] + x[i][m + 1];
     }
-    for (; j < tiles; ++j) sum += p[j * one + q * 64];
-    const int s = q * 4 + (item & 3);
-    if (s < io.states && t < io.steps) out[s] = (T)sum;
-  }
+    for (; j < tiles; ++j)
+#pragma unroll
+      for (int i = 0; i < K; ++i) sum[i] += p[j * one + (q + i * split) * 64];
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const int s = (q + i * split) * 4 + (item & 3);
+      if (s < io.states && t < io.steps) out[s] = (T)sum[i];
+    }
+  };
+  int q = (int)first;
+  for (; q + 3 * split < n4; q += 4 * split) sums(q, std::integral_constant<int, 4>{});
+  for (; q < n4; q += split) sums(q, std::integral_constant<int, 1>{});
 }
 
 // ---------------------------------------------------------------- the host's side
@@ -991,10 +1023,13 @@ int prepare(const ms_scan_io& io, const Plan& p, const Work& w, bool back, hipSt
   const int shares = p.ns * p.nw / p.unit;
   const int64_t each = 64 / shares, blocks = (p.units * io.rows * io.groups + each - 1) / each;
   if (too_many(blocks) || too_many(io.rows * io.groups)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
+  const int64_t elem = io.dtype == 0 ? 4 : 2;
+  const bool vec = p.unit >= 4 && aligned(io.B, io.B_t, io.B_r, elem, 4) && aligned(io.C, io.C_t, io.C_r, elem, 4) &&
+                   (io.groups == 1 || (io.B_g % 4 == 0 && io.C_g % 4 == 0));
   const dim3 grid((unsigned)blocks), block(256);
-  if (io.dtype == 0) hipLaunchKernelGGL(widen<float>, grid, block, 0, stream, io, p.unit, shares, p.units, w.bc);
-  else if (io.dtype == 1) hipLaunchKernelGGL(widen<bf16>, grid, block, 0, stream, io, p.unit, shares, p.units, w.bc);
-  else hipLaunchKernelGGL(widen<f16>, grid, block, 0, stream, io, p.unit, shares, p.units, w.bc);
+  if (io.dtype == 0) hipLaunchKernelGGL(widen<float>, grid, block, 0, stream, io, p.unit, shares, p.units, vec, w.bc);
+  else if (io.dtype == 1) hipLaunchKernelGGL(widen<bf16>, grid, block, 0, stream, io, p.unit, shares, p.units, vec, w.bc);
+  else hipLaunchKernelGGL(widen<f16>, grid, block, 0, stream, io, p.unit, shares, p.units, vec, w.bc);
   return launched(who);
 }
 
