@@ -21,7 +21,7 @@
 // sums over channels, folded over the wave's lanes with v_permlane swaps and DPP, and over the channel
 // blocks by a last kernel.
 // Measured at 16 states (time; share of the vector units' cycles that issue): forward 8 rows of 2,048
-// steps x 2,048 channels bf16 260 us, 58 %; one row of 16,411 x 1,536 bf16 in 31 chunks 106 + 133 us,
+// steps x 2,048 channels bf16 233 us, 65 %; one row of 16,411 x 1,536 bf16 in 31 chunks 106 + 133 us,
 // 77 and 72 %; with gradients 2,048 rows of 128 x 128 f32 243 us forward, 59 %, and 600 us backward,
 // 67 % (107 vector instructions a wave, step and four states).
 #include <type_traits>
@@ -129,17 +129,22 @@ __device__ __forceinline__ int64_t checkpoint_at(const Args& a, int64_t k, int64
   return (((k * a.io.rows + r) * a.p.blocks_d + td) * (a.p.ns * a.p.nw / 4) + state / 4) * 256 + lane * 4 + state % 4;
 }
 
-// Which steps of a tile begin an episode, as a mask the whole wave shares: lane l looks at step l
+// Which steps of a tile begin an episode, as a mask the whole wave shares: lane l looks at step l, a tile
+// ahead as every other load
 struct Starts {
   const uint8_t* p;
   int64_t by;
-  __device__ __forceinline__ Starts(const ms_scan_io& io, int64_t r, int64_t t0, int64_t steps)
-      : p(io.starts ? io.starts + r * io.starts_r + (t0 + (threadIdx.x & 63)) * io.starts_t : nullptr), by(steps * io.starts_t) {}
-  __device__ __forceinline__ uint64_t mask(int steps) const {  // of the tile's first `steps` steps
-    return p ? __ballot((int)(threadIdx.x & 63) < steps && *p != 0) : 0;
+  int now;
+  // `steps`: how many steps of the first tile there are; a tile further is `tile` steps
+  __device__ __forceinline__ Starts(const ms_scan_io& io, int64_t r, int64_t t0, int64_t tile, int steps)
+      : p(io.starts ? io.starts + r * io.starts_r + (t0 + (threadIdx.x & 63)) * io.starts_t : nullptr), by(tile * io.starts_t) {
+    read(steps);
   }
-  __device__ __forceinline__ void move() {
+  __device__ __forceinline__ void read(int steps) { now = p && (int)(threadIdx.x & 63) < steps ? *p : 0; }
+  __device__ __forceinline__ uint64_t mask() const { return p ? __ballot(now != 0) : 0; }
+  __device__ __forceinline__ void move(int steps) {  // to the next tile, of which `steps` steps are there
     if (p) p += by;
+    read(steps);
   }
 };
 
@@ -180,6 +185,10 @@ template <typename T, int NS, int NW, bool LOCAL>
 __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
   constexpr int TT = NW < 4 ? 8 * NW : 32, E = TT / NW, TPR = 64 / E;  // a tile: TT steps x 64 channels, E channels of one step a thread
   constexpr int G = 16 / NS;                                          // steps of a unit
+  // With one block a CU nothing runs beside the steps between two tiles: the next tile's rates are then
+  // computed under the loads of this one's parts (8 rows of 2,048 x 2,048: 262 -> 233 us). Where three
+  // blocks share a CU that takes 2 % longer.
+  constexpr bool TOGETHER = NW == 8;
   static_assert(TT % G == 0 && TT % 8 == 0, "tiles are whole units");
   __shared__ float s_rate[TT + G][64], s_ru[TT + G][64];  // the last unit is only fetched
   __shared__ float s_y[LOCAL ? 1 : NW][LOCAL ? 1 : TT][64];
@@ -235,25 +244,30 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
     dl += d_step;
     if (z) z += z_step;
   };
-  int left = (int)(t_end - t_begin);  // steps of the chunk not done yet
-  fetch(lt < left);
-  Scalars s = scalars(next);
-  Starts flags(io, at.r, t_begin, TT);
-  for (; left > 0; left -= TT) {
-    const V cu = vu, cz = vz;
-    const bool mine = lt < left;
+  // a tile's rates into LDS (a step past the end has rate 0: it changes nothing)
+  auto stage = [&](bool mine) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {  // a step past the end has rate 0: it changes nothing
+    for (int e = 0; e < E; ++e) {
       float slope, rate = (float)vd[e] + bias[e];
       if (soft) rate = softplus(rate, slope);
       rate = mine ? rate : 0.0f;
       s_rate[lt][column<E>(lc + e, lt)] = rate;
-      s_ru[lt][column<E>(lc + e, lt)] = rate * (float)cu[e];
+      s_ru[lt][column<E>(lc + e, lt)] = rate * (float)vu[e];
     }
-    const uint64_t starts = flags.mask(left < TT ? left : TT);
-    flags.move();
+  };
+  int left = (int)(t_end - t_begin);  // steps of the chunk not done yet
+  fetch(lt < left);
+  Scalars s = scalars(next);
+  Starts flags(io, at.r, t_begin, TT, left < TT ? left : TT);
+  if constexpr (TOGETHER) stage(lt < left);
+  for (; left > 0; left -= TT) {
+    const V cu = vu, cz = vz;
+    const bool mine = lt < left;
+    if constexpr (!TOGETHER) stage(mine);
+    const uint64_t starts = flags.mask();
     __syncthreads();
     fetch(lt + TT < left);
+    flags.move(left - TT < TT ? left - TT : TT);
     float rate[G], ru[G];
 #pragma unroll
     for (int j = 0; j < G; ++j) {
@@ -312,14 +326,26 @@ __global__ __launch_bounds__(64 * NW) void forward(const Args a) {
       }
     }
     __syncthreads();
-    if (!LOCAL) {
+    float part[TOGETHER ? NW : 1][E];
+    if constexpr (TOGETHER) {
+#pragma unroll
+      for (int k = 0; k < NW; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) part[k][e] = s_y[k][lt][column<E>(lc + e, lt)];
+      __builtin_amdgcn_sched_barrier(0);
+      if (left > TT) stage(lt + TT < left);
+    }
+    if constexpr (!LOCAL) {
       if (mine && n > 0) {
         float y[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          float v = s_y[0][lt][column<E>(lc + e, lt)];
+          float v = 0.0f;
 #pragma unroll
-          for (int k = 1; k < NW; ++k) v += s_y[k][lt][column<E>(lc + e, lt)];
+          for (int k = 0; k < NW; ++k) {
+            const float x = TOGETHER ? part[TOGETHER ? k : 0][e] : s_y[k][lt][column<E>(lc + e, lt)];
+            v = k ? v + x : x;
+          }
           y[e] = __builtin_fmaf(skip[e], (float)cu[e], v);
           if (z) y[e] *= silu((float)cz[e]);
         }
@@ -534,7 +560,7 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
     if (z) vz = load<T, E>(z + (t + lt) * io.z_t, in ? n : 0, vec);
   };
   fetch(t_begin + (tiles - 1) * TT);
-  Starts flags(io, at.r, t_begin + (tiles - 1) * TT, -TT);
+  Starts flags(io, at.r, t_begin + (tiles - 1) * TT, -TT, (int)(t_end - t_begin - (tiles - 1) * TT));
   for (int64_t k = tiles - 1; k >= 0; --k) {
     const int64_t t0 = t_begin + k * TT, t1 = t0 + TT < t_end ? t0 + TT : t_end;
     const bool mine = t0 + lt < t1;
@@ -545,10 +571,10 @@ __global__ __launch_bounds__(64 * NW) void backward_local(const Args a) {
       s_rate[lt][column<E>(lc + e, lt)] = mine ? rate : 0.0f;
       s_dy[lt][column<E>(lc + e, lt)] = z ? (float)vy[e] * silu((float)vz[e]) : (float)vy[e];
     }
-    const uint64_t starts = flags.mask((int)(t1 - t0));
-    flags.move();
+    const uint64_t starts = flags.mask();
     __syncthreads();
     fetch(t0 - TT);
+    flags.move(k > 0 ? TT : 0);
     for (int t = TT - G; t >= 0; t -= G) {
       f32x16 c[NS / 4];
 #pragma unroll
@@ -641,7 +667,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
   const float* from = io.checkpoints + checkpoint_at(a, t_begin / KC + tiles - 1, at.r, at.td, w * NS, 0);
   const int64_t to_step = io.rows * a.p.blocks_d * (NS * NW / 4) * 64;
   float* to = a.parts_bc + (((t_begin / KC + tiles - 1) * io.rows + at.r) * a.p.blocks_d + at.td) * (NS * NW / 4) * 64 + w * (NS / 4) * 64;
-  Starts flags(io, at.r, t_begin + (tiles - 1) * TT, -TT);
+  Starts flags(io, at.r, t_begin + (tiles - 1) * TT, -TT, len - (tiles - 1) * TT);
   auto fetch = [&](bool in) __attribute__((always_inline)) {
     vu = load<T, E>(pu, in ? n : 0, vec);
     vd = load<T, E>(pd, in ? n : 0, vec);
@@ -671,14 +697,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
       s_kept[SLOPE][lt][c] = slope;
       s_kept[GATE][lt][c] = gate;
     }
-    const uint64_t starts = flags.mask(len - k * TT < TT ? len - k * TT : TT);
-    flags.move();
+    const uint64_t starts = flags.mask();
     __syncthreads();
     pu -= TT * io.u_t;
     pd -= TT * io.delta_t;
     po -= TT * io.dout_t;
     if (pz) pz -= TT * io.z_t;
     fetch(k > 0);
+    flags.move(k > 0 ? TT : 0);
     if (k > 0) from -= ckpt_step;
     auto tile = [&](auto any) __attribute__((always_inline)) {
       constexpr bool CUTS = decltype(any)::value;
@@ -907,20 +933,23 @@ __global__ __launch_bounds__(256) void finish_bc(const Args a, int split) {
 // 2,048 x 2,048 a row unless stated (forward alone; forward with backward for the backward's rule):
 //   * four states a wave, four waves a block. One wave with all 16 has less to add up but leaves the
 //     SIMDs idle: 64 rows of 256 steps 259 us against 181, 8 rows 996 against 310.
-//   * forward with one block a CU (193 to 256 blocks, 8 rows): two states a wave and eight waves, 254 us
-//     against 310; with more blocks the four have it (12 rows of 1,024 steps: 204 against 253).
-//   * fewer blocks: chunks of time, 768 blocks in all. 4 rows 180 us against 301 unsplit, 6 rows (192
-//     blocks) 247 against 303, one row of 16,411 steps x 1,536 241 against 2,300.
+//   * forward of 9 to 16 states with at most one block a CU: two states a wave and eight waves, 8 rows
+//     221 us against 310; with more blocks the four have it (12 rows of 1,024 steps: 204 against 253).
+//   * fewer blocks: chunks of time, 768 blocks in all, where the steps saved pay for three more launches
+//     and twice the exponentials: a call takes 25 us + blocks x steps x 0.56 ns split, 5 us + steps x 0.106
+//     us unsplit. 3 rows (96 blocks) 136 us against 221, 4 rows 173 against 222, but 500 steps of them 66
+//     against 62; 5 rows 243 against 221; 1 row of 200 steps 39 against 30, of 16,411 x 1,536 241 against
+//     1,800. Other numbers of states, with other waves: up to 192 blocks.
 //   * backward: chunks up to 511 blocks, 1,536 blocks in all. 6 rows of 1,024 steps 406 us against 581,
 //     12 rows 714 against 805; 16 rows (512 blocks) 872 against 825, so not there.
-//   * chunks of 64 steps at least: 512 steps x 256 channels 39 us, 128 steps 50, 32 steps 41.
+//   * chunks of 64 steps at least: 512 steps x 256 channels 39 us, 128 steps at least 50, 32 steps 41.
 Plan plan(const ms_scan_io& io, bool back) {
   Plan p = {};
   p.tiles = (io.channels / io.groups + 63) / 64;
   p.blocks_d = p.tiles * io.groups;
   const int64_t blocks = p.blocks_d * io.rows;
   const int np = io.states <= 4 ? 4 : io.states <= 8 ? 8 : io.states <= 16 ? 16 : io.states <= 32 ? 32 : 64;
-  const bool split = blocks > 0 && blocks <= (back ? 511 : 192);
+  const bool split = blocks > 0 && (back ? blocks <= 511 : np == 16 ? (160 - blocks) * io.steps > 30000 : blocks <= 192);
   p.ns = np <= 16 ? 4 : np / 4;
   if (!back && np == 16 && !split && blocks <= 256) p.ns = 2;
   p.nw = np / p.ns;

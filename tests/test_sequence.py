@@ -513,6 +513,18 @@ def test_ssm_scan_chunk_edges(T, N):
 
 
 @gpu
+@pytest.mark.parametrize("N", [9, 16])
+@pytest.mark.parametrize("T", [1, 31, 32, 33, 95, 191, 193, 225, 352])
+def test_ssm_scan_around_the_split_of_16_states(T, N):
+    """Lengths around whole tiles of the unsplit form of 9 to 16 states, and around those where it splits."""
+    need_gpu()
+    v = scan_inputs(T, 3, 100, N, 1, torch.bfloat16, 131, "cuda", state=True)
+    v["starts"] = (torch.rand((T, 3), generator=gen(132)) < 0.02).cuda()
+    g = gen(133)
+    check_scan(v, True, torch.randn((T, 3, 100), generator=g).bfloat16().cuda(), torch.randn((3, 100, N), generator=g).cuda())
+
+
+@gpu
 def test_strides_past_32_bits():
     """Steps that lie more than 2^31 elements apart."""
     need_gpu()
