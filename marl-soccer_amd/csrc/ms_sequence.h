@@ -103,18 +103,16 @@ template <int WAVES>
 __device__ __forceinline__ double sum_share(const float* __restrict__ in, int64_t first, int64_t last, int64_t columns,
                                             int64_t c, double (&s)[WAVES][64]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
+  constexpr int AHEAD = 8;  // loads in flight
+  double x[AHEAD] = {};
   if (c < columns) {
     int64_t i = first + w;
-    for (; i + 3 * WAVES < last; i += 4 * WAVES) {
-      a0 += in[i * columns + c];
-      a1 += in[(i + WAVES) * columns + c];
-      a2 += in[(i + 2 * WAVES) * columns + c];
-      a3 += in[(i + 3 * WAVES) * columns + c];
-    }
-    for (; i < last; i += WAVES) a0 += in[i * columns + c];
+    for (; i + (AHEAD - 1) * WAVES < last; i += AHEAD * WAVES)
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) x[k] += in[(i + k * WAVES) * columns + c];
+    for (; i < last; i += WAVES) x[0] += in[i * columns + c];
   }
-  s[w][lane] = (a0 + a1) + (a2 + a3);
+  s[w][lane] = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
   __syncthreads();
   double a = 0.0;
   if (w == 0)
