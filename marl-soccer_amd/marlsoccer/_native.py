@@ -219,14 +219,22 @@ def lib():
 _cuda = None  # (torch.cuda, the current raw stream of a device), looked up at the first launch
 
 
+def _look_up():
+    global _cuda
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _cuda = torch.cuda, raw or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _cuda
+
+
+def current_raw_stream(index: int) -> int:
+    """The current stream of device `index`, as hipStream_t."""
+    return (_cuda or _look_up())[1](index)
+
+
 def on_current_stream(index: int, fn, *args) -> int:
     """fn(*args, the current stream of device `index`) with that device current: its status."""
-    global _cuda
-    if _cuda is None:
-        import torch
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        _cuda = torch.cuda, raw or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-    cuda, raw_stream = _cuda
+    cuda, raw_stream = _cuda or _look_up()
     if cuda.current_device() == index:
         return fn(*args, raw_stream(index))
     with cuda.device(index):

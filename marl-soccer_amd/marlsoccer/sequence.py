@@ -26,6 +26,7 @@ computed from) that no eager autograd graph of these operators holds any more.
 from __future__ import annotations
 
 import struct
+import threading
 import weakref
 
 import torch
@@ -67,7 +68,7 @@ def _renewed(t):
 
 
 # the autograd nodes of eager forwards that some graph still holds
-_living = weakref.WeakSet()
+_living, _living_lock = weakref.WeakSet(), threading.Lock()
 
 
 def _leaves(nodes):
@@ -90,7 +91,8 @@ def _refuse_held(*inputs):
     eager graph still holds: their gradient accumulators belong to that graph's stream, and the captured
     backward would have to wait for it, at which torch ends the process."""
     here = torch.cuda.current_stream().cuda_stream
-    others = [node for node in list(_living) if node.stream != here]
+    with _living_lock:
+        others = [node for node in _living if node.stream != here]
     if not others:
         return
     grad = [t for t in inputs if t is not None and t.requires_grad]
@@ -100,10 +102,11 @@ def _refuse_held(*inputs):
                            "of earlier forward passes before capturing")
 
 
-def _lives(ctx):
-    """A forward's node, noted with its stream for as long as a graph holds it."""
-    ctx.stream = torch.cuda.current_stream().cuda_stream
-    _living.add(ctx)
+def _lives(ctx, stream=None):
+    """A forward's node, noted with its stream (None: the current one) for as long as a graph holds it."""
+    ctx.stream = torch.cuda.current_stream().cuda_stream if stream is None else stream
+    with _living_lock:
+        _living.add(ctx)
 
 
 def _with_workspace(io, work):
@@ -253,7 +256,7 @@ class _ShortConv(torch.autograd.Function):
         ctx.save_for_backward(x, weight, bias, state, starts)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
-        _lives(ctx)
+        _lives(ctx, N.current_raw_stream(x.get_device()))
         return out, new
 
     @staticmethod
@@ -401,7 +404,7 @@ class _Scan(torch.autograd.Function):
         ctx.save_for_backward(u, delta, A, B, Cm, D, z, delta_bias, state, starts, keep)
         ctx.soft = soft
         ctx.set_materialize_grads(False)
-        _lives(ctx)
+        _lives(ctx, N.current_raw_stream(u.get_device()))
         return out, new
 
     @staticmethod
