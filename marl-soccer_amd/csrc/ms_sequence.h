@@ -35,6 +35,17 @@ __device__ __forceinline__ typename Vec<T, E>::type load(const T* p, int n, bool
   return v;
 }
 template <typename T, int E>
+__device__ __forceinline__ typename Vec<T, E>::type load(const T* p) {  // all of them, aligned
+  return *(const typename Vec<T, E>::type*)p;
+}
+template <typename T, int E>
+__device__ __forceinline__ void store(T* p, const float (&x)[E]) {
+  typename Vec<T, E>::type v;
+#pragma unroll
+  for (int i = 0; i < E; ++i) v[i] = (T)x[i];
+  *(typename Vec<T, E>::type*)p = v;
+}
+template <typename T, int E>
 __device__ __forceinline__ void store(T* p, const float (&x)[E], int n, bool vec) {
   if (vec && n >= E) {
     typename Vec<T, E>::type v;
