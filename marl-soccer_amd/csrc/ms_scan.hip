@@ -1025,16 +1025,6 @@ const char* check(const ms_scan_io* io, bool back, bool step) {
   return nullptr;
 }
 
-bool vec_ok(const ms_scan_io& io, bool back) {
-  const int64_t elem = io.dtype == 0 ? 4 : 2, E = 8;
-  if (io.groups > 1 && (io.channels / io.groups) % 8) return false;
-  bool ok = aligned(io.u, io.u_t, io.u_r, elem, E) && aligned(io.delta, io.delta_t, io.delta_r, elem, E) &&
-            (!io.z || aligned(io.z, io.z_t, io.z_r, elem, E));
-  if (!back) return ok && aligned(io.out, io.out_t, io.out_r, elem, E);
-  return ok && aligned(io.dout, io.dout_t, io.dout_r, elem, E) && aligned(io.du, io.du_t, io.du_r, elem, E) &&
-         aligned(io.ddelta, io.ddelta_t, io.ddelta_r, elem, E) && (!io.z || aligned(io.dz, io.dz_t, io.dz_r, elem, E));
-}
-
 // out of 32-bit grids: refused
 bool too_many(int64_t blocks) { return blocks > 0x7fffffff; }
 
@@ -1047,7 +1037,6 @@ int prepare(const ms_scan_io& io, const Plan& p, const Work& w, bool back, hipSt
   a.cut = w.cut;
   a.parts_bc = w.parts_bc;
   a.parts = w.parts;
-  a.vec = vec_ok(io, back);
   if (back && kept_scalars(io, p)) return MS_OK;
   const int shares = p.ns * p.nw / p.unit;
   const int64_t each = 64 / shares, blocks = (p.units * io.rows * io.groups + each - 1) / each;
@@ -1063,6 +1052,20 @@ int prepare(const ms_scan_io& io, const Plan& p, const Work& w, bool back, hipSt
 }
 
 enum Pass { LOCAL, MAIN, BACK_LOCAL, BACK };
+
+// Whether a pass may move the E channels of a thread at once (2,048 steps of 8 rows x 2,044 bf16, where
+// rows are aligned to 8 B: 261 us with four channels at once, 315 guarded one by one)
+bool vec_ok(const ms_scan_io& io, Pass pass, int nw) {
+  const int64_t elem = io.dtype == 0 ? 4 : 2, E = pass == BACK ? KC / nw : nw == 8 ? 4 : 8;
+  if (io.groups > 1 && (io.channels / io.groups) % E) return false;
+  auto ok = [&](const void* p, int64_t t, int64_t r) { return !p || aligned(p, t, r, elem, E); };
+  bool all = ok(io.delta, io.delta_t, io.delta_r) && ok(io.z, io.z_t, io.z_r);
+  if (pass != BACK_LOCAL) all = all && ok(io.u, io.u_t, io.u_r);
+  if (pass == MAIN) all = all && ok(io.out, io.out_t, io.out_r);
+  if (pass >= BACK_LOCAL) all = all && ok(io.dout, io.dout_t, io.dout_r);
+  if (pass == BACK) all = all && ok(io.du, io.du_t, io.du_r) && ok(io.ddelta, io.ddelta_t, io.ddelta_r) && (!io.z || ok(io.dz, io.dz_t, io.dz_r));
+  return all;
+}
 
 template <typename T, int NS, int NW>
 void launch_as(Pass pass, const Args& a, dim3 grid, hipStream_t stream) {
@@ -1081,7 +1084,8 @@ void launch_type(Pass pass, const Args& a, dim3 grid, hipStream_t stream) {
   else if (a.p.ns == 8) launch_as<T, 8, 4>(pass, a, grid, stream);
   else launch_as<T, 16, 4>(pass, a, grid, stream);
 }
-int launch(Pass pass, const Args& a, hipStream_t stream, const char* who) {
+int launch(Pass pass, Args& a, hipStream_t stream, const char* who) {
+  a.vec = vec_ok(a.io, pass, a.p.nw);
   const int64_t blocks = a.p.blocks_d * a.io.rows * a.p.chunks;
   if (too_many(blocks)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
   const dim3 grid((unsigned)blocks);

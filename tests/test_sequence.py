@@ -525,6 +525,38 @@ def test_ssm_scan_around_the_split_of_16_states(T, N):
 
 
 @gpu
+@pytest.mark.parametrize("T", [1, 3])
+@pytest.mark.parametrize("R,D,dtype", [(1500, 2048, torch.bfloat16), (700, 1028, torch.float32), (4200, 516, torch.float16), (9, 3001, torch.float32),
+                                       (11, 1030, torch.bfloat16)])
+def test_short_conv_many_rows_and_every_width_of_access(T, R, D, dtype):
+    """More rows than the blocks take at once, and channels that 8, 4, 2 or 1 of them a thread divide; the
+    step's form against the sequence's, whose first step it is."""
+    need_gpu()
+    c = conv_inputs(T, R, D, 4, dtype, 141, "cuda", starts=True, state=True)
+    out, new = seq.short_conv(**c, activation="silu", return_state=True)
+    want, want_new = ref.conv(**c)[:2]
+    ref.assert_close("out", out, want, ref.conv(**c, absolute=True)[0], 4 + 20)
+    assert torch.equal(new.double().cpu(), want_new)
+    state = c["state"].clone()
+    for t in range(T):
+        y = seq.short_conv_step(c["x"][t], state, c["weight"], c["bias"], starts=c["starts"][t], activation="silu")
+        assert torch.equal(y, out[t])
+    assert torch.equal(state, new)
+
+
+@gpu
+@pytest.mark.parametrize("G", [1, 2])
+@pytest.mark.parametrize("D,N,T", [(132, 16, 70), (130, 16, 70), (268, 5, 40), (262, 16, 400), (136, 33, 40)])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS.get)
+def test_ssm_scan_every_width_of_access(D, N, T, G, dtype):
+    """Channels whose rows are aligned to 16, 8 or 4 B, in groups that end inside them."""
+    need_gpu()
+    v = scan_inputs(T, 3, D, N, G, dtype, 151, "cuda", state=True, starts=True)
+    g = gen(152)
+    check_scan(v, True, torch.randn((T, 3, D), generator=g).to(dtype).cuda(), torch.randn((3, D, N), generator=g).cuda())
+
+
+@gpu
 def test_strides_past_32_bits():
     """Steps that lie more than 2^31 elements apart."""
     need_gpu()
