@@ -939,7 +939,9 @@ __global__ __launch_bounds__(256) void finish_bc(const Args a, int split) {
 //     and twice the exponentials: a call takes 25 us + blocks x steps x 0.56 ns split, 5 us + steps x 0.106
 //     us unsplit. 3 rows (96 blocks) 136 us against 221, 4 rows 173 against 222, but 500 steps of them 66
 //     against 62; 5 rows 243 against 221; 1 row of 200 steps 39 against 30, of 16,411 x 1,536 241 against
-//     1,800. Other numbers of states, with other waves: up to 192 blocks.
+//     1,800. Other numbers of states: up to 192 blocks of four waves, or as many waves in smaller ones (4
+//     states, 16 rows of 2,048 x 512: 94 us against 526 unsplit and 170 with 768 blocks; 8 states, 40 rows
+//     of 377 x 448: 68 against 94).
 //   * backward: chunks up to 511 blocks, 1,536 blocks in all. 6 rows of 1,024 steps 406 us against 581,
 //     12 rows 714 against 805; 16 rows (512 blocks) 872 against 825, so not there.
 //   * chunks of 64 steps at least: 512 steps x 256 channels 39 us, 128 steps at least 50, 32 steps 41.
@@ -949,12 +951,13 @@ Plan plan(const ms_scan_io& io, bool back) {
   p.blocks_d = p.tiles * io.groups;
   const int64_t blocks = p.blocks_d * io.rows;
   const int np = io.states <= 4 ? 4 : io.states <= 8 ? 8 : io.states <= 16 ? 16 : io.states <= 32 ? 32 : 64;
-  const bool split = blocks > 0 && (back ? blocks <= 511 : np == 16 ? (160 - blocks) * io.steps > 30000 : blocks <= 192);
   p.ns = np <= 16 ? 4 : np / 4;
+  const int64_t small = 4 * p.ns / np > 1 ? 4 * p.ns / np : 1;  // blocks of one or two waves: as many times the blocks
+  const bool split = blocks > 0 && (back ? blocks <= 511 * small : np == 16 ? (160 - blocks) * io.steps > 30000 : blocks <= 192 * small);
   if (!back && np == 16 && !split && blocks <= 256) p.ns = 2;
   p.nw = np / p.ns;
   const int64_t pieces = (io.steps + 31) / 32;
-  int64_t chunks = split ? ((back ? 1536 : 768) + blocks - 1) / blocks : 1;
+  int64_t chunks = split ? ((back ? 1536 : 768) * small + blocks - 1) / blocks : 1;
   if (chunks > pieces / 2) chunks = pieces / 2;
   if (chunks < 1) chunks = 1;
   p.chunk = (pieces + chunks - 1) / chunks * 32;

@@ -77,11 +77,10 @@ def _entries(params, grads, exp_avg, exp_avg_sq, steps, scales, sq_scales):
             _explain(p, g, m, v, s, moment, params[0].device)
     sizes = list(map(_numel, params))
     if bits8:
-        where = params[0].get_device()
-        for k, *pair in zip(sizes, scales, sq_scales):
-            for t in pair:
-                if t.dtype != torch.float32 or t.numel() != scales_for(k) or not t.is_contiguous() or t.get_device() != where:
-                    _bad("scales", f"contiguous float32 of {scales_for(k)} values on {params[0].device} (one for every {BLOCK} values)")
+        both = [*scales, *sq_scales]
+        if not (list(map(_numel, both)) == [-(-k // BLOCK) for k in sizes] * 2 and set(map(_DTYPE, both)) == {torch.float32}
+                and all(map(_packed, both)) and set(map(_where, both)) == {params[0].get_device()}):
+            _bad("scales", f"contiguous float32 on {params[0].device}, one for every {BLOCK} values of their parameter")
         a, b = map(_ptr_of, scales), map(_ptr_of, sq_scales)
     else:
         a = b = repeat(0)
