@@ -307,9 +307,6 @@ def _adamw_plain(s):
 
 
 def _package(name):
-    """The framework's module, imported once as a program imports it."""
-    if (got := sys.modules.get("marlsoccer." + name)) is not None:
-        return got
     if "marlsoccer" not in sys.modules:
         at = os.path.join(os.getcwd(), "marl-soccer_amd")
         if at not in sys.path:
