@@ -470,7 +470,12 @@ const char *ms_sequence_last_error(void);
  *   param, grad: dtype 0 float32, 1 bfloat16, 2 float16 (the same for both), numel elements in a row.
  *   state_bits 32: exp_avg, exp_avg_sq float32. state_bits 8: OCP e4m3 bytes, exp_avg the codes of
  *   m and exp_avg_sq those of sqrt(v), each with a float32 scale for every MS_ADAMW_BLOCK elements
- *   (value = code * scale, scale = max|.| / 448) in the *_scale arrays.
+ *   (value = code * scale, scale = max|.| / 448) in the *_scale arrays. Codes are rounded to nearest:
+ *   a change of less than half a step of the code (2^-5 to 2^-4 of the value) is then lost at every step,
+ *   however many follow, so with beta2 near 1 values keep their ratio to the block's largest for good.
+ *   state_bits 8 | MS_ADAMW_STOCHASTIC rounds them to one of the two neighbours (off by less than a
+ *   step), at random from a hash of the step count and the element's place, so that the expected value is
+ *   the unrounded one and moments follow the 32-bit ones in the mean; the same step gives the same bits.
  * ms_grad_clip: factor = min(1, max_norm / (norm + 1e-6)), norm the Euclidean norm of all the
  *   tensors' gradients (summed in float64, in a fixed order; a non-finite one passes into the
  *   update, as clip_grad_norm_ has it); also written to *grad_norm (float32, device) when non-NULL.
@@ -481,6 +486,7 @@ const char *ms_sequence_last_error(void);
 #define MS_OPTIM_WORKSPACE 4096
 #define MS_OPTIM_TENSORS 48
 #define MS_ADAMW_BLOCK 256
+#define MS_ADAMW_STOCHASTIC 256
 typedef struct ms_optim_tensor {
   void *param;
   const void *grad;

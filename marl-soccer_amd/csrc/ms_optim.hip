@@ -95,10 +95,39 @@ __device__ __forceinline__ void put_any(void* p, int dtype, int64_t i, int64_t n
   else put4<f16x4>((f16*)p, i, n, vec, v);
 }
 
-// OCP e4m3 codes, rounded to nearest even by the hardware's conversions; four in a dword
+// OCP e4m3 codes, four in a dword: rounded to nearest even by the hardware's conversions, or to one of the
+// two neighbours with the odds that keep the expected value. For these v_cvt_sr_fp8_f32 adds the upper 20
+// bits of `odds` to what e4m3 has no bits for and cuts (checked against that on the card, subnormals too);
+// 16 random bits will do: the last four stay 0, so that 448 and a unit in the last place is not carried to
+// the code after it, which is no number.
 __device__ __forceinline__ uint32_t encode(f32x4 v) {
   int c = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], c, true);
+}
+struct Odds {
+  uint32_t h[2];  // 16 bits for each of four values
+};
+__device__ __forceinline__ uint32_t encode(f32x4 v, Odds o) {
+  int c = __builtin_amdgcn_cvt_sr_fp8_f32(v[0], (int)(o.h[0] & 0xffff0000u), 0, 0);
+  c = __builtin_amdgcn_cvt_sr_fp8_f32(v[1], (int)(o.h[0] << 16), c, 1);
+  c = __builtin_amdgcn_cvt_sr_fp8_f32(v[2], (int)(o.h[1] & 0xffff0000u), c, 2);
+  return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(v[3], (int)(o.h[1] << 16), c, 3);
+}
+// A hash of a tensor's step count (one key a block) and of where in it four values lie, so that a step
+// repeats bit for bit: multiplications by odd constants and shifted xors (the constants: the golden ratio,
+// the roots of 2, 3, 5 and 7 in 32 bits).
+__device__ __forceinline__ uint32_t key_of(int64_t t) {
+  uint32_t x = (uint32_t)t * 0x9E3779B9u + (uint32_t)(t >> 32) * 0x6A09E667u;
+  x = (x ^ x >> 15) * 0xBB67AE85u;
+  return x ^ x >> 13;
+}
+__device__ __forceinline__ Odds odds_of(int64_t i, uint32_t key) {
+  uint32_t x = (uint32_t)(i / E) * 0x9E3779B9u + (uint32_t)((i / E) >> 32) * 0x6A09E667u + key;
+  x = (x ^ x >> 16) * 0xBB67AE85u;
+  x = (x ^ x >> 15) * 0x3C6EF373u;
+  x ^= x >> 16;
+  const uint32_t y = x * 0xA54FF53Bu;
+  return {{x, y ^ y >> 15}};
 }
 __device__ __forceinline__ f32x4 decode(uint32_t c) {
   f32x4 v;
@@ -146,11 +175,17 @@ __device__ __forceinline__ float wave_max(float x) {
 }
 
 // Eight bits for a moment: a wave's 256 values share the scale max|.| / 448, so the largest is held
-// to a unit in the last place of float32 and the others to e4m3's half step, 2^-4 of the value, down
-// to 2^-15 of the largest. The second moment is held as its root, which halves the range it spans. A
-// change of less than half a step is not kept, except by the largest, through the scale. Blocks under
-// 2^-100 are held as zeros, where the scale's inverse would overflow.
-__device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_lane) {
+// to a unit in the last place of float32 and the others to steps of e4m3, 2^-4 to 2^-3 of the value, down
+// to 2^-14.8 of the largest (2^-6 of the scale), and to 2^-9 of the scale below that. The second moment
+// is held as its root, which halves the range it spans. Blocks under 2^-100 are held as zeros, where the
+// scale's inverse would overflow.
+// Rounded to nearest, a step's change of less than half a unit of the codes is lost for good, and with
+// beta2 = 0.999 a root moves by some 0.05 % a step: then only the largest moves, by the scale, and the others
+// follow it (roots 0.3 to 9 times the 32-bit ones after thousands of steps whose gradients change in
+// size). SR keeps such changes in the mean: each rounding is right in expectation, and the held root
+// wanders about the 32-bit one, by some 17 % of it at beta2 = 0.999.
+template <bool SR>
+__device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_lane, Odds odds) {
   float top = 0.0f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) top = fmaxf(top, __builtin_fabsf(v[k]));
@@ -160,7 +195,8 @@ __device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_l
   if (first_lane) *scale = some ? top / 448.0f : 0.0f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) v[k] = v[k] * inv;
-  return encode(v);
+  if constexpr (SR) return encode(v, odds);
+  else return encode(v);
 }
 
 __device__ __forceinline__ bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
@@ -178,13 +214,14 @@ __device__ __forceinline__ double power(double b, int64_t t) {
 // What all of a tensor's blocks share: the step size and the root's factor of step t
 struct Factors {
   float fix1, fix2, keep, clip;
+  uint32_t key;
 };
 
 struct Moments {
   f32x4 m, v;
 };
 
-template <int BITS>
+template <int BITS, bool SR>
 __global__ __launch_bounds__(THREADS) void adamw(const List list, const Hyper hp, const Ws ws) {
   __shared__ Factors shared;
   // this block's tensor: as many as end at or before it come before it (the last end is the grid's size)
@@ -226,6 +263,7 @@ __global__ __launch_bounds__(THREADS) void adamw(const List list, const Hyper hp
     f.fix2 = (float)(1.0 / sqrt(1.0 - power(hp.beta2, t)));
     f.keep = (float)(1.0 - lr * hp.weight_decay);
     f.clip = hp.use_clip ? ws.f[0] : 1.0f;
+    f.key = SR ? key_of(t) : 0;
     if (threadIdx.x == 0) shared = f;
   }
   __syncthreads();
@@ -262,8 +300,10 @@ __global__ __launch_bounds__(THREADS) void adamw(const List list, const Hyper hp
       for (int e = 0; e < E; ++e)
         if (i + e >= n) m[e] = r[e] = 0.0f;  // values past the end count for no scale
       const int64_t q = i / MS_ADAMW_BLOCK;
-      put_codes((uint8_t*)a.exp_avg, i, n, vs, quantise(m, a.exp_avg_scale + q, lane == 0));
-      put_codes((uint8_t*)a.exp_avg_sq, i, n, vs, quantise(r, a.exp_avg_sq_scale + q, lane == 0));
+      Odds o = {};
+      if constexpr (SR) o = odds_of(i, f.key);
+      put_codes((uint8_t*)a.exp_avg, i, n, vs, quantise<SR>(m, a.exp_avg_scale + q, lane == 0, o));
+      put_codes((uint8_t*)a.exp_avg_sq, i, n, vs, quantise<SR>(r, a.exp_avg_sq_scale + q, lane == 0, {{o.h[1], o.h[0]}}));
     }
   }
   // every block has read its count (and used it) by its ticket; the last one raises them all. The ticket
@@ -422,7 +462,10 @@ int ms_adamw_step(const ms_optim_tensor* tensors, int64_t count, int state_bits,
                   void* stream) {
   const char* who = "ms_adamw_step";
   if (const char* why = opt::check(tensors, count, workspace)) return opt::fail(MS_ERR_INVALID_ARGUMENT, who, why);
-  if (state_bits != 32 && state_bits != 8) return opt::fail(MS_ERR_INVALID_ARGUMENT, who, "state_bits must be 32 or 8");
+  const bool stochastic = state_bits == (8 | MS_ADAMW_STOCHASTIC);
+  if (stochastic) state_bits = 8;
+  if (state_bits != 32 && state_bits != 8)
+    return opt::fail(MS_ERR_INVALID_ARGUMENT, who, "state_bits must be 32, 8 or 8 | MS_ADAMW_STOCHASTIC");
   if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0 && weight_decay >= 0.0) ||
       (!lr_device && !(lr >= 0.0)))
     return opt::fail(MS_ERR_INVALID_ARGUMENT, who, "lr, eps and weight_decay must be >= 0, the betas in [0, 1)");
@@ -460,9 +503,11 @@ int ms_adamw_step(const ms_optim_tensor* tensors, int64_t count, int state_bits,
     list.rounds = per;
     const dim3 grid((unsigned)blocks), block(opt::THREADS);
     if (state_bits == 32)
-      hipLaunchKernelGGL(opt::adamw<32>, grid, block, 0, (hipStream_t)stream, list, hp, opt::Ws{workspace});
+      hipLaunchKernelGGL((opt::adamw<32, false>), grid, block, 0, (hipStream_t)stream, list, hp, opt::Ws{workspace});
+    else if (stochastic)
+      hipLaunchKernelGGL((opt::adamw<8, true>), grid, block, 0, (hipStream_t)stream, list, hp, opt::Ws{workspace});
     else
-      hipLaunchKernelGGL(opt::adamw<8>, grid, block, 0, (hipStream_t)stream, list, hp, opt::Ws{workspace});
+      hipLaunchKernelGGL((opt::adamw<8, false>), grid, block, 0, (hipStream_t)stream, list, hp, opt::Ws{workspace});
     if (int rc = opt::launched(who)) return rc;
   }
   return MS_OK;

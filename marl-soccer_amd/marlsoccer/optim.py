@@ -10,14 +10,22 @@ the step itself may be captured.
     loss.backward(); opt.step(); opt.zero_grad()
 
 state_bits=8 holds both moments as OCP e4m3 bytes with a float32 scale for every 256 values: 2 B a
-value instead of 8. The second moment is held as its root. Rounding is to nearest: against moments in
-32 bits a value is off by up to 2^-4 of itself down to 2^-15 of its block's largest (by 2^-19 of the
-largest below that), and a change of less than half a step waits until it is more, so use it where
-memory counts.
+value instead of 8. The second moment is held as its root. A step of the codes is 2^-4 to 2^-3 of the value
+down to 2^-14.8 of its block's largest, and 2^-17.8 of the largest below that.
+
+rounding="stochastic" is for training: each value goes to one of its two neighbours with the odds that
+keep its expectation, from a hash of the step count and its place (the same step gives the same bits). The
+moments then follow the 32-bit ones in the mean; with beta2 = 0.999 a held root wanders by some 17 % about
+the 32-bit one. rounding="nearest" holds each step's moments to half a step of the codes, but what a step
+changes by less than that is lost, at every step, however many follow: with beta2 = 0.999 a root moves by
+some 0.05 % a step, so all but the block's largest only follow that one, through the scale. When gradients
+change in size their roots stay off: by 0.3 to 9 times after thousands of steps where some of a block's
+values grew four times or shrank ten times against the others.
 """
 from __future__ import annotations
 
 import struct
+import warnings
 from itertools import chain, repeat
 from operator import attrgetter
 
@@ -29,6 +37,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 WORKSPACE = 4096   # MS_OPTIM_WORKSPACE, floats
 BLOCK = 256        # MS_ADAMW_BLOCK: values that share a scale
 F8 = torch.float8_e4m3fn
+ROUNDINGS = {"nearest": 0, "stochastic": 256}  # MS_ADAMW_STOCHASTIC
 
 
 def scales_for(numel: int) -> int:
@@ -125,18 +134,21 @@ def _launch(device, params, calls):
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, steps, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
-               max_grad_norm=None, exp_avg_scales=None, exp_avg_sq_scales=None, workspace=None, grad_norm=None):
+               max_grad_norm=None, exp_avg_scales=None, exp_avg_sq_scales=None, workspace=None, grad_norm=None, rounding="nearest"):
     """One AdamW step over a list of tensors, in place (see ms_adamw_step in include/marl_soccer.h):
     parameters and gradients float32, bfloat16 or float16, contiguous; moments float32, or float8_e4m3fn
     with scales; steps: one int64 on the device for each. What is written must not overlap (the same
     tensor twice is refused). lr: a float, or one float32 on the device.
     max_grad_norm: clip all gradients together by their norm (the gradients themselves stay as they
     are); grad_norm: one float32 on the device that receives the norm. workspace: WORKSPACE zeroed
-    floats, kept by a caller that steps often (None: made here); one step at a time may use it."""
+    floats, kept by a caller that steps often (None: made here); one step at a time may use it.
+    rounding: of moments with scales, "nearest" or "stochastic" (the module's comment)."""
     if not len(params):
         return
     if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
         _bad("exp_avg_scales and exp_avg_sq_scales", "both given or both None")
+    if rounding not in ROUNDINGS:
+        _bad("rounding", f"'nearest' or 'stochastic', got {rounding!r}")
     rows, device = _entries(params, grads, exp_avg, exp_avg_sq, steps, exp_avg_scales, exp_avg_sq_scales)
     if max_grad_norm is not None and not max_grad_norm > 0:
         _bad("max_grad_norm", "positive")
@@ -149,7 +161,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, steps, *, lr, betas=(0.9, 0.9
     calls = []
     if max_grad_norm is not None:
         calls.append(_clip_call(rows, max_grad_norm, grad_norm, workspace))
-    calls.append(_step_call(rows, 8 if exp_avg_scales is not None else 32, lr, betas, eps, weight_decay,
+    calls.append(_step_call(rows, 8 | ROUNDINGS[rounding] if exp_avg_scales is not None else 32, lr, betas, eps, weight_decay,
                             max_grad_norm is not None, workspace, device))
     _launch(device, params, calls)
 
@@ -176,11 +188,12 @@ class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update (decoupled weight decay, no amsgrad) with every tensor of a group in
     one launch; weight_decay=0 is the notebook's Adam. max_grad_norm clips the gradients of all groups
     together inside the step (.grad stays unclipped; `last_grad_norm`, on the device, holds the norm).
-    A parameter without a gradient is left alone, its step count too. state_bits: 32 or 8 (the
-    module's comment). lr may be one float32 on the device, which a captured step reads anew. State:
+    A parameter without a gradient is left alone, its step count too. state_bits: 32 or 8; rounding: of 8
+    bits, "stochastic" or "nearest" (the module's comment; None: nearest, with a warning). lr may be one float32 on the device, which a captured step reads anew. State:
     step, exp_avg, exp_avg_sq and, with 8 bits, their scales; state_dict() carries all of it."""
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None, state_bits=32):
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None, state_bits=32,
+                 rounding=None):
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
         if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
@@ -189,15 +202,21 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("betas must be in [0, 1), eps and weight_decay >= 0")
         if max_grad_norm is not None and not max_grad_norm > 0:
             raise ValueError(f"max_grad_norm must be positive, got {max_grad_norm}")
-        self.max_grad_norm, self.state_bits = max_grad_norm, state_bits
+        if rounding is not None and (rounding not in ROUNDINGS or state_bits != 8):
+            raise ValueError(f"rounding must be 'nearest' or 'stochastic', of moments in 8 bits, got {rounding!r} with {state_bits}")
+        if state_bits == 8 and rounding is None:
+            warnings.warn("AdamW: moments in 8 bits, rounded to nearest, lose small changes for good; rounding='stochastic' keeps them "
+                          "in the mean", stacklevel=2)
+        self.max_grad_norm, self.state_bits, self.rounding = max_grad_norm, state_bits, rounding
         self._work = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def __getstate__(self):
-        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "state_bits": self.state_bits}
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "state_bits": self.state_bits, "rounding": self.rounding}
 
     def __setstate__(self, state):
         super().__setstate__(state)
+        self.rounding = state.get("rounding")
         self._work = {}  # a copy's own
 
     @property
@@ -271,8 +290,9 @@ class AdamW(torch.optim.Optimizer):
         if self.max_grad_norm is not None:
             every = b"".join(rows for _, rows, _ in groups)
             calls.append(_clip_call(every, self.max_grad_norm, norm, work))
+        bits = self.state_bits | ROUNDINGS[self.rounding or "nearest"]
         for group, rows, _ in groups:
-            calls.append(_step_call(rows, self.state_bits, group["lr"], group["betas"], group["eps"], group["weight_decay"],
+            calls.append(_step_call(rows, bits, group["lr"], group["betas"], group["eps"], group["weight_decay"],
                                     self.max_grad_norm is not None, work, device))
         _launch(device, every_param, calls)
         return loss

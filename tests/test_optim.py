@@ -422,3 +422,133 @@ def test_a_saved_parameter_that_was_stepped_refuses_its_backward():
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+# ---------------------------------------------------------------- 8-bit moments over many steps
+
+def eight_bit_lists(m, r, steps=None):
+    """The lists of one tensor whose held moments are m and r (root of the second), as quantised to nearest."""
+    def held(x):
+        f = torch.nn.functional.pad(x.reshape(-1), (0, -x.numel() % optim.BLOCK)).view(-1, optim.BLOCK)
+        top = f.abs().amax(1)
+        return (f * (448 / top)[:, None]).to(optim.F8).view(-1)[:x.numel()].view(x.shape).contiguous(), top / 448
+    (mc, ms), (rc, rs) = held(m), held(r)
+    return dict(exp_avg=[mc], exp_avg_sq=[rc], exp_avg_scales=[ms], exp_avg_sq_scales=[rs])
+
+
+@gpu
+def test_stochastic_rounding_keeps_the_expected_moments():
+    """One step from the same state under many step counts: the moments are off by less than a step of their
+    codes each time, and their mean over the counts is the unrounded value. A mean of K draws between two
+    neighbours has a deviation of at most step / (2 sqrt(K)); 6 of them hold for 2 x 5,003 values with a
+    probability of 1 - 10,006 x 2e-9. The odds have 16 bits, cut: a bias of at most 2^-16 steps, and
+    float32's roundings of the moment before it (9 u and 8 u of its terms, the module's comment) and of the
+    scaled value (2 u). The same count gives the same bits."""
+    need_gpu()
+    n, K, b1, b2 = 5003, 600, 0.9, 0.999
+    g = torch.Generator().manual_seed(11)
+    size = torch.exp(1.5 * torch.randn(n, generator=g))
+    m0, r0, grad = (torch.randn(n, generator=g) * size).cuda(), (torch.rand(n, generator=g) * size).cuda(), (torch.randn(n, generator=g) * size).cuda()
+    start = eight_bit_lists(m0, r0)
+    held_m = optim.moment_values(start["exp_avg"][0], start["exp_avg_scales"][0]).double()
+    held_r = optim.moment_values(start["exp_avg_sq"][0], start["exp_avg_sq_scales"][0]).double()
+    terms = b1 * held_m.abs() + (1 - b1) * grad.double().abs()
+    want = (b1 * held_m + (1 - b1) * grad.double(), (b2 * held_r.square() + (1 - b2) * grad.double().square()).sqrt())
+    sums = [torch.zeros(n, dtype=torch.float64, device="cuda") for _ in range(2)]
+    for k in range(K):
+        outs = []
+        for again in range(2 if k == 0 else 1):
+            count = torch.tensor([k], device="cuda")
+            lists = {key: [t[0].clone()] for key, t in start.items()}
+            optim.adamw_step([torch.zeros(n, device="cuda")], [grad], steps=[count], lr=1e-3, betas=(b1, b2), rounding="stochastic", **lists)
+            outs.append([optim.moment_values(lists[c][0], lists[s][0]).double() for c, s in (("exp_avg", "exp_avg_scales"), ("exp_avg_sq", "exp_avg_sq_scales"))])
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], outs[-1]))
+        for j, (got, s) in enumerate(zip(outs[0], ("exp_avg_scales", "exp_avg_sq_scales"))):
+            scale = lists[s][0].double().repeat_interleave(optim.BLOCK)[:n]
+            unit = torch.exp2(torch.floor(torch.log2((want[j].abs() / scale).clamp(min=2.0 ** -6))) - 3) * scale  # a step of the codes there
+            err = (9 * U * terms if j == 0 else 8 * U * want[1]) + 2 * U * want[j].abs()
+            assert bool(((got - want[j]).abs() <= unit + err).all()), (k, j)
+            sums[j] += got
+            if k == K - 1:
+                off = (sums[j] / K - want[j]).abs()
+                bound = unit * (6 / (2 * math.sqrt(K)) + 2.0 ** -16) + err
+                assert bool((off <= bound).all()), (j, float((off / bound).max()))
+
+
+@gpu
+@pytest.mark.parametrize("change", ["steady", "half of them grow four times", "half of them shrink to a tenth", "one was large for half the time"])
+def test_stochastic_moments_follow_64_bits_over_thousands_of_steps(change):
+    """Never brought back to the 64-bit moments. A root r moves by at most 0.0005 |g^2 / v - 1| of itself a step,
+    0.001 on average, and so does the largest, whose scale shifts the codes; a rounding's variance is at most
+    its step (2^-3 r) times the shift: 2.5e-4 r^2 a step, forgotten at 0.001 a step, so 0.125 r^2 in all; where
+    gradients fall, v falls by 0.001 a step and what was off stays as it was against it: 1.25e-4 for up to
+    3,000 steps and what was there, 0.5 r^2. The mean of the roots: v is too large by that variance on
+    average, a root by half of it at most while steady (0.0625), and by a quarter where it is not
+    stationary; the mean of 2,048 independent values is known to 0.016."""
+    need_gpu()
+    n, T, at, b2 = 2048, 4000, 1000, 0.999
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    opt = optim.AdamW([p], lr=1e-6, betas=(0.9, b2), weight_decay=0.0, state_bits=8, rounding="stochastic")
+    some = torch.arange(n, device="cuda") % 2 == 0
+    one = torch.arange(n, device="cuda") % optim.BLOCK == 3
+    v = torch.zeros(n, dtype=torch.float64, device="cuda")
+    for t in range(T):
+        g = torch.randn(n, generator=gen, device="cuda")
+        if change == "half of them grow four times" and t >= at:
+            g = torch.where(some, 4 * g, g)
+        elif change == "half of them shrink to a tenth" and t >= at:
+            g = torch.where(some, 0.1 * g, g)
+        elif change == "one was large for half the time" and t < T // 2:
+            g = torch.where(one, 30 * g, g)
+        p.grad = g
+        opt.step()
+        v = b2 * v + (1 - b2) * g.double().square()
+    s = opt.state[p]
+    ratio = optim.moment_values(s["exp_avg_sq"], s["exp_avg_sq_scale"]).double() / v.sqrt()
+    falls = change in ("half of them shrink to a tenth", "one was large for half the time")
+    for part in (some & ~one, ~some & ~one):
+        assert abs(float(ratio[part].mean()) - 1) <= (0.25 if falls else 0.0625 + 0.05), change
+        assert float((ratio[part] - 1).square().mean()) <= (0.5 if falls else 0.125), change
+
+
+@gpu
+def test_stochastic_first_moment_reaches_a_constant_gradient():
+    """m goes from 0 to g by a tenth of the distance a step; to nearest it stops where a tenth is half a step
+    of the codes, far below g. The deviation of a rounding that keeps the expectation: at most half a step (2^-4
+    of the value) each, forgotten by 0.9 a step: 2^-4 / sqrt(1 - 0.81) = 0.144 of the value, and the
+    mean over 1,024 of them is known to 0.0045."""
+    need_gpu()
+    n = 1024
+    g = torch.linspace(0.05, 1.0, n, device="cuda")[torch.randperm(n, generator=torch.Generator().manual_seed(3)).cuda()]
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    opt = optim.AdamW([p], lr=1e-6, state_bits=8, rounding="stochastic")
+    for _ in range(200):  # 0.9^200 = 7e-10 is left of the start
+        p.grad = g
+        opt.step()
+    ratio = optim.moment_values(opt.state[p]["exp_avg"], opt.state[p]["exp_avg_scale"]) / g
+    assert abs(float(ratio.mean()) - 1) <= 6 * 0.0045
+    assert float((ratio - 1).square().mean()) <= 0.144 ** 2
+
+
+def test_rounding_is_checked_and_named():
+    p = torch.nn.Parameter(torch.zeros(4))
+    for kw in (dict(state_bits=8, rounding="up"), dict(state_bits=32, rounding="stochastic"), dict(rounding="nearest")):
+        with pytest.raises(ValueError, match="rounding"):
+            optim.AdamW([p], **kw)
+    with pytest.warns(UserWarning, match="stochastic"):
+        optim.AdamW([p], state_bits=8)
+    import copy
+    import warnings
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        optim.AdamW([p])
+        optim.AdamW([p], state_bits=8, rounding="nearest")
+        assert copy.deepcopy(optim.AdamW([p], state_bits=8, rounding="stochastic")).rounding == "stochastic"
+    one = dict(params=[torch.zeros(4)], grads=[torch.zeros(4)], exp_avg=[torch.zeros(4)], exp_avg_sq=[torch.zeros(4)], steps=[torch.zeros(1, dtype=torch.int64)], lr=1e-3)
+    with pytest.raises(ValueError, match="rounding"):
+        optim.adamw_step(**one, rounding="down")
+    from marlsoccer import _native as N
+    rows = (N.MsOptimTensor * 1)(N.MsOptimTensor(numel=4, grad=16, step=16, param=16, exp_avg=16, exp_avg_sq=16))
+    for bits in (256, 32 | 256, 8 | 512):
+        assert N.lib().ms_adamw_step(rows, 1, bits, 1e-3, None, 0.9, 0.99, 1e-8, 0.0, 0, 16, None) == N.MS_ERR_INVALID_ARGUMENT
