@@ -190,6 +190,12 @@ __device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_l
 #pragma unroll
   for (int k = 0; k < 4; ++k) top = fmaxf(top, __builtin_fabsf(v[k]));
   top = wave_max(top);
+  if (top > 3.4028234663852886e38f) {  // an infinite one is held as no number, by itself: the scale is the others'
+    top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = __builtin_isinf(v[k]) ? top : fmaxf(top, __builtin_fabsf(v[k]));
+    top = wave_max(top);
+  }
   const bool some = top >= 7.8886090522101181e-31f;
   const float inv = some ? 448.0f / top : 0.0f;
   if (first_lane) *scale = some ? top / 448.0f : 0.0f;

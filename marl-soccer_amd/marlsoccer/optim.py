@@ -20,7 +20,8 @@ the 32-bit one. rounding="nearest" holds each step's moments to half a step of t
 changes by less than that is lost, at every step, however many follow: with beta2 = 0.999 a root moves by
 some 0.05 % a step, so all but the block's largest only follow that one, through the scale. When gradients
 change in size their roots stay off: by 0.3 to 9 times after thousands of steps where some of a block's
-values grew four times or shrank ten times against the others.
+values grew four times or shrank ten times against the others. A moment that is infinite or no number is
+held as no number, and reaches no other value of its block.
 """
 from __future__ import annotations
 

@@ -552,3 +552,32 @@ def test_rounding_is_checked_and_named():
     rows = (N.MsOptimTensor * 1)(N.MsOptimTensor(numel=4, grad=16, step=16, param=16, exp_avg=16, exp_avg_sq=16))
     for bits in (256, 32 | 256, 8 | 512):
         assert N.lib().ms_adamw_step(rows, 1, bits, 1e-3, None, 0.9, 0.99, 1e-8, 0.0, 0, 16, None) == N.MS_ERR_INVALID_ARGUMENT
+
+
+@gpu
+@pytest.mark.parametrize("rounding", ["nearest", "stochastic"])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan"), 1e25], ids=["inf", "minus inf", "nan", "a square past float32"])
+def test_a_non_finite_moment_of_8_bits_stays_alone(bad, rounding):
+    """Its own parameter is lost (as with 32 bits); the rest of its block goes on as without it. 1e25: only
+    the second moment overflows, and the first is the block's largest, so there only the second is compared."""
+    need_gpu()
+    runs = []
+    for value in (0.0, bad):
+        (p,), _ = make([(700,)], torch.float32, 90)
+        p = torch.nn.Parameter(p)
+        opt = optim.AdamW([p], lr=1e-2, state_bits=8, rounding=rounding)
+        for k in range(4):
+            _, (g,) = make([(700,)], torch.float32, 91 + k)
+            g[300] = value if k == 1 else 0.0
+            p.grad = g
+            opt.step()
+            s = opt.state[p]
+            if k == 1:
+                m, r = (optim.moment_values(s[c], s[c + "_scale"]) for c in ("exp_avg", "exp_avg_sq"))
+                m1, r1 = m.clone(), r.clone()
+        runs.append((p.detach(), m1, r1))
+    (p0, m0, r0), (p1, m1, r1) = runs
+    others = torch.arange(700, device="cuda") != 300
+    assert torch.isnan(p1[300]) and torch.isnan(r1[300]) and torch.equal(r0[others], r1[others])
+    if not math.isfinite(bad):
+        assert torch.isnan(m1[300]) and torch.equal(m0[others], m1[others]) and torch.equal(p0[others], p1[others])
