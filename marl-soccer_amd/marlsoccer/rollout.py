@@ -171,7 +171,8 @@ class DeviceRollout:
     An agent with a memory (Agent(memory=...)) runs with policy="torch" (its default then): every
     step the memory of all 2 N rows is stepped in place, from zeros where an episode ended before it.
     collect() then also returns "memory_state", the state before the rollout's first step, with which
-    agent.memory(x, dones.reshape(T, -1).bool(), memory_state) replays the rollout for the update. A
+    agent.memory(x, dones.reshape(T, -1).bool(), memory_state) replays the rollout for the update.
+    Its get_value alone sees no memory: the value of next_obs, for bootstrapping, is next_value()'s. A
     caller that resets the batch between rollouts zeroes the tensors of `memory_state` too.
     """
 
@@ -245,10 +246,7 @@ class DeviceRollout:
             return
         else:
             x = self.normalizer.normalize(self.next_obs.reshape(-1, OBS_DIM))
-            # no autocast weight-cast cache: its casts would be allocated and reused across a graph
-            # capture (the casts of ~0.4 M parameters per step are negligible)
-            with torch.autocast("cuda", dtype=torch.bfloat16, enabled=self.policy_dtype == torch.bfloat16,
-                                cache_enabled=False):
+            with self._autocast():
                 if self.memory_state is not None:
                     x = self.agent.memory.step(x, self.memory_state, self.next_done.reshape(-1) != 0)
                 if self.deterministic:
@@ -287,6 +285,22 @@ class DeviceRollout:
             self.step(t)
         if self._fused is not None:  # the fused step reads the env's obs rows directly
             self.next_obs.copy_(self.batch.obs[:, :2])
+
+    def _autocast(self):
+        # no autocast weight-cast cache: its casts would be allocated and reused across a graph
+        # capture (the casts of ~0.4 M parameters per step are negligible)
+        return torch.autocast("cuda", dtype=torch.bfloat16, enabled=self.policy_dtype == torch.bfloat16, cache_enabled=False)
+
+    @torch.no_grad()
+    def next_value(self) -> torch.Tensor:
+        """The critic's value of next_obs (N, 2), for bootstrapping after a collect() and before the
+        update; through the memory where the agent has one, as the next step's policy would see it.
+        Changes nothing: not the memory's state, not the generator."""
+        x = self.normalizer.normalize(self.next_obs.reshape(-1, OBS_DIM))
+        with self._autocast():
+            if self.memory_state is not None:
+                x = self.agent.memory.step(x, tuple(s.clone() for s in self.memory_state), self.next_done.reshape(-1) != 0)
+            return self.agent.get_value(x).float().reshape(self.N, 2)
 
     def _inputs_identity(self) -> tuple:
         """The tensors a captured rollout reads in place (their storage)."""

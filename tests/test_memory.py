@@ -158,3 +158,46 @@ def test_collect_update_loop(bits):
         assert all(bool(torch.isfinite(p).all()) for p in agent.parameters())
         assert any(not torch.equal(p, q) for p, q in zip(before, agent.parameters()))
     b.close()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
+def test_next_value_is_the_next_rollouts_first(graph, dtype):
+    """The value for bootstrapping goes through the memory and leaves its state and the generator alone: the
+    next rollout, with the same parameters and statistics, stores it first. The products may be summed in
+    another order: 1e-4 in float32 as above, and in bfloat16 the five layers' roundings of a different
+    order, 2^-8 each of values of the size of 1."""
+    need_gpu()
+    N, T = 24, 15
+    agent, b, ro = make(N, T, graph, short_config(13), policy_dtype=dtype)
+    for _ in range(3):
+        ro.collect()
+        before, draws = [s.clone() for s in ro.memory_state], ro.gen.get_state()
+        value = ro.next_value()
+        assert value.shape == (N, 2) and value.dtype == torch.float32
+        assert all(torch.equal(a, c) for a, c in zip(before, ro.memory_state)) and torch.equal(draws, ro.gen.get_state())
+        x = ro.normalizer.normalize(ro.next_obs.reshape(-1, 66))
+        plain = agent.get_value(x).view(N, 2).detach()
+        first = ro.collect()["values"][0]
+        assert float((value - first).abs().max()) <= (1e-4 if dtype == torch.float32 else 5 * 2.0 ** -8)
+        if dtype == torch.float32:
+            # a value without the memory would fail the line above: all that is asked of it is to be further off than that allows
+            assert float((plain - first).abs().max()) > 1e-4
+    b.close()
+
+
+@gpu
+@pytest.mark.parametrize("policy", ["fused", "torch"])
+def test_next_value_without_memory(policy):
+    need_gpu()
+    from marlsoccer import SoccerBatch
+    torch.manual_seed(0)
+    agent = Agent().cuda()
+    b = SoccerBatch(16, config=short_config(13))
+    b.reset(seed=3)
+    ro = DeviceRollout(b, agent, RunningMeanStd((66,), device="cuda"), 8, seed=5, update_normalizer=False, policy=policy)
+    ro.collect()
+    value = ro.next_value()
+    assert float((value - ro.collect()["values"][0]).abs().max()) <= 1e-4
+    b.close()
