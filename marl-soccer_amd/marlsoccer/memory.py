@@ -55,9 +55,13 @@ class SequenceMemory(nn.Module):
 
     def forward(self, x, starts=None, state=None):
         """x (T, R, width); starts (T, R) bool: row r begins an episode at step t (the rollout's dones);
-        state: init_state's or a call's (None: zeros). Returns y (T, R, width) and the state after."""
+        state: init_state's or a call's (None: zeros; the convolution's is taken in the type that x is
+        projected to, so a bfloat16 rollout's state replays in float32 too). Returns y (T, R, width) and
+        the state after."""
         conv_state, scan_state = (None, None) if state is None else state
         u, z = self.in_proj(x).chunk(2, dim=-1)
+        if conv_state is not None:
+            conv_state = conv_state.to(u.dtype)
         u, conv_state = short_conv(u, self.conv_weight, self.conv_bias, conv_state, starts, "silu", return_state=True)
         rate, B, C = self._rates(u)
         y, scan_state = ssm_scan(u, rate, -torch.exp(self.A_log), B, C, D=self.skip, z=z, delta_bias=self.rate_bias,

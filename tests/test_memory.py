@@ -201,3 +201,53 @@ def test_next_value_without_memory(policy):
     value = ro.next_value()
     assert float((value - ro.collect()["values"][0]).abs().max()) <= 1e-4
     b.close()
+
+
+def test_a_state_of_another_type_is_taken_in_the_activations_type():
+    """Without a device: the state's type is no longer what the call is refused for."""
+    m = SequenceMemory()
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        with pytest.raises(ValueError, match="HIP device"):
+            m(torch.zeros(3, 2, 66), None, m.init_state(2, dtype=dtype))
+
+
+@gpu
+@pytest.mark.parametrize("again", ["float32", "autocast"])
+def test_bf16_rollout_replays(again):
+    """A rollout under bfloat16 replayed by the update in float32, as documented, and under the same autocast.
+    The critic under bfloat16 is within 2e-2 of float32 (tests/test_policy.py); the memory adds 128 products
+    of roundings to 2^-8 (the projections' in and out, the activations between them), some four of them in a
+    row, of a sum below 0.5: 8e-3 a feature, 0.064 over 66 of them at most, through layers whose gain is about one."""
+    need_gpu()
+    N, T = 24, 30
+    agent, b, ro = make(N, T, config=short_config(13), policy_dtype=torch.bfloat16)
+    for _ in range(2):
+        out = ro.collect()
+        assert out["memory_state"][0].dtype == torch.bfloat16
+        x = ro.normalizer.normalize(out["obs"].reshape(-1, 66)).view(T, 2 * N, 66)
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=again == "autocast"):
+            y, state = agent.memory(x, out["dones"].reshape(T, -1).bool(), out["memory_state"])
+            value = agent.get_value(y.reshape(-1, 66)).float().view(T, N, 2)
+        assert float((value - out["values"]).detach().abs().max()) <= 2e-2 + 0.064
+        for a, c in zip(state, ro.memory_state):
+            assert a.dtype == (torch.float32 if again == "float32" else c.dtype)
+            assert float((a.float() - c.float()).detach().abs().max()) <= 4 * 2.0 ** -8 * (1 + float(c.float().abs().max()))
+        value.square().mean().backward()
+        assert all(bool(torch.isfinite(p.grad).all()) for p in agent.memory.parameters())
+    b.close()
+
+
+@gpu
+def test_gradients_reach_a_state_of_another_type():
+    """The same as those of the state in float32, rounded to the state's type."""
+    need_gpu()
+    torch.manual_seed(0)
+    m = SequenceMemory(channels=32).cuda()
+    x = torch.randn(5, 3, 66, device="cuda")
+    state = tuple(torch.randn_like(s) for s in m.init_state(3, "cuda", torch.bfloat16))
+    grads = []
+    for conv in (state[0], state[0].float()):
+        leaves = conv.clone().requires_grad_(), state[1].clone().requires_grad_()
+        grads.append(torch.autograd.grad(m(x, None, leaves)[0].sum(), leaves))
+    (a, b), (c, d) = grads
+    assert a.dtype == torch.bfloat16 and bool(a.any()) and torch.equal(a, c.bfloat16()) and torch.equal(b, d)
