@@ -18,7 +18,8 @@ and for one step, with the states renewed in place:
 
 Everything that varies in time has one type (float32, bfloat16 or float16); weights, A, D, biases and
 the scan's states are float32. Results are rounded once, and repeat bit for bit (no atomics). The
-sequence forms carry gradients to every input but `starts` (once: no double backward). Calls are
+sequence forms carry gradients to every input but `starts` (once: no double backward); forward-mode
+derivatives are refused (NotImplementedError), by the steps too. Calls are
 asynchronous on the current stream of the tensors' device and may be captured into a HIP graph; a
 captured backward needs its forward in the same capture, and leaves (the inputs', or those they were
 computed from) that no eager autograd graph of these operators holds any more.
@@ -30,6 +31,7 @@ import threading
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -107,6 +109,12 @@ def _lives(ctx, stream=None):
     ctx.stream = torch.cuda.current_stream().cuda_stream if stream is None else stream
     with _living_lock:
         _living.add(ctx)
+
+
+def _refuse_tangents(who, *inputs):
+    """A dual tensor has no requires_grad: without this its tangent would be lost silently."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in inputs):
+        raise NotImplementedError(f"{who}: forward-mode derivatives are not implemented")
 
 
 def _with_workspace(io, work):
@@ -287,6 +295,7 @@ def short_conv(x, weight, bias=None, state=None, starts=None, activation=None, r
     step 0, oldest first (None: zeros); starts (T, R). activation: None or "silu". Returns y like x,
     and with return_state the state after the last step (inputs from before the last start as
     zeros). Gradients flow to x, weight, bias, state and back from the returned state."""
+    _refuse_tangents("short_conv", x, weight, bias, state)
     _conv_check("short_conv", x, weight, bias, state, starts, activation, 3)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, state)):
         if torch.cuda.is_current_stream_capturing():
@@ -301,6 +310,7 @@ def short_conv_step(x, state, weight, bias=None, starts=None, activation=None):
     """One step of short_conv for every row: x (R, D), starts (R,); state (R, W - 1, D) is renewed in
     place. Returns y (R, D). No gradients."""
     who = "short_conv_step"
+    _refuse_tangents(who, x, state, weight, bias)
     if not isinstance(state, torch.Tensor):
         raise ValueError(f"{who}: state must be a tensor")
     _conv_check(who, x, weight, bias, state, starts, activation, 2)
@@ -444,6 +454,7 @@ def ssm_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, state=None, sta
     Returns y like u, and with return_state the states after the last step. Gradients flow to every
     input but starts, and back from the returned state; with them the forward also keeps the states
     of every 8th step (4 N bytes a channel), and B and C in float32, until the backward."""
+    _refuse_tangents("ssm_scan", u, delta, A, B, C, D, z, delta_bias, state)
     _scan_check("ssm_scan", u, delta, A, B, C, D, z, delta_bias, state, starts, 3)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (u, delta, A, B, C, D, z, delta_bias, state)):
         if torch.cuda.is_current_stream_capturing():
@@ -458,6 +469,7 @@ def ssm_step(state, u, delta, A, B, C, D=None, z=None, delta_bias=None, starts=N
     """One step of ssm_scan for every row: u, delta, z (R, D), B, C (R, N) or (R, G, N), starts (R,);
     state (R, D, N) is renewed in place. Returns y (R, D). No gradients."""
     who = "ssm_step"
+    _refuse_tangents(who, state, u, delta, A, B, C, D, z, delta_bias)
     if not isinstance(state, torch.Tensor):
         raise ValueError(f"{who}: state must be a tensor")
     _scan_check(who, u, delta, A, B, C, D, z, delta_bias, state, starts, 2)

@@ -693,3 +693,41 @@ def test_capture_refuses_leaves_that_an_eager_graph_holds():
         torch.cuda.synchronize()
         for a, b in zip(want, got):
             assert torch.equal(a, b)
+
+
+def tangent_calls(device):
+    """Each operator with one of its inputs a dual tensor, by name."""
+    v = scan_inputs(4, 2, 6, 5, 1, torch.float32, 161, device, state=True, starts=True)
+    c = conv_inputs(4, 2, 6, 4, torch.float32, 162, device, state=True, starts=True)
+    at = {k: (t[0] if k in ("u", "delta", "B", "C", "z", "starts") else t) for k, t in v.items()}
+    cat = {k: (t[0] if k in ("x", "starts") else t) for k, t in c.items()}
+    for fn, args in ((seq.ssm_scan, v), (seq.ssm_step, at), (seq.short_conv, c), (seq.short_conv_step, cat)):
+        for k in args:
+            if k != "starts":
+                yield fn, args, k
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Raised before anything runs, so without a device too; an input without a tangent is none of its business."""
+    from torch.autograd import forward_ad
+    for fn, args, k in tangent_calls("cpu"):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(args[k], torch.ones_like(args[k]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fn(**{**args, k: dual})
+            refuses(fn, "HIP device", **args)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda x: seq.short_conv(x, torch.ones(6, 4)), (torch.ones(4, 2, 6),), (torch.ones(4, 2, 6),))
+
+
+@gpu
+def test_a_level_of_forward_mode_alone_changes_nothing():
+    need_gpu()
+    from torch.autograd import forward_ad
+    v = scan_inputs(4, 2, 6, 5, 1, torch.float32, 163, "cuda")
+    with forward_ad.dual_level():
+        again = seq.ssm_scan(**v)
+        other = forward_ad.make_dual(torch.ones(3, device="cuda"), torch.ones(3, device="cuda")) * 2
+    assert torch.equal(seq.ssm_scan(**v), again) and other is not None
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        seq.ssm_scan(**{**v, "u": forward_ad.make_dual(v["u"], torch.ones_like(v["u"]))})
