@@ -59,12 +59,13 @@ __device__ __forceinline__ void store(T* p, const float (&x)[E], int n, bool vec
   }
 }
 
-// 1 / (1 + exp(-x)) and its product with x. The argument is held where exp is finite; a NaN is lost
-// here and comes back with x in every use. v_exp_f32's argument is rounded, which costs |x| 2^-24 of
-// exp: less than a unit in the last place of the result where it is not small.
+// 1 / (1 + exp(-x)) and its product with x. v_exp_f32's argument is rounded, which costs |x| 2^-24 of
+// exp: less than a unit in the last place of the result where it is not small. Below x = -87.3 the
+// result would be subnormal and is 0, and so are the product, off by at most 89 x 2^-126 there, and the
+// slope: exp may pass to infinity, whose reciprocal is 0 (holding the argument at 126 left 2^-126, which a
+// large x makes large again: silu(-3e38) was -3.5).
 __device__ __forceinline__ float sigmoid(float x) {
-  const float t = __builtin_amdgcn_fmed3f(x * -1.44269504f, -126.0f, 126.0f);
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f));
 }
 __device__ __forceinline__ float silu(float x) { return x * sigmoid(x); }
 __device__ __forceinline__ float silu_slope(float x) {

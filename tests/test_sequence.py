@@ -731,3 +731,54 @@ def test_a_level_of_forward_mode_alone_changes_nothing():
     assert torch.equal(seq.ssm_scan(**v), again) and other is not None
     with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         seq.ssm_scan(**{**v, "u": forward_ad.make_dual(v["u"], torch.ones_like(v["u"]))})
+
+
+LARGE = [0.0, 1e-30, 0.5, 1.0, 1.28, 5.0, 17.0, 20.0, 40.0, 80.0, 87.0, 87.5, 88.0, 89.0, 100.0, 127.5, 1e3, 6e4, 1e10, 1e30, 1e37, 3e38]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS.get)
+def test_activations_of_large_values(dtype):
+    """The convolution's activation and the scan's gate, and their slopes, from 1e-30 to the types' ends and of
+    both signs. exp's argument is off by |x| 2 u, so its value by that much of itself; 1 - s is known to u,
+    which the slope multiplies by x while s is not yet 1 (x < 17); a sigmoid below 2^-126 is 0, which costs at
+    most 89 x 2^-126. The products and sums: 24 u as in test_short_conv."""
+    need_gpu()
+    x = torch.tensor([v for v in LARGE if v < torch.finfo(dtype).max])
+    x = torch.cat([x, -x]).to(dtype)
+    n = x.numel()
+    d = x.double()
+    s = 1 / (1 + torch.exp(-d))
+    want, slope = torch.where(s > 0, d * s, 0.0), s * (1 + d * (1 - s))
+    u, lost = 2.0 ** -24, 89 * 2.0 ** -126
+    near = d.abs().clamp(max=100)
+    err = (24 + 2 * near) * u * want.abs() + lost
+    slope_err = (24 + 2 * near) * u * s * (1 + d.abs() * (1 - s)) + 2 * u * near * s * (d > 0) + lost
+
+    def check(name, got, want, err):
+        eps = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+        tiny = torch.finfo(dtype).smallest_normal * (torch.finfo(dtype).eps if dtype == torch.float16 else 1.0)
+        off = (got.double().cpu() - want).abs()
+        bad = ~(off <= err + eps * (want.abs() + err) + tiny)
+        assert not bad.any(), (name, d[bad], got.double().cpu()[bad], want[bad])
+
+    weight = torch.zeros((n, 4), device="cuda")
+    weight[:, 3] = 1
+    at = x.cuda()[None, None].requires_grad_()
+    out = seq.short_conv(at, weight, activation="silu")
+    (g,) = torch.autograd.grad(out, at, torch.ones_like(out))
+    check("convolution", out[0, 0], want, err)
+    check("its slope", g[0, 0], slope, slope_err)
+    one, zero = torch.ones((1, 1, n), dtype=dtype, device="cuda"), torch.zeros((1, 1, 1), dtype=dtype, device="cuda")
+    A, skip = -torch.ones((n, 1), device="cuda"), torch.ones(n, device="cuda")
+    out = seq.ssm_scan(one, one, A, zero, zero, D=skip, z=at)
+    (g,) = torch.autograd.grad(out, at, torch.ones_like(out))
+    check("gate", out[0, 0], want, err)
+    check("its slope", g[0, 0], slope, slope_err)
+    y = seq.ssm_step(torch.zeros((1, n, 1), device="cuda"), one[0], one[0], A, zero[0], zero[0], D=skip, z=at.detach()[0])
+    check("a step's gate", y[0], want, err)
+    wide = at.detach().expand(40, 3, n).requires_grad_()  # several tiles and rows
+    out = seq.ssm_scan(one.expand(40, 3, n), one.expand(40, 3, n), A, zero.expand(40, 3, 1), zero.expand(40, 3, 1), D=skip, z=wide)
+    (g,) = torch.autograd.grad(out, wide, torch.ones_like(out))
+    check("gate of a sequence", out, want.expand(40, 3, n), err)
+    check("its slope", g, slope.expand(40, 3, n), slope_err)
