@@ -85,7 +85,8 @@ def pack_net(seq: torch.nn.Sequential) -> torch.Tensor:
 
 class FusedPolicy:
     """ms_policy_forward for one Agent: pack() after every parameter change (DeviceRollout
-    does it once per collect, inside its graph), then forward()."""
+    does it once per collect, inside its graph), then forward(). The kernel goes from the
+    observations to the actor and critic: an Agent with a memory between them is refused."""
 
     def __init__(self, agent):
         self.agent = agent
@@ -95,6 +96,8 @@ class FusedPolicy:
         self.pack()
 
     def pack(self) -> None:
+        if getattr(self.agent, "memory", None) is not None:
+            raise ValueError("FusedPolicy has no memory: run the modules of an Agent with one (DeviceRollout(policy='torch'))")
         with torch.no_grad():
             self.packed[0].copy_(pack_net(self.agent.actor_mean))
             self.packed[1].copy_(pack_net(self.agent.critic))

@@ -251,3 +251,13 @@ def test_gradients_reach_a_state_of_another_type():
         grads.append(torch.autograd.grad(m(x, None, leaves)[0].sum(), leaves))
     (a, b), (c, d) = grads
     assert a.dtype == torch.bfloat16 and bool(a.any()) and torch.equal(a, c.bfloat16()) and torch.equal(b, d)
+
+
+def test_the_fused_policy_refuses_an_agent_with_memory():
+    from marlsoccer.policy import FusedPolicy
+    with pytest.raises(ValueError, match="no memory"):
+        FusedPolicy(Agent(memory=SequenceMemory()))
+    fused = FusedPolicy(Agent())
+    fused.agent.memory = SequenceMemory()  # given one later
+    with pytest.raises(ValueError, match="no memory"):
+        fused.pack()
