@@ -243,7 +243,26 @@ class AdamW(torch.optim.Optimizer):
         if p.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: take one step before the capture: a graph that made the moments would zero them at every replay")
 
+    @staticmethod
+    def _refuse_settings(group):
+        for name in ("maximize", "amsgrad"):
+            if group.get(name):
+                raise ValueError(f"AdamW: {name}=True is set, which this update does not do")
+        if group.get("weight_decay", 0) != 0 and not group.get("decoupled_weight_decay", True):
+            raise ValueError("AdamW: a weight decay that is part of the gradient (torch.optim.Adam's) is set; this one's is decoupled")
+
+    def add_param_group(self, param_group):
+        self._refuse_settings(param_group)
+        super().add_param_group(param_group)
+
     def load_state_dict(self, state_dict):
+        """Its own state_dict() or that of torch.optim.AdamW. One whose update is another is refused:
+        maximize, amsgrad, a weight decay that is not decoupled (torch.optim.Adam's), moments of other bits."""
+        for g in state_dict["param_groups"]:
+            self._refuse_settings(g)
+        for s in state_dict["state"].values():
+            if "exp_avg" in s and (s["exp_avg"].dtype == F8) != (self.state_bits == 8):
+                raise ValueError(f"AdamW: the saved moments are {s['exp_avg'].dtype}, this optimizer holds them in {self.state_bits} bits")
         super().load_state_dict(state_dict)
         # Optimizer.load_state_dict casts floating-point state to the parameter's type: take it as it was saved
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]

@@ -581,3 +581,41 @@ def test_a_non_finite_moment_of_8_bits_stays_alone(bad, rounding):
     assert torch.isnan(p1[300]) and torch.isnan(r1[300]) and torch.equal(r0[others], r1[others])
     if not math.isfinite(bad):
         assert torch.isnan(m1[300]) and torch.equal(m0[others], m1[others]) and torch.equal(p0[others], p1[others])
+
+
+def test_a_state_of_another_update_is_refused_when_loaded():
+    """Saved by torch's optimizers with settings that this update does not have, or with moments of other
+    bits; nothing of it is taken over."""
+    def params():
+        return [torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(3))]
+
+    def saved(cls, **kw):
+        ps = params()
+        opt = cls(ps, **kw)
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        opt.step()
+        return opt.state_dict()
+
+    T = torch.optim
+    mine = lambda bits=32: optim.AdamW(params(), lr=0.5, state_bits=bits, rounding="stochastic" if bits == 8 else None)  # noqa: E731
+    for cls, kw, match in ((T.AdamW, dict(maximize=True), "maximize"), (T.AdamW, dict(amsgrad=True), "amsgrad"),
+                           (T.Adam, dict(weight_decay=0.1), "decoupled")):
+        opt = mine()
+        with pytest.raises(ValueError, match=match):
+            opt.load_state_dict(saved(cls, **kw))
+        assert not opt.state and opt.param_groups[0]["lr"] == 0.5
+    with pytest.raises(ValueError, match="maximize"):
+        optim.AdamW([dict(params=params(), maximize=True)])
+    with pytest.raises(ValueError, match="moments are"):
+        mine(8).load_state_dict(saved(T.AdamW))
+    eight = mine(8)
+    for p in eight.param_groups[0]["params"]:
+        eight._state_of(p)
+    with pytest.raises(ValueError, match="moments are"):
+        mine().load_state_dict(eight.state_dict())
+    mine(8).load_state_dict(eight.state_dict())
+    for cls, kw in ((T.AdamW, dict(weight_decay=0.1, lr=0.25)), (T.Adam, dict(lr=0.25))):
+        opt = mine()
+        opt.load_state_dict(saved(cls, **kw))
+        assert opt.param_groups[0]["lr"] == 0.25 and all(int(s["step"]) == 1 for s in opt.state.values())
