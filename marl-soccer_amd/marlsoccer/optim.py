@@ -91,13 +91,14 @@ def _entries(params, grads, exp_avg, exp_avg_sq, steps, scales, sq_scales):
         if not (list(map(_numel, both)) == [-(-k // BLOCK) for k in sizes] * 2 and set(map(_DTYPE, both)) == {torch.float32}
                 and all(map(_packed, both)) and set(map(_where, both)) == {params[0].get_device()}):
             _bad("scales", f"contiguous float32 on {params[0].device}, one for every {BLOCK} values of their parameter")
-        a, b = map(_ptr_of, scales), map(_ptr_of, sq_scales)
+        a, b = list(map(_ptr_of, scales)), list(map(_ptr_of, sq_scales))
     else:
         a = b = repeat(0)
     at, counts = list(map(_ptr_of, every)), list(map(_ptr_of, steps))
-    written = [q for q, k in zip(at[:n] + at[2 * n:], sizes * 3) if k]
-    if len(set(written)) != len(written) or len(set(counts)) != n:
-        _bad("every parameter, moment and step count", "a tensor of its own: one is given twice")
+    written = [q for q, k in zip(at[:n] + at[2 * n:] + (a + b if bits8 else []), sizes * 5) if k]
+    alone = set(written)
+    if len(alone) != len(written) or len(set(counts)) != n or not alone.isdisjoint(q for q, k in zip(at[n:2 * n], sizes) if k):
+        _bad("every parameter, moment, scale and step count", "a tensor of its own: one is given twice")
     rows = zip(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], a, b, counts, sizes,
                [_DTYPES[dt] for dt in of_params], repeat(0))
     return struct.pack("<" + _ROW * n, *chain.from_iterable(rows)), params[0].device
@@ -138,8 +139,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, steps, *, lr, betas=(0.9, 0.9
                max_grad_norm=None, exp_avg_scales=None, exp_avg_sq_scales=None, workspace=None, grad_norm=None, rounding="nearest"):
     """One AdamW step over a list of tensors, in place (see ms_adamw_step in include/marl_soccer.h):
     parameters and gradients float32, bfloat16 or float16, contiguous; moments float32, or float8_e4m3fn
-    with scales; steps: one int64 on the device for each. What is written must not overlap (the same
-    tensor twice is refused). lr: a float, or one float32 on the device.
+    with scales; steps: one int64 on the device for each. What is written must not overlap what else is
+    read or written (the same tensor twice is refused). lr: a float, or one float32 on the device.
     max_grad_norm: clip all gradients together by their norm (the gradients themselves stay as they
     are); grad_norm: one float32 on the device that receives the norm. workspace: WORKSPACE zeroed
     floats, kept by a caller that steps often (None: made here); one step at a time may use it.

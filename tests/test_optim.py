@@ -619,3 +619,25 @@ def test_a_state_of_another_update_is_refused_when_loaded():
         opt = mine()
         opt.load_state_dict(saved(cls, **kw))
         assert opt.param_groups[0]["lr"] == 0.25 and all(int(s["step"]) == 1 for s in opt.state.values())
+
+
+def test_scales_and_gradients_that_are_written_elsewhere_are_refused():
+    """Waves of one launch would race on them: a scale array for both moments or for two tensors, and a
+    gradient that is also another tensor's parameter or moment."""
+    def two(dt=torch.float32, n=4):
+        return [torch.zeros(n, dtype=dt), torch.zeros(n, dtype=dt)]
+
+    good = dict(params=two(), grads=two(), exp_avg=two(optim.F8), exp_avg_sq=two(optim.F8), steps=two(torch.int64, 1), exp_avg_scales=two(n=1),
+                exp_avg_sq_scales=two(n=1), lr=1e-3)
+    for bad in (dict(exp_avg_scales=good["exp_avg_sq_scales"]), dict(exp_avg_scales=[good["exp_avg_scales"][0]] * 2),
+                dict(exp_avg_sq_scales=[good["exp_avg_sq_scales"][1]] * 2), dict(grads=good["params"][::-1])):
+        with pytest.raises(ValueError, match="given twice"):
+            optim.adamw_step(**{**good, **bad})
+    moments = two()
+    with pytest.raises(ValueError, match="given twice"):
+        optim.adamw_step(two(), moments, moments, two(), two(torch.int64, 1), lr=1e-3)
+    with pytest.raises(ValueError, match="HIP device"):
+        optim.adamw_step(**good)
+    with pytest.raises(ValueError, match="HIP device"):  # empty tensors have no address
+        none = [torch.zeros(0), torch.zeros(0)]
+        optim.adamw_step(two(n=0), two(n=0), two(optim.F8, 0), two(optim.F8, 0), two(torch.int64, 1), lr=1e-3, exp_avg_scales=none, exp_avg_sq_scales=none)
