@@ -142,7 +142,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, steps, *, lr, betas=(0.9, 0.9
     with scales; steps: one int64 on the device for each. What is written must not overlap what else is
     read or written (the same tensor twice is refused). lr: a float, or one float32 on the device.
     max_grad_norm: clip all gradients together by their norm (the gradients themselves stay as they
-    are); grad_norm: one float32 on the device that receives the norm. workspace: WORKSPACE zeroed
+    are); grad_norm: one float32 on the device that receives the norm (max_grad_norm inf: the norm alone). workspace: WORKSPACE zeroed
     floats, kept by a caller that steps often (None: made here); one step at a time may use it.
     rounding: of moments with scales, "nearest" or "stochastic" (the module's comment)."""
     if not len(params):
@@ -154,6 +154,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, steps, *, lr, betas=(0.9, 0.9
     rows, device = _entries(params, grads, exp_avg, exp_avg_sq, steps, exp_avg_scales, exp_avg_sq_scales)
     if max_grad_norm is not None and not max_grad_norm > 0:
         _bad("max_grad_norm", "positive")
+    if grad_norm is not None and max_grad_norm is None:
+        _bad("grad_norm", "given with max_grad_norm: without it no norm is computed (inf computes it and clips nothing)")
     if grad_norm is not None and (grad_norm.dtype != torch.float32 or grad_norm.numel() != 1 or grad_norm.device != device):
         _bad("grad_norm", f"one float32 on {device}")
     if device.type == "cuda" and workspace is None:

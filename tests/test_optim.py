@@ -641,3 +641,24 @@ def test_scales_and_gradients_that_are_written_elsewhere_are_refused():
     with pytest.raises(ValueError, match="HIP device"):  # empty tensors have no address
         none = [torch.zeros(0), torch.zeros(0)]
         optim.adamw_step(two(n=0), two(n=0), two(optim.F8, 0), two(optim.F8, 0), two(torch.int64, 1), lr=1e-3, exp_avg_scales=none, exp_avg_sq_scales=none)
+
+
+def test_a_norm_that_nothing_computes_is_refused():
+    one = dict(params=[torch.zeros(4)], grads=[torch.zeros(4)], exp_avg=[torch.zeros(4)], exp_avg_sq=[torch.zeros(4)], steps=[torch.zeros(1, dtype=torch.int64)], lr=1e-3)
+    with pytest.raises(ValueError, match="no norm is computed"):
+        optim.adamw_step(**one, grad_norm=torch.zeros(1))
+    with pytest.raises(ValueError, match="HIP device"):
+        optim.adamw_step(**one, grad_norm=torch.zeros(1), max_grad_norm=float("inf"))
+
+
+@gpu
+def test_an_infinite_max_grad_norm_gives_the_norm_and_clips_nothing():
+    need_gpu()
+    ps, gs = make([(300,), (7,)], torch.float32, 95)
+    outs = []
+    for kw in ({}, dict(max_grad_norm=float("inf"), grad_norm=torch.zeros((), device="cuda"))):
+        lists = [[t.clone() for t in ps], gs, [torch.zeros_like(t) for t in ps], [torch.zeros_like(t) for t in ps], [torch.zeros(1, dtype=torch.int64, device="cuda") for _ in ps]]
+        optim.adamw_step(*lists, lr=1e-2, **kw)
+        outs.append(lists[0])
+    norm = math.sqrt(sum(float(g.double().square().sum()) for g in gs))
+    assert all(torch.equal(a, b) for a, b in zip(*outs)) and abs(float(kw["grad_norm"]) - norm) <= 2 * U * norm
