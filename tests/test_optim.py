@@ -662,3 +662,35 @@ def test_an_infinite_max_grad_norm_gives_the_norm_and_clips_nothing():
         outs.append(lists[0])
     norm = math.sqrt(sum(float(g.double().square().sum()) for g in gs))
     assert all(torch.equal(a, b) for a, b in zip(*outs)) and abs(float(kw["grad_norm"]) - norm) <= 2 * U * norm
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_deep_copy_steps_like_the_original(bits):
+    """The copy's parameters come without gradients (a Parameter's deep copy has none): given the same ones,
+    copy and original take the same steps, each with its own moments, counts and workspace."""
+    import copy
+    need_gpu()
+    shapes = [(20, 5), (700,)]
+    ps, _ = make(shapes, torch.float32, 97)
+    mine = optim.AdamW([torch.nn.Parameter(p) for p in ps], lr=1e-2, max_grad_norm=0.5, state_bits=bits, rounding="stochastic" if bits == 8 else None)
+
+    def step(opt, k):
+        for p, g in zip(opt.param_groups[0]["params"], make(shapes, torch.float32, 98 + k)[1]):
+            p.grad = g
+        opt.step()
+
+    def held(opt):
+        return [t for p in opt.param_groups[0]["params"] for t in (p.detach(), *opt.state[p].values())]
+
+    for k in range(2):
+        step(mine, k)
+    twin = copy.deepcopy(mine)
+    assert {t.data_ptr() for t in held(mine)}.isdisjoint(t.data_ptr() for t in held(twin)) and not twin._work
+    for k in (2, 3):
+        step(mine, k)
+        assert all(int(twin.state[p]["step"]) == k for p in twin.param_groups[0]["params"])  # not moved by the original's step
+        step(twin, k)
+        assert all(torch.equal(a.float(), b.float()) for a, b in zip(held(mine), held(twin)))
+        assert torch.equal(mine.last_grad_norm, twin.last_grad_norm)
+    assert {w.data_ptr() for w in mine._work[ps[0].device]}.isdisjoint(w.data_ptr() for w in twin._work[ps[0].device])
