@@ -158,7 +158,7 @@ class DeviceRollout:
     that graph — one launch per rollout instead of ~40 kernel launches per step. The captured
     graph reads the agent's parameters and the normalizer's mean/var in place, so the PPO
     update must modify them in place (optimizer steps and RunningMeanStd.update do); a replay
-    checks that those tensors are still the captured ones and captures again if not.
+    checks that those tensors, and a memory's state, are still the captured ones and captures again if not.
     policy="fused" (the default for fp32): the normalisation and both MLPs run as ONE gfx950
     kernel (ms_policy_forward: f32-input MFMA, activations in registers; marlsoccer.policy),
     within 1e-5 of the torch modules; "torch": the modules themselves (hipBLASLt GEMMs).
@@ -304,8 +304,8 @@ class DeviceRollout:
 
     def _inputs_identity(self) -> tuple:
         """The tensors a captured rollout reads in place (their storage)."""
-        return tuple(p.data_ptr() for p in self.agent.parameters()) + (self.normalizer.mean.data_ptr(),
-                                                                          self.normalizer.var.data_ptr())
+        state = () if self.memory_state is None else (*self.memory_state, *self.memory_start)
+        return tuple(t.data_ptr() for t in (*self.agent.parameters(), self.normalizer.mean, self.normalizer.var, *state))
 
     def _capture(self) -> None:
         b, dev = self.batch, self.batch.device

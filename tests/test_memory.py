@@ -261,3 +261,22 @@ def test_the_fused_policy_refuses_an_agent_with_memory():
     fused.agent.memory = SequenceMemory()  # given one later
     with pytest.raises(ValueError, match="no memory"):
         fused.pack()
+
+
+@gpu
+def test_a_replaced_state_is_captured_again():
+    """A caller that puts new tensors in memory_state's place, where zeroing them was asked for: a replayed
+    graph would go on from the old ones."""
+    need_gpu()
+    runs = []
+    for graph in (False, True):
+        agent, b, ro = make(24, 9, graph, short_config(7))
+        outs = []
+        for k in range(5):
+            if k == 3:
+                ro.memory_state = agent.memory.init_state(48, "cuda")
+            out = ro.collect()
+            outs += [out[k].clone() for k in ("obs", "actions", "values")] + [s.clone() for s in ro.memory_state + out["memory_state"]]
+        runs.append(outs)
+        b.close()
+    assert all(torch.equal(a, c) for a, c in zip(*runs))
