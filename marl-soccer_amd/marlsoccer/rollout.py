@@ -324,6 +324,8 @@ class DeviceRollout:
         self._graph = g
 
     def collect(self) -> dict:
+        if (getattr(self.agent, "memory", None) is None) != (self.memory_state is None):
+            raise ValueError("the agent's memory came or went after this DeviceRollout was made: make another")
         if self.graph and self._collects > 0:
             if self._graph is not None and self._graph_inputs != self._inputs_identity():
                 self._graph = None  # parameters or normaliser tensors were replaced: capture again

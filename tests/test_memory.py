@@ -280,3 +280,20 @@ def test_a_replaced_state_is_captured_again():
         runs.append(outs)
         b.close()
     assert all(torch.equal(a, c) for a, c in zip(*runs))
+
+
+@gpu
+def test_a_memory_that_comes_or_goes_is_refused():
+    need_gpu()
+    agent, b, ro = make(8, 3)
+    ro.collect()
+    memory, agent.memory = agent.memory, None
+    with pytest.raises(ValueError, match="came or went"):
+        ro.collect()
+    plain = DeviceRollout(b, agent, ro.normalizer, 3)
+    plain.collect()
+    agent.memory = memory
+    with pytest.raises(ValueError, match="came or went"):
+        plain.collect()
+    ro.collect()
+    b.close()
