@@ -370,8 +370,10 @@ int ms_rollout_record(int64_t n_envs, const float *rew, const uint8_t *term, con
  *   for those before the last start. It may be `state` itself when T <= 1 (a step in place).
  * ms_conv_backward: gradients for dout and dnew_state (NULL: zero) with the same inputs: dx,
  *   dstate [io], dweight (D, W), dbias (D); NULL gradients are not written (dx is required).
- *   workspace: ms_conv_workspace() bytes, 16-B aligned.
+ *   workspace: ms_conv_workspace() bytes, 16-B aligned. dweight and dbias add at most MS_SUM_CHAIN steps
+ *   in a row in float32, and these sums in float64.
  */
+#define MS_SUM_CHAIN 512
 typedef struct ms_conv_io {
   int32_t dtype, width, silu, pad0;
   int64_t steps, rows, channels;

@@ -266,7 +266,7 @@ __global__ __launch_bounds__(THREADS) void backward(const ms_conv_io io, const S
       }
     }
   }
-  // the block's sums: slots of the same channels in turn, in a fixed order
+  // the block's sums: slots of the same channels in turn, in a fixed order and in float64 as what follows
   float* to = parts + bp * (W + 1) * D;
 #pragma unroll
   for (int k = 0; k <= W; ++k)
@@ -276,9 +276,9 @@ __global__ __launch_bounds__(THREADS) void backward(const ms_conv_io io, const S
       red[threadIdx.x] = k < W ? dw[k < W ? k : 0][e] : db[e];
       __syncthreads();
       if (slot == 0 && some) {
-        float a = 0.0f;
+        double a = 0.0;
         for (int s = 0; s < slots; ++s) a += red[s * cols + col];
-        to[(c + e) * (W + 1) + k] = a;
+        to[(c + e) * (W + 1) + k] = (float)a;
       }
     }
 }
@@ -302,6 +302,7 @@ __global__ __launch_bounds__(64 * WAVES) void finish(const float* __restrict__ i
 
 // How the work is cut: spans of steps long enough that the W - 1 re-read steps cost little, short
 // enough that there are threads for every SIMD several times over.
+constexpr int64_t CHAIN = MS_SUM_CHAIN;  // steps that a thread adds up in float32 for dw and db
 Shape shape(const ms_conv_io& io, bool back, int E) {
   Shape s = {};
   s.groups = io.channels / E;
@@ -313,6 +314,7 @@ Shape shape(const ms_conv_io& io, bool back, int E) {
   int64_t spans = have > 0 ? (want + have - 1) / have : 1;
   const int64_t most = (io.steps + 15) / 16;  // 16 steps at least: 3 re-read
   spans = spans > most ? most : spans;
+  if (back && spans * CHAIN < io.steps) spans = (io.steps + CHAIN - 1) / CHAIN;
   spans = spans < 1 ? 1 : spans;
   s.span = (io.steps + spans - 1) / spans;
   s.span = s.span < 1 ? 1 : s.span;
@@ -325,7 +327,11 @@ Shape shape(const ms_conv_io& io, bool back, int E) {
   // 1,024 blocks at a time (65,536 rows of one step x 128 bf16: 27 us, 40 uncapped); fewer bytes take four
   // rounds (7,697 x 2,692 f16: 46 us, with 1,024 49, uncapped 52).
   const bool wide = E * (io.dtype == 0 ? 4 : 2) == 16;
-  const int64_t cap = ((back ? 1536 : wide ? 1024 : 4096) + s.blocks_c - 1) / s.blocks_c;
+  int64_t cap = ((back ? 1536 : wide ? 1024 : 4096) + s.blocks_c - 1) / s.blocks_c;
+  if (back) {  // more where a thread's items would be more than CHAIN steps
+    const int64_t turn = slots * (CHAIN / s.span > 1 ? CHAIN / s.span : 1), least = (s.items + turn - 1) / turn;
+    cap = cap < least ? least : cap;
+  }
   if (s.blocks_p > cap) s.blocks_p = cap;
   return s;
 }

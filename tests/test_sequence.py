@@ -782,3 +782,35 @@ def test_activations_of_large_values(dtype):
     (g,) = torch.autograd.grad(out, wide, torch.ones_like(out))
     check("gate of a sequence", out, want.expand(40, 3, n), err)
     check("its slope", g, slope.expand(40, 3, n), slope_err)
+
+
+def drifting(n):
+    """A float32 constant whose n-fold sum, added up one by one in float32, drifts far from n times it."""
+    import numpy as np
+    c = np.linspace(0.1, 0.2, 257, dtype=np.float32)
+    total = np.zeros_like(c)
+    for _ in range(n):
+        total += c
+    off = np.abs(total.astype(np.float64) / (n * c.astype(np.float64)) - 1)
+    return float(c[off.argmax()]), float(off.max())
+
+
+@gpu
+def test_short_conv_sums_long_sequences_in_short_chains():
+    """dweight and dbias over 2^30 steps and rows, all adding the same: each thread adds at most 512 of them
+    in float32 (511 roundings of half a unit, of sums no larger than the last), the rest is float64, with
+    one rounding for a block's part and one at the end. Chains of 4,096, which these rows would make, drift further."""
+    need_gpu()
+    T, R, W = 4096, 262144, 4
+    c, off = drifting(T)
+    bound = 514 * 2.0 ** -24
+    assert off > bound  # the input shows it
+    x = torch.ones((1, 1, 1), device="cuda").expand(T, R, 1)
+    weight, bias = torch.ones((1, W), device="cuda", requires_grad=True), torch.zeros(1, device="cuda", requires_grad=True)
+    out = seq.short_conv(x, weight, bias)
+    dout = torch.full((1, 1, 1), c, device="cuda").expand(T, R, 1)
+    dw, db = torch.autograd.grad(out, (weight, bias), dout)
+    value = float(torch.tensor(c))
+    want = torch.tensor([value * R * (T - W + 1 + k) for k in range(W)], dtype=torch.float64)
+    assert float((dw.double().cpu()[0] / want - 1).abs().max()) <= bound
+    assert abs(float(db) / (value * R * T) - 1) <= bound
