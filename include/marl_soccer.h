@@ -418,7 +418,8 @@ int ms_conv_backward(const ms_conv_io *io, void *stream);
  * ms_scan_backward: gradients for dout and dnew_state (NULL: zero) with the inputs and checkpoints
  *   of the forward: du, ddelta, dz [io, the strides given], dB, dC [io, (T, R, G, N) contiguous],
  *   dA, dD, ddelta_bias, dstate (contiguous). du, ddelta, dB, dC and dA are required, dz with z;
- *   the others may be NULL. workspace: ms_scan_workspace(io, 1) bytes. */
+ *   the others may be NULL. workspace: ms_scan_workspace(io, 1) bytes. dA, dD and ddelta_bias add at
+ *   most MS_SUM_CHAIN steps in a row in float32, and these sums in float64. */
 typedef struct ms_scan_io {
   int32_t dtype, softplus, states, groups;
   int64_t steps, rows, channels;

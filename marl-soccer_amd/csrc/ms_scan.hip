@@ -32,6 +32,8 @@ namespace scan {
 using namespace seq;
 
 constexpr int KC = 8;  // steps between checkpoints
+constexpr int SEGMENT = MS_SUM_CHAIN;  // steps that the backward adds up in float32 for dA, dD and ddelta_bias
+static_assert(SEGMENT % KC == 0, "whole tiles");
 constexpr float LOG2E = 1.44269504f, LN2 = 0.69314718f;
 
 #define CONSTANT(T) const __attribute__((address_space(4))) T
@@ -44,6 +46,7 @@ struct Plan {
   int64_t tiles, blocks_d;  // tiles per group, tiles * groups
   int64_t chunks, chunk;    // over time; steps per chunk (a multiple of 32)
   int64_t kc;               // checkpoints, tiles of the backward pass
+  int64_t segments;         // of a chunk: the backward's sums over time are handed on after each
 };
 
 struct Work {  // the workspace, in floats
@@ -674,6 +677,30 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
     vo = load<T, E>(po, in ? n : 0, vec);
     if (pz) vz = load<T, E>(pz, in ? n : 0, vec);
   };
+  // a segment's parts of dA (D, N), dD (D) and ddelta_bias (D), in one row; the sums begin anew
+  auto hand_on = [&](int64_t g) __attribute__((always_inline)) {
+    const int64_t D = io.channels;
+    float* part = a.parts + ((at.chunk * a.p.segments + g) * io.rows + at.r) * D * (N + 2);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      if (live && w * NS + i < N) part[ch * N + w * NS + i] = dA[i];
+      dA[i] = 0.0f;
+    }
+    __syncthreads();
+    if (threadIdx.x < 64 && live) {  // the threads of the same channels add up
+      double dskip = 0.0, dbias = 0.0;
+#pragma unroll
+      for (int i = 0; i < TT; ++i) {
+        dskip += s_kept[DSKIP][i][lane];
+        dbias += s_kept[DBIAS][i][lane];
+      }
+      part[D * N + ch] = (float)dskip;
+      part[D * (N + 1) + ch] = (float)dbias;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_kept[DSKIP][lt][lc + e] = s_kept[DBIAS][lt][lc + e] = 0.0f;
+  };
   fetch((tiles - 1) * TT + lt < len);
 #pragma unroll
   for (int q = 0; q < NS / 4; ++q) start[q] = *(const float4*)(from + q * 256 + lane * 4);
@@ -842,33 +869,18 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
     qu -= TT * io.du_t;
     qd -= TT * io.ddelta_t;
     if (pz) qz -= TT * io.dz_t;
+    if (k % (SEGMENT / TT) == 0) hand_on(k / (SEGMENT / TT));
   }
-  // this chunk's parts of dA (D, N), dD (D) and ddelta_bias (D), in one row
-  const int64_t D = io.channels;
-  float* part = a.parts + (at.chunk * io.rows + at.r) * D * (N + 2);
-  if (live) {
+  // a last chunk that is shorter than the others has nothing to add in their last segments
+  for (int g = (tiles + SEGMENT / TT - 1) / (SEGMENT / TT); g < a.p.segments; ++g) hand_on(g);
+  if (live && io.dstate && t_begin == 0) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
-      if (w * NS + i < N) {
-        part[ch * N + w * NS + i] = dA[i];
-        if (io.dstate && t_begin == 0) io.dstate[slot + w * NS + i] = carry[i];
-      }
-  }
-  // dD and ddelta_bias: the threads of the same channels add up
-  __syncthreads();
-  if (threadIdx.x < 64 && live) {
-    float dskip = 0.0f, dbias = 0.0f;
-#pragma unroll
-    for (int i = 0; i < TT; ++i) {
-      dskip += s_kept[DSKIP][i][lane];
-      dbias += s_kept[DBIAS][i][lane];
-    }
-    part[D * N + ch] = dskip;
-    part[D * (N + 1) + ch] = dbias;
+      if (w * NS + i < N) io.dstate[slot + w * NS + i] = carry[i];
   }
 }
 
-// The second stage of the sums over rows and chunks, put in place: dA, dD, ddelta_bias
+// The second stage of the sums over rows, chunks and segments, put in place: dA, dD, ddelta_bias
 template <int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void finish_weights(const float* __restrict__ in, int64_t parts, ms_scan_io io) {
   __shared__ double s[WAVES][64];
@@ -964,6 +976,7 @@ Plan plan(const ms_scan_io& io, bool back) {
   p.chunk = p.chunk < 32 ? 32 : p.chunk;
   p.chunks = io.steps > 0 ? (io.steps + p.chunk - 1) / p.chunk : 1;
   p.kc = (io.steps + KC - 1) / KC;
+  p.segments = ((p.chunks > 1 ? p.chunk : io.steps) + SEGMENT - 1) / SEGMENT;
   p.unit = back ? 4 : p.ns;
   // whole tiles of 32 steps, and a unit past the end
   p.units = (io.steps + 31) / 32 * 32 * p.unit / 16 + 1;
@@ -972,7 +985,7 @@ Plan plan(const ms_scan_io& io, bool back) {
 
 int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
 
-// how many parts the sums over rows and chunks add in the first of their two stages
+// how many parts the sums over rows, chunks and segments add in the first of their two stages
 int64_t share_of(int64_t parts) { return parts <= 64 ? parts : parts <= 4096 ? 64 : (parts + 63) / 64; }
 
 int64_t scalar_floats(const ms_scan_io& io, const Plan& p) { return io.rows * io.groups * (p.ns * p.nw / p.unit) * p.units * 32; }
@@ -999,9 +1012,9 @@ Work work(const ms_scan_io& io, const Plan& p, bool back) {
   }
   if (back) {
     w.parts_bc = take(p.kc * io.rows * p.blocks_d * (p.ns * p.nw / 4) * 64);
-    w.parts = take(parts * row);
-    const int64_t share = share_of(parts);
-    w.sums = share ? take((parts + share - 1) / share * row) : nullptr;
+    const int64_t sums = parts * p.segments, share = share_of(sums);
+    w.parts = take(sums * row);
+    w.sums = share ? take((sums + share - 1) / share * row) : nullptr;
   }
   w.floats = used;
   return w;
@@ -1214,7 +1227,7 @@ int ms_scan_backward(const ms_scan_io* io, void* stream) {
   if (io->dtype == 0) hipLaunchKernelGGL(scan::finish_bc<float>, grid, block, 0, st, a, split);
   else if (io->dtype == 1) hipLaunchKernelGGL(scan::finish_bc<seq::bf16>, grid, block, 0, st, a, split);
   else hipLaunchKernelGGL(scan::finish_bc<seq::f16>, grid, block, 0, st, a, split);
-  const int64_t parts = p.chunks * io->rows, share = scan::share_of(parts), row = io->channels * (io->states + 2);
+  const int64_t parts = p.chunks * p.segments * io->rows, share = scan::share_of(parts), row = io->channels * (io->states + 2);
   const unsigned columns = (unsigned)((row + 63) / 64), shares = (unsigned)((parts + share - 1) / share);
   if (shares > 1)
     hipLaunchKernelGGL(seq::sum_parts<4>, dim3(columns, shares), dim3(256), 0, st, w.parts, parts, share, row, w.sums);

@@ -814,3 +814,45 @@ def test_short_conv_sums_long_sequences_in_short_chains():
     want = torch.tensor([value * R * (T - W + 1 + k) for k in range(W)], dtype=torch.float64)
     assert float((dw.double().cpu()[0] / want - 1).abs().max()) <= bound
     assert abs(float(db) / (value * R * T) - 1) <= bound
+
+
+@gpu
+def test_ssm_scan_sums_long_sequences_in_short_chains():
+    """dA, dD and ddelta_bias over 65,536 steps of 512 rows that all add nearly the same: at most 512 steps are
+    added up in float32, the rest in float64. The 64-bit values: every row is the same, and once the states have
+    settled (exp(-0.5) a step at the slowest) each step adds the same again. dD's terms are exact: 514 u as for
+    the convolution. A term of dA or ddelta_bias has two states that have settled, each off by at most 12 u (a
+    decay by (3 x 0.5 + 2) u, which 1 / (1 - a) = 2.5 makes 9, and two roundings a step), the slope, the products
+    and the sum over 16 states: below 64 u."""
+    need_gpu()
+    T, R, N, short = 65536, 512, 16, 512
+    c, off = drifting(T // 8)  # of the eight sums in turn that a row's steps make
+    u = 2.0 ** -24
+    assert off > 578 * u
+    one = lambda x: torch.tensor([[[x]]], dtype=torch.float32)  # noqa: E731
+    A, B, C = -torch.arange(1, N + 1, dtype=torch.float32)[None], torch.full((1, 1, N), 0.75), torch.linspace(0.5, 1.0, N)[None, None]
+    skip, bias = torch.ones(1), torch.zeros(1)
+    wants = []
+    for t in (short - 1, short):
+        far = lambda x: x.expand(t, 1, x.shape[2])  # noqa: E731
+        wants.append(ref.scan(far(one(1.0)), far(one(0.5)), A, far(B), far(C), skip, None, bias, soft=False, dout=far(one(c)))[2])
+    leaves = [x.cuda().requires_grad_() for x in (A, skip, bias)]
+    far = lambda x: x.cuda().expand(T, R, x.shape[2])  # noqa: E731
+    out = seq.ssm_scan(far(one(1.0)), far(one(0.5)), leaves[0], far(B), far(C), D=leaves[1], delta_bias=leaves[2], delta_softplus=False)
+    grads = torch.autograd.grad(out, leaves, far(one(c)))
+    for name, g, k in (("A", grads[0], 578), ("D", grads[1], 514), ("delta_bias", grads[2], 578)):
+        want = (wants[1][name] + (T - short) * (wants[1][name] - wants[0][name])) * R
+        rel = float((g.double().cpu() / want - 1).abs().max())
+        assert rel <= k * u, (name, rel / u)
+
+
+@gpu
+@pytest.mark.parametrize("T,R,D,N", [(513, 520, 64, 16), (1030, 520, 3, 5), (1600, 2, 64, 16), (4200, 1, 70, 33)])
+def test_ssm_scan_around_the_segments_of_its_sums(T, R, D, N):
+    """Lengths past whole segments, with the time axis whole (many rows) and in chunks."""
+    need_gpu()
+    v = scan_inputs(T, R, D, N, 1, torch.float32, 171, "cuda", state=True)
+    v["starts"] = (torch.rand((T, R), generator=gen(172)) < 0.01).cuda()
+    g = gen(173)
+    dout, dnew = torch.randn((T, R, D), generator=g).cuda(), torch.randn((R, D, N), generator=g).cuda()
+    check_scan(v, True, dout, dnew)
