@@ -97,7 +97,8 @@ def _entries(params, grads, exp_avg, exp_avg_sq, steps, scales, sq_scales):
     at, counts = list(map(_ptr_of, every)), list(map(_ptr_of, steps))
     written = [q for q, k in zip(at[:n] + at[2 * n:] + (a + b if bits8 else []), sizes * 5) if k]
     alone = set(written)
-    if len(alone) != len(written) or len(set(counts)) != n or not alone.isdisjoint(q for q, k in zip(at[n:2 * n], sizes) if k):
+    if (len(alone) != len(written) or len(set(counts)) != n
+            or not alone.isdisjoint(at[n:2 * n]) and any(k and q in alone for q, k in zip(at[n:2 * n], sizes))):
         _bad("every parameter, moment, scale and step count", "a tensor of its own: one is given twice")
     rows = zip(at[:n], at[n:2 * n], at[2 * n:3 * n], at[3 * n:], a, b, counts, sizes,
                [_DTYPES[dt] for dt in of_params], repeat(0))
