@@ -362,7 +362,8 @@ int ms_rollout_record(int64_t n_envs, const float *rew, const uint8_t *term, con
  * new episode at step t, and nothing before t, the given state included, reaches step t or later.
  * dtype: 0 float32, 1 bfloat16, 2 float16 for the arrays marked [io]; all others are float32.
  * Asynchronous on `stream`; no atomics, so results repeat bit for bit. Arrays must not overlap
- * unless stated. T = 0 and R = 0 are allowed (state copied through, gradients zero).
+ * unless stated. T = 0 and R = 0 are allowed (state copied through, gradients zero). Calls that would
+ * need a launch of 2^32 threads (a scan's R x D from 2^30 on) are refused; ms_scan_step takes several.
  *
  * ms_conv_forward: out[t][r][d] = act(bias[d] + sum_k weight[d][k] x[t - W + 1 + k][r][d]), W = width
  *   in 2..4, act SiLU or none; steps before 0 come from state (R, W-1, D) [io], oldest first

@@ -373,7 +373,7 @@ template <typename T, int E>
 int run_forward(const ms_conv_io& io, hipStream_t stream) {
   const Shape s = shape(io, false, E);
   const int64_t blocks = s.blocks_c * s.blocks_p;
-  if (blocks > 0x7fffffff) return fail(MS_ERR_INVALID_ARGUMENT, "ms_conv_forward", "too large");
+  if (too_many(blocks, THREADS)) return fail(MS_ERR_INVALID_ARGUMENT, "ms_conv_forward", "too large");
   const dim3 grid((unsigned)blocks), block(THREADS);
   switch (io.width) {
     case 2: hipLaunchKernelGGL((forward<T, E, 2>), grid, block, 0, stream, io, s); break;
@@ -393,10 +393,11 @@ int forward_as(const ms_conv_io& io, hipStream_t stream) {
 template <typename T, int E, bool FULL>
 int run_backward(const ms_conv_io& io, hipStream_t stream) {
   const Shape s = shape(io, true, E);
-  if (s.blocks_c * s.blocks_p > 0x7fffffff) return fail(MS_ERR_INVALID_ARGUMENT, "ms_conv_backward", "too large");
+  const int64_t columns = io.channels * (io.width + 1);
+  if (too_many(s.blocks_c * s.blocks_p, THREADS) || too_many((columns + 63) / 64, 1024))
+    return fail(MS_ERR_INVALID_ARGUMENT, "ms_conv_backward", "too large");
   const dim3 grid((unsigned)(s.blocks_c * s.blocks_p)), block(THREADS);
   float* parts = (float*)io.workspace;
-  const int64_t columns = io.channels * (io.width + 1);
   switch (io.width) {
     case 2: hipLaunchKernelGGL((backward<T, E, 2, FULL>), grid, block, 0, stream, io, s, parts); break;
     case 3: hipLaunchKernelGGL((backward<T, E, 3, FULL>), grid, block, 0, stream, io, s, parts); break;

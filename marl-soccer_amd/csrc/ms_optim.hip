@@ -498,7 +498,7 @@ int ms_adamw_step(const ms_optim_tensor* tensors, int64_t count, int state_bits,
       list.t[i] = tensors[first + i];
       const int64_t one = (int64_t)per * opt::ROUND;
       blocks += (uint64_t)((list.t[i].numel + one - 1) / one);
-      if (blocks > 0x7fffffff) return opt::fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
+      if (blocks > 0xffffffffu / opt::THREADS) return opt::fail(MS_ERR_INVALID_ARGUMENT, who, "too large");  // a launch's threads are counted in 32 bits
       list.end[i] = (uint32_t)blocks;
     }
     if (blocks == 0) {  // only empty tensors: a block still raises their counts

@@ -1041,8 +1041,20 @@ const char* check(const ms_scan_io* io, bool back, bool step) {
   return nullptr;
 }
 
-// out of 32-bit grids: refused
-bool too_many(int64_t blocks) { return blocks > 0x7fffffff; }
+int64_t widen_blocks(const ms_scan_io& io, const Plan& p) {
+  const int64_t each = 64 / (p.ns * p.nw / p.unit);
+  return (p.units * io.rows * io.groups + each - 1) / each;
+}
+int64_t join_blocks(const ms_scan_io& io) { return (io.rows * io.channels * io.states + 255) / 256; }
+int64_t finish_waves(const ms_scan_io& io) { return (io.steps + 7) / 8 * io.rows * io.groups; }
+
+// Whether every launch's threads fit 32 bits, looked at before the first of them
+bool fits(const ms_scan_io& io, const Plan& p, bool back) {
+  if (io.rows > ((int64_t)1 << 40) / io.channels || io.rows > ((int64_t)1 << 40) / (io.steps + 64)) return false;
+  if (too_many(p.blocks_d * io.rows * p.chunks, 64 * p.nw) || too_many(widen_blocks(io, p), 256) || io.rows * io.groups > 0x7fffffff) return false;
+  if (p.chunks > 1 && too_many(join_blocks(io), 256)) return false;
+  return !back || !(too_many((finish_waves(io) * (p.ns * p.nw / 4) + 3) / 4, 256) || too_many((io.channels * (io.states + 2) + 63) / 64, 256));
+}
 
 int prepare(const ms_scan_io& io, const Plan& p, const Work& w, bool back, hipStream_t stream, const char* who, Args& a) {
   a.io = io;
@@ -1055,12 +1067,10 @@ int prepare(const ms_scan_io& io, const Plan& p, const Work& w, bool back, hipSt
   a.parts = w.parts;
   if (back && kept_scalars(io, p)) return MS_OK;
   const int shares = p.ns * p.nw / p.unit;
-  const int64_t each = 64 / shares, blocks = (p.units * io.rows * io.groups + each - 1) / each;
-  if (too_many(blocks) || too_many(io.rows * io.groups)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
   const int64_t elem = io.dtype == 0 ? 4 : 2;
   const bool vec = p.unit >= 4 && aligned(io.B, io.B_t, io.B_r, elem, 4) && aligned(io.C, io.C_t, io.C_r, elem, 4) &&
                    (io.groups == 1 || (io.B_g % 4 == 0 && io.C_g % 4 == 0));
-  const dim3 grid((unsigned)blocks), block(256);
+  const dim3 grid((unsigned)widen_blocks(io, p)), block(256);
   if (io.dtype == 0) hipLaunchKernelGGL(widen<float>, grid, block, 0, stream, io, p.unit, shares, p.units, vec, w.bc);
   else if (io.dtype == 1) hipLaunchKernelGGL(widen<bf16>, grid, block, 0, stream, io, p.unit, shares, p.units, vec, w.bc);
   else hipLaunchKernelGGL(widen<f16>, grid, block, 0, stream, io, p.unit, shares, p.units, vec, w.bc);
@@ -1102,9 +1112,7 @@ void launch_type(Pass pass, const Args& a, dim3 grid, hipStream_t stream) {
 }
 int launch(Pass pass, Args& a, hipStream_t stream, const char* who) {
   a.vec = vec_ok(a.io, pass, a.p.nw);
-  const int64_t blocks = a.p.blocks_d * a.io.rows * a.p.chunks;
-  if (too_many(blocks)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
-  const dim3 grid((unsigned)blocks);
+  const dim3 grid((unsigned)(a.p.blocks_d * a.io.rows * a.p.chunks));
   if (a.io.dtype == 0) launch_type<float>(pass, a, grid, stream);
   else if (a.io.dtype == 1) launch_type<bf16>(pass, a, grid, stream);
   else launch_type<f16>(pass, a, grid, stream);
@@ -1112,9 +1120,7 @@ int launch(Pass pass, Args& a, hipStream_t stream, const char* who) {
 }
 template <bool BACK>
 int launch_join(const Args& a, hipStream_t stream, const char* who) {
-  const int64_t blocks = (a.io.rows * a.io.channels * a.io.states + 255) / 256;
-  if (too_many(blocks)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
-  hipLaunchKernelGGL(join<BACK>, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(join<BACK>, dim3((unsigned)join_blocks(a.io)), dim3(256), 0, stream, a);
   return launched(who);
 }
 
@@ -1124,24 +1130,48 @@ __global__ __launch_bounds__(256) void copy_state(const float* __restrict__ from
 }
 int copied(const float* from, int64_t n, float* to, hipStream_t stream, const char* who) {
   if (!to || n == 0 || to == from) return MS_OK;
-  if (too_many((n + 255) / 256)) return fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
-  hipLaunchKernelGGL(copy_state, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, from, n, to);
-  return launched(who);
+  constexpr int64_t MOST = (int64_t)1 << 31;  // values a launch
+  for (int64_t i = 0; i < n; i += MOST) {
+    const int64_t m = n - i < MOST ? n - i : MOST;
+    hipLaunchKernelGGL(copy_state, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, stream, from ? from + i : nullptr, m, to + i);
+    if (int rc = launched(who)) return rc;
+  }
+  return MS_OK;
 }
 
+// A step of as many rows at a time as a launch has threads for
 template <typename T>
-void launch_step(const ms_scan_io& io, hipStream_t stream) {
-  const int64_t rc = io.rows * io.channels;
+int launch_step(ms_scan_io io, hipStream_t stream) {
   const int q = io.states / 4;
   const bool four = io.states % 4 == 0 && (q & (q - 1)) == 0 && ((uintptr_t)io.A & 15u) == 0 &&
                     ((uintptr_t)io.new_state & 15u) == 0 && (!io.state || ((uintptr_t)io.state & 15u) == 0);
-  const dim3 grid((unsigned)((rc * (four ? q : 1) + 255) / 256)), block(256);
-  if (!four) hipLaunchKernelGGL(step1<T>, grid, block, 0, stream, io);
-  else if (q == 1) hipLaunchKernelGGL((step4<T, 1>), grid, block, 0, stream, io);
-  else if (q == 2) hipLaunchKernelGGL((step4<T, 2>), grid, block, 0, stream, io);
-  else if (q == 4) hipLaunchKernelGGL((step4<T, 4>), grid, block, 0, stream, io);
-  else if (q == 8) hipLaunchKernelGGL((step4<T, 8>), grid, block, 0, stream, io);
-  else hipLaunchKernelGGL((step4<T, 16>), grid, block, 0, stream, io);
+  const int64_t one = io.channels * (four ? q : 1), most = 0xffffff00ll / one;  // a row's threads
+  if (most < 1) return fail(MS_ERR_INVALID_ARGUMENT, "ms_scan_step", "too large");
+  auto move = [](auto*& p, int64_t by) {
+    typedef std::remove_reference_t<decltype(p)> P;
+    if (p) p = (P)((const T*)p + by);
+  };
+  for (int64_t left = io.rows; left > 0; left -= most) {
+    io.rows = left < most ? left : most;
+    const dim3 grid((unsigned)((io.rows * one + 255) / 256)), block(256);
+    if (!four) hipLaunchKernelGGL(step1<T>, grid, block, 0, stream, io);
+    else if (q == 1) hipLaunchKernelGGL((step4<T, 1>), grid, block, 0, stream, io);
+    else if (q == 2) hipLaunchKernelGGL((step4<T, 2>), grid, block, 0, stream, io);
+    else if (q == 4) hipLaunchKernelGGL((step4<T, 4>), grid, block, 0, stream, io);
+    else if (q == 8) hipLaunchKernelGGL((step4<T, 8>), grid, block, 0, stream, io);
+    else hipLaunchKernelGGL((step4<T, 16>), grid, block, 0, stream, io);
+    if (int rc = launched("ms_scan_step")) return rc;
+    move(io.u, most * io.u_r);
+    move(io.delta, most * io.delta_r);
+    move(io.z, most * io.z_r);
+    move(io.B, most * io.B_r);
+    move(io.C, most * io.C_r);
+    move(io.out, most * io.out_r);
+    if (io.starts) io.starts += most * io.starts_r;
+    if (io.state) io.state += most * io.channels * io.states;
+    io.new_state += most * io.channels * io.states;
+  }
+  return MS_OK;
 }
 
 bool space(const ms_scan_io& io, int64_t bytes) {
@@ -1172,6 +1202,7 @@ int ms_scan_forward(const ms_scan_io* io, void* stream) {
   if (io->rows == 0) return MS_OK;
   if (io->steps == 0) return scan::copied(io->state, io->rows * io->channels * io->states, io->new_state, st, who);
   const scan::Plan p = scan::plan(*io, false);
+  if (!scan::fits(*io, p, false)) return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
   const scan::Work w = scan::work(*io, p, false);
   if (!scan::space(*io, w.floats * 4))
     return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "the workspace is missing, misaligned or too small");
@@ -1189,12 +1220,8 @@ int ms_scan_forward(const ms_scan_io* io, void* stream) {
 int ms_scan_step(const ms_scan_io* io, void* stream) {
   if (const char* why = scan::check(io, false, true)) return seq::fail(MS_ERR_INVALID_ARGUMENT, "ms_scan_step", why);
   if (io->rows == 0) return MS_OK;
-  if (scan::too_many((io->rows * io->channels * 16 + 255) / 256))
-    return seq::fail(MS_ERR_INVALID_ARGUMENT, "ms_scan_step", "too large");
-  if (io->dtype == 0) scan::launch_step<float>(*io, (hipStream_t)stream);
-  else if (io->dtype == 1) scan::launch_step<seq::bf16>(*io, (hipStream_t)stream);
-  else scan::launch_step<seq::f16>(*io, (hipStream_t)stream);
-  return seq::launched("ms_scan_step");
+  const hipStream_t st = (hipStream_t)stream;
+  return io->dtype == 0 ? scan::launch_step<float>(*io, st) : io->dtype == 1 ? scan::launch_step<seq::bf16>(*io, st) : scan::launch_step<seq::f16>(*io, st);
 }
 
 int ms_scan_backward(const ms_scan_io* io, void* stream) {
@@ -1209,6 +1236,7 @@ int ms_scan_backward(const ms_scan_io* io, void* stream) {
     return scan::copied(io->dnew_state, io->rows * dn, io->dstate, st, who);
   }
   const scan::Plan p = scan::plan(*io, true);
+  if (!scan::fits(*io, p, true)) return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
   const scan::Work w = scan::work(*io, p, true);
   if (!scan::space(*io, w.floats * 4) || ((uintptr_t)io->checkpoints & 15u))
     return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "the workspace or the checkpoints are missing, misaligned or too small");
@@ -1219,10 +1247,9 @@ int ms_scan_backward(const ms_scan_io* io, void* stream) {
     if (int rc = scan::launch_join<true>(a, st, who)) return rc;
   }
   if (int rc = scan::launch(scan::BACK, a, st, who)) return rc;
-  int64_t waves = (io->steps + 7) / 8 * io->rows * io->groups;
+  int64_t waves = scan::finish_waves(*io);
   const int split = waves < 32768 ? p.ns * p.nw / 4 : 1;
   waves *= split;
-  if (scan::too_many(waves + 4)) return seq::fail(MS_ERR_INVALID_ARGUMENT, who, "too large");
   const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
   if (io->dtype == 0) hipLaunchKernelGGL(scan::finish_bc<float>, grid, block, 0, st, a, split);
   else if (io->dtype == 1) hipLaunchKernelGGL(scan::finish_bc<seq::bf16>, grid, block, 0, st, a, split);

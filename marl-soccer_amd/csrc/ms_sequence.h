@@ -99,6 +99,9 @@ inline bool aligned(const void* p, int64_t a, int64_t b, int64_t elem, int64_t v
   return ((uintptr_t)p % (uint64_t)bytes) == 0 && a % unit == 0 && b % unit == 0;
 }
 
+// A launch's threads are counted in 32 bits: past them the runtime cuts the grid without an error
+inline bool too_many(int64_t blocks, int64_t threads) { return blocks > 0xffffffffll / threads; }
+
 inline int fail(int code, const char* who, const char* why) {
   snprintf(g_sequence_error, sizeof(g_sequence_error), "%s: %s", who, why);
   return code;

@@ -856,3 +856,36 @@ def test_ssm_scan_around_the_segments_of_its_sums(T, R, D, N):
     g = gen(173)
     dout, dnew = torch.randn((T, R, D), generator=g).cuda(), torch.randn((R, D, N), generator=g).cuda()
     check_scan(v, True, dout, dnew)
+
+
+@gpu
+@pytest.mark.parametrize("N", [16, 1])
+def test_a_step_of_more_rows_than_a_launch_has_threads(N):
+    """2^32 threads and some (four states a thread, or a channel each): the same as the rows by themselves."""
+    need_gpu()
+    D = 64 if N == 16 else 256
+    R = 2 ** 24 + 3
+    if torch.cuda.mem_get_info()[0] < 120 * 2 ** 30:
+        pytest.skip("needs 120 GiB of device memory")
+    g = torch.Generator(device="cuda").manual_seed(181)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    u, delta, B, C = r(R, D), r(1, D).expand(R, D), r(R, N), r(R, N)
+    A, state = -torch.rand((D, N), generator=g, device="cuda") - 0.5, torch.ones((R, D, N), device="cuda")
+    y = seq.ssm_step(state, u, delta, A, B, C)
+    for at in (slice(0, 5), slice(R // 2, R // 2 + 5), slice(2 ** 24 - 2, R)):
+        alone = torch.ones((at.stop - at.start, D, N), device="cuda")
+        same = torch.equal(y[at], seq.ssm_step(alone, u[at], delta[at], A, B[at], C[at])), torch.equal(state[at], alone)
+        assert same == (True, True), at
+
+
+def test_sequences_past_a_launchs_threads_are_refused_before_anything_runs():
+    """No device is needed to hear it: nothing was launched."""
+    import ctypes as C
+
+    from marlsoccer import _native as N
+    L = N.lib()
+    many = 2 ** 27  # rows of 64 channels: 2^27 blocks of 256 threads
+    io = N.MsScanIO(dtype=1, states=16, groups=1, steps=1, rows=many, channels=64, u=16, delta=16, B=16, C=16, A=16, out=16, workspace=16,
+                    workspace_bytes=2 ** 62, dout=16, du=16, ddelta=16, dB=16, dC=16, dA=16, checkpoints=16)
+    for fn in (L.ms_scan_forward, L.ms_scan_backward):
+        assert fn(C.byref(io), None) == N.MS_ERR_INVALID_ARGUMENT and b"too large" in L.ms_sequence_last_error()
