@@ -213,7 +213,7 @@ class AdamW(torch.optim.Optimizer):
             warnings.warn("AdamW: moments in 8 bits, rounded to nearest, lose small changes for good; rounding='stochastic' keeps them "
                           "in the mean", stacklevel=2)
         self.max_grad_norm, self.state_bits, self.rounding = max_grad_norm, state_bits, rounding
-        self._work = {}
+        self._work, self._clipped = {}, False
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def __getstate__(self):
@@ -222,12 +222,12 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self.rounding = state.get("rounding")
-        self._work = {}  # a copy's own
+        self._work, self._clipped = {}, False  # a copy's own
 
     @property
     def last_grad_norm(self):
         """The norm of the last clipped step, one float32 on the device (None before it)."""
-        return next((w[1] for w in self._work.values()), None)
+        return next((w[1] for w in self._work.values()), None) if self._clipped else None
 
     def _state_of(self, p):
         s = self.state[p]
@@ -319,4 +319,5 @@ class AdamW(torch.optim.Optimizer):
             calls.append(_step_call(rows, bits, group["lr"], group["betas"], group["eps"], group["weight_decay"],
                                     self.max_grad_norm is not None, work, device))
         _launch(device, every_param, calls)
+        self._clipped |= self.max_grad_norm is not None
         return loss

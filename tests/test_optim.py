@@ -694,3 +694,16 @@ def test_a_deep_copy_steps_like_the_original(bits):
         assert all(torch.equal(a.float(), b.float()) for a, b in zip(held(mine), held(twin)))
         assert torch.equal(mine.last_grad_norm, twin.last_grad_norm)
     assert {w.data_ptr() for w in mine._work[ps[0].device]}.isdisjoint(w.data_ptr() for w in twin._work[ps[0].device])
+
+
+@gpu
+def test_there_is_no_norm_before_a_clipped_step():
+    need_gpu()
+    p = torch.nn.Parameter(torch.ones(4, device="cuda"))
+    p.grad = torch.full_like(p, 3.0)
+    opt = optim.AdamW([p])
+    opt.step()
+    assert opt.last_grad_norm is None
+    opt.max_grad_norm = 1.0
+    opt.step()
+    assert float(opt.last_grad_norm) == 6.0
