@@ -183,8 +183,10 @@ __device__ __forceinline__ float wave_max(float x) {
 // beta2 = 0.999 a root moves by some 0.05 % a step: then only the largest moves, by the scale, and the others
 // follow it (roots 0.3 to 9 times the 32-bit ones after thousands of steps whose gradients change in
 // size). SR keeps such changes in the mean: each rounding is right in expectation, and the held root
-// wanders about the 32-bit one, by some 17 % of it at beta2 = 0.999.
-template <bool SR>
+// wanders about the 32-bit one, by some 17 % of it at beta2 = 0.999. ROOT: the second moment's, which SR
+// does not round down to nothing: a value that the first moment was rounded up at would be divided by it
+// (values of 1e-6 of their block's largest: steps of 100 times lr and more).
+template <bool SR, bool ROOT>
 __device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_lane, Odds odds) {
   float top = 0.0f;
 #pragma unroll
@@ -200,7 +202,11 @@ __device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_l
   const float inv = some ? 448.0f / top : 0.0f;
   if (first_lane) *scale = some ? top / 448.0f : 0.0f;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = v[k] * inv;
+  for (int k = 0; k < 4; ++k) {
+    const float x = v[k];
+    v[k] = x * inv;
+    if constexpr (SR && ROOT) v[k] = v[k] < 0x1p-9f && x > 0.0f ? 0x1p-9f : v[k];
+  }
   if constexpr (SR) return encode(v, odds);
   else return encode(v);
 }
@@ -308,8 +314,8 @@ __global__ __launch_bounds__(THREADS) void adamw(const List list, const Hyper hp
       const int64_t q = i / MS_ADAMW_BLOCK;
       Odds o = {};
       if constexpr (SR) o = odds_of(i, f.key);
-      put_codes((uint8_t*)a.exp_avg, i, n, vs, quantise<SR>(m, a.exp_avg_scale + q, lane == 0, o));
-      put_codes((uint8_t*)a.exp_avg_sq, i, n, vs, quantise<SR>(r, a.exp_avg_sq_scale + q, lane == 0, {{o.h[1], o.h[0]}}));
+      put_codes((uint8_t*)a.exp_avg, i, n, vs, quantise<SR, false>(m, a.exp_avg_scale + q, lane == 0, o));
+      put_codes((uint8_t*)a.exp_avg_sq, i, n, vs, quantise<SR, true>(r, a.exp_avg_sq_scale + q, lane == 0, {{o.h[1], o.h[0]}}));
     }
   }
   // every block has read its count (and used it) by its ticket; the last one raises them all. The ticket

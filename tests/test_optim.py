@@ -443,7 +443,7 @@ def test_stochastic_rounding_keeps_the_expected_moments():
     neighbours has a deviation of at most step / (2 sqrt(K)); 6 of them hold for 2 x 5,003 values with a
     probability of 1 - 10,006 x 2e-9. The odds have 16 bits, cut: a bias of at most 2^-16 steps, and
     float32's roundings of the moment before it (9 u and 8 u of its terms, the module's comment) and of the
-    scaled value (2 u). The same count gives the same bits."""
+    scaled value (2 u). A root below the smallest code is held as that code. The same count gives the same bits."""
     need_gpu()
     n, K, b1, b2 = 5003, 600, 0.9, 0.999
     g = torch.Generator().manual_seed(11)
@@ -465,6 +465,8 @@ def test_stochastic_rounding_keeps_the_expected_moments():
         assert all(torch.equal(a, b) for a, b in zip(outs[0], outs[-1]))
         for j, (got, s) in enumerate(zip(outs[0], ("exp_avg_scales", "exp_avg_sq_scales"))):
             scale = lists[s][0].double().repeat_interleave(optim.BLOCK)[:n]
+            if j == 1 and k == 0:
+                want = (want[0], torch.maximum(want[1], scale * 2.0 ** -9))
             unit = torch.exp2(torch.floor(torch.log2((want[j].abs() / scale).clamp(min=2.0 ** -6))) - 3) * scale  # a step of the codes there
             err = (9 * U * terms if j == 0 else 8 * U * want[1]) + 2 * U * want[j].abs()
             assert bool(((got - want[j]).abs() <= unit + err).all()), (k, j)
@@ -707,3 +709,29 @@ def test_there_is_no_norm_before_a_clipped_step():
     opt.max_grad_norm = 1.0
     opt.step()
     assert float(opt.last_grad_norm) == 6.0
+
+
+@gpu
+@pytest.mark.parametrize("small", [1e-5, 1e-6, 1e-7])
+def test_values_far_below_their_blocks_largest_take_no_long_steps(small):
+    """One value of 256 has gradients of size 1, the others of `small`, near or under the smallest code
+    (4.4e-6 of the largest). Unrounded, |m| <= (1 - b1) / sqrt((1 - b2) (1 - b1^2 / b2)) r = 7.3 r by
+    Cauchy and Schwarz: no step is longer than 7.3 lr. Rounded,
+    m is up to a code higher and r as much lower, but not below one code: 4.4e-6 of the largest, whose
+    own m / r is at most 7.3 too. So (7.3 small + 7.3 x 4.4e-6) over 4.4e-6 at most where r is one code, less
+    above, and the bias corrections of the first 20 steps raise it by sqrt(1 - 0.999^t) / (1 - 0.9^t) < 1."""
+    need_gpu()
+    n, lr = 1024, 1e-3
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    size = torch.where(torch.arange(n, device="cuda") % optim.BLOCK == 5, 1.0, small)
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    opt = optim.AdamW([p], lr=lr, eps=1e-8, weight_decay=0.0, state_bits=8, rounding="stochastic")
+    longest = torch.zeros((), device="cuda")
+    for t in range(500):
+        before = p.detach().clone()
+        g = torch.randn(n, generator=gen, device="cuda") * size
+        p.grad = g * (torch.rand(n, generator=gen, device="cuda") < 0.5)  # half of them without a gradient
+        opt.step()
+        longest = torch.maximum(longest, (p.detach() - before).abs().max())
+    one = 2.0 ** -9 / 448
+    assert float(longest) <= lr * 7.3 * (1 + min(small, one) / one) * (1 + 2.0 ** -3)
