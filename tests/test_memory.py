@@ -297,3 +297,47 @@ def test_a_memory_that_comes_or_goes_is_refused():
         plain.collect()
     ro.collect()
     b.close()
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_whole_update_in_a_graph(bits):
+    """Memory, loss, backward and AdamW's step captured once and replayed, with new inputs and learning rates
+    between, against the eager updates."""
+    from marlsoccer.optim import AdamW
+    need_gpu()
+    T, R, runs = 12, 20, []
+    for graph in (False, True):
+        torch.manual_seed(0)
+        m, head = SequenceMemory(channels=32).cuda(), torch.nn.Linear(66, 3).cuda()
+        params = [*m.parameters(), *head.parameters()]
+        opt = AdamW(params, lr=torch.full((), 1e-3, device="cuda"), max_grad_norm=0.5, state_bits=bits, rounding="stochastic" if bits == 8 else None)
+        x, starts = torch.randn(T, R, 66, device="cuda"), torch.rand(T, R, device="cuda") < 0.1
+
+        def update():
+            opt.zero_grad(set_to_none=True)
+            loss = head(m(x, starts)[0]).square().mean()
+            loss.backward()
+            opt.step()
+            return loss.detach()
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            update()
+        torch.cuda.current_stream().wait_stream(side)
+        if graph:
+            opt.zero_grad(set_to_none=True)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                captured = update()
+        losses = []
+        for _ in range(5):
+            x.mul_(1.01)
+            opt.param_groups[0]["lr"].mul_(0.9)
+            if graph:
+                g.replay()
+            losses.append(captured.clone() if graph else update())
+            torch.cuda.synchronize()
+        runs.append(losses + [p.detach().clone() for p in params])
+    assert all(torch.equal(a, b) for a, b in zip(*runs))

@@ -889,3 +889,73 @@ def test_sequences_past_a_launchs_threads_are_refused_before_anything_runs():
                     workspace_bytes=2 ** 62, dout=16, du=16, ddelta=16, dB=16, dC=16, dA=16, checkpoints=16)
     for fn in (L.ms_scan_forward, L.ms_scan_backward):
         assert fn(C.byref(io), None) == N.MS_ERR_INVALID_ARGUMENT and b"too large" in L.ms_sequence_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("T,R,D,N,G,dtype", [(100, 2, 24, 16, 24, torch.float32), (300, 1, 63, 16, 3, torch.bfloat16), (70, 3, 127, 4, 1, torch.float16),
+                                             (33, 2, 130, 8, 130, torch.float32), (3, 2, 1, 1, 1, torch.float32), (9, 600, 2, 2, 1, torch.bfloat16),
+                                             (257, 3, 192, 16, 3, torch.bfloat16), (40, 2, 66, 20, 6, torch.float16)])
+@pytest.mark.parametrize("every", [False, True], ids=["some starts", "all starts"])
+def test_ssm_scan_odd_groups_and_every_step_a_start(T, R, D, N, G, dtype, every):
+    """Groups of one channel and of odd numbers; starts of any non-zero value, expanded over the rows."""
+    need_gpu()
+    v = scan_inputs(T, R, D, N, G, dtype, 191, "cuda", starts=True, state=True, grouped=True)
+    if every:
+        v["starts"] = torch.full((T, 1), 255, dtype=torch.uint8, device="cuda").expand(T, R)
+    g = gen(192)
+    check_scan(v, True, torch.randn((T, R, D), generator=g).to(dtype).cuda(), torch.randn((R, D, N), generator=g).cuda())
+
+
+@gpu
+def test_only_the_states_gradient_and_a_graph_used_twice():
+    need_gpu()
+    T, R, D, N = 20, 2, 40, 16
+    v = scan_inputs(T, R, D, N, 1, torch.float32, 193, "cuda", state=True)
+    dnew = torch.randn((R, D, N), generator=gen(194)).cuda()
+    leaves = {k: t.detach().requires_grad_() for k, t in v.items() if t is not None}
+    _, new = seq.ssm_scan(**{**v, **leaves}, return_state=True)
+    names = ["u", "delta", "A", "B", "delta_bias", "state"]
+    first = torch.autograd.grad(new, [leaves[k] for k in names], dnew, retain_graph=True)
+    again = torch.autograd.grad(new, [leaves[k] for k in names], dnew)
+    none = torch.zeros(T, R, D)
+    want, size = (ref.scan(**v, dout=none, dnew=dnew, absolute=a)[2] for a in (False, True))
+    for k, x, y in zip(names, first, again):
+        assert torch.equal(x, y)
+        ref.assert_close(k, x, want[k], size[k], ref.scan_chain(T, R, D, N, True))
+
+
+@gpu
+def test_calls_from_several_threads():
+    """Each on its own stream, with gradients: the bits of a call by itself."""
+    import threading
+    need_gpu()
+    v = scan_inputs(60, 3, 70, 16, 1, torch.float32, 195, "cuda", starts=True, state=True)
+    c = conv_inputs(60, 3, 70, 4, torch.float32, 196, "cuda", starts=True, state=True)
+    dout = torch.randn((60, 3, 70), generator=gen(197)).cuda()
+
+    def once():
+        leaves = {k: t.detach().requires_grad_() if k != "starts" else t for k, t in v.items()}
+        x = c["x"].detach().requires_grad_()
+        out = seq.ssm_scan(**{**leaves, "u": seq.short_conv(x, c["weight"], c["bias"], c["state"], c["starts"], "silu")})
+        return [out, *torch.autograd.grad(out, [x, leaves["A"], leaves["B"]], dout)]
+
+    want, wrong = once(), []
+    torch.cuda.synchronize()
+
+    def work():
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    got = once()
+                    stream.synchronize()
+                    wrong.extend(i for i, (a, b) in enumerate(zip(want, got)) if not torch.equal(a, b))
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
