@@ -46,7 +46,7 @@ struct Plan {
   int64_t tiles, blocks_d;  // tiles per group, tiles * groups
   int64_t chunks, chunk;    // over time; steps per chunk (a multiple of 32)
   int64_t kc;               // checkpoints, tiles of the backward pass
-  int64_t segments;         // of a chunk: the backward's sums over time are handed on after each
+  int64_t segments, sums;   // of a chunk and of all: the backward's sums over time are handed on after each
 };
 
 struct Work {  // the workspace, in floats
@@ -871,8 +871,6 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && NS == 4 ? 3 : NW == 1 ? 1 : 2) 
     if (pz) qz -= TT * io.dz_t;
     if (k % (SEGMENT / TT) == 0) hand_on(k / (SEGMENT / TT));
   }
-  // a last chunk that is shorter than the others has nothing to add in their last segments
-  for (int g = (tiles + SEGMENT / TT - 1) / (SEGMENT / TT); g < a.p.segments; ++g) hand_on(g);
   if (live && io.dstate && t_begin == 0) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
@@ -976,7 +974,8 @@ Plan plan(const ms_scan_io& io, bool back) {
   p.chunk = p.chunk < 32 ? 32 : p.chunk;
   p.chunks = io.steps > 0 ? (io.steps + p.chunk - 1) / p.chunk : 1;
   p.kc = (io.steps + KC - 1) / KC;
-  p.segments = ((p.chunks > 1 ? p.chunk : io.steps) + SEGMENT - 1) / SEGMENT;
+  p.segments = (p.chunk + SEGMENT - 1) / SEGMENT;
+  p.sums = (p.chunks - 1) * p.segments + (io.steps - (p.chunks - 1) * p.chunk + SEGMENT - 1) / SEGMENT;  // the last chunk may be shorter
   p.unit = back ? 4 : p.ns;
   // whole tiles of 32 steps, and a unit past the end
   p.units = (io.steps + 31) / 32 * 32 * p.unit / 16 + 1;
@@ -1012,7 +1011,7 @@ Work work(const ms_scan_io& io, const Plan& p, bool back) {
   }
   if (back) {
     w.parts_bc = take(p.kc * io.rows * p.blocks_d * (p.ns * p.nw / 4) * 64);
-    const int64_t sums = parts * p.segments, share = share_of(sums);
+    const int64_t sums = p.sums * io.rows, share = share_of(sums);
     w.parts = take(sums * row);
     w.sums = share ? take((sums + share - 1) / share * row) : nullptr;
   }
@@ -1254,7 +1253,7 @@ int ms_scan_backward(const ms_scan_io* io, void* stream) {
   if (io->dtype == 0) hipLaunchKernelGGL(scan::finish_bc<float>, grid, block, 0, st, a, split);
   else if (io->dtype == 1) hipLaunchKernelGGL(scan::finish_bc<seq::bf16>, grid, block, 0, st, a, split);
   else hipLaunchKernelGGL(scan::finish_bc<seq::f16>, grid, block, 0, st, a, split);
-  const int64_t parts = p.chunks * p.segments * io->rows, share = scan::share_of(parts), row = io->channels * (io->states + 2);
+  const int64_t parts = p.sums * io->rows, share = scan::share_of(parts), row = io->channels * (io->states + 2);
   const unsigned columns = (unsigned)((row + 63) / 64), shares = (unsigned)((parts + share - 1) / share);
   if (shares > 1)
     hipLaunchKernelGGL(seq::sum_parts<4>, dim3(columns, shares), dim3(256), 0, st, w.parts, parts, share, row, w.sums);
