@@ -1,11 +1,12 @@
 // ms_optim.hip — AdamW over a list of tensors, and the gradients' norm that clips them (gfx950).
 //
 // Bound by HBM: p, m and v read and written, g read (28 B a value in float32, 16 B with moments in
-// 8 bits), some 30 operations between. The list travels in the kernel's arguments (48 tensors of 64 B),
+// 8 bits), some 30 operations between. The list travels in the kernel's arguments (48 tensors of 72 B),
 // so a step is one launch whatever the tensors' sizes, needs no table in memory, and a captured graph
 // holds its own copy. A block finds its tensor from the running block counts, 4 values a thread and
 // round. A short list of small tensors (a policy's) is cut finer than a long one, to fill the chip.
-// 201 M values in 8 bits, clipped: 0.78 ms a call, 5.2 TB/s with the norm's read of g; the Agent's 423 k
+// 201 M values in 8 bits, clipped: 0.78 ms a call, 5.2 TB/s with the norm's read of g (rounded to nearest
+// or stochastically alike), in 32 bits 1.25 ms, 5.2 TB/s; the Agent's 423 k
 // values: 10 us for the norm and 10 for the step, which is a launch and a chain of two dependent reads.
 //
 // Step counts stay on the device, one a tensor: every block reads its tensor's count before it takes

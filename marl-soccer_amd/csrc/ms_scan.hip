@@ -22,8 +22,8 @@
 // blocks by a last kernel.
 // Measured at 16 states (time; share of the vector units' cycles that issue): forward 8 rows of 2,048
 // steps x 2,048 channels bf16 233 us, 65 %; one row of 16,411 x 1,536 bf16 in 31 chunks 106 + 133 us,
-// 77 and 72 %; with gradients 2,048 rows of 128 x 128 f32 243 us forward, 59 %, and 600 us backward,
-// 67 % (107 vector instructions a wave, step and four states).
+// 77 and 72 %; with gradients 2,048 rows of 128 x 128 f32 244 us forward, 59 %, and 600 us backward,
+// 67 % (108 vector instructions a wave, step and four states).
 #include <type_traits>
 
 #include "ms_sequence.h"
