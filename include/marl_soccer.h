@@ -479,8 +479,8 @@ const char *ms_sequence_last_error(void);
  *   however many follow, so with beta2 near 1 values keep their ratio to the block's largest for good.
  *   state_bits 8 | MS_ADAMW_STOCHASTIC rounds them to one of the two neighbours (off by less than a
  *   step), at random from a hash of the step count and the element's place, so that the expected value is
- *   the unrounded one and moments follow the 32-bit ones in the mean; the same step gives the same bits. A
- *   root under the smallest code, 2^-9 of the scale, is held as that one.
+ *   the unrounded one and moments follow the 32-bit ones in the mean; the same step gives the same bits.
+ *   With either a root under the smallest code, 2^-9 of the scale, is held as that one.
  *   A moment that is infinite or no number is held as no number, alone.
  * ms_grad_clip: factor = min(1, max_norm / (norm + 1e-6)), norm the Euclidean norm of all the
  *   tensors' gradients (summed in float64, in a fixed order; a non-finite one passes into the

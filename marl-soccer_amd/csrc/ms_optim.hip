@@ -184,9 +184,9 @@ __device__ __forceinline__ float wave_max(float x) {
 // beta2 = 0.999 a root moves by some 0.05 % a step: then only the largest moves, by the scale, and the others
 // follow it (roots 0.3 to 9 times the 32-bit ones after thousands of steps whose gradients change in
 // size). SR keeps such changes in the mean: each rounding is right in expectation, and the held root
-// wanders about the 32-bit one, by some 17 % of it at beta2 = 0.999. ROOT: the second moment's, which SR
-// does not round down to nothing: a value that the first moment was rounded up at would be divided by it
-// (values of 1e-6 of their block's largest: steps of 100 times lr and more).
+// wanders about the 32-bit one, by some 17 % of it at beta2 = 0.999. ROOT: the second moment's, which is
+// not rounded down to nothing: the next step without a gradient would divide the first moment by it (values
+// of 1e-5 of their block's largest took steps of 400 lr, in either rounding).
 template <bool SR, bool ROOT>
 __device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_lane, Odds odds) {
   float top = 0.0f;
@@ -206,7 +206,7 @@ __device__ __forceinline__ uint32_t quantise(f32x4 v, float* scale, bool first_l
   for (int k = 0; k < 4; ++k) {
     const float x = v[k];
     v[k] = x * inv;
-    if constexpr (SR && ROOT) v[k] = v[k] < 0x1p-9f && x > 0.0f ? 0x1p-9f : v[k];
+    if constexpr (ROOT) v[k] = v[k] < 0x1p-9f && x > 0.0f ? 0x1p-9f : v[k];
   }
   if constexpr (SR) return encode(v, odds);
   else return encode(v);

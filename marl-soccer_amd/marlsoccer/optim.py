@@ -16,13 +16,13 @@ down to 2^-14.8 of its block's largest, and 2^-17.8 of the largest below that.
 rounding="stochastic" is for training: each value goes to one of its two neighbours with the odds that
 keep its expectation, from a hash of the step count and its place (the same step gives the same bits). The
 moments then follow the 32-bit ones in the mean; with beta2 = 0.999 a held root wanders by some 17 % about
-the 32-bit one. A root below the smallest code (2^-17.8 of its block's largest) is held as that code, so
-no step is longer for it. rounding="nearest" holds each step's moments to half a step of the codes, but what a step
+the 32-bit one. rounding="nearest" holds each step's moments to half a step of the codes, but what a step
 changes by less than that is lost, at every step, however many follow: with beta2 = 0.999 a root moves by
 some 0.05 % a step, so all but the block's largest only follow that one, through the scale. When gradients
 change in size their roots stay off: by 0.3 to 9 times after thousands of steps where some of a block's
-values grew four times or shrank ten times against the others; and a root below half the smallest code is held
-as 0, which leaves the next step's gradient and eps alone to divide by. A moment that is infinite or no number is
+values grew four times or shrank ten times against the others. With either a
+root below the smallest code (2^-17.8 of its block's largest) is held as that code: held as 0 it would leave
+the next step's gradient and eps alone to divide by. A moment that is infinite or no number is
 held as no number, and reaches no other value of its block.
 """
 from __future__ import annotations

@@ -712,20 +712,22 @@ def test_there_is_no_norm_before_a_clipped_step():
 
 
 @gpu
+@pytest.mark.parametrize("rounding", ["stochastic", "nearest"])
 @pytest.mark.parametrize("small", [1e-5, 1e-6, 1e-7])
-def test_values_far_below_their_blocks_largest_take_no_long_steps(small):
+def test_values_far_below_their_blocks_largest_take_no_long_steps(small, rounding):
     """One value of 256 has gradients of size 1, the others of `small`, near or under the smallest code
     (4.4e-6 of the largest). Unrounded, |m| <= (1 - b1) / sqrt((1 - b2) (1 - b1^2 / b2)) r = 7.3 r by
     Cauchy and Schwarz: no step is longer than 7.3 lr. Rounded,
     m is up to a code higher and r as much lower, but not below one code: 4.4e-6 of the largest, whose
     own m / r is at most 7.3 too. So (7.3 small + 7.3 x 4.4e-6) over 4.4e-6 at most where r is one code, less
-    above, and the bias corrections of the first 20 steps raise it by sqrt(1 - 0.999^t) / (1 - 0.9^t) < 1."""
+    above, and the bias corrections of the first 20 steps raise it by sqrt(1 - 0.999^t) / (1 - 0.9^t) < 1. To
+    nearest a root of one code stays there until 0.999 + 0.001 g^2 passes 1.5^2: g, and so m, is below 36 of it."""
     need_gpu()
     n, lr = 1024, 1e-3
     gen = torch.Generator(device="cuda").manual_seed(7)
     size = torch.where(torch.arange(n, device="cuda") % optim.BLOCK == 5, 1.0, small)
     p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
-    opt = optim.AdamW([p], lr=lr, eps=1e-8, weight_decay=0.0, state_bits=8, rounding="stochastic")
+    opt = optim.AdamW([p], lr=lr, eps=1e-8, weight_decay=0.0, state_bits=8, rounding=rounding)
     longest = torch.zeros((), device="cuda")
     for t in range(500):
         before = p.detach().clone()
@@ -734,4 +736,4 @@ def test_values_far_below_their_blocks_largest_take_no_long_steps(small):
         opt.step()
         longest = torch.maximum(longest, (p.detach() - before).abs().max())
     one = 2.0 ** -9 / 448
-    assert float(longest) <= lr * 7.3 * (1 + min(small, one) / one) * (1 + 2.0 ** -3)
+    assert float(longest) <= lr * (7.3 if rounding == "stochastic" else 36) * (1 + min(small, one) / one) * (1 + 2.0 ** -3)
