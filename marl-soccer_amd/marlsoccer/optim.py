@@ -258,7 +258,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: a weight decay that is part of the gradient (torch.optim.Adam's) is set; this one's is decoupled")
 
     def add_param_group(self, param_group):
-        self._refuse_settings(param_group)
+        if isinstance(param_group, dict):
+            self._refuse_settings(param_group)
         super().add_param_group(param_group)
 
     def load_state_dict(self, state_dict):

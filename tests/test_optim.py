@@ -609,6 +609,8 @@ def test_a_state_of_another_update_is_refused_when_loaded():
         assert not opt.state and opt.param_groups[0]["lr"] == 0.5
     with pytest.raises(ValueError, match="maximize"):
         optim.AdamW([dict(params=params(), maximize=True)])
+    with pytest.raises(TypeError, match="dict"):  # torch's own
+        mine().add_param_group(params())
     with pytest.raises(ValueError, match="moments are"):
         mine(8).load_state_dict(saved(T.AdamW))
     eight = mine(8)
