@@ -13,6 +13,7 @@ from __future__ import annotations
 import torch
 
 from .batch import SoccerBatch
+from .policy import memory_of
 from .rollout import ACT_DIM, OBS_DIM, TRAINABLE, Agent, RunningMeanStd
 
 
@@ -54,7 +55,7 @@ def evaluate(agent: Agent, normalizer: RunningMeanStd, num_episodes: int, seed=N
             from .render import render_batch
         blue = torch.tensor(TRAINABLE, dtype=torch.int64, device=dev)  # on the device: a host index would copy per step
 
-        memory = getattr(agent, "memory", None)
+        memory = memory_of(agent)
         memory_state = None if memory is None else memory.init_state(2 * n, dev)
 
         def body():

@@ -83,6 +83,13 @@ def pack_net(seq: torch.nn.Sequential) -> torch.Tensor:
     return torch.where(ok, flat[src], torch.zeros((), dtype=torch.float32, device=dev))
 
 
+def memory_of(agent):
+    """An Agent's sequence memory (marlsoccer.memory), or None: what an agent of one's own may hold
+    under that name is something else unless it has a state to begin with and steps it."""
+    memory = getattr(agent, "memory", None)
+    return memory if callable(getattr(memory, "init_state", None)) and callable(getattr(memory, "step", None)) else None
+
+
 class FusedPolicy:
     """ms_policy_forward for one Agent: pack() after every parameter change (DeviceRollout
     does it once per collect, inside its graph), then forward(). The kernel goes from the
@@ -96,7 +103,7 @@ class FusedPolicy:
         self.pack()
 
     def pack(self) -> None:
-        if getattr(self.agent, "memory", None) is not None:
+        if memory_of(self.agent) is not None:
             raise ValueError("FusedPolicy has no memory: run the modules of an Agent with one (DeviceRollout(policy='torch'))")
         with torch.no_grad():
             self.packed[0].copy_(pack_net(self.agent.actor_mean))

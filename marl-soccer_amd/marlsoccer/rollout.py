@@ -21,7 +21,7 @@ import torch
 import torch.nn as nn
 from torch.distributions.normal import Normal
 
-from .policy import rollout_record
+from .policy import memory_of, rollout_record
 
 OBS_DIM, ACT_DIM = 66, 3
 TRAINABLE = (0, 1)   # agent_0, agent_1 (blue) — notebook L243
@@ -187,7 +187,7 @@ class DeviceRollout:
         if policy_dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"policy_dtype must be torch.float32 or torch.bfloat16, got {policy_dtype}")
         self.policy_dtype = policy_dtype
-        memory = getattr(agent, "memory", None)
+        memory = memory_of(agent)
         if policy is None:
             policy = "fused" if policy_dtype == torch.float32 and memory is None else "torch"
         if policy not in ("fused", "torch") or (policy == "fused" and policy_dtype != torch.float32):
@@ -324,7 +324,7 @@ class DeviceRollout:
         self._graph = g
 
     def collect(self) -> dict:
-        if (getattr(self.agent, "memory", None) is None) != (self.memory_state is None):
+        if (memory_of(self.agent) is None) != (self.memory_state is None):
             raise ValueError("the agent's memory came or went after this DeviceRollout was made: make another")
         if self.graph and self._collects > 0:
             if self._graph is not None and self._graph_inputs != self._inputs_identity():

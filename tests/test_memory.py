@@ -341,3 +341,36 @@ def test_a_whole_update_in_a_graph(bits):
             torch.cuda.synchronize()
         runs.append(losses + [p.detach().clone() for p in params])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+class Collector(Agent):
+    """An agent with something of its own under the name: no policy's memory."""
+
+    def __init__(self):
+        super().__init__()
+        self.memory = [1, 2, 3]
+
+
+def test_another_kind_of_memory_is_none_of_the_policys():
+    from marlsoccer.policy import FusedPolicy
+    FusedPolicy(Collector())
+
+
+@gpu
+def test_agents_with_another_kind_of_memory_run_as_before():
+    need_gpu()
+    from marlsoccer import SoccerBatch
+    from marlsoccer.evaluate import evaluate
+    runs = []
+    for cls in (Agent, Collector):
+        torch.manual_seed(0)
+        agent, rms = cls().cuda(), RunningMeanStd((66,), device="cuda")
+        b = SoccerBatch(8, config=short_config(20))
+        b.reset(seed=3)
+        ro = DeviceRollout(b, agent, rms, 6, seed=5)
+        assert ro.policy == "fused"
+        out = ro.collect()
+        assert "memory_state" not in out
+        runs.append((out["values"].clone(), torch.from_numpy(evaluate(agent, rms, 4, seed=3, config=short_config(20))["returns"])))
+        b.close()
+    assert all(torch.equal(a, c) for a, c in zip(*runs))
